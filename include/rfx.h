@@ -480,6 +480,125 @@ typedef struct rfx_vit_attn_desc {
 } rfx_vit_attn_desc;
 int rfx_vit_attention(const rfx_vit_attn_desc* desc, void* stream);
 
+/* --------------------------------------------------- int8 layer path ---- */
+/* Operators of a transformer layer whose weights and activations are held as
+ * 8-bit integers (the reference has them in bf16 only: QKVLinear and
+ * MergedColumnLinear, reflex/layers/linear.py:72-148, RotaryEmbedding,
+ * reflex/layers/rope.py:34-132, AdaRMSNorm and the gated residual,
+ * reflex/policies/pi05/modeling_pi05.py:47-99).  In a layer they run as
+ * block_norm (int8 rows) -> linear_i8 (QKV) -> rope -> attention ->
+ * quant_rows -> linear_i8 -> block_norm -> linear_i8 (GEGLU) -> quant_rows ->
+ * linear_i8 -> block_norm.  T == 0 is a no-op in each of them. */
+
+/* Rows to int8 with one scale per row (activations per token, weights per
+ * output channel), the scheme of RFX_QUANT_I8_SYM: scale[t] = absmax_t / 127
+ * (fp32), q = clamp(rne(x / scale), -127, 127); scale == 0 gives q 0.  A row
+ * that holds a NaN or an infinity gets that as its scale and q = 0, so that
+ * what is computed from it is NaN.  1 <= K <= 16384, any alignment of
+ * elements; 16-byte aligned rows (8-byte for q) with K % 8 == 0 take wide
+ * accesses. */
+typedef struct rfx_quant_rows_desc {
+  int T, K;
+  int in_dtype;  /* RFX_DTYPE_BF16 or RFX_DTYPE_F32 */
+  const void* x; /* [T][ldx] */
+  long ldx;
+  void* q; /* int8 [T][ldq] */
+  long ldq;
+  float* scale; /* [T] */
+} rfx_quant_rows_desc;
+int rfx_quant_rows(const rfx_quant_rows_desc* desc, void* stream);
+
+/* y[t][o] = act(x_scale[t] * w_scale[o] * sum_k x[t][k] * w[o][k] + bias[o]).
+ * The integer sum is exact (s32; K <= 65536); scales, bias and activation are
+ * fp32, rounded once to the output type.  epilogue: RFX_EPI_STORE, RFX_EPI_SILU,
+ * RFX_EPI_GELU (tanh form), or RFX_EPI_GEGLU: w holds O/2 gate rows and then
+ * O/2 up rows as they are ([Wgate; Wup], no repacking) and
+ * y[t][f] = gelu_tanh(gate_f) * up_f, O/2 columns.  Any T, O and K; rows of x
+ * and w begin on 16-byte boundaries (pad ldx / ldw; the padding is not read). */
+typedef struct rfx_linear_i8_desc {
+  int T, O, K;
+  int epilogue;
+  int out_dtype; /* RFX_DTYPE_BF16 or RFX_DTYPE_F32 */
+  const void* x; /* int8 [T][ldx] */
+  long ldx;
+  const float* x_scale; /* [T] */
+  const void* w;        /* int8 [O][ldw] */
+  long ldw;
+  const float* w_scale; /* [O] */
+  const float* bias;    /* [O] or NULL */
+  void* y;              /* [T][ldy] */
+  long ldy;
+} rfx_linear_i8_desc;
+int rfx_linear_i8(const rfx_linear_i8_desc* desc, void* stream);
+
+/* What lies between two blocks, in one pass over the rows:
+ *   u  = y                                       the block's output, or
+ *   u  = y * rsqrt(mean y^2 + eps) * post_w      with a norm after the block
+ *   h' = h + residual_scale * gate[b] * u        rounded to dtype, to h_out
+ *   z  = h' * rsqrt(mean h'^2 + eps) * a1 * a2[b] + b2[b]   the next block's norm
+ * b = t / tokens_per_batch; post_w, gate, a1, a2 are 1 and b2 is 0 when NULL.
+ * The next norm reads h' as rounded.  z goes to `z` (dtype) or, as int8 rows
+ * with the scheme of rfx_quant_rows, to z_q / z_scale; with neither, only the
+ * stream is updated; with y == NULL only the norm is computed (h' = h).
+ * h_out may be h and z may be h or y (same stride).  1 <= K <= 16384. */
+typedef struct rfx_block_norm_desc {
+  int T, K, tokens_per_batch;
+  int dtype;     /* of h, y, h_out and z: RFX_DTYPE_BF16 or RFX_DTYPE_F32 */
+  const void* h; /* [T][ldh] residual stream */
+  long ldh;
+  const void* y; /* [T][ldy] or NULL */
+  long ldy;
+  const float* post_w; /* [K] or NULL */
+  const float* gate;   /* [B][K] at stride gate_stride, or NULL */
+  long gate_stride;
+  float residual_scale;
+  void* h_out; /* [T][ldho] */
+  long ldho;
+  const float* norm_a1; /* [K] or NULL */
+  const float* norm_a2; /* [B][K] at stride norm_ab_stride, or NULL */
+  const float* norm_b2;
+  long norm_ab_stride;
+  float eps;
+  void* z; /* [T][ldz] or NULL */
+  long ldz;
+  void* z_q; /* int8 [T][ldzq] or NULL */
+  long ldzq;
+  float* z_scale; /* [T], with z_q */
+} rfx_block_norm_desc;
+int rfx_block_norm(const rfx_block_norm_desc* desc, void* stream);
+
+/* Rotary positions on QKV rows x[b*S + s] = [num_q_heads q heads | num_kv_heads
+ * k heads | num_kv_heads v heads (with v_out)], split into q, k and v, element
+ * (b, h, s, d) at b * stride_b + h * stride_h + s * stride_s + d (so head-major
+ * and token-major outputs, and an output over x itself, are all strides).
+ * Pair i < rot_dim/2 of a q or k head is dims (i, i + rot_dim/2)
+ * (RFX_ROPE_HALF) or (2i, 2i + 1) (RFX_ROPE_INTERLEAVED) and turns by
+ * positions[b*S + s] * inv_freq[i] radians, times `magnitude`; dims past
+ * rot_dim and v are copied.  inv_freq is fp64 on the device (positions far
+ * beyond fp32's reach keep their angle), scaled by the caller for long
+ * contexts.  head_dim <= 256, rot_dim even. */
+#define RFX_ROPE_HALF 0
+#define RFX_ROPE_INTERLEAVED 1
+typedef struct rfx_rope_desc {
+  int B, S;
+  int num_q_heads, num_kv_heads; /* num_kv_heads 0: q only */
+  int head_dim, rot_dim;
+  int pairs; /* RFX_ROPE_* */
+  int dtype; /* RFX_DTYPE_BF16 or RFX_DTYPE_F32 */
+  const void* x; /* [B*S][ldx] */
+  long ldx;
+  const int* positions;   /* [B*S] */
+  const double* inv_freq; /* [rot_dim/2] */
+  float magnitude;
+  void* q_out;
+  long qs_b, qs_h, qs_s;
+  void* k_out; /* NULL with num_kv_heads 0 */
+  long ks_b, ks_h, ks_s;
+  void* v_out; /* NULL: rows of x end after the k heads */
+  long vs_b, vs_h, vs_s;
+} rfx_rope_desc;
+int rfx_rope(const rfx_rope_desc* desc, void* stream);
+
 /* ------------------------------------------------ fused chunk executor ---- */
 /* The whole PI0.5 denoising loop of one chunk (all Euler steps x layers:
  * input norm, QKV+RoPE, partitioned attention over the context ring,
@@ -582,6 +701,10 @@ int rfx_plan_add_rms_norm(rfx_plan* plan, const rfx_norm_desc* desc);
 int rfx_plan_add_patches(rfx_plan* plan, const rfx_patches_desc* desc);
 int rfx_plan_add_layer_norm(rfx_plan* plan, const rfx_layer_norm_desc* desc);
 int rfx_plan_add_vit_attention(rfx_plan* plan, const rfx_vit_attn_desc* desc);
+int rfx_plan_add_quant_rows(rfx_plan* plan, const rfx_quant_rows_desc* desc);
+int rfx_plan_add_linear_i8(rfx_plan* plan, const rfx_linear_i8_desc* desc);
+int rfx_plan_add_block_norm(rfx_plan* plan, const rfx_block_norm_desc* desc);
+int rfx_plan_add_rope(rfx_plan* plan, const rfx_rope_desc* desc);
 /* The chunk (not owned by the plan) is run at this point: counter clear + one launch. */
 int rfx_plan_add_chunk(rfx_plan* plan, rfx_chunk* chunk);
 /* The next op added is launched without programmatic dependent launch: it

@@ -43,6 +43,9 @@ RFX_EPI_GELU = 5
 RFX_PACK_QKV_ROPE = 0
 RFX_PACK_GATE_UP = 1
 
+RFX_ROPE_HALF = 0
+RFX_ROPE_INTERLEAVED = 1
+
 RFX_ADARMS_GATE = 0
 RFX_ADARMS_SSG = 1
 
@@ -204,6 +207,45 @@ class EmbedCacheDesc(ctypes.Structure):
     ]
 
 
+class QuantRowsDesc(Structure):
+    _fields_ = [
+        ("T", c_int), ("K", c_int), ("in_dtype", c_int), ("x", c_void_p), ("ldx", c_long),
+        ("q", c_void_p), ("ldq", c_long), ("scale", c_void_p),
+    ]
+
+
+class LinearI8Desc(Structure):
+    _fields_ = [
+        ("T", c_int), ("O", c_int), ("K", c_int), ("epilogue", c_int), ("out_dtype", c_int),
+        ("x", c_void_p), ("ldx", c_long), ("x_scale", c_void_p),
+        ("w", c_void_p), ("ldw", c_long), ("w_scale", c_void_p),
+        ("bias", c_void_p), ("y", c_void_p), ("ldy", c_long),
+    ]
+
+
+class BlockNormDesc(Structure):
+    _fields_ = [
+        ("T", c_int), ("K", c_int), ("tokens_per_batch", c_int), ("dtype", c_int),
+        ("h", c_void_p), ("ldh", c_long), ("y", c_void_p), ("ldy", c_long),
+        ("post_w", c_void_p), ("gate", c_void_p), ("gate_stride", c_long), ("residual_scale", c_float),
+        ("h_out", c_void_p), ("ldho", c_long),
+        ("norm_a1", c_void_p), ("norm_a2", c_void_p), ("norm_b2", c_void_p), ("norm_ab_stride", c_long),
+        ("eps", c_float), ("z", c_void_p), ("ldz", c_long), ("z_q", c_void_p), ("ldzq", c_long),
+        ("z_scale", c_void_p),
+    ]
+
+
+class RopeDesc(Structure):
+    _fields_ = [
+        ("B", c_int), ("S", c_int), ("num_q_heads", c_int), ("num_kv_heads", c_int),
+        ("head_dim", c_int), ("rot_dim", c_int), ("pairs", c_int), ("dtype", c_int),
+        ("x", c_void_p), ("ldx", c_long), ("positions", c_void_p), ("inv_freq", c_void_p), ("magnitude", c_float),
+        ("q_out", c_void_p), ("qs_b", c_long), ("qs_h", c_long), ("qs_s", c_long),
+        ("k_out", c_void_p), ("ks_b", c_long), ("ks_h", c_long), ("ks_s", c_long),
+        ("v_out", c_void_p), ("vs_b", c_long), ("vs_h", c_long), ("vs_s", c_long),
+    ]
+
+
 # Every entry point declared in include/rfx.h: name -> (argtypes, restype).
 SIGNATURES = {
     "rfx_version": ([], c_int),
@@ -235,6 +277,14 @@ SIGNATURES = {
     "rfx_plan_add_patches": ([c_void_p, POINTER(PatchesDesc)], c_int),
     "rfx_plan_add_layer_norm": ([c_void_p, POINTER(LayerNormDesc)], c_int),
     "rfx_plan_add_vit_attention": ([c_void_p, POINTER(VitAttnDesc)], c_int),
+    "rfx_quant_rows": ([POINTER(QuantRowsDesc), c_void_p], c_int),
+    "rfx_linear_i8": ([POINTER(LinearI8Desc), c_void_p], c_int),
+    "rfx_block_norm": ([POINTER(BlockNormDesc), c_void_p], c_int),
+    "rfx_rope": ([POINTER(RopeDesc), c_void_p], c_int),
+    "rfx_plan_add_quant_rows": ([c_void_p, POINTER(QuantRowsDesc)], c_int),
+    "rfx_plan_add_linear_i8": ([c_void_p, POINTER(LinearI8Desc)], c_int),
+    "rfx_plan_add_block_norm": ([c_void_p, POINTER(BlockNormDesc)], c_int),
+    "rfx_plan_add_rope": ([c_void_p, POINTER(RopeDesc)], c_int),
     "rfx_plan_add_chunk": ([c_void_p, c_void_p], c_int),
     "rfx_chunk_workspace_size": ([POINTER(ChunkDesc), POINTER(c_size_t)], c_int),
     "rfx_chunk_create": ([POINTER(ChunkDesc), c_void_p, c_size_t, POINTER(c_void_p)], c_int),
@@ -295,6 +345,6 @@ def ptr(t) -> int | None:
 
 __all__ = [n for n in dir() if n.startswith(("RFX_", "Rfx"))] + [
     "KvQuantDesc", "LinearDesc", "AttnDesc", "TimeCondDesc", "ModulationDesc", "ActionIoDesc", "CopyRowsDesc",
-    "NormDesc", "ChunkDesc",
+    "NormDesc", "ChunkDesc", "QuantRowsDesc", "LinearI8Desc", "BlockNormDesc", "RopeDesc",
     "SIGNATURES", "load", "check", "call", "ptr", "LIB_PATH", "c_ubyte",
 ]

@@ -1,0 +1,435 @@
+// Linear layers in 8-bit integers: y = act(x_scale[t] * w_scale[o] * (x_q · w_qᵀ) + bias[o]).
+//
+// The integer products are summed exactly (tcgen05.mma kind::i8, s32
+// accumulators in TMEM), so neither the order of the sum nor a split of K
+// changes a result: the only roundings are the int -> fp32 conversion, the two
+// scales, bias and activation in fp32, and one rounding to the output type.
+//
+// Tokens are the MMA's M (a TMEM lane is a token, so a thread of the epilogue
+// holds consecutive outputs of one row) and weight rows its N.  Operands are
+// K-major rows of 128 bytes per K step, staged by TMA with 128-byte swizzle;
+// what lies past T, O or K is filled with zeros by the copy and not stored.
+// For GeGLU a tile's N is half gate rows and half up rows of [Wgate; Wup].
+#include "rfx_internal.h"
+
+#include <algorithm>
+
+namespace rfx {
+namespace {
+
+constexpr int kTileM = 128;
+constexpr int kStepK = 128;  // int8 elements (bytes) of K per stage
+constexpr int kSmemMax = 227 * 1024;
+constexpr int kMaxK = 65536;  // 65536 * 128 * 128 = 2^30: an s32 sum cannot overflow
+
+struct I8Params {
+  int T, O, K;
+  int F;           // output columns: O, or O / 2 with GeGLU
+  int m_tiles;     // 128-token tiles
+  int k_steps;
+  int splits;      // CTAs per cluster, each a part of K
+  int stages;
+  int rows_a;      // token rows per copy: 128, or T rounded up to 8
+  int recv_off;    // receive buffer of the split sums
+  int small_off;
+  const float* x_scale;
+  const float* w_scale;
+  const float* bias;
+  void* y;
+  long ldy;
+  int* status;
+};
+
+enum { kActNone, kActSilu, kActGelu, kActGeglu };
+
+// GELU-tanh as v * sigmoid(2u), u = sqrt(2/pi) (v + 0.044715 v^3):
+// 0.5 (1 + tanh u) = 1 / (1 + e^-2u), one exponential and one division.
+__device__ __forceinline__ float gelu_i8(float v) {
+  const float u2 = 1.5957691216057308f * fmaf(0.044715f * v * v, v, v);
+  return __fdividef(v, 1.f + __expf(-u2));
+}
+__device__ __forceinline__ float silu_i8(float v) { return __fdividef(v, 1.f + __expf(-v)); }
+
+template <int ACT>
+__device__ __forceinline__ float activate(float v) {
+  if (ACT == kActSilu) return silu_i8(v);
+  if (ACT == kActGelu) return gelu_i8(v);
+  return v;
+}
+
+// Scales, bias and activation of 4 accumulators of token scale sx; for GeGLU
+// `up` are the 4 accumulators of the matching up rows.  o is the first output
+// column; columns past F read nothing.
+template <int ACT>
+__device__ __forceinline__ void finish4(const I8Params& p, const int (&acc)[4], const int (&up)[4], float sx, int o,
+                                        float (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (o + j >= p.F) {
+      v[j] = 0.f;
+      continue;
+    }
+    float a = static_cast<float>(acc[j]) * sx * __ldg(p.w_scale + o + j);
+    if (p.bias) a += __ldg(p.bias + o + j);
+    if (ACT == kActGeglu) {
+      float u = static_cast<float>(up[j]) * sx * __ldg(p.w_scale + p.F + o + j);
+      if (p.bias) u += __ldg(p.bias + p.F + o + j);
+      v[j] = gelu_i8(a) * u;
+    } else {
+      v[j] = activate<ACT>(a);
+    }
+  }
+}
+
+__device__ __forceinline__ void put4(float* y, int n, bool wide, const float (&v)[4]) {
+  if (wide && n >= 4) {
+    *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) y[j] = v[j];
+  }
+}
+__device__ __forceinline__ void put4(__nv_bfloat16* y, int n, bool wide, const float (&v)[4]) {
+  if (wide && n >= 4) {
+    *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) y[j] = __float2bfloat16_rn(v[j]);
+  }
+}
+
+__device__ __forceinline__ void st_dsmem_i4(uint32_t addr, const int (&v)[4]) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+
+// One tile of 128 tokens x NT weight rows per cluster, K split over its CTAs.
+// Warp 0 issues the copies, warp 1 the MMAs, warps 2-5 read the accumulators.
+// With a split, every CTA pushes the s32 sums of the columns that CTA r owns
+// (1/splits of the tile) into r's receive buffer through DSMEM, and after a
+// cluster barrier r adds them and runs the epilogue of its columns.
+constexpr int kI8Threads = 192;
+constexpr int kI8MaxStages = 8;
+
+template <int NT, int ACT, typename Tout>
+__global__ void __launch_bounds__(kI8Threads, 1)
+    linear_i8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                     const I8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr bool kGeglu = ACT == kActGeglu;
+  constexpr int kStage = (kTileM + NT) * kStepK;
+  constexpr int kOutCols = kGeglu ? NT / 2 : NT;  // output columns of a tile
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool clustered = p.splits > 1;
+  const int split = clustered ? static_cast<int>(cluster_ctarank()) : 0;
+  const int tile = blockIdx.x / p.splits;
+  const int t0 = tile % p.m_tiles * kTileM;
+  const int o0 = tile / p.m_tiles * kOutCols;
+  const int k0 = static_cast<int>(static_cast<long>(split) * p.k_steps / p.splits);
+  const int nk = static_cast<int>(static_cast<long>(split + 1) * p.k_steps / p.splits) - k0;
+
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.small_off);
+  uint64_t* empty = full + kI8MaxStages;
+  uint64_t* acc_bar = empty + kI8MaxStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_bar + 1);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(acc_bar, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmW);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, NT);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  // the cluster's CTAs have all started before anyone writes into a peer
+  if (clustered)
+    cluster_sync();
+  else
+    __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  int issued = 0;
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t bytes = static_cast<uint32_t>((p.rows_a + NT) * kStepK);
+      for (int i = 0; i < nk; ++i) {
+        const int s = i % p.stages;
+        if (i >= p.stages && !mbar_wait(&empty[s], ((i / p.stages) - 1) & 1, p.status, kDevTimeoutStageEmpty)) break;
+        uint8_t* st = smem + s * kStage;
+        const int kx = (k0 + i) * kStepK;
+        mbar_arrive_expect_tx(&full[s], bytes);
+        if (kGeglu) {
+          tma_load_2d(st + kTileM * kStepK, &tmW, &full[s], kx, o0);
+          tma_load_2d(st + (kTileM + NT / 2) * kStepK, &tmW, &full[s], kx, p.F + o0);
+        } else {
+          tma_load_2d(st + kTileM * kStepK, &tmW, &full[s], kx, o0);
+        }
+        tma_load_2d(st, &tmX, &full[s], kx, t0);
+        issued = i + 1;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_i8(kTileM, NT);
+      bool ok = true;
+      for (int i = 0; i < nk; ++i) {
+        const int s = i % p.stages;
+        if (!(ok = mbar_wait(&full[s], (i / p.stages) & 1, p.status, kDevTimeoutTmaFull))) break;
+        tc_fence_after();
+        const uint32_t a = smem_u32(smem + s * kStage);
+        const uint64_t ad = make_sdesc_sw128(a, 16, 1024);
+        const uint64_t bd = make_sdesc_sw128(a + kTileM * kStepK, 16, 1024);
+#pragma unroll
+        for (int kk = 0; kk < kStepK / 32; ++kk)
+          umma_i8_ss(tmem, ad + kk * 2, bd + kk * 2, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&empty[s]);
+      }
+      if (ok) umma_commit(acc_bar);
+    }
+    __syncwarp();
+  } else {
+    bool ok = true;
+    if (lane == 0) ok = mbar_wait(acc_bar, 0, p.status, kDevTimeoutMmaDone);
+    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    if (ok) {
+      tc_fence_after();
+      if (!clustered) {
+        const int t = t0 + row;
+        const bool live = t < p.T;
+        const float sx = live ? p.x_scale[t] : 0.f;
+        Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy;
+        const bool wide = (p.ldy * sizeof(Tout)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
+#pragma unroll 1
+        for (int c = 0; c < kOutCols; c += 16) {
+          uint32_t r[16], u[16];
+          tmem_ld16(acc + c, r);
+          if (kGeglu) tmem_ld16(acc + NT / 2 + c, u);
+          tmem_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int g = 0; g < 16; g += 4) {
+              const int o = o0 + c + g;
+              int a4[4], u4[4];
+              float v[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                a4[j] = static_cast<int>(r[g + j]);
+                u4[j] = kGeglu ? static_cast<int>(u[g + j]) : 0;
+              }
+              finish4<ACT>(p, a4, u4, sx, o, v);
+              if (o < p.F) put4(y + o, p.F - o, wide, v);
+            }
+          }
+          __syncwarp();
+        }
+      } else {
+        // groups of 4 accumulator columns; the output columns of owner r are
+        // r * own .. , the gate and up halves of a GeGLU tile alike
+        const int own = kOutCols / p.splits;       // output columns per owner
+        const int groups = NT / 4 / p.splits;      // accumulator groups per owner
+        const int ld = p.rows_a + 2;               // rows per group slot (+2: conflict-free reads)
+        const uint32_t base = smem_u32(smem + p.recv_off) + static_cast<uint32_t>(split * groups * ld + row) * 16u;
+#pragma unroll 1
+        for (int c = 0; c < NT; c += 16) {
+          uint32_t r[16];
+          tmem_ld16(acc + c, r);
+          tmem_wait_ld();
+          if (row < p.rows_a) {
+#pragma unroll
+            for (int g = 0; g < 16; g += 4) {
+              const int col = kGeglu ? (c + g) % (NT / 2) : c + g;
+              const int owner = col / own;
+              const int slot = (col - owner * own) / 4 + (kGeglu && c + g >= NT / 2 ? own / 4 : 0);
+              const int v[4] = {static_cast<int>(r[g]), static_cast<int>(r[g + 1]), static_cast<int>(r[g + 2]),
+                                static_cast<int>(r[g + 3])};
+              st_dsmem_i4(mapa_shared(base + static_cast<uint32_t>(slot * ld) * 16u, owner), v);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+  if (clustered) {
+    tc_fence_before();
+    cluster_sync();
+    const int own = kOutCols / p.splits;
+    const int groups = NT / 4 / p.splits;
+    const int ld = p.rows_a + 2;
+    const int4* recv = reinterpret_cast<const int4*>(smem + p.recv_off);
+    const int og = own / 4;  // output groups
+    const int rows = min(p.T - t0, kTileM);
+    const bool wide = (p.ldy * sizeof(Tout)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
+    for (int i = threadIdx.x; i < rows * og; i += kI8Threads) {
+      const int row = i / og, g = i - row * og;
+      int a4[4] = {0, 0, 0, 0}, u4[4] = {0, 0, 0, 0};
+#pragma unroll 4
+      for (int q = 0; q < p.splits; ++q) {
+        const int4 v = recv[(q * groups + g) * ld + row];
+        a4[0] += v.x; a4[1] += v.y; a4[2] += v.z; a4[3] += v.w;
+        if (kGeglu) {
+          const int4 w = recv[(q * groups + og + g) * ld + row];
+          u4[0] += w.x; u4[1] += w.y; u4[2] += w.z; u4[3] += w.w;
+        }
+      }
+      const int t = t0 + row, o = o0 + split * own + g * 4;
+      float v[4];
+      finish4<ACT>(p, a4, u4, p.x_scale[t], o, v);
+      if (o < p.F) put4(static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy + o, p.F - o, wide, v);
+    }
+  }
+  // a producer that stopped early waits (bounded) for its copies in flight
+  if (warp == 0 && lane == 0)
+    for (int i = (issued > p.stages ? issued - p.stages : 0); i < issued; ++i)
+      mbar_wait(&full[i % p.stages], (i / p.stages) & 1, p.status, kDevTimeoutTmaFull);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, NT);
+  }
+}
+
+// ------------------------------------------------------------ host side ---
+struct I8Plan {
+  int nt, splits, stages, rows_a, recv_off, small_off, smem, m_tiles, n_tiles;
+};
+
+int out_cols(const rfx_linear_i8_desc& d) { return d.epilogue == RFX_EPI_GEGLU ? d.O / 2 : d.O; }
+
+I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
+  I8Plan c{};
+  c.nt = 128;
+  const int tile_cols = d.epilogue == RFX_EPI_GEGLU ? c.nt / 2 : c.nt;
+  c.m_tiles = (d.T + kTileM - 1) / kTileM;
+  c.n_tiles = (out_cols(d) + tile_cols - 1) / tile_cols;
+  c.rows_a = std::min(kTileM, (d.T + 7) / 8 * 8);
+  const int k_steps = (d.K + kStepK - 1) / kStepK;
+  c.splits = 1;
+  for (int s : {2, 4, 8})
+    if (s <= k_steps && static_cast<long>(c.m_tiles) * c.n_tiles * s <= nsm) c.splits = s;
+  const int stage = (kTileM + c.nt) * kStepK;
+  const int recv = c.splits > 1 ? c.nt / 4 * (c.rows_a + 2) * 16 : 0;
+  const int small = 256;
+  const int per = (k_steps + c.splits - 1) / c.splits;
+  c.stages = std::min({kI8MaxStages, per, (kSmemMax - 1024 - recv - small) / stage});
+  c.recv_off = c.stages * stage;
+  c.small_off = c.recv_off + recv;
+  c.smem = c.small_off + small + 1024;
+  return c;
+}
+
+template <int ACT>
+const void* i8_ptr(int out_dtype) {
+  return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_kernel<128, ACT, __nv_bfloat16>)
+                                 : reinterpret_cast<const void*>(linear_i8_kernel<128, ACT, float>);
+}
+const void* i8_kernel(int epilogue, int out_dtype) {
+  switch (epilogue) {
+    case RFX_EPI_STORE: return i8_ptr<kActNone>(out_dtype);
+    case RFX_EPI_SILU: return i8_ptr<kActSilu>(out_dtype);
+    case RFX_EPI_GELU: return i8_ptr<kActGelu>(out_dtype);
+    case RFX_EPI_GEGLU: return i8_ptr<kActGeglu>(out_dtype);
+  }
+  return nullptr;
+}
+
+bool al(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+}  // namespace
+
+int validate_linear_i8(const rfx_linear_i8_desc& d) {
+  if (d.T < 0 || d.O < 1 || d.K < 1 || d.K > kMaxK)
+    return set_error(RFX_E_INVAL, "rfx_linear_i8: need T>=0, O>=1, 1<=K<=%d (T=%d O=%d K=%d)", kMaxK, d.T, d.O, d.K);
+  if (d.epilogue != RFX_EPI_STORE && d.epilogue != RFX_EPI_SILU && d.epilogue != RFX_EPI_GELU &&
+      d.epilogue != RFX_EPI_GEGLU)
+    return set_error(RFX_E_INVAL, "rfx_linear_i8: epilogue must be STORE, SILU, GELU or GEGLU");
+  if (d.epilogue == RFX_EPI_GEGLU && d.O % 2)
+    return set_error(RFX_E_INVAL, "rfx_linear_i8: GEGLU needs an even O (gate rows, then as many up rows)");
+  if (d.out_dtype != kDtypeBF16 && d.out_dtype != kDtypeF32)
+    return set_error(RFX_E_INVAL, "rfx_linear_i8: output dtype must be bf16 or f32");
+  if (d.T == 0) return RFX_OK;
+  if (!d.x || !d.w || !d.x_scale || !d.w_scale || !d.y)
+    return set_error(RFX_E_INVAL, "rfx_linear_i8: null pointer");
+  if (!al(d.x, 16) || !al(d.w, 16) || d.ldx < d.K || d.ldw < d.K || d.ldx % 16 || d.ldw % 16)
+    return set_error(RFX_E_INVAL,
+                     "rfx_linear_i8: int8 rows must begin on 16-byte boundaries (aligned x and w, ldx and ldw >= K and "
+                     "multiples of 16)");
+  if (d.ldy < out_cols(d) || !al(d.y, d.out_dtype == kDtypeBF16 ? 2 : 4) || !al(d.x_scale, 4) || !al(d.w_scale, 4) ||
+      !al(d.bias, 4))
+    return set_error(RFX_E_INVAL, "rfx_linear_i8: ldy below the output's columns, or a misaligned pointer");
+  if ((static_cast<long>(d.T) / kTileM + 1) * (d.O / 32 + 1) > 0x7fffffffL / 8)
+    return set_error(RFX_E_INVAL, "rfx_linear_i8: too many output tiles (T=%d O=%d)", d.T, d.O);
+  return RFX_OK;
+}
+
+int build_linear_i8_maps(const rfx_linear_i8_desc& d, CUtensorMap* tmX, CUtensorMap* tmW) {
+  int rc = validate_linear_i8(d);
+  if (rc || d.T == 0) return rc;
+  int nsm = 148;
+  rfx_num_sms(&nsm);
+  const I8Plan c = plan_i8(d, nsm);
+  rc = make_tmap_2d(tmX, d.x, 1, d.K, d.T, d.ldx, kStepK, c.rows_a, true);
+  if (rc) return rc;
+  return make_tmap_2d(tmW, d.w, 1, d.K, d.O, d.ldw, kStepK, d.epilogue == RFX_EPI_GEGLU ? c.nt / 2 : c.nt, true);
+}
+
+int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const CUtensorMap* tmW, cudaStream_t stream,
+                     bool pdl) {
+  if (d.T == 0) return RFX_OK;
+  int nsm = 148;
+  rfx_num_sms(&nsm);
+  const I8Plan c = plan_i8(d, nsm);
+  const void* fn = i8_kernel(d.epilogue, d.out_dtype);
+  const int rc = ensure_smem_attr(fn, c.smem);
+  if (rc) return rc;
+  I8Params p{};
+  p.T = d.T;
+  p.O = d.O;
+  p.K = d.K;
+  p.F = out_cols(d);
+  p.m_tiles = c.m_tiles;
+  p.k_steps = (d.K + kStepK - 1) / kStepK;
+  p.splits = c.splits;
+  p.stages = c.stages;
+  p.rows_a = c.rows_a;
+  p.recv_off = c.recv_off;
+  p.small_off = c.small_off;
+  p.x_scale = d.x_scale;
+  p.w_scale = d.w_scale;
+  p.bias = d.bias;
+  p.y = d.y;
+  p.ldy = d.ldy;
+  p.status = device_status_ptr();
+  CUtensorMap x = *tmX, w = *tmW;
+  const unsigned grid = static_cast<unsigned>(c.m_tiles) * c.n_tiles * c.splits;
+  return launch_kernel(fn, dim3(grid), dim3(kI8Threads), static_cast<size_t>(c.smem), stream, pdl, c.splits, x, w, p);
+}
+
+}  // namespace rfx
+
+extern "C" int rfx_linear_i8(const rfx_linear_i8_desc* d, void* stream) {
+  using namespace rfx;
+  if (!d) return set_error(RFX_E_INVAL, "rfx_linear_i8: null descriptor");
+  CUtensorMap x, w;
+  const int rc = build_linear_i8_maps(*d, &x, &w);
+  if (rc) return rc;
+  return launch_linear_i8(*d, &x, &w, static_cast<cudaStream_t>(stream), pdl_enabled());
+}

@@ -103,6 +103,10 @@ int validate_rms_norm(const rfx_norm_desc& d);
 int validate_patches(const rfx_patches_desc& d);
 int validate_layer_norm(const rfx_layer_norm_desc& d);
 int validate_vit_attention(const rfx_vit_attn_desc& d);
+int validate_quant_rows(const rfx_quant_rows_desc& d);
+int validate_block_norm(const rfx_block_norm_desc& d);
+int validate_rope(const rfx_rope_desc& d);
+int validate_linear_i8(const rfx_linear_i8_desc& d);
 
 int launch_time_cond(const rfx_time_cond_desc& d, cudaStream_t stream, bool pdl);
 int launch_modulation(const rfx_modulation_desc& d, cudaStream_t stream, bool pdl);
@@ -113,6 +117,12 @@ int launch_rms_norm(const rfx_norm_desc& d, cudaStream_t stream, bool pdl);
 int launch_patches(const rfx_patches_desc& d, cudaStream_t stream, bool pdl);
 int launch_layer_norm(const rfx_layer_norm_desc& d, cudaStream_t stream, bool pdl);
 int launch_vit_attention(const rfx_vit_attn_desc& d, cudaStream_t stream, bool pdl);
+int launch_quant_rows(const rfx_quant_rows_desc& d, cudaStream_t stream, bool pdl);
+int launch_block_norm(const rfx_block_norm_desc& d, cudaStream_t stream, bool pdl);
+int launch_rope(const rfx_rope_desc& d, cudaStream_t stream, bool pdl);
+int build_linear_i8_maps(const rfx_linear_i8_desc& d, CUtensorMap* tmX, CUtensorMap* tmW);
+int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const CUtensorMap* tmW, cudaStream_t stream,
+                     bool pdl);
 int run_chunk_op(rfx_chunk* c, cudaStream_t s);
 
 }  // namespace rfx

@@ -348,12 +348,25 @@ struct LayerNormOp {
 struct VitAttnOp {
   rfx_vit_attn_desc d;
 };
+struct QuantRowsOp {
+  rfx_quant_rows_desc d;
+};
+struct BlockNormOp {
+  rfx_block_norm_desc d;
+};
+struct RopeOp {
+  rfx_rope_desc d;
+};
+struct LinearI8Op {
+  rfx_linear_i8_desc d;
+  CUtensorMap x, w;
+};
 struct BarrierOp {};
 struct ChunkOp {
   rfx_chunk* c;
 };
 using Op = std::variant<LinearOp, AttnOp, QuantOp, TimeOp, ModOp, InOp, TailOp, CopyOp, NormOp, BarrierOp, ChunkOp,
-                        PatchOp, LayerNormOp, VitAttnOp>;
+                        PatchOp, LayerNormOp, VitAttnOp, QuantRowsOp, BlockNormOp, RopeOp, LinearI8Op>;
 }  // namespace
 
 struct rfx_plan {
@@ -379,6 +392,10 @@ int run_op(const Op& op, cudaStream_t s, bool pdl) {
   if (auto* o = std::get_if<PatchOp>(&op)) return launch_patches(o->d, s, pdl);
   if (auto* o = std::get_if<LayerNormOp>(&op)) return launch_layer_norm(o->d, s, pdl);
   if (auto* o = std::get_if<VitAttnOp>(&op)) return launch_vit_attention(o->d, s, pdl);
+  if (auto* o = std::get_if<QuantRowsOp>(&op)) return launch_quant_rows(o->d, s, pdl);
+  if (auto* o = std::get_if<BlockNormOp>(&op)) return launch_block_norm(o->d, s, pdl);
+  if (auto* o = std::get_if<RopeOp>(&op)) return launch_rope(o->d, s, pdl);
+  if (auto* o = std::get_if<LinearI8Op>(&op)) return launch_linear_i8(o->d, &o->x, &o->w, s, pdl);
   return set_error(RFX_E_STATE, "plan: unknown op");
 }
 // Launches every op in order; an op that follows a BarrierOp runs without PDL.
@@ -526,6 +543,40 @@ extern "C" int rfx_plan_add_vit_attention(rfx_plan* plan, const rfx_vit_attn_des
   if (rc) return rc;
   plan->ops.emplace_back(VitAttnOp{*desc});
   plan->launches += 1;
+  return RFX_OK;
+}
+
+extern "C" int rfx_plan_add_quant_rows(rfx_plan* plan, const rfx_quant_rows_desc* desc) {
+  PLAN_GUARD(plan);
+  const int rc = validate_quant_rows(*desc);
+  if (rc) return rc;
+  plan->ops.emplace_back(QuantRowsOp{*desc});
+  plan->launches += desc->T > 0 ? 1 : 0;
+  return RFX_OK;
+}
+extern "C" int rfx_plan_add_block_norm(rfx_plan* plan, const rfx_block_norm_desc* desc) {
+  PLAN_GUARD(plan);
+  const int rc = validate_block_norm(*desc);
+  if (rc) return rc;
+  plan->ops.emplace_back(BlockNormOp{*desc});
+  plan->launches += desc->T > 0 ? 1 : 0;
+  return RFX_OK;
+}
+extern "C" int rfx_plan_add_rope(rfx_plan* plan, const rfx_rope_desc* desc) {
+  PLAN_GUARD(plan);
+  const int rc = validate_rope(*desc);
+  if (rc) return rc;
+  plan->ops.emplace_back(RopeOp{*desc});
+  plan->launches += desc->B > 0 && desc->S > 0 ? 1 : 0;
+  return RFX_OK;
+}
+extern "C" int rfx_plan_add_linear_i8(rfx_plan* plan, const rfx_linear_i8_desc* desc) {
+  PLAN_GUARD(plan);
+  LinearI8Op op{*desc, {}, {}};
+  const int rc = build_linear_i8_maps(op.d, &op.x, &op.w);
+  if (rc) return rc;
+  plan->ops.emplace_back(op);
+  plan->launches += desc->T > 0 ? 1 : 0;
   return RFX_OK;
 }
 

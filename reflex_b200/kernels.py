@@ -7,6 +7,7 @@ live on a CUDA device: there is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 
 import torch
@@ -348,6 +349,218 @@ def copy_rows(**kw) -> None:
     L.call("rfx_copy_rows", ctypes.byref(d), _stream())
 
 
+# -------------------------------------------------------- int8 layer path ---
+_CODES = {torch.bfloat16: L.RFX_DTYPE_BF16, torch.float32: L.RFX_DTYPE_F32}
+
+
+def _here(*ts) -> None:
+    """Every tensor lies on the current CUDA device (whose stream is used)."""
+    for t in ts:
+        if t is not None and t.get_device() < 0:
+            raise ValueError("rfx kernels take CUDA tensors only (there is no CPU fallback)")
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensor on cuda:{t.get_device()}, current device cuda:{dev}")
+
+
+def _rows(name: str, t: torch.Tensor, T: int, K: int, align: int = 1) -> int:
+    """Row stride of a [T, K] tensor with contiguous rows (a single row's
+    stride is never used: the smallest that is a multiple of `align`)."""
+    if t.dim() != 2 or t.shape[0] != T or t.shape[1] != K or (K > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be [{T}, {K}] with contiguous rows")
+    if T > 0x7FFFFFFF:
+        raise ValueError(f"{name}: at most 2^31 - 1 rows")
+    ld = t.stride(0)
+    if T <= 1:
+        return -(-K // align) * align
+    if ld < K:
+        raise ValueError(f"{name}: rows overlap (stride {ld}, length {K})")
+    return ld
+
+
+def _dtype(name: str, t: torch.Tensor, *allowed) -> None:
+    if t.dtype not in allowed:
+        raise ValueError(f"{name} is {t.dtype}, not {' or '.join(str(a) for a in allowed)}")
+
+
+def _vector(name: str, t: torch.Tensor | None, K: int) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != K or (K > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a contiguous fp32 [{K}]")
+    return t.data_ptr()
+
+
+def _per_batch(name: str, t: torch.Tensor | None, T: int, S: int, K: int) -> int:
+    """Batch stride of an fp32 vector per stream [B, K], or [K] for all of them."""
+    if t is None:
+        return 0
+    if t.dtype != torch.float32 or t.dim() not in (1, 2) or t.shape[-1] != K or (K > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be fp32 [B, {K}] or [{K}] with contiguous rows")
+    if t.dim() == 1:
+        return 0
+    if t.shape[0] * S < T:
+        raise ValueError(f"{name} has {t.shape[0]} rows for {T} tokens of {S} per stream")
+    return t.stride(0)
+
+
+def quant_rows_desc(*, x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> L.QuantRowsDesc:
+    """Rows x [T, K] (bf16 or fp32) to int8 q [T, K] and fp32 scale [T]."""
+    _here(x, q, scale)
+    _dtype("x", x, torch.bfloat16, torch.float32)
+    _dtype("q", q, torch.int8)
+    T, K = x.shape
+    ldx, ldq = _rows("x", x, T, K), _rows("q", q, T, K)
+    return L.QuantRowsDesc(T, K, _CODES[x.dtype], x.data_ptr(), ldx, q.data_ptr(), ldq, _vector("scale", scale, T))
+
+
+def quant_rows(*, x, q, scale) -> None:
+    """int8 rows with one scale per row: scale = absmax / 127, q = rne(x / scale)."""
+    d = quant_rows_desc(x=x, q=q, scale=scale)
+    L.call("rfx_quant_rows", ctypes.byref(d), _stream())
+
+
+def linear_i8_desc(*, w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, y: torch.Tensor,
+                   epilogue: int = L.RFX_EPI_STORE, bias: torch.Tensor | None = None) -> L.LinearI8Desc:
+    """y = act((x_scale * w_scale) * (x @ w^T) + bias): int8 x [T, K] and
+    w [O, K] whose rows begin on 16-byte boundaries, fp32 scales [T] and [O],
+    y [T, O] bf16 or fp32 ([T, O/2] with RFX_EPI_GEGLU, w = [Wgate; Wup])."""
+    _here(w, w_scale, x, x_scale, y, bias)
+    _dtype("x", x, torch.int8)
+    _dtype("w", w, torch.int8)
+    _dtype("y", y, torch.bfloat16, torch.float32)
+    T, K = x.shape
+    O = w.shape[0]
+    ldx, ldw = _rows("x", x, T, K, 16), _rows("w", w, O, K, 16)
+    ldy = _rows("y", y, T, O // 2 if epilogue == L.RFX_EPI_GEGLU else O)
+    return L.LinearI8Desc(T, O, K, epilogue, _CODES[y.dtype], x.data_ptr(), ldx, _vector("x_scale", x_scale, T),
+                          w.data_ptr(), ldw, _vector("w_scale", w_scale, O), _vector("bias", bias, O), y.data_ptr(),
+                          ldy)
+
+
+def linear_i8(*, w, w_scale, x, x_scale, y, epilogue=L.RFX_EPI_STORE, bias=None) -> None:
+    """Linear layer in 8-bit integers with a scale per token and per output channel."""
+    d = linear_i8_desc(w=w, w_scale=w_scale, x=x, x_scale=x_scale, y=y, epilogue=epilogue, bias=bias)
+    L.call("rfx_linear_i8", ctypes.byref(d), _stream())
+
+
+def block_norm_desc(*, h: torch.Tensor, S: int, y: torch.Tensor | None = None, post_w=None, gate=None,
+                    residual_scale: float = 1.0, h_out: torch.Tensor | None = None, norm_a1=None, norm_a2=None,
+                    norm_b2=None, eps: float = 1e-6, z: torch.Tensor | None = None, z_q: torch.Tensor | None = None,
+                    z_scale: torch.Tensor | None = None) -> L.BlockNormDesc:
+    """Residual stream h [T, K], the block's output y [T, K] (same dtype), S
+    tokens per stream; post_w and norm_a1 [K], gate, norm_a2 and norm_b2
+    [B, K] or [K] (fp32).  h_out takes the updated stream (h for in place),
+    z or z_q and z_scale the next norm's output."""
+    _here(h, y, post_w, gate, h_out, norm_a1, norm_a2, norm_b2, z, z_q, z_scale)
+    _dtype("h", h, torch.bfloat16, torch.float32)
+    T, K = h.shape
+    if S < 1:
+        raise ValueError("S (tokens per stream) must be at least 1")
+    ld = {"h": _rows("h", h, T, K), "y": 0, "h_out": 0, "z": 0, "z_q": 0}
+    for name, t in (("y", y), ("h_out", h_out), ("z", z)):
+        if t is not None:
+            _dtype(name, t, h.dtype)
+            ld[name] = _rows(name, t, T, K)
+    if z_q is not None:
+        _dtype("z_q", z_q, torch.int8)
+        ld["z_q"] = _rows("z_q", z_q, T, K)
+    sa, sb = _per_batch("norm_a2", norm_a2, T, S, K), _per_batch("norm_b2", norm_b2, T, S, K)
+    if norm_a2 is not None and norm_b2 is not None and sa != sb and T > S:
+        raise ValueError("norm_a2 and norm_b2 must have one batch stride")
+    return L.BlockNormDesc(T, K, min(S, 0x7FFFFFFF), _CODES[h.dtype], h.data_ptr(), ld["h"], L.ptr(y), ld["y"],
+                           _vector("post_w", post_w, K), L.ptr(gate), _per_batch("gate", gate, T, S, K),
+                           residual_scale, L.ptr(h_out), ld["h_out"], _vector("norm_a1", norm_a1, K), L.ptr(norm_a2),
+                           L.ptr(norm_b2), sa if norm_a2 is not None else sb, eps, L.ptr(z), ld["z"], L.ptr(z_q),
+                           ld["z_q"], _vector("z_scale", z_scale, T))
+
+
+def block_norm(**kw) -> None:
+    """The norm of a block's output, its gate and residual scale, the residual
+    add and the next block's norm (as it is, or as int8 rows), in one pass."""
+    d = block_norm_desc(**kw)
+    L.call("rfx_block_norm", ctypes.byref(d), _stream())
+
+
+def rope_frequencies(rot_dim: int, theta: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
+                     trained_len: int | None = None, device="cuda") -> tuple[torch.Tensor, float]:
+    """(inv_freq, magnitude) for `rope`: fp64 radians per position of each of
+    the rot_dim / 2 pairs, theta^(-2i / rot_dim), stretched by `factor` for
+    contexts longer than the trained one:
+
+    * ``"linear"``: every frequency divided by the factor;
+    * ``"ntk"``: theta raised so that the slowest pair is divided by it;
+    * ``"yarn"`` (Peng et al. 2023): pairs that turn more than 32 times over
+      `trained_len` positions are kept, those that turn less than once are
+      divided, linearly in between; q and k grow by 0.1 ln(factor) + 1.
+    """
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError("rot_dim must be even and at least 2")
+    if factor < 1.0:
+        raise ValueError("factor must be at least 1")
+    if scaling == "ntk":
+        if rot_dim == 2:
+            raise ValueError("ntk scaling needs more than one pair")
+        theta = theta * factor ** (rot_dim / (rot_dim - 2))
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    f = theta ** (-2.0 * i / rot_dim)
+    magnitude = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        if not trained_len or trained_len < 1:
+            raise ValueError("yarn scaling needs trained_len")
+        turns = trained_len * f / (2.0 * math.pi)
+        keep = ((turns - 1.0) / 31.0).clamp(0.0, 1.0)
+        f = keep * f + (1.0 - keep) * f / factor
+        magnitude = 0.1 * math.log(factor) + 1.0
+    elif scaling not in ("none", "ntk"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    return f.to(device), magnitude
+
+
+def rope_desc(*, x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, q_out: torch.Tensor,
+              k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None, pairs: int = L.RFX_ROPE_HALF,
+              magnitude: float = 1.0) -> L.RopeDesc:
+    """x [B*S, (Hq + Hkv + Hkv) * D] QKV rows (Hkv once less without v_out);
+    q_out [B, Hq, S, D], k_out and v_out [B, Hkv, S, D] views of any strides
+    with contiguous D (also over x itself); positions int32 [B*S]; inv_freq
+    fp64 [rot_dim / 2]."""
+    _here(x, positions, inv_freq, q_out, k_out, v_out)
+    _dtype("x", x, torch.bfloat16, torch.float32)
+    _dtype("positions", positions, torch.int32)
+    _dtype("inv_freq", inv_freq, torch.float64)
+    if q_out.dim() != 4:
+        raise ValueError("q_out must be [B, Hq, S, D]")
+    B, Hq, S, D = q_out.shape
+    Hkv = k_out.shape[1] if k_out is not None else 0
+    for name, t in (("q_out", q_out), ("k_out", k_out), ("v_out", v_out)):
+        if t is None:
+            continue
+        _dtype(name, t, x.dtype)
+        if t.dim() != 4 or t.shape != (B, Hq if name == "q_out" else Hkv, S, D) or (D > 1 and t.stride(3) != 1):
+            raise ValueError(f"{name} must be [{B}, heads, {S}, {D}] with contiguous heads")
+        if any(n > 1 and st < D for n, st in zip(t.shape[:3], t.stride()[:3])):
+            raise ValueError(f"{name}: heads overlap (strides {t.stride()})")
+    heads = Hq + Hkv * (2 if v_out is not None else 1)
+    ldx = _rows("x", x, B * S, heads * D, 8)
+    if positions.dim() != 1 or positions.shape[0] != B * S or not positions.is_contiguous():
+        raise ValueError(f"positions must be a contiguous int32 [{B * S}]")
+    if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous fp64 vector")
+    st = lambda t: t.stride()[:3] if t is not None else (0, 0, 0)  # noqa: E731
+    return L.RopeDesc(B, S, Hq, Hkv, D, 2 * inv_freq.shape[0], pairs, _CODES[x.dtype], x.data_ptr(), ldx,
+                      positions.data_ptr(), inv_freq.data_ptr(), magnitude, q_out.data_ptr(), *st(q_out),
+                      L.ptr(k_out), *st(k_out), L.ptr(v_out), *st(v_out))
+
+
+def rope(**kw) -> None:
+    """Rotary positions on QKV rows, split into q, k and v on the way."""
+    d = rope_desc(**kw)
+    L.call("rfx_rope", ctypes.byref(d), _stream())
+
+
 def device_status() -> int:
     v = ctypes.c_int(0)
     L.call("rfx_device_status", _stream(), ctypes.byref(v))
@@ -369,6 +582,10 @@ class Plan:
         L.PatchesDesc: "rfx_plan_add_patches",
         L.LayerNormDesc: "rfx_plan_add_layer_norm",
         L.VitAttnDesc: "rfx_plan_add_vit_attention",
+        L.QuantRowsDesc: "rfx_plan_add_quant_rows",
+        L.LinearI8Desc: "rfx_plan_add_linear_i8",
+        L.BlockNormDesc: "rfx_plan_add_block_norm",
+        L.RopeDesc: "rfx_plan_add_rope",
     }
     # direct (non-plan) entry point of each descriptor kind, for eager execution
     DIRECT = {
@@ -382,6 +599,10 @@ class Plan:
         L.PatchesDesc: "rfx_patches",
         L.LayerNormDesc: "rfx_layer_norm",
         L.VitAttnDesc: "rfx_vit_attention",
+        L.QuantRowsDesc: "rfx_quant_rows",
+        L.LinearI8Desc: "rfx_linear_i8",
+        L.BlockNormDesc: "rfx_block_norm",
+        L.RopeDesc: "rfx_rope",
     }
 
     @classmethod

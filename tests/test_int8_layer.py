@@ -1,0 +1,203 @@
+"""The int8 layer operators without a GPU: struct layouts, the refusals of the
+C entry points and of the tensor wrappers, empty calls, and the scaled rotary
+frequencies against their formulas."""
+import ctypes
+import math
+import os
+import subprocess
+
+import pytest
+import torch
+
+from reflex_b200 import _lib
+from reflex_b200 import kernels as K
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+STRUCTS = {"rfx_quant_rows_desc": "QuantRowsDesc", "rfx_linear_i8_desc": "LinearI8Desc",
+           "rfx_block_norm_desc": "BlockNormDesc", "rfx_rope_desc": "RopeDesc"}
+ENTRIES = {"rfx_quant_rows": "quant_rows", "rfx_linear_i8": "linear_i8", "rfx_block_norm": "block_norm",
+           "rfx_rope": "rope"}
+A = 1 << 20  # an aligned address that is never dereferenced
+
+
+def test_structs_match_c_layout(tmp_path):
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "rfx.h"', "int main(void) {"]
+    for c_name, py_name in STRUCTS.items():
+        lines.append(f'  printf("{py_name} size %zu\\n", sizeof({c_name}));')
+        for field, _ in getattr(_lib, py_name)._fields_:
+            lines.append(f'  printf("{py_name} {field} %zu\\n", offsetof({c_name}, {field}));')
+    lines.append("  return 0; }")
+    c = tmp_path / "layout.c"
+    c.write_text("\n".join(lines))
+    subprocess.run(["gcc", "-std=c99", "-I", os.path.join(ROOT, "include"), str(c), "-o", str(tmp_path / "layout")],
+                   check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split("\n")
+    for line in filter(None, out):
+        py_name, key, val = line.split()
+        cls = getattr(_lib, py_name)
+        got = ctypes.sizeof(cls) if key == "size" else getattr(cls, key).offset
+        assert got == int(val), f"{py_name}.{key}: ctypes {got}, C {val}"
+
+
+@pytest.mark.parametrize("name", sorted(ENTRIES))
+def test_null_descriptor_is_rejected(name):
+    assert getattr(_lib.load(), name)(None, None) == _lib.RFX_E_INVAL
+
+
+def quant():
+    return _lib.QuantRowsDesc(4, 64, _lib.RFX_DTYPE_BF16, A, 64, A, 64, A)
+
+
+def linear():
+    return _lib.LinearI8Desc(4, 64, 64, _lib.RFX_EPI_STORE, _lib.RFX_DTYPE_BF16, A, 64, A, A, 64, A, None, A, 64)
+
+
+def norm():
+    d = _lib.BlockNormDesc()
+    d.T, d.K, d.tokens_per_batch, d.dtype = 4, 64, 4, _lib.RFX_DTYPE_BF16
+    d.h, d.y, d.h_out, d.z = A, 2 * A, 3 * A, 4 * A
+    d.ldh = d.ldy = d.ldho = d.ldz = d.ldzq = 64
+    d.residual_scale, d.eps = 1.0, 1e-6
+    return d
+
+
+def rope():
+    d = _lib.RopeDesc()
+    d.B, d.S, d.num_q_heads, d.num_kv_heads, d.head_dim, d.rot_dim = 1, 4, 2, 1, 64, 64
+    d.pairs, d.dtype, d.magnitude = _lib.RFX_ROPE_HALF, _lib.RFX_DTYPE_BF16, 1.0
+    d.x = d.positions = d.inv_freq = d.q_out = d.k_out = d.v_out = A
+    d.ldx = 4 * 64
+    return d
+
+
+BAD = [
+    ("rfx_quant_rows", quant, dict(T=-1)), ("rfx_quant_rows", quant, dict(K=0)),
+    ("rfx_quant_rows", quant, dict(K=16385, ldx=16385, ldq=16385)), ("rfx_quant_rows", quant, dict(in_dtype=2)),
+    ("rfx_quant_rows", quant, dict(x=None)), ("rfx_quant_rows", quant, dict(q=None)),
+    ("rfx_quant_rows", quant, dict(scale=None)), ("rfx_quant_rows", quant, dict(ldx=63)),
+    ("rfx_quant_rows", quant, dict(ldq=63)), ("rfx_quant_rows", quant, dict(x=A + 1)),
+    ("rfx_quant_rows", quant, dict(scale=A + 2)),
+    ("rfx_linear_i8", linear, dict(T=-1)), ("rfx_linear_i8", linear, dict(O=0)), ("rfx_linear_i8", linear, dict(K=0)),
+    ("rfx_linear_i8", linear, dict(K=65537, ldx=65552, ldw=65552)),
+    ("rfx_linear_i8", linear, dict(epilogue=_lib.RFX_EPI_RESIDUAL)),
+    ("rfx_linear_i8", linear, dict(epilogue=_lib.RFX_EPI_QKV_ROPE)), ("rfx_linear_i8", linear, dict(epilogue=6)),
+    ("rfx_linear_i8", linear, dict(epilogue=_lib.RFX_EPI_GEGLU, O=63)), ("rfx_linear_i8", linear, dict(out_dtype=5)),
+    ("rfx_linear_i8", linear, dict(x=A + 8)), ("rfx_linear_i8", linear, dict(w=A + 1)),
+    ("rfx_linear_i8", linear, dict(ldx=72)), ("rfx_linear_i8", linear, dict(ldw=48)),
+    ("rfx_linear_i8", linear, dict(ldy=63)), ("rfx_linear_i8", linear, dict(y=None)),
+    ("rfx_linear_i8", linear, dict(x_scale=None)), ("rfx_linear_i8", linear, dict(w_scale=A + 2)),
+    ("rfx_linear_i8", linear, dict(T=2147483647, O=2147483646, ldy=2147483646)),
+    ("rfx_block_norm", norm, dict(T=-1)), ("rfx_block_norm", norm, dict(K=16385)),
+    ("rfx_block_norm", norm, dict(tokens_per_batch=0)), ("rfx_block_norm", norm, dict(dtype=3)),
+    ("rfx_block_norm", norm, dict(h=None)), ("rfx_block_norm", norm, dict(h_out=None)),
+    ("rfx_block_norm", norm, dict(y=None)), ("rfx_block_norm", norm, dict(y=None, h_out=None, gate=A)),
+    ("rfx_block_norm", norm, dict(y=None, h_out=None, z=None)), ("rfx_block_norm", norm, dict(z_q=A, z_scale=A)),
+    ("rfx_block_norm", norm, dict(z=None, z_q=A)), ("rfx_block_norm", norm, dict(z=None, norm_a1=A)),
+    ("rfx_block_norm", norm, dict(ldz=63)), ("rfx_block_norm", norm, dict(h_out=A, ldho=128)),
+    ("rfx_block_norm", norm, dict(z=3 * A)), ("rfx_block_norm", norm, dict(post_w=A + 2)),
+    ("rfx_rope", rope, dict(B=-1)), ("rfx_rope", rope, dict(num_q_heads=0)), ("rfx_rope", rope, dict(head_dim=257)),
+    ("rfx_rope", rope, dict(rot_dim=63)), ("rfx_rope", rope, dict(rot_dim=66)), ("rfx_rope", rope, dict(rot_dim=0)),
+    ("rfx_rope", rope, dict(pairs=2)), ("rfx_rope", rope, dict(dtype=7)), ("rfx_rope", rope, dict(ldx=255)),
+    ("rfx_rope", rope, dict(k_out=None)), ("rfx_rope", rope, dict(num_kv_heads=0)),
+    ("rfx_rope", rope, dict(positions=None)), ("rfx_rope", rope, dict(inv_freq=A + 4)),
+    ("rfx_rope", rope, dict(B=65536, S=65536)),
+]
+
+
+@pytest.mark.parametrize("entry,make,change", BAD)
+def test_bad_descriptors_are_refused(entry, make, change):
+    """Refused by the direct call and by the plan add, with a message that
+    names the entry point; the plan stays empty."""
+    lib = _lib.load()
+    d = make()
+    for k, v in change.items():
+        setattr(d, k, v)
+    assert getattr(lib, entry)(ctypes.byref(d), None) == _lib.RFX_E_INVAL
+    assert entry.encode() in lib.rfx_last_error()
+    plan = ctypes.c_void_p()
+    assert lib.rfx_plan_create(ctypes.byref(plan)) == _lib.RFX_OK
+    try:
+        add = getattr(lib, "rfx_plan_add_" + ENTRIES[entry])
+        assert add(plan, ctypes.byref(d)) == _lib.RFX_E_INVAL
+        n = ctypes.c_int(-1)
+        assert lib.rfx_plan_num_launches(plan, ctypes.byref(n)) == _lib.RFX_OK and n.value == 0
+    finally:
+        lib.rfx_plan_destroy(plan)
+
+
+@pytest.mark.parametrize("entry,make,change", [
+    ("rfx_quant_rows", quant, dict(T=0, x=None, q=None, scale=None)),
+    ("rfx_linear_i8", linear, dict(T=0, x=None, y=None, x_scale=None)),
+    ("rfx_block_norm", norm, dict(T=0, h=None, y=None, h_out=None, z=None)),
+    ("rfx_rope", rope, dict(S=0, x=None)),
+])
+def test_no_rows_is_a_no_op(entry, make, change):
+    """No rows: accepted without a device, nothing launched."""
+    lib = _lib.load()
+    d = make()
+    for k, v in change.items():
+        setattr(d, k, v)
+    assert getattr(lib, entry)(ctypes.byref(d), None) == _lib.RFX_OK
+    plan = ctypes.c_void_p()
+    assert lib.rfx_plan_create(ctypes.byref(plan)) == _lib.RFX_OK
+    try:
+        assert getattr(lib, "rfx_plan_add_" + ENTRIES[entry])(plan, ctypes.byref(d)) == _lib.RFX_OK
+        n = ctypes.c_int(-1)
+        assert lib.rfx_plan_num_launches(plan, ctypes.byref(n)) == _lib.RFX_OK and n.value == 0
+    finally:
+        lib.rfx_plan_destroy(plan)
+
+
+def test_plan_counts_launches():
+    lib = _lib.load()
+    plan = ctypes.c_void_p()
+    assert lib.rfx_plan_create(ctypes.byref(plan)) == _lib.RFX_OK
+    try:
+        for name, d in (("quant_rows", quant()), ("block_norm", norm()), ("rope", rope())):
+            assert getattr(lib, "rfx_plan_add_" + name)(plan, ctypes.byref(d)) == _lib.RFX_OK
+        n = ctypes.c_int(-1)
+        assert lib.rfx_plan_num_launches(plan, ctypes.byref(n)) == _lib.RFX_OK and n.value == 3
+    finally:
+        lib.rfx_plan_destroy(plan)
+
+
+def test_cpu_tensors_are_refused():
+    x, q, s = torch.zeros(2, 16), torch.zeros(2, 16, dtype=torch.int8), torch.zeros(2)
+    with pytest.raises(ValueError, match="CUDA"):
+        K.quant_rows(x=x, q=q, scale=s)
+    with pytest.raises(ValueError, match="CUDA"):
+        K.linear_i8(w=q, w_scale=s, x=q, x_scale=s, y=torch.zeros(2, 2))
+    with pytest.raises(ValueError, match="CUDA"):
+        K.block_norm(h=x, S=2, z=x)
+    with pytest.raises(ValueError, match="CUDA"):
+        K.rope(x=x, positions=torch.zeros(2, dtype=torch.int32), inv_freq=torch.ones(4, dtype=torch.float64),
+               q_out=torch.zeros(1, 1, 2, 16))
+
+
+def test_rope_frequencies():
+    """The published formulas, pair by pair (fp64)."""
+    rot, theta, s, L0 = 64, 10000.0, 8.0, 4096
+    base = [theta ** (-2 * i / rot) for i in range(rot // 2)]
+    f, m = K.rope_frequencies(rot, theta, device="cpu")
+    assert f.dtype == torch.float64 and m == 1.0
+    assert torch.allclose(f, torch.tensor(base, dtype=torch.float64), rtol=1e-14, atol=0)
+    f, m = K.rope_frequencies(rot, theta, scaling="linear", factor=s, device="cpu")
+    assert torch.allclose(f, torch.tensor([b / s for b in base], dtype=torch.float64), rtol=1e-14, atol=0) and m == 1.0
+    f, m = K.rope_frequencies(rot, theta, scaling="ntk", factor=s, device="cpu")
+    # the fastest pair is kept, the slowest divided by the factor
+    assert f[0] == 1.0 and math.isclose(f[-1].item(), base[-1] / s, rel_tol=1e-12) and m == 1.0
+    f, m = K.rope_frequencies(rot, theta, scaling="yarn", factor=s, trained_len=L0, device="cpu")
+    for i, b in enumerate(base):
+        turns = L0 * b / (2 * math.pi)
+        g = min(max((turns - 1.0) / (32.0 - 1.0), 0.0), 1.0)
+        assert math.isclose(f[i].item(), (1 - g) * b / s + g * b, rel_tol=1e-12)
+    assert f[0].item() == base[0] and math.isclose(f[-1].item(), base[-1] / s, rel_tol=1e-12)
+    assert math.isclose(m, 0.1 * math.log(s) + 1.0)
+
+
+@pytest.mark.parametrize("kw", [dict(rot_dim=0), dict(rot_dim=7), dict(rot_dim=64, factor=0.5),
+                                dict(rot_dim=64, scaling="yarn", factor=4.0), dict(rot_dim=2, scaling="ntk", factor=2.0),
+                                dict(rot_dim=64, scaling="other")])
+def test_rope_frequencies_refusals(kw):
+    with pytest.raises(ValueError):
+        K.rope_frequencies(device="cpu", **kw)
