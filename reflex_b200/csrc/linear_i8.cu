@@ -25,10 +25,12 @@ constexpr int kMaxK = 65536;  // 65536 * 128 * 128 = 2^30: an s32 sum cannot ove
 struct I8Params {
   int T, O, K;
   int F;           // output columns: O, or O / 2 with GeGLU
-  int m_tiles;     // 128-token tiles
+  int m_tiles;     // 128-token tiles (CTA pairs: 256)
   int k_steps;
   int splits;      // CTAs per cluster, each a part of K
   int stages;
+  int n_tile;      // CTA pairs: weight rows per tile
+  int units;       // CTA pairs: tiles
   int rows_a;      // token rows per copy: 128, or T rounded up to 8
   int recv_off;    // receive buffer of the split sums
   int small_off;
@@ -307,15 +309,300 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   }
 }
 
+// ------------------------------------------------------- CTA-pair tiles ---
+// Many tokens: a pair of CTAs computes 256 tokens x N weight rows (N a
+// multiple of 32 up to 256) with cta_group::2 MMAs: each CTA stages its 128
+// tokens and half of the weight rows per K step, so a step moves 16 KB + 64 N
+// bytes into each SM for 2 N clocks of MMA, and with N = 256 the L2 -> SM
+// stream (64 B/clk) just keeps up.  With GeGLU the even CTA stages the gate
+// rows and the odd one the up rows, and a thread of either finds both halves of
+// its outputs in its own TMEM lane.
+//
+// splits == 1: persistent.  The pair walks the tiles, the two accumulators of
+// 256 TMEM columns alternate, and a tile's epilogue (8 warps) runs under the
+// next tile's MMAs.
+// splits > 1: a cluster of `splits` pairs computes one tile, each pair a part
+// of K; at the end each CTA pushes the s32 sums of the columns that another
+// split owns into that CTA's (now idle) operand ring through DSMEM and adds
+// what it receives to its own.
+constexpr int kPairThreads = 320;
+constexpr int kPairStages = 6;
+constexpr int kPairStage = 2 * kTileM * kStepK;  // 128 token rows + at most 128 weight rows
+constexpr int kPairOffVec = kPairStages * kPairStage;       // [2][w_scale | bias][256]
+constexpr int kPairOffBars = kPairOffVec + 2 * 2 * 256 * 4;
+constexpr int kPairSmem = kPairOffBars + 256 + 1024;
+static_assert(kPairSmem <= kSmemMax, "pair tiles fit in shared memory");
+
+// 16 outputs of one token: scales and bias from shared memory.
+template <int ACT>
+__device__ __forceinline__ void finish16(const uint32_t (&acc)[16], const uint32_t (&up)[16], float sx,
+                                         const float* ws, const float* bs, int half, float (&v)[16]) {
+#pragma unroll
+  for (int g = 0; g < 16; g += 4) {
+    const float4 w = *reinterpret_cast<const float4*>(ws + g);
+    const float4 b = *reinterpret_cast<const float4*>(bs + g);
+    const float wv[4] = {w.x, w.y, w.z, w.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[g + j] = fmaf(static_cast<float>(static_cast<int>(acc[g + j])) * sx, wv[j], bv[j]);
+    if (ACT == kActGeglu) {
+      const float4 w2 = *reinterpret_cast<const float4*>(ws + half + g);
+      const float4 b2 = *reinterpret_cast<const float4*>(bs + half + g);
+      const float wu[4] = {w2.x, w2.y, w2.z, w2.w}, bu[4] = {b2.x, b2.y, b2.z, b2.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[g + j] = gelu_i8(v[g + j]) * fmaf(static_cast<float>(static_cast<int>(up[g + j])) * sx, wu[j], bu[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[g + j] = activate<ACT>(v[g + j]);
+    }
+  }
+}
+
+// A thread's 16 neighbouring outputs, in 32-byte sectors where the rows allow
+// it (`wide`), clipped to n columns.
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void put16(__nv_bfloat16* y, int n, bool wide, const float (&v)[16]) {
+  if (wide && n >= 16) {
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    st_global_v8(y, u);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < n) y[j] = __float2bfloat16_rn(v[j]);
+  }
+}
+__device__ __forceinline__ void put16(float* y, int n, bool wide, const float (&v)[16]) {
+  if (wide && n >= 16) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t u[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(v[8 * h + i]);
+      st_global_v8(y + 8 * h, u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < n) y[j] = v[j];
+  }
+}
+
+template <int ACT, typename Tout>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    linear_i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                          const I8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr bool kGeglu = ACT == kActGeglu;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* vec = reinterpret_cast<float*>(smem + kPairOffVec);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairOffBars);
+  uint64_t* empty = full + kPairStages;
+  uint64_t* acc_full = empty + kPairStages;  // [2]
+  uint64_t* acc_free = acc_full + 2;         // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_free + 2);
+  const uint32_t crank = cluster_ctarank();
+  const uint32_t rank = crank & 1u;  // in the pair
+  const bool leader = rank == 0;
+  const int split = static_cast<int>(crank >> 1);
+  const int N = p.n_tile, nh = N / 2;
+  const int oc = kGeglu ? nh : N;  // output columns of a tile
+  const int csize = 2 * p.splits;
+  const int unit0 = blockIdx.x / csize, ustep = gridDim.x / csize;
+  const int k0 = static_cast<int>(static_cast<long>(split) * p.k_steps / p.splits);
+  const int nk = static_cast<int>(static_cast<long>(split + 1) * p.k_steps / p.splits) - k0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPairStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_free[i], 16);  // both CTAs' epilogue warps, on the even CTA's barrier
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmW);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();  // every CTA's barriers are initialised before a remote arrival
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  int issued = 0;
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      const uint32_t bytes = 2u * (kTileM + nh) * kStepK;  // both CTAs' copies count on the even CTA's barrier
+      for (int un = unit0; un < p.units && ok; un += ustep) {
+        const int t0 = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM;
+        const int o0 = (un / p.m_tiles) * oc;
+        const int wrow = kGeglu ? (rank ? p.F + o0 : o0) : o0 + static_cast<int>(rank) * nh;
+        for (int i = 0; i < nk; ++i) {
+          const int s = issued % kPairStages;
+          if (issued >= kPairStages &&
+              !(ok = mbar_wait(&empty[s], ((issued / kPairStages) - 1) & 1, p.status, kDevTimeoutStageEmpty)))
+            break;
+          uint8_t* st = smem + s * kPairStage;
+          const uint32_t fb = mapa_shared(smem_u32(&full[s]), crank & ~1u);
+          if (leader) mbar_arrive_expect_tx(&full[s], bytes);
+          tma_load_2d_pair(st, &tmX, fb, (k0 + i) * kStepK, t0);
+          tma_load_2d_pair(st + kTileM * kStepK, &tmW, fb, (k0 + i) * kStepK, wrow);
+          ++issued;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      const uint32_t idesc = make_idesc_i8(2 * kTileM, N);
+      const uint64_t a0 = make_sdesc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t b0 = make_sdesc_sw128(smem_u32(smem + kTileM * kStepK), 16, 1024);
+      bool ok = true;
+      int it = 0, tl = 0;
+      for (int un = unit0; un < p.units && ok; un += ustep, ++tl) {
+        const int buf = tl & 1;
+        if (tl >= 2 && !(ok = mbar_wait(&acc_free[buf], ((tl >> 1) - 1) & 1, p.status, kDevTimeoutMmaDone))) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + buf * 256;
+        for (int i = 0; i < nk; ++i, ++it) {
+          const int s = it % kPairStages;
+          if (!(ok = mbar_wait(&full[s], (it / kPairStages) & 1, p.status, kDevTimeoutTmaFull))) break;
+          tc_fence_after();
+          const uint64_t off = static_cast<uint64_t>((s * kPairStage) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kStepK / 32; ++kk)
+            umma_i8_ss_pair(acc, a0 + off + kk * 2, b0 + off + kk * 2, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+          umma_commit_pair(smem_u32(&empty[s]));
+          umma_commit_pair(mapa_shared(smem_u32(&empty[s]), crank | 1u));
+        }
+        if (ok) {
+          umma_commit_pair(smem_u32(&acc_full[buf]));
+          umma_commit_pair(mapa_shared(smem_u32(&acc_full[buf]), crank | 1u));
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const int et = threadIdx.x - 64;  // 0..255
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const int hw = (warp - 2) >> 2;  // which of the two warps of this TMEM quadrant
+    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t free_bar = mapa_shared(smem_u32(&acc_free[0]), crank & ~1u);
+    const bool wide = (p.ldy * sizeof(Tout)) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 31u) == 0 &&
+                      (oc * sizeof(Tout)) % 32 == 0;
+    int tl = 0;
+    for (int un = unit0; un < p.units; un += ustep, ++tl) {
+      const int buf = tl & 1;
+      const int t = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM + row;
+      const int o0 = (un / p.m_tiles) * oc;
+      // this tile's scales and bias, while its products are still computed
+      float* ws = vec + buf * 512;
+      float* bs = ws + 256;
+      if (et < N) {
+        const int c = kGeglu ? (et < nh ? et : et - nh) : et;
+        const bool in = o0 + c < p.F;
+        const int o = o0 + c + (kGeglu && et >= nh ? p.F : 0);
+        ws[et] = in ? __ldg(p.w_scale + o) : 0.f;
+        bs[et] = in && p.bias ? __ldg(p.bias + o) : 0.f;
+      }
+      const bool live = t < p.T;
+      const float sx = live ? __ldg(p.x_scale + t) : 0.f;
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait(&acc_full[buf], (tl >> 1) & 1, p.status, kDevTimeoutMmaDone);
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      uint32_t all;  // every epilogue warp agrees before anyone leaves the loop
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(all)
+          : "r"(ok ? 1u : 0u)
+          : "memory");
+      if (!all) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * 256 + lane_base;
+      Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy;
+      if (p.splits == 1) {
+#pragma unroll 1
+        for (int c = hw * 16; c < oc; c += 32) {
+          uint32_t r[16], u[16];
+          tmem_ld16(acc + c, r);
+          if (kGeglu) tmem_ld16(acc + nh + c, u);
+          tmem_wait_ld();
+          if (c + 32 >= oc) {  // this warp's last read of the accumulator
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(free_bar + 8u * buf);
+          }
+          if (live && o0 + c < p.F) {
+            float v[16];
+            finish16<ACT>(r, u, sx, ws + c, bs + c, nh, v);
+            put16(y + o0 + c, p.F - o0 - c, wide, v);
+          }
+          __syncwarp();
+        }
+        if (hw * 16 >= oc && lane == 0) mbar_arrive_cluster(free_bar + 8u * buf);  // a warp without columns
+      }
+    }
+  }
+  tc_fence_before();
+  // a producer that stopped early waits (bounded) for the pair's copies in flight
+  if (warp == 0 && lane == 0 && leader)
+    for (int i = (issued > kPairStages ? issued - kPairStages : 0); i < issued; ++i)
+      mbar_wait(&full[i % kPairStages], (i / kPairStages) & 1, p.status, kDevTimeoutTmaFull);
+  __syncwarp();
+  cluster_sync();  // neither CTA leaves while the pair's copies or MMAs may touch it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
 // ------------------------------------------------------------ host side ---
 struct I8Plan {
-  int nt, splits, stages, rows_a, recv_off, small_off, smem, m_tiles, n_tiles;
+  bool pair;
+  int nt, splits, stages, rows_a, recv_off, small_off, smem, m_tiles, n_tiles, clusters;
 };
 
 int out_cols(const rfx_linear_i8_desc& d) { return d.epilogue == RFX_EPI_GEGLU ? d.O / 2 : d.O; }
 
 I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   I8Plan c{};
+  if (d.T > 128) {
+    const int pairs = nsm / 2;
+    const int m = (d.T + 2 * kTileM - 1) / (2 * kTileM);
+    long best = -1;
+    for (int nt = 64; nt <= 256; nt += 32) {
+      const int cols = d.epilogue == RFX_EPI_GEGLU ? nt / 2 : nt;
+      const long tiles = static_cast<long>(m) * ((out_cols(d) + cols - 1) / cols);
+      const long cost = (tiles + pairs - 1) / pairs * (nt + 64);
+      if (best < 0 || cost <= best) {
+        best = cost;
+        c.nt = nt;
+        c.n_tiles = (out_cols(d) + cols - 1) / cols;
+      }
+    }
+    c.pair = true;
+    c.splits = 1;
+    c.m_tiles = m;
+    c.rows_a = kTileM;
+    c.smem = kPairSmem;
+    c.clusters = static_cast<int>(std::min<long>(static_cast<long>(m) * c.n_tiles, pairs));
+    return c;
+  }
   c.nt = 128;
   const int tile_cols = d.epilogue == RFX_EPI_GEGLU ? c.nt / 2 : c.nt;
   c.m_tiles = (d.T + kTileM - 1) / kTileM;
@@ -337,16 +624,19 @@ I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
 }
 
 template <int ACT>
-const void* i8_ptr(int out_dtype) {
+const void* i8_ptr(int out_dtype, bool pair) {
+  if (pair)
+    return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, __nv_bfloat16>)
+                                   : reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, float>);
   return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_kernel<128, ACT, __nv_bfloat16>)
                                  : reinterpret_cast<const void*>(linear_i8_kernel<128, ACT, float>);
 }
-const void* i8_kernel(int epilogue, int out_dtype) {
+const void* i8_kernel(int epilogue, int out_dtype, bool pair) {
   switch (epilogue) {
-    case RFX_EPI_STORE: return i8_ptr<kActNone>(out_dtype);
-    case RFX_EPI_SILU: return i8_ptr<kActSilu>(out_dtype);
-    case RFX_EPI_GELU: return i8_ptr<kActGelu>(out_dtype);
-    case RFX_EPI_GEGLU: return i8_ptr<kActGeglu>(out_dtype);
+    case RFX_EPI_STORE: return i8_ptr<kActNone>(out_dtype, pair);
+    case RFX_EPI_SILU: return i8_ptr<kActSilu>(out_dtype, pair);
+    case RFX_EPI_GELU: return i8_ptr<kActGelu>(out_dtype, pair);
+    case RFX_EPI_GEGLU: return i8_ptr<kActGeglu>(out_dtype, pair);
   }
   return nullptr;
 }
@@ -388,7 +678,8 @@ int build_linear_i8_maps(const rfx_linear_i8_desc& d, CUtensorMap* tmX, CUtensor
   const I8Plan c = plan_i8(d, nsm);
   rc = make_tmap_2d(tmX, d.x, 1, d.K, d.T, d.ldx, kStepK, c.rows_a, true);
   if (rc) return rc;
-  return make_tmap_2d(tmW, d.w, 1, d.K, d.O, d.ldw, kStepK, d.epilogue == RFX_EPI_GEGLU ? c.nt / 2 : c.nt, true);
+  return make_tmap_2d(tmW, d.w, 1, d.K, d.O, d.ldw, kStepK,
+                      c.pair || d.epilogue == RFX_EPI_GEGLU ? c.nt / 2 : c.nt, true);
 }
 
 int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const CUtensorMap* tmW, cudaStream_t stream,
@@ -397,7 +688,7 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const 
   int nsm = 148;
   rfx_num_sms(&nsm);
   const I8Plan c = plan_i8(d, nsm);
-  const void* fn = i8_kernel(d.epilogue, d.out_dtype);
+  const void* fn = i8_kernel(d.epilogue, d.out_dtype, c.pair);
   const int rc = ensure_smem_attr(fn, c.smem);
   if (rc) return rc;
   I8Params p{};
@@ -408,6 +699,8 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const 
   p.m_tiles = c.m_tiles;
   p.k_steps = (d.K + kStepK - 1) / kStepK;
   p.splits = c.splits;
+  p.n_tile = c.nt;
+  p.units = c.m_tiles * c.n_tiles;
   p.stages = c.stages;
   p.rows_a = c.rows_a;
   p.recv_off = c.recv_off;
@@ -419,6 +712,9 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const 
   p.ldy = d.ldy;
   p.status = device_status_ptr();
   CUtensorMap x = *tmX, w = *tmW;
+  if (c.pair)
+    return launch_kernel(fn, dim3(2 * c.splits * c.clusters), dim3(kPairThreads), static_cast<size_t>(c.smem), stream,
+                         pdl, 2 * c.splits, x, w, p);
   const unsigned grid = static_cast<unsigned>(c.m_tiles) * c.n_tiles * c.splits;
   return launch_kernel(fn, dim3(grid), dim3(kI8Threads), static_cast<size_t>(c.smem), stream, pdl, c.splits, x, w, p);
 }
