@@ -44,13 +44,17 @@ struct I8Params {
 
 enum { kActNone, kActSilu, kActGelu, kActGeglu };
 
-// GELU-tanh as v * sigmoid(2u), u = sqrt(2/pi) (v + 0.044715 v^3):
-// 0.5 (1 + tanh u) = 1 / (1 + e^-2u), one exponential and one division.
+// GELU-tanh as v * sigmoid(2u), u = sqrt(2/pi) (v + 0.044715 v^3), since
+// 0.5 (1 + tanh u) = 1 / (1 + e^-2u): one exponential and one reciprocal, the
+// exponent formed in base 2.  An e^-2u that overflows leaves v * 0.
 __device__ __forceinline__ float gelu_i8(float v) {
-  const float u2 = 1.5957691216057308f * fmaf(0.044715f * v * v, v, v);
-  return __fdividef(v, 1.f + __expf(-u2));
+  constexpr float kA = -2.3022081986f;  // -2 sqrt(2/pi) log2(e)
+  constexpr float kB = kA * 0.044715f;
+  return v * rcp_approx(1.f + ex2_approx(v * fmaf(kB, v * v, kA)));
 }
-__device__ __forceinline__ float silu_i8(float v) { return __fdividef(v, 1.f + __expf(-v)); }
+__device__ __forceinline__ float silu_i8(float v) {
+  return v * rcp_approx(1.f + ex2_approx(v * -1.4426950409f));
+}
 
 template <int ACT>
 __device__ __forceinline__ float activate(float v) {
@@ -185,24 +189,24 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc_i8(kTileM, NT);
-      bool ok = true;
-      for (int i = 0; i < nk; ++i) {
-        const int s = i % p.stages;
-        if (!(ok = mbar_wait(&full[s], (i / p.stages) & 1, p.status, kDevTimeoutTmaFull))) break;
-        tc_fence_after();
-        const uint32_t a = smem_u32(smem + s * kStage);
-        const uint64_t ad = make_sdesc_sw128(a, 16, 1024);
-        const uint64_t bd = make_sdesc_sw128(a + kTileM * kStepK, 16, 1024);
+    // the whole warp walks the steps and one elected lane issues (uniform operands)
+    constexpr uint32_t idesc = make_idesc_i8(kTileM, NT);
+    const uint64_t a0 = make_sdesc_sw128(smem_u32(smem), 16, 1024);
+    const uint64_t b0 = make_sdesc_sw128(smem_u32(smem + kTileM * kStepK), 16, 1024);
+    for (int i = 0; i < nk; ++i) {
+      const int s = i % p.stages;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (i / p.stages) & 1, p.status, kDevTimeoutTmaFull))) break;
+      tc_fence_after();
+      const uint64_t off = static_cast<uint64_t>((s * kStage) >> 4);
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kStepK / 32; ++kk)
-          umma_i8_ss(tmem, ad + kk * 2, bd + kk * 2, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+          umma_i8_ss(tmem, a0 + off + kk * 2, b0 + off + kk * 2, idesc, (i > 0 || kk > 0) ? 1u : 0u);
         umma_commit(&empty[s]);
+        if (i == nk - 1) umma_commit(acc_bar);
       }
-      if (ok) umma_commit(acc_bar);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     bool ok = true;
     if (lane == 0) ok = mbar_wait(acc_bar, 0, p.status, kDevTimeoutMmaDone);
@@ -326,12 +330,25 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 // split owns into that CTA's (now idle) operand ring through DSMEM and adds
 // what it receives to its own.
 constexpr int kPairThreads = 320;
-constexpr int kPairStages = 6;
-constexpr int kPairStage = 2 * kTileM * kStepK;  // 128 token rows + at most 128 weight rows
-constexpr int kPairOffVec = kPairStages * kPairStage;       // [2][w_scale | bias][256]
+constexpr int kPairMaxStages = 10;
+constexpr int kPairRing = 6 * 2 * kTileM * kStepK;     // operand ring: 6 stages of N = 256, more of a narrower N
+constexpr int kPairOffVec = kPairRing;                 // [2][w_scale | bias][256]
 constexpr int kPairOffBars = kPairOffVec + 2 * 2 * 256 * 4;
 constexpr int kPairSmem = kPairOffBars + 256 + 1024;
+constexpr int kMaxSplits = 4;                          // clusters of at most 8 CTAs
 static_assert(kPairSmem <= kSmemMax, "pair tiles fit in shared memory");
+static_assert((kPairMaxStages * 2 + 4) * 8 + 4 <= 256, "barriers fit");
+
+// Whether every epilogue thread's wait succeeded (also a barrier of the 256).
+__device__ __forceinline__ bool epi_agree(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(ok ? 1u : 0u)
+      : "memory");
+  return all != 0;
+}
 
 // 16 outputs of one token: scales and bias from shared memory.
 template <int ACT>
@@ -403,8 +420,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float* vec = reinterpret_cast<float*>(smem + kPairOffVec);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairOffBars);
-  uint64_t* empty = full + kPairStages;
-  uint64_t* acc_full = empty + kPairStages;  // [2]
+  uint64_t* empty = full + kPairMaxStages;
+  uint64_t* acc_full = empty + kPairMaxStages;  // [2]
   uint64_t* acc_free = acc_full + 2;         // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_free + 2);
   const uint32_t crank = cluster_ctarank();
@@ -413,13 +430,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const int split = static_cast<int>(crank >> 1);
   const int N = p.n_tile, nh = N / 2;
   const int oc = kGeglu ? nh : N;  // output columns of a tile
+  const int stages = p.stages, stage = (kTileM + nh) * kStepK;
   const int csize = 2 * p.splits;
   const int unit0 = blockIdx.x / csize, ustep = gridDim.x / csize;
   const int k0 = static_cast<int>(static_cast<long>(split) * p.k_steps / p.splits);
   const int nk = static_cast<int>(static_cast<long>(split + 1) * p.k_steps / p.splits) - k0;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kPairStages; ++i) {
+    for (int i = 0; i < stages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
@@ -442,60 +460,76 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
+  const bool wide = (p.ldy * sizeof(Tout)) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 31u) == 0;
+  bool failed = false;
   int issued = 0;
   if (warp == 0) {
     if (lane == 0) {
       bool ok = true;
+      int s = 0;
+      uint32_t phase = 0;
       const uint32_t bytes = 2u * (kTileM + nh) * kStepK;  // both CTAs' copies count on the even CTA's barrier
       for (int un = unit0; un < p.units && ok; un += ustep) {
         const int t0 = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM;
         const int o0 = (un / p.m_tiles) * oc;
         const int wrow = kGeglu ? (rank ? p.F + o0 : o0) : o0 + static_cast<int>(rank) * nh;
         for (int i = 0; i < nk; ++i) {
-          const int s = issued % kPairStages;
-          if (issued >= kPairStages &&
-              !(ok = mbar_wait(&empty[s], ((issued / kPairStages) - 1) & 1, p.status, kDevTimeoutStageEmpty)))
-            break;
-          uint8_t* st = smem + s * kPairStage;
+          if (issued >= stages && !(ok = mbar_wait(&empty[s], phase ^ 1, p.status, kDevTimeoutStageEmpty))) break;
+          uint8_t* st = smem + s * stage;
           const uint32_t fb = mapa_shared(smem_u32(&full[s]), crank & ~1u);
           if (leader) mbar_arrive_expect_tx(&full[s], bytes);
           tma_load_2d_pair(st, &tmX, fb, (k0 + i) * kStepK, t0);
           tma_load_2d_pair(st + kTileM * kStepK, &tmW, fb, (k0 + i) * kStepK, wrow);
           ++issued;
+          if (++s == stages) {
+            s = 0;
+            phase ^= 1;
+          }
         }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
+      // the whole warp walks the steps and one elected lane issues: the loop's
+      // values stay uniform, where a loop inside `if (lane == 0)` spends more
+      // clocks on each instruction's operands than the MMA takes
       const uint32_t idesc = make_idesc_i8(2 * kTileM, N);
       const uint64_t a0 = make_sdesc_sw128(smem_u32(smem), 16, 1024);
       const uint64_t b0 = make_sdesc_sw128(smem_u32(smem + kTileM * kStepK), 16, 1024);
       bool ok = true;
-      int it = 0, tl = 0;
+      int s = 0, tl = 0;
+      uint32_t phase = 0;
       for (int un = unit0; un < p.units && ok; un += ustep, ++tl) {
         const int buf = tl & 1;
-        if (tl >= 2 && !(ok = mbar_wait(&acc_free[buf], ((tl >> 1) - 1) & 1, p.status, kDevTimeoutMmaDone))) break;
+        if (tl >= 2 &&
+            !(ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[buf], ((tl >> 1) - 1) & 1, p.status, kDevTimeoutMmaDone))))
+          break;
         tc_fence_after();
         const uint32_t acc = tmem + buf * 256;
-        for (int i = 0; i < nk; ++i, ++it) {
-          const int s = it % kPairStages;
-          if (!(ok = mbar_wait(&full[s], (it / kPairStages) & 1, p.status, kDevTimeoutTmaFull))) break;
+        for (int i = 0; i < nk; ++i) {
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase, p.status, kDevTimeoutTmaFull)))) break;
           tc_fence_after();
-          const uint64_t off = static_cast<uint64_t>((s * kPairStage) >> 4);
+          const uint64_t off = static_cast<uint64_t>((s * stage) >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kStepK / 32; ++kk)
-            umma_i8_ss_pair(acc, a0 + off + kk * 2, b0 + off + kk * 2, idesc, (i > 0 || kk > 0) ? 1u : 0u);
-          umma_commit_pair(smem_u32(&empty[s]));
-          umma_commit_pair(mapa_shared(smem_u32(&empty[s]), crank | 1u));
-        }
-        if (ok) {
-          umma_commit_pair(smem_u32(&acc_full[buf]));
-          umma_commit_pair(mapa_shared(smem_u32(&acc_full[buf]), crank | 1u));
+            for (int kk = 0; kk < kStepK / 32; ++kk)
+              umma_i8_ss_pair(acc, a0 + off + kk * 2, b0 + off + kk * 2, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+            umma_commit_pair(smem_u32(&empty[s]));
+            umma_commit_pair(mapa_shared(smem_u32(&empty[s]), crank | 1u));
+            if (i == nk - 1) {
+              umma_commit_pair(smem_u32(&acc_full[buf]));
+              umma_commit_pair(mapa_shared(smem_u32(&acc_full[buf]), crank | 1u));
+            }
+          }
+          __syncwarp();
+          if (++s == stages) {
+            s = 0;
+            phase ^= 1;
+          }
         }
       }
     }
-    __syncwarp();
   } else {
     const int et = threadIdx.x - 64;  // 0..255
     const int quad = warp & 3;
@@ -503,8 +537,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int hw = (warp - 2) >> 2;  // which of the two warps of this TMEM quadrant
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t free_bar = mapa_shared(smem_u32(&acc_free[0]), crank & ~1u);
-    const bool wide = (p.ldy * sizeof(Tout)) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 31u) == 0 &&
-                      (oc * sizeof(Tout)) % 32 == 0;
     int tl = 0;
     for (int un = unit0; un < p.units; un += ustep, ++tl) {
       const int buf = tl & 1;
@@ -522,47 +554,116 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       const bool live = t < p.T;
       const float sx = live ? __ldg(p.x_scale + t) : 0.f;
-      bool ok = true;
-      if (lane == 0) ok = mbar_wait(&acc_full[buf], (tl >> 1) & 1, p.status, kDevTimeoutMmaDone);
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      uint32_t all;  // every epilogue warp agrees before anyone leaves the loop
-      asm volatile(
-          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-          : "=r"(all)
-          : "r"(ok ? 1u : 0u)
-          : "memory");
-      if (!all) break;
+      // every epilogue warp agrees before anyone leaves the loop
+      if (!epi_agree(mbar_wait(&acc_full[buf], (tl >> 1) & 1, p.status, kDevTimeoutMmaDone))) {
+        failed = true;
+        break;
+      }
       tc_fence_after();
       const uint32_t acc = tmem + buf * 256 + lane_base;
-      Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy;
-      if (p.splits == 1) {
+      Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy + o0;
+      if (p.splits > 1) break;  // one tile per cluster: summed below
 #pragma unroll 1
-        for (int c = hw * 16; c < oc; c += 32) {
-          uint32_t r[16], u[16];
-          tmem_ld16(acc + c, r);
-          if (kGeglu) tmem_ld16(acc + nh + c, u);
-          tmem_wait_ld();
-          if (c + 32 >= oc) {  // this warp's last read of the accumulator
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(free_bar + 8u * buf);
-          }
-          if (live && o0 + c < p.F) {
-            float v[16];
-            finish16<ACT>(r, u, sx, ws + c, bs + c, nh, v);
-            put16(y + o0 + c, p.F - o0 - c, wide, v);
-          }
+      for (int c = hw * 16; c < oc; c += 32) {
+        uint32_t r[16], u[16];
+        tmem_ld16(acc + c, r);
+        if (kGeglu) tmem_ld16(acc + nh + c, u);
+        tmem_wait_ld();
+        if (c + 32 >= oc) {  // this warp's last read of the accumulator
+          tc_fence_before();
           __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(free_bar + 8u * buf);
         }
-        if (hw * 16 >= oc && lane == 0) mbar_arrive_cluster(free_bar + 8u * buf);  // a warp without columns
+        if (live && o0 + c < p.F) {
+          float v[16];
+          finish16<ACT>(r, u, sx, ws + c, bs + c, nh, v);
+          put16(y + c, p.F - o0 - c, wide, v);
+        }
+        __syncwarp();
       }
     }
+  }
+  if (p.splits > 1) {
+    // Every CTA's products are summed and its ring is idle: each pushes the
+    // 16-column chunks that another split owns (chunk j: split j % splits) to
+    // the CTA of the same token half there, [chunk][source][4 columns][token],
+    // and adds what it receives to its own.  s32 sums: any order is exact.
+    const int rowt = (warp & 3) * 32 + lane;
+    const int hw = (warp - 2) >> 2;
+    const uint32_t acc = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    constexpr int kParts = kGeglu ? 2 : 1;
+    const int chunks = oc / 16, others = p.splits - 1;
+    cluster_sync();
+    if (warp >= 2 && !failed) {
+      const uint32_t base = smem_u32(smem) + static_cast<uint32_t>(rowt) * 16u;
+#pragma unroll 1
+      for (int j = hw; j < chunks; j += 2) {
+        const int owner = j % p.splits;
+        if (owner == split) continue;
+        const int src = split < owner ? split : split - 1;
+        const uint32_t dst = mapa_shared(base, static_cast<uint32_t>(owner) * 2u + rank);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          uint32_t r[16];
+          tmem_ld16(acc + part * nh + j * 16, r);
+          tmem_wait_ld();
+          const int slot = ((j / p.splits) * others + src) * kParts + part;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int v[4] = {static_cast<int>(r[4 * g]), static_cast<int>(r[4 * g + 1]), static_cast<int>(r[4 * g + 2]),
+                              static_cast<int>(r[4 * g + 3])};
+            st_dsmem_i4(dst + static_cast<uint32_t>((slot * 4 + g) * kTileM * 16), v);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 2 && !failed) {
+      const int un = unit0;
+      const int t = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM + rowt;
+      const int o0 = (un / p.m_tiles) * oc;
+      const bool live = t < p.T;
+      const float sx = live ? __ldg(p.x_scale + t) : 0.f;
+      Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy + o0;
+      const int4* recv = reinterpret_cast<const int4*>(smem) + rowt;
+#pragma unroll 1
+      for (int lc = hw; lc * p.splits + split < chunks; lc += 2) {
+        const int c = (lc * p.splits + split) * 16;
+        uint32_t r[kParts][16];
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) tmem_ld16(acc + part * nh + c, r[part]);
+        tmem_wait_ld();
+#pragma unroll 1
+        for (int src = 0; src < others; ++src) {
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) {
+            const int slot = (lc * others + src) * kParts + part;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int4 v = recv[(slot * 4 + g) * kTileM];
+              r[part][4 * g] += static_cast<uint32_t>(v.x);
+              r[part][4 * g + 1] += static_cast<uint32_t>(v.y);
+              r[part][4 * g + 2] += static_cast<uint32_t>(v.z);
+              r[part][4 * g + 3] += static_cast<uint32_t>(v.w);
+            }
+          }
+        }
+        if (live && o0 + c < p.F) {
+          float v[16];
+          finish16<ACT>(r[0], r[kParts - 1], sx, vec + c, vec + 256 + c, nh, v);
+          put16(y + c, p.F - o0 - c, wide, v);
+        }
+        __syncwarp();
+      }
+    }
+    __syncwarp();
   }
   tc_fence_before();
   // a producer that stopped early waits (bounded) for the pair's copies in flight
   if (warp == 0 && lane == 0 && leader)
-    for (int i = (issued > kPairStages ? issued - kPairStages : 0); i < issued; ++i)
-      mbar_wait(&full[i % kPairStages], (i / kPairStages) & 1, p.status, kDevTimeoutTmaFull);
+    for (int i = (issued > stages ? issued - stages : 0); i < issued; ++i)
+      mbar_wait(&full[i % stages], (i / stages) & 1, p.status, kDevTimeoutTmaFull);
   __syncwarp();
   cluster_sync();  // neither CTA leaves while the pair's copies or MMAs may touch it
   if (warp == 1) {
@@ -579,28 +680,55 @@ struct I8Plan {
 
 int out_cols(const rfx_linear_i8_desc& d) { return d.epilogue == RFX_EPI_GEGLU ? d.O / 2 : d.O; }
 
+template <int ACT>
+const void* i8_ptr(int out_dtype, bool pair) {
+  if (pair)
+    return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, __nv_bfloat16>)
+                                   : reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, float>);
+  return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_kernel<128, ACT, __nv_bfloat16>)
+                                 : reinterpret_cast<const void*>(linear_i8_kernel<128, ACT, float>);
+}
+const void* i8_kernel(int epilogue, int out_dtype, bool pair) {
+  switch (epilogue) {
+    case RFX_EPI_STORE: return i8_ptr<kActNone>(out_dtype, pair);
+    case RFX_EPI_SILU: return i8_ptr<kActSilu>(out_dtype, pair);
+    case RFX_EPI_GELU: return i8_ptr<kActGelu>(out_dtype, pair);
+    case RFX_EPI_GEGLU: return i8_ptr<kActGeglu>(out_dtype, pair);
+  }
+  return nullptr;
+}
+
 I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   I8Plan c{};
   if (d.T > 128) {
-    const int pairs = nsm / 2;
     const int m = (d.T + 2 * kTileM - 1) / (2 * kTileM);
-    long best = -1;
-    for (int nt = 64; nt <= 256; nt += 32) {
-      const int cols = d.epilogue == RFX_EPI_GEGLU ? nt / 2 : nt;
-      const long tiles = static_cast<long>(m) * ((out_cols(d) + cols - 1) / cols);
-      const long cost = (tiles + pairs - 1) / pairs * (nt + 64);
-      if (best < 0 || cost <= best) {
-        best = cost;
-        c.nt = nt;
-        c.n_tiles = (out_cols(d) + cols - 1) / cols;
+    const int k_steps = (d.K + kStepK - 1) / kStepK;
+    const void* fn = i8_kernel(d.epilogue, d.out_dtype, true);
+    double best = 0;
+    for (int s = 1; s <= std::min(kMaxSplits, k_steps); ++s) {
+      // clusters of 2s CTAs that are resident at once (GPCs hold whole clusters)
+      int slots = max_active_clusters(fn, kPairThreads, kPairSmem, 2 * s);
+      if (slots <= 0) slots = nsm / (2 * s) - (s > 1 ? 3 : 0);
+      for (int nt = 64; nt <= 256; nt += 32) {
+        const int cols = d.epilogue == RFX_EPI_GEGLU ? nt / 2 : nt;
+        const long tiles = static_cast<long>(m) * ((out_cols(d) + cols - 1) / cols);
+        const long rounds = (tiles + slots - 1) / slots;
+        if (s > 1 && rounds > 1) continue;
+        const double cost = rounds * ((k_steps + s - 1) / s) * (100.0 + 0.95 * nt) + 6.0 * nt + (s > 1 ? 1500.0 : 0.0);
+        if (c.nt == 0 || cost < best) {
+          best = cost;
+          c.nt = nt;
+          c.splits = s;
+          c.n_tiles = static_cast<int>(tiles / m);
+          c.clusters = static_cast<int>(s > 1 ? tiles : std::min<long>(tiles, slots));
+        }
       }
     }
     c.pair = true;
-    c.splits = 1;
     c.m_tiles = m;
     c.rows_a = kTileM;
+    c.stages = std::min(kPairMaxStages, kPairRing / ((kTileM + c.nt / 2) * kStepK));
     c.smem = kPairSmem;
-    c.clusters = static_cast<int>(std::min<long>(static_cast<long>(m) * c.n_tiles, pairs));
     return c;
   }
   c.nt = 128;
@@ -621,24 +749,6 @@ I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   c.small_off = c.recv_off + recv;
   c.smem = c.small_off + small + 1024;
   return c;
-}
-
-template <int ACT>
-const void* i8_ptr(int out_dtype, bool pair) {
-  if (pair)
-    return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, __nv_bfloat16>)
-                                   : reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, float>);
-  return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_kernel<128, ACT, __nv_bfloat16>)
-                                 : reinterpret_cast<const void*>(linear_i8_kernel<128, ACT, float>);
-}
-const void* i8_kernel(int epilogue, int out_dtype, bool pair) {
-  switch (epilogue) {
-    case RFX_EPI_STORE: return i8_ptr<kActNone>(out_dtype, pair);
-    case RFX_EPI_SILU: return i8_ptr<kActSilu>(out_dtype, pair);
-    case RFX_EPI_GELU: return i8_ptr<kActGelu>(out_dtype, pair);
-    case RFX_EPI_GEGLU: return i8_ptr<kActGeglu>(out_dtype, pair);
-  }
-  return nullptr;
 }
 
 bool al(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }

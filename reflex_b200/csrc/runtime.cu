@@ -5,8 +5,10 @@
 
 #include <atomic>
 #include <cstdarg>
+#include <map>
 #include <memory>
 #include <mutex>
+#include <tuple>
 #include <unordered_map>
 #include <variant>
 #include <vector>
@@ -153,6 +155,38 @@ bool cluster_fits(const void* func, dim3 grid, int threads, int smem, int cluste
   std::lock_guard<std::mutex> lk(mu);
   memo[key] = ok;
   return ok;
+}
+
+int max_active_clusters(const void* func, int threads, int smem, int cluster_x) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, int, int>, int> memo;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  const auto key = std::make_tuple(func, smem, cluster_x, dev);
+  std::lock_guard<std::mutex> lk(mu);
+  auto it = memo.find(key);
+  if (it != memo.end()) return it->second;
+  int n = 0;
+  if (ensure_smem_attr(func, smem) == RFX_OK) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(cluster_x));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(cluster_x);
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess) n = 0;
+    cudaGetLastError();
+  }
+  memo[key] = n;
+  return n;
 }
 
 // ------------------------------------------------------------ tensor maps ---
