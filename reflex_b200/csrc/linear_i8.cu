@@ -333,7 +333,8 @@ constexpr int kPairThreads = 320;
 constexpr int kPairMaxStages = 10;
 constexpr int kPairRing = 6 * 2 * kTileM * kStepK;     // operand ring: 6 stages of N = 256, more of a narrower N
 constexpr int kPairOffVec = kPairRing;                 // [2][w_scale | bias][256]
-constexpr int kPairOffBars = kPairOffVec + 2 * 2 * 256 * 4;
+constexpr int kPairOffOut = kPairOffVec + 2 * 2 * 256 * 4;  // output staging per lane quadrant
+constexpr int kPairOffBars = kPairOffOut + 4 * 32 * 144;
 constexpr int kPairSmem = kPairOffBars + 256 + 1024;
 constexpr int kMaxSplits = 4;                          // clusters of at most 8 CTAs
 static_assert(kPairSmem <= kSmemMax, "pair tiles fit in shared memory");
@@ -375,39 +376,55 @@ __device__ __forceinline__ void finish16(const uint32_t (&acc)[16], const uint32
   }
 }
 
-// A thread's 16 neighbouring outputs, in 32-byte sectors where the rows allow
-// it (`wide`), clipped to n columns.
-__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
+// 16 outputs packed as they are stored.
+__device__ __forceinline__ void pack16(const float (&v)[16], uint32_t* w, const __nv_bfloat16*) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
 }
-__device__ __forceinline__ void put16(__nv_bfloat16* y, int n, bool wide, const float (&v)[16]) {
-  if (wide && n >= 16) {
-    uint32_t u[8];
+__device__ __forceinline__ void pack16(const float (&v)[16], uint32_t* w, const float*) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-    st_global_v8(y, u);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j < n) y[j] = __float2bfloat16_rn(v[j]);
-  }
+  for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i]);
 }
-__device__ __forceinline__ void put16(float* y, int n, bool wide, const float (&v)[16]) {
-  if (wide && n >= 16) {
+
+// 32 rows x 128 bytes of outputs to memory through 32 x 144 bytes of shared
+// memory.  The two warps of a TMEM lane quadrant hold 64 bytes of each row
+// (lane = row, warp hw the columns of half hw) and then store 16 rows each, a
+// store instruction writing whole 128-byte lines of 4 rows: with a lane
+// writing 32 bytes of its own row the stores took 4.8 us of a 3200 x 2560
+// output.  `y` is the first row's first column; `rows` rows and `n` columns
+// are live.  `bar`: the named barrier of the two warps.
+constexpr int kStageLd = 144;
+__device__ __forceinline__ void quad_bar(int bar) { asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory"); }
+template <typename Tout>
+__device__ __forceinline__ void store_group(uint8_t* st, const uint32_t (&w)[16], Tout* y, long ldy, int rows, int n,
+                                            bool wide, int hw, int lane, int bar) {
+  constexpr int kUnit = 16 / static_cast<int>(sizeof(Tout));  // elements per 16 bytes
+  constexpr int kCols = 128 / static_cast<int>(sizeof(Tout));
+  uint4* d = reinterpret_cast<uint4*>(st + lane * kStageLd + hw * 64);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t u[8];
+  for (int j = 0; j < 4; ++j) d[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  quad_bar(bar);
+  if (wide) {
+    const int unit = lane & 7;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(v[8 * h + i]);
-      st_global_v8(y + 8 * h, u);
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * hw + 4 * i + (lane >> 3);
+      if (r >= rows) continue;
+      const uint8_t* src = st + r * kStageLd + unit * 16;
+      Tout* dst = y + r * ldy + unit * kUnit;
+      if ((unit + 1) * kUnit <= n) {
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+      } else {
+        for (int e = 0; unit * kUnit + e < n; ++e) dst[e] = reinterpret_cast<const Tout*>(src)[e];
+      }
     }
   } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j < n) y[j] = v[j];
+    for (int i = lane; i < 16 * kCols; i += 32) {
+      const int r = 16 * hw + i / kCols, c = i % kCols;
+      if (r < rows && c < n) y[r * ldy + c] = reinterpret_cast<const Tout*>(st + r * kStageLd)[c];
+    }
   }
+  quad_bar(bar);  // the buffer is free again
 }
 
 template <int ACT, typename Tout>
@@ -460,35 +477,40 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  const bool wide = (p.ldy * sizeof(Tout)) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 31u) == 0;
+  const bool wide = (p.ldy * sizeof(Tout)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
+  constexpr int kGroup = 128 / static_cast<int>(sizeof(Tout));  // output columns of 128 bytes
+  constexpr int kHalf = kGroup / 2;                              // of which a warp finishes half
+  uint8_t* out_st = smem + kPairOffOut + (warp & 3) * 32 * kStageLd;
   bool failed = false;
   int issued = 0;
   if (warp == 0) {
-    if (lane == 0) {
-      bool ok = true;
-      int s = 0;
-      uint32_t phase = 0;
-      const uint32_t bytes = 2u * (kTileM + nh) * kStepK;  // both CTAs' copies count on the even CTA's barrier
-      for (int un = unit0; un < p.units && ok; un += ustep) {
-        const int t0 = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM;
-        const int o0 = (un / p.m_tiles) * oc;
-        const int wrow = kGeglu ? (rank ? p.F + o0 : o0) : o0 + static_cast<int>(rank) * nh;
-        for (int i = 0; i < nk; ++i) {
-          if (issued >= stages && !(ok = mbar_wait(&empty[s], phase ^ 1, p.status, kDevTimeoutStageEmpty))) break;
+    // as in the MMA warp, the whole warp walks the steps and one lane issues
+    bool ok = true;
+    int s = 0;
+    uint32_t phase = 0;
+    const uint32_t bytes = 2u * (kTileM + nh) * kStepK;  // both CTAs' copies count on the even CTA's barrier
+    const uint32_t full0 = mapa_shared(smem_u32(full), crank & ~1u);
+    for (int un = unit0; un < p.units && ok; un += ustep) {
+      const int t0 = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM;
+      const int o0 = (un / p.m_tiles) * oc;
+      const int wrow = kGeglu ? (rank ? p.F + o0 : o0) : o0 + static_cast<int>(rank) * nh;
+      for (int i = 0; i < nk; ++i) {
+        if (issued >= stages && !(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase ^ 1, p.status, kDevTimeoutStageEmpty))))
+          break;
+        if (elect_one()) {
           uint8_t* st = smem + s * stage;
-          const uint32_t fb = mapa_shared(smem_u32(&full[s]), crank & ~1u);
           if (leader) mbar_arrive_expect_tx(&full[s], bytes);
-          tma_load_2d_pair(st, &tmX, fb, (k0 + i) * kStepK, t0);
-          tma_load_2d_pair(st + kTileM * kStepK, &tmW, fb, (k0 + i) * kStepK, wrow);
-          ++issued;
-          if (++s == stages) {
-            s = 0;
-            phase ^= 1;
-          }
+          tma_load_2d_pair(st, &tmX, full0 + 8u * s, (k0 + i) * kStepK, t0);
+          tma_load_2d_pair(st + kTileM * kStepK, &tmW, full0 + 8u * s, (k0 + i) * kStepK, wrow);
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == stages) {
+          s = 0;
+          phase ^= 1;
         }
       }
     }
-    __syncwarp();
   } else if (warp == 1) {
     if (leader) {
       // the whole warp walks the steps and one elected lane issues: the loop's
@@ -533,14 +555,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   } else {
     const int et = threadIdx.x - 64;  // 0..255
     const int quad = warp & 3;
-    const int row = quad * 32 + lane;
     const int hw = (warp - 2) >> 2;  // which of the two warps of this TMEM quadrant
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t free_bar = mapa_shared(smem_u32(&acc_free[0]), crank & ~1u);
     int tl = 0;
     for (int un = unit0; un < p.units; un += ustep, ++tl) {
       const int buf = tl & 1;
-      const int t = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM + row;
+      const int tw = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32;  // the warp's first token
+      const int t = tw + lane;
+      Tout* y0 = static_cast<Tout*>(p.y) + static_cast<long>(tw) * p.ldy;
       const int o0 = (un / p.m_tiles) * oc;
       // this tile's scales and bias, while its products are still computed
       float* ws = vec + buf * 512;
@@ -552,8 +575,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         ws[et] = in ? __ldg(p.w_scale + o) : 0.f;
         bs[et] = in && p.bias ? __ldg(p.bias + o) : 0.f;
       }
-      const bool live = t < p.T;
-      const float sx = live ? __ldg(p.x_scale + t) : 0.f;
+      const float sx = t < p.T ? __ldg(p.x_scale + t) : 0.f;
       // every epilogue warp agrees before anyone leaves the loop
       if (!epi_agree(mbar_wait(&acc_full[buf], (tl >> 1) & 1, p.status, kDevTimeoutMmaDone))) {
         failed = true;
@@ -561,45 +583,53 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       tc_fence_after();
       const uint32_t acc = tmem + buf * 256 + lane_base;
-      Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy + o0;
       if (p.splits > 1) break;  // one tile per cluster: summed below
 #pragma unroll 1
-      for (int c = hw * 16; c < oc; c += 32) {
-        uint32_t r[16], u[16];
-        tmem_ld16(acc + c, r);
-        if (kGeglu) tmem_ld16(acc + nh + c, u);
-        tmem_wait_ld();
-        if (c + 32 >= oc) {  // this warp's last read of the accumulator
+      for (int g = 0; g < oc; g += kGroup) {
+        uint32_t w[16];
+#pragma unroll
+        for (int q = 0; q < kHalf / 16; ++q) {
+          const int c = g + hw * kHalf + 16 * q;
+          if (c < oc) {
+            uint32_t r[16], u[16];
+            tmem_ld16(acc + c, r);
+            if (kGeglu) tmem_ld16(acc + nh + c, u);
+            tmem_wait_ld();
+            float v[16];
+            finish16<ACT>(r, u, sx, ws + c, bs + c, nh, v);
+            pack16(v, w + q * 8, static_cast<const Tout*>(nullptr));
+          }
+        }
+        if (g + kGroup >= oc) {  // the last read of the accumulator
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(free_bar + 8u * buf);
         }
-        if (live && o0 + c < p.F) {
-          float v[16];
-          finish16<ACT>(r, u, sx, ws + c, bs + c, nh, v);
-          put16(y + c, p.F - o0 - c, wide, v);
-        }
-        __syncwarp();
+        store_group(out_st, w, y0 + o0 + g, p.ldy, p.T - tw, min(min(kGroup, oc - g), p.F - o0 - g), wide, hw, lane,
+                    2 + quad);
       }
     }
   }
   if (p.splits > 1) {
     // Every CTA's products are summed and its ring is idle: each pushes the
-    // 16-column chunks that another split owns (chunk j: split j % splits) to
-    // the CTA of the same token half there, [chunk][source][4 columns][token],
-    // and adds what it receives to its own.  s32 sums: any order is exact.
-    const int rowt = (warp & 3) * 32 + lane;
-    const int hw = (warp - 2) >> 2;
-    const uint32_t acc = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    // groups of 128 output bytes that another split owns (group j: split
+    // j % splits) to the CTA of the same token half there, as
+    // [group][source][gate | up][4 columns][token], and adds what it receives
+    // to its own.  s32 sums: any order is exact.
+    const int quad = warp & 3, hw = (warp - 2) >> 2;
+    const int rowt = quad * 32 + lane;
+    const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     constexpr int kParts = kGeglu ? 2 : 1;
-    const int chunks = oc / 16, others = p.splits - 1;
+    constexpr int kSlot = kGroup / 4 * kTileM * 16;  // bytes of one part of one group
+    const int groups = (oc + kGroup - 1) / kGroup, others = p.splits - 1;
     cluster_sync();
     if (warp >= 2 && !failed) {
       const uint32_t base = smem_u32(smem) + static_cast<uint32_t>(rowt) * 16u;
 #pragma unroll 1
-      for (int j = hw; j < chunks; j += 2) {
-        const int owner = j % p.splits;
-        if (owner == split) continue;
+      for (int j = hw; j < groups * (kGroup / 16); j += 2) {  // 16-column chunks
+        const int grp = j / (kGroup / 16), q = j % (kGroup / 16);
+        const int owner = grp % p.splits;
+        if (owner == split || j * 16 >= oc) continue;
         const int src = split < owner ? split : split - 1;
         const uint32_t dst = mapa_shared(base, static_cast<uint32_t>(owner) * 2u + rank);
 #pragma unroll
@@ -607,12 +637,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           uint32_t r[16];
           tmem_ld16(acc + part * nh + j * 16, r);
           tmem_wait_ld();
-          const int slot = ((j / p.splits) * others + src) * kParts + part;
+          const int slot = ((grp / p.splits) * others + src) * kParts + part;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const int v[4] = {static_cast<int>(r[4 * g]), static_cast<int>(r[4 * g + 1]), static_cast<int>(r[4 * g + 2]),
                               static_cast<int>(r[4 * g + 3])};
-            st_dsmem_i4(dst + static_cast<uint32_t>((slot * 4 + g) * kTileM * 16), v);
+            st_dsmem_i4(dst + static_cast<uint32_t>(slot * kSlot + (q * 4 + g) * kTileM * 16), v);
           }
         }
       }
@@ -621,40 +651,46 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     cluster_sync();
     if (warp >= 2 && !failed) {
       const int un = unit0;
-      const int t = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM + rowt;
+      const int tw = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32;
       const int o0 = (un / p.m_tiles) * oc;
-      const bool live = t < p.T;
-      const float sx = live ? __ldg(p.x_scale + t) : 0.f;
-      Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy + o0;
-      const int4* recv = reinterpret_cast<const int4*>(smem) + rowt;
+      const float sx = tw + lane < p.T ? __ldg(p.x_scale + tw + lane) : 0.f;
+      Tout* y0 = static_cast<Tout*>(p.y) + static_cast<long>(tw) * p.ldy + o0;
 #pragma unroll 1
-      for (int lc = hw; lc * p.splits + split < chunks; lc += 2) {
-        const int c = (lc * p.splits + split) * 16;
-        uint32_t r[kParts][16];
+      for (int lg = 0; lg * p.splits + split < groups; ++lg) {
+        const int g0 = (lg * p.splits + split) * kGroup;
+        uint32_t w[16];
 #pragma unroll
-        for (int part = 0; part < kParts; ++part) tmem_ld16(acc + part * nh + c, r[part]);
-        tmem_wait_ld();
+        for (int qq = 0; qq < kHalf / 16; ++qq) {
+          const int q = hw * (kHalf / 16) + qq;
+          const int c = g0 + 16 * q;
+          if (c < oc) {
+            uint32_t r[kParts][16];
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) tmem_ld16(acc + part * nh + c, r[part]);
+            tmem_wait_ld();
 #pragma unroll 1
-        for (int src = 0; src < others; ++src) {
+            for (int src = 0; src < others; ++src) {
 #pragma unroll
-          for (int part = 0; part < kParts; ++part) {
-            const int slot = (lc * others + src) * kParts + part;
+              for (int part = 0; part < kParts; ++part) {
+                const int4* recv = reinterpret_cast<const int4*>(smem + ((lg * others + src) * kParts + part) * kSlot) +
+                                   q * 4 * kTileM + rowt;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int4 v = recv[(slot * 4 + g) * kTileM];
-              r[part][4 * g] += static_cast<uint32_t>(v.x);
-              r[part][4 * g + 1] += static_cast<uint32_t>(v.y);
-              r[part][4 * g + 2] += static_cast<uint32_t>(v.z);
-              r[part][4 * g + 3] += static_cast<uint32_t>(v.w);
+                for (int g = 0; g < 4; ++g) {
+                  const int4 v = recv[g * kTileM];
+                  r[part][4 * g] += static_cast<uint32_t>(v.x);
+                  r[part][4 * g + 1] += static_cast<uint32_t>(v.y);
+                  r[part][4 * g + 2] += static_cast<uint32_t>(v.z);
+                  r[part][4 * g + 3] += static_cast<uint32_t>(v.w);
+                }
+              }
             }
+            float v[16];
+            finish16<ACT>(r[0], r[kParts - 1], sx, vec + c, vec + 256 + c, nh, v);
+            pack16(v, w + qq * 8, static_cast<const Tout*>(nullptr));
           }
         }
-        if (live && o0 + c < p.F) {
-          float v[16];
-          finish16<ACT>(r[0], r[kParts - 1], sx, vec + c, vec + 256 + c, nh, v);
-          put16(y + c, p.F - o0 - c, wide, v);
-        }
-        __syncwarp();
+        store_group(out_st, w, y0 + g0, p.ldy, p.T - tw, min(min(kGroup, oc - g0), p.F - o0 - g0), wide, hw, lane,
+                    2 + quad);
       }
     }
     __syncwarp();
