@@ -30,7 +30,8 @@ struct I8Params {
   int splits;      // CTAs per cluster, each a part of K
   int stages;
   int n_tile;      // CTA pairs: weight rows per tile
-  int units;       // CTA pairs: tiles
+  int n_tail;      // of the tiles from units_a on
+  int units_a, units;
   int rows_a;      // token rows per copy: 128, or T rounded up to 8
   int recv_off;    // receive buffer of the split sums
   int small_off;
@@ -333,8 +334,8 @@ constexpr int kPairThreads = 320;
 constexpr int kPairMaxStages = 10;
 constexpr int kPairRing = 6 * 2 * kTileM * kStepK;     // operand ring: 6 stages of N = 256, more of a narrower N
 constexpr int kPairOffVec = kPairRing;                 // [2][w_scale | bias][256]
-constexpr int kPairOffOut = kPairOffVec + 2 * 2 * 256 * 4;  // output staging per lane quadrant
-constexpr int kPairOffBars = kPairOffOut + 4 * 32 * 144;
+constexpr int kPairOffOut = kPairOffVec + 2 * 2 * 256 * 4;  // output staging, 2 KB per epilogue warp
+constexpr int kPairOffBars = kPairOffOut + 8 * 32 * 64;
 constexpr int kPairSmem = kPairOffBars + 256 + 1024;
 constexpr int kMaxSplits = 4;                          // clusters of at most 8 CTAs
 static_assert(kPairSmem <= kSmemMax, "pair tiles fit in shared memory");
@@ -386,50 +387,48 @@ __device__ __forceinline__ void pack16(const float (&v)[16], uint32_t* w, const 
   for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i]);
 }
 
-// 32 rows x 128 bytes of outputs to memory through 32 x 144 bytes of shared
-// memory.  The two warps of a TMEM lane quadrant hold 64 bytes of each row
-// (lane = row, warp hw the columns of half hw) and then store 16 rows each, a
-// store instruction writing whole 128-byte lines of 4 rows: with a lane
-// writing 32 bytes of its own row the stores took 4.8 us of a 3200 x 2560
-// output.  `y` is the first row's first column; `rows` rows and `n` columns
-// are live.  `bar`: the named barrier of the two warps.
-constexpr int kStageLd = 144;
-__device__ __forceinline__ void quad_bar(int bar) { asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory"); }
+// A warp's 32 rows x 64 bytes of outputs (lane = row) to memory through its own
+// 2 KB of shared memory: one TMA store, which also clips rows past T and
+// columns past F, where y's rows begin on 16-byte boundaries (`tma`), else
+// coalesced elements.  `rows` and `n` are the live rows and columns from (t, o).
 template <typename Tout>
-__device__ __forceinline__ void store_group(uint8_t* st, const uint32_t (&w)[16], Tout* y, long ldy, int rows, int n,
-                                            bool wide, int hw, int lane, int bar) {
-  constexpr int kUnit = 16 / static_cast<int>(sizeof(Tout));  // elements per 16 bytes
-  constexpr int kCols = 128 / static_cast<int>(sizeof(Tout));
-  uint4* d = reinterpret_cast<uint4*>(st + lane * kStageLd + hw * 64);
+__device__ __forceinline__ void store_part(const I8Params& p, const CUtensorMap* tmY, uint8_t* st,
+                                           const uint32_t (&w)[16], int t, int o, int rows, int n, bool tma, int lane) {
+  constexpr int kCols = 64 / static_cast<int>(sizeof(Tout));
+  if (n <= 0 || rows <= 0) return;
+  if (tma) {
+    if (lane == 0) bulk_wait_read();  // the previous store has left the buffer
+    __syncwarp();
+  }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) d[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-  quad_bar(bar);
-  if (wide) {
-    const int unit = lane & 7;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 16 * hw + 4 * i + (lane >> 3);
-      if (r >= rows) continue;
-      const uint8_t* src = st + r * kStageLd + unit * 16;
-      Tout* dst = y + r * ldy + unit * kUnit;
-      if ((unit + 1) * kUnit <= n) {
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-      } else {
-        for (int e = 0; unit * kUnit + e < n; ++e) dst[e] = reinterpret_cast<const Tout*>(src)[e];
-      }
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  if (tma) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(tmY, st, o, t);
+      bulk_commit();
     }
   } else {
-    for (int i = lane; i < 16 * kCols; i += 32) {
-      const int r = 16 * hw + i / kCols, c = i % kCols;
-      if (r < rows && c < n) y[r * ldy + c] = reinterpret_cast<const Tout*>(st + r * kStageLd)[c];
+    __syncwarp();
+    Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy + o;
+    for (int i = lane; i < 32 * kCols; i += 32) {
+      const int r = i / kCols, c = i % kCols;
+      const int byte = c * static_cast<int>(sizeof(Tout));
+      if (r < rows && c < n)
+        y[r * p.ldy + c] =
+            *reinterpret_cast<const Tout*>(st + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
     }
+    __syncwarp();
   }
-  quad_bar(bar);  // the buffer is free again
 }
 
 template <int ACT, typename Tout>
 __global__ void __launch_bounds__(kPairThreads, 1)
     linear_i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                          const __grid_constant__ CUtensorMap tmW2, const __grid_constant__ CUtensorMap tmY,
                           const I8Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -445,9 +444,23 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t rank = crank & 1u;  // in the pair
   const bool leader = rank == 0;
   const int split = static_cast<int>(crank >> 1);
-  const int N = p.n_tile, nh = N / 2;
-  const int oc = kGeglu ? nh : N;  // output columns of a tile
-  const int stages = p.stages, stage = (kTileM + nh) * kStepK;
+  // Units: first `units_a` tiles of N = n_tile, then tiles of N = n_tail over
+  // the remaining columns, so that the last round of tiles is a narrow one.
+  struct Unit {
+    int m, o0, N;
+  };
+  auto unit_of = [&](int un) {
+    const bool tail = un >= p.units_a;
+    const int v = tail ? un - p.units_a : un;
+    const int n = v / p.m_tiles;
+    const int w = kGeglu ? p.n_tile / 2 : p.n_tile;
+    Unit u;
+    u.m = v - n * p.m_tiles;
+    u.N = tail ? p.n_tail : p.n_tile;
+    u.o0 = tail ? p.units_a / p.m_tiles * w + n * (kGeglu ? u.N / 2 : u.N) : n * w;
+    return u;
+  };
+  const int stages = p.stages, stage = (kTileM + p.n_tile / 2) * kStepK;
   const int csize = 2 * p.splits;
   const int unit0 = blockIdx.x / csize, ustep = gridDim.x / csize;
   const int k0 = static_cast<int>(static_cast<long>(split) * p.k_steps / p.splits);
@@ -477,10 +490,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  const bool wide = (p.ldy * sizeof(Tout)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
+  const bool tma_y = (p.ldy * sizeof(Tout)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
   constexpr int kGroup = 128 / static_cast<int>(sizeof(Tout));  // output columns of 128 bytes
   constexpr int kHalf = kGroup / 2;                              // of which a warp finishes half
-  uint8_t* out_st = smem + kPairOffOut + (warp & 3) * 32 * kStageLd;
+  uint8_t* out_st = smem + kPairOffOut + (warp - 2) * 32 * 64;
   bool failed = false;
   int issued = 0;
   if (warp == 0) {
@@ -488,12 +501,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     bool ok = true;
     int s = 0;
     uint32_t phase = 0;
-    const uint32_t bytes = 2u * (kTileM + nh) * kStepK;  // both CTAs' copies count on the even CTA's barrier
     const uint32_t full0 = mapa_shared(smem_u32(full), crank & ~1u);
     for (int un = unit0; un < p.units && ok; un += ustep) {
-      const int t0 = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM;
-      const int o0 = (un / p.m_tiles) * oc;
-      const int wrow = kGeglu ? (rank ? p.F + o0 : o0) : o0 + static_cast<int>(rank) * nh;
+      const Unit tile = unit_of(un);
+      const int t0 = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM;
+      const int wrow = kGeglu ? (rank ? p.F + tile.o0 : tile.o0) : tile.o0 + static_cast<int>(rank) * (tile.N / 2);
+      const CUtensorMap* tw = un < p.units_a ? &tmW : &tmW2;
+      const uint32_t bytes = 2u * (kTileM + tile.N / 2) * kStepK;  // both CTAs' copies count on the even CTA's barrier
       for (int i = 0; i < nk; ++i) {
         if (issued >= stages && !(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase ^ 1, p.status, kDevTimeoutStageEmpty))))
           break;
@@ -501,7 +515,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           uint8_t* st = smem + s * stage;
           if (leader) mbar_arrive_expect_tx(&full[s], bytes);
           tma_load_2d_pair(st, &tmX, full0 + 8u * s, (k0 + i) * kStepK, t0);
-          tma_load_2d_pair(st + kTileM * kStepK, &tmW, full0 + 8u * s, (k0 + i) * kStepK, wrow);
+          tma_load_2d_pair(st + kTileM * kStepK, tw, full0 + 8u * s, (k0 + i) * kStepK, wrow);
         }
         __syncwarp();
         ++issued;
@@ -516,7 +530,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // the whole warp walks the steps and one elected lane issues: the loop's
       // values stay uniform, where a loop inside `if (lane == 0)` spends more
       // clocks on each instruction's operands than the MMA takes
-      const uint32_t idesc = make_idesc_i8(2 * kTileM, N);
       const uint64_t a0 = make_sdesc_sw128(smem_u32(smem), 16, 1024);
       const uint64_t b0 = make_sdesc_sw128(smem_u32(smem + kTileM * kStepK), 16, 1024);
       bool ok = true;
@@ -524,6 +537,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       uint32_t phase = 0;
       for (int un = unit0; un < p.units && ok; un += ustep, ++tl) {
         const int buf = tl & 1;
+        const uint32_t idesc = make_idesc_i8(2 * kTileM, un < p.units_a ? p.n_tile : p.n_tail);
         if (tl >= 2 &&
             !(ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[buf], ((tl >> 1) - 1) & 1, p.status, kDevTimeoutMmaDone))))
           break;
@@ -561,10 +575,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     int tl = 0;
     for (int un = unit0; un < p.units; un += ustep, ++tl) {
       const int buf = tl & 1;
-      const int tw = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32;  // the warp's first token
+      const Unit tile = unit_of(un);
+      const int N = tile.N, nh = N / 2, oc = kGeglu ? nh : N;  // oc output columns
+      const int tw = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32;  // the warp's first token
       const int t = tw + lane;
-      Tout* y0 = static_cast<Tout*>(p.y) + static_cast<long>(tw) * p.ldy;
-      const int o0 = (un / p.m_tiles) * oc;
+      const int o0 = tile.o0;
       // this tile's scales and bias, while its products are still computed
       float* ws = vec + buf * 512;
       float* bs = ws + 256;
@@ -584,30 +599,36 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       tc_fence_after();
       const uint32_t acc = tmem + buf * 256 + lane_base;
       if (p.splits > 1) break;  // one tile per cluster: summed below
+      // groups of 128 output bytes, of which each warp of the quadrant finishes
+      // and stores 64
 #pragma unroll 1
-      for (int g = 0; g < oc; g += kGroup) {
+      for (int g = hw * kHalf; g < oc; g += kGroup) {
         uint32_t w[16];
+        uint32_t r[kHalf / 16][16], u[kHalf / 16][16];
 #pragma unroll
         for (int q = 0; q < kHalf / 16; ++q) {
-          const int c = g + hw * kHalf + 16 * q;
-          if (c < oc) {
-            uint32_t r[16], u[16];
-            tmem_ld16(acc + c, r);
-            if (kGeglu) tmem_ld16(acc + nh + c, u);
-            tmem_wait_ld();
-            float v[16];
-            finish16<ACT>(r, u, sx, ws + c, bs + c, nh, v);
-            pack16(v, w + q * 8, static_cast<const Tout*>(nullptr));
+          if (g + 16 * q < oc) {
+            tmem_ld16(acc + g + 16 * q, r[q]);
+            if (kGeglu) tmem_ld16(acc + nh + g + 16 * q, u[q]);
           }
         }
-        if (g + kGroup >= oc) {  // the last read of the accumulator
+        tmem_wait_ld();
+        if (g + kGroup >= oc) {  // this warp's last read of the accumulator
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(free_bar + 8u * buf);
         }
-        store_group(out_st, w, y0 + o0 + g, p.ldy, p.T - tw, min(min(kGroup, oc - g), p.F - o0 - g), wide, hw, lane,
-                    2 + quad);
+#pragma unroll
+        for (int q = 0; q < kHalf / 16; ++q) {
+          if (g + 16 * q < oc) {
+            float v[16];
+            finish16<ACT>(r[q], u[q], sx, ws + g + 16 * q, bs + g + 16 * q, nh, v);
+            pack16(v, w + q * 8, static_cast<const Tout*>(nullptr));
+          }
+        }
+        store_part<Tout>(p, &tmY, out_st, w, tw, o0 + g, p.T - tw, min(min(kHalf, oc - g), p.F - o0 - g), tma_y, lane);
       }
+      if (hw * kHalf >= oc && lane == 0) mbar_arrive_cluster(free_bar + 8u * buf);  // a warp without columns
     }
   }
   if (p.splits > 1) {
@@ -616,6 +637,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     // j % splits) to the CTA of the same token half there, as
     // [group][source][gate | up][4 columns][token], and adds what it receives
     // to its own.  s32 sums: any order is exact.
+    const Unit tile = unit_of(unit0);
+    const int nh = tile.N / 2, oc = kGeglu ? nh : tile.N;
     const int quad = warp & 3, hw = (warp - 2) >> 2;
     const int rowt = quad * 32 + lane;
     const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16);
@@ -650,11 +673,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     __syncwarp();
     cluster_sync();
     if (warp >= 2 && !failed) {
-      const int un = unit0;
-      const int tw = (un % p.m_tiles) * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32;
-      const int o0 = (un / p.m_tiles) * oc;
+      const int tw = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32;
+      const int o0 = tile.o0;
       const float sx = tw + lane < p.T ? __ldg(p.x_scale + tw + lane) : 0.f;
-      Tout* y0 = static_cast<Tout*>(p.y) + static_cast<long>(tw) * p.ldy + o0;
 #pragma unroll 1
       for (int lg = 0; lg * p.splits + split < groups; ++lg) {
         const int g0 = (lg * p.splits + split) * kGroup;
@@ -689,12 +710,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             pack16(v, w + qq * 8, static_cast<const Tout*>(nullptr));
           }
         }
-        store_group(out_st, w, y0 + g0, p.ldy, p.T - tw, min(min(kGroup, oc - g0), p.F - o0 - g0), wide, hw, lane,
-                    2 + quad);
+        const int g = g0 + hw * kHalf;
+        store_part<Tout>(p, &tmY, out_st, w, tw, o0 + g, p.T - tw, min(min(kHalf, oc - g), p.F - o0 - g), tma_y, lane);
       }
     }
     __syncwarp();
   }
+  if (warp >= 2 && lane == 0) bulk_wait_all();  // the output's stores are complete
   tc_fence_before();
   // a producer that stopped early waits (bounded) for the pair's copies in flight
   if (warp == 0 && lane == 0 && leader)
@@ -712,6 +734,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 struct I8Plan {
   bool pair;
   int nt, splits, stages, rows_a, recv_off, small_off, smem, m_tiles, n_tiles, clusters;
+  int nt2, n_tiles2;  // CTA pairs: the narrow last tiles' width and count per token tile
 };
 
 int out_cols(const rfx_linear_i8_desc& d) { return d.epilogue == RFX_EPI_GEGLU ? d.O / 2 : d.O; }
@@ -740,23 +763,54 @@ I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
     const int m = (d.T + 2 * kTileM - 1) / (2 * kTileM);
     const int k_steps = (d.K + kStepK - 1) / kStepK;
     const void* fn = i8_kernel(d.epilogue, d.out_dtype, true);
+    const int div = d.epilogue == RFX_EPI_GEGLU ? 2 : 1;  // weight rows per output column
+    const int F = out_cols(d);
+    const int step = 32 * div;  // tiles of whole 64-byte pieces of output rows
+    auto tiles_of = [&](int cols, int nt) { return (cols * div + nt - 1) / nt; };
+    // A tile's time in ns: its K steps, each bound by the copies into the SM
+    // for narrow tiles and by the MMAs for wide ones, or its epilogue.
+    auto tile_ns = [&](int nt, int s) {
+      return std::max((k_steps + s - 1) / s * (100.0 + 0.95 * nt), 10.0 * nt);
+    };
     double best = 0;
     for (int s = 1; s <= std::min(kMaxSplits, k_steps); ++s) {
       // clusters of 2s CTAs that are resident at once (GPCs hold whole clusters)
       int slots = max_active_clusters(fn, kPairThreads, kPairSmem, 2 * s);
-      if (slots <= 0) slots = nsm / (2 * s) - (s > 1 ? 3 : 0);
-      for (int nt = 64; nt <= 256; nt += 32) {
-        const int cols = d.epilogue == RFX_EPI_GEGLU ? nt / 2 : nt;
-        const long tiles = static_cast<long>(m) * ((out_cols(d) + cols - 1) / cols);
+      if (slots <= 0) slots = std::max(1, nsm / (2 * s) - (s > 1 ? 3 : 0));
+      for (int nt = 64; nt <= 256; nt += step) {
+        const int n = tiles_of(F, nt);
+        const long tiles = static_cast<long>(m) * n;
         const long rounds = (tiles + slots - 1) / slots;
         if (s > 1 && rounds > 1) continue;
-        const double cost = rounds * ((k_steps + s - 1) / s) * (100.0 + 0.95 * nt) + 6.0 * nt + (s > 1 ? 1500.0 : 0.0);
-        if (c.nt == 0 || cost < best) {
+        auto consider = [&](double cost, int n_a, int nt2, int n_b) {
+          if (c.nt != 0 && cost >= best) return;
           best = cost;
           c.nt = nt;
           c.splits = s;
-          c.n_tiles = static_cast<int>(tiles / m);
-          c.clusters = static_cast<int>(s > 1 ? tiles : std::min<long>(tiles, slots));
+          c.n_tiles = n_a;
+          c.nt2 = nt2;
+          c.n_tiles2 = n_b;
+          c.clusters = static_cast<int>(std::min<long>(static_cast<long>(m) * (n_a + n_b), slots));
+        };
+        consider(rounds * tile_ns(nt, s) + 10.0 * nt + (s > 1 ? 1500.0 : 0.0), n, nt, 0);
+        if (s > 1 || rounds < 2) continue;
+        // the full rounds at this width, the rest in narrower tiles
+        const int n_a = static_cast<int>((rounds - 1) * slots / m);
+        if (n_a < 1 || n_a >= n) continue;
+        for (int nt2 = 64; nt2 < nt; nt2 += step) {
+          const int n_b = tiles_of(F - n_a * (nt / div), nt2);
+          const long ua = static_cast<long>(n_a) * m, ub = static_cast<long>(n_b) * m;
+          // the tiles go round the slots: the busiest slot's time
+          const double ta = tile_ns(nt, 1), tb = tile_ns(nt2, 1);
+          const long qa = ua / slots, ra = ua % slots, first = slots - ra;  // `first` slots have one tile less
+          double t;
+          if (ub <= first) {
+            t = std::max(qa * ta + tb, (qa + (ra ? 1 : 0)) * ta);
+          } else {
+            const long qb = (ub - first) / slots, rb = (ub - first) % slots;
+            t = std::max(ra ? (qa + 1) * ta + (qb + (rb ? 1 : 0)) * tb : 0.0, qa * ta + (1 + qb + (rb > ra ? 1 : 0)) * tb);
+          }
+          consider(t + 10.0 * nt2, n_a, nt2, n_b);
         }
       }
     }
@@ -816,20 +870,30 @@ int validate_linear_i8(const rfx_linear_i8_desc& d) {
   return RFX_OK;
 }
 
-int build_linear_i8_maps(const rfx_linear_i8_desc& d, CUtensorMap* tmX, CUtensorMap* tmW) {
+int build_linear_i8_maps(const rfx_linear_i8_desc& d, LinearI8Maps* maps) {
   int rc = validate_linear_i8(d);
   if (rc || d.T == 0) return rc;
   int nsm = 148;
   rfx_num_sms(&nsm);
   const I8Plan c = plan_i8(d, nsm);
-  rc = make_tmap_2d(tmX, d.x, 1, d.K, d.T, d.ldx, kStepK, c.rows_a, true);
+  const bool geglu = d.epilogue == RFX_EPI_GEGLU;
+  rc = make_tmap_2d(&maps->x, d.x, 1, d.K, d.T, d.ldx, kStepK, c.rows_a, true);
   if (rc) return rc;
-  return make_tmap_2d(tmW, d.w, 1, d.K, d.O, d.ldw, kStepK,
-                      c.pair || d.epilogue == RFX_EPI_GEGLU ? c.nt / 2 : c.nt, true);
+  rc = make_tmap_2d(&maps->w, d.w, 1, d.K, d.O, d.ldw, kStepK, c.pair || geglu ? c.nt / 2 : c.nt, true);
+  if (rc || !c.pair) return rc;
+  maps->w2 = maps->w;
+  if (c.n_tiles2 > 0) {
+    rc = make_tmap_2d(&maps->w2, d.w, 1, d.K, d.O, d.ldw, kStepK, c.nt2 / 2, true);
+    if (rc) return rc;
+  }
+  const int esz = d.out_dtype == kDtypeBF16 ? 2 : 4;
+  maps->y = maps->w;  // not used where y's rows are not 16-byte aligned
+  if (al(d.y, 16) && (d.ldy * esz) % 16 == 0)
+    rc = make_tmap_2d_swizzle(&maps->y, d.y, esz, out_cols(d), d.T, d.ldy * esz, 64 / esz, 32, 64);
+  return rc;
 }
 
-int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const CUtensorMap* tmW, cudaStream_t stream,
-                     bool pdl) {
+int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cudaStream_t stream, bool pdl) {
   if (d.T == 0) return RFX_OK;
   int nsm = 148;
   rfx_num_sms(&nsm);
@@ -846,7 +910,9 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const 
   p.k_steps = (d.K + kStepK - 1) / kStepK;
   p.splits = c.splits;
   p.n_tile = c.nt;
-  p.units = c.m_tiles * c.n_tiles;
+  p.n_tail = c.nt2;
+  p.units_a = c.m_tiles * c.n_tiles;
+  p.units = p.units_a + c.m_tiles * c.n_tiles2;
   p.stages = c.stages;
   p.rows_a = c.rows_a;
   p.recv_off = c.recv_off;
@@ -857,10 +923,10 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const 
   p.y = d.y;
   p.ldy = d.ldy;
   p.status = device_status_ptr();
-  CUtensorMap x = *tmX, w = *tmW;
+  CUtensorMap x = maps.x, w = maps.w, w2 = maps.w2, y = maps.y;
   if (c.pair)
     return launch_kernel(fn, dim3(2 * c.splits * c.clusters), dim3(kPairThreads), static_cast<size_t>(c.smem), stream,
-                         pdl, 2 * c.splits, x, w, p);
+                         pdl, 2 * c.splits, x, w, w2, y, p);
   const unsigned grid = static_cast<unsigned>(c.m_tiles) * c.n_tiles * c.splits;
   return launch_kernel(fn, dim3(grid), dim3(kI8Threads), static_cast<size_t>(c.smem), stream, pdl, c.splits, x, w, p);
 }
@@ -870,8 +936,8 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const 
 extern "C" int rfx_linear_i8(const rfx_linear_i8_desc* d, void* stream) {
   using namespace rfx;
   if (!d) return set_error(RFX_E_INVAL, "rfx_linear_i8: null descriptor");
-  CUtensorMap x, w;
-  const int rc = build_linear_i8_maps(*d, &x, &w);
+  LinearI8Maps maps;
+  const int rc = build_linear_i8_maps(*d, &maps);
   if (rc) return rc;
-  return launch_linear_i8(*d, &x, &w, static_cast<cudaStream_t>(stream), pdl_enabled());
+  return launch_linear_i8(*d, maps, static_cast<cudaStream_t>(stream), pdl_enabled());
 }

@@ -65,6 +65,9 @@ int ensure_smem_attr(const void* func, int bytes, bool nonportable_cluster = fal
 // {box_cols, box_rows}; swizzle 128B when swizzle128 is set.
 int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t cols, uint64_t rows,
                  uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows, bool swizzle128);
+// The same with a 128-, 64- or 0-byte swizzle (64: 16-byte chunk ^= (row / 2) % 4 of 64-byte rows).
+int make_tmap_2d_swizzle(CUtensorMap* out, const void* base, int elem_bytes, uint64_t cols, uint64_t rows,
+                         uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows, int swizzle_bytes);
 
 // ------------------------------------------------------- kernel launchers ---
 struct KvQuantDesc {
@@ -123,9 +126,11 @@ int launch_vit_attention(const rfx_vit_attn_desc& d, cudaStream_t stream, bool p
 int launch_quant_rows(const rfx_quant_rows_desc& d, cudaStream_t stream, bool pdl);
 int launch_block_norm(const rfx_block_norm_desc& d, cudaStream_t stream, bool pdl);
 int launch_rope(const rfx_rope_desc& d, cudaStream_t stream, bool pdl);
-int build_linear_i8_maps(const rfx_linear_i8_desc& d, CUtensorMap* tmX, CUtensorMap* tmW);
-int launch_linear_i8(const rfx_linear_i8_desc& d, const CUtensorMap* tmX, const CUtensorMap* tmW, cudaStream_t stream,
-                     bool pdl);
+struct LinearI8Maps {
+  CUtensorMap x, w, w2, y;
+};
+int build_linear_i8_maps(const rfx_linear_i8_desc& d, LinearI8Maps* maps);
+int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cudaStream_t stream, bool pdl);
 int run_chunk_op(rfx_chunk* c, cudaStream_t s);
 
 }  // namespace rfx

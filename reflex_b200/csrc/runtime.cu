@@ -210,6 +210,12 @@ EncodeTiledFn encode_fn() {
 
 int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t cols, uint64_t rows,
                  uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows, bool swizzle128) {
+  return make_tmap_2d_swizzle(out, base, elem_bytes, cols, rows, row_stride_bytes, box_cols, box_rows,
+                              swizzle128 ? 128 : 0);
+}
+
+int make_tmap_2d_swizzle(CUtensorMap* out, const void* base, int elem_bytes, uint64_t cols, uint64_t rows,
+                         uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows, int swizzle_bytes) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return set_error(RFX_E_CUDA, "cuTensorMapEncodeTiled unavailable");
   if (!base || (reinterpret_cast<uintptr_t>(base) & 15u) || (row_stride_bytes & 15u) || rows == 0 || cols == 0)
@@ -226,7 +232,9 @@ int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t co
   cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(out, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  swizzle_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                  : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                        : CU_TENSOR_MAP_SWIZZLE_NONE,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(RFX_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
   return RFX_OK;
@@ -393,7 +401,7 @@ struct RopeOp {
 };
 struct LinearI8Op {
   rfx_linear_i8_desc d;
-  CUtensorMap x, w;
+  LinearI8Maps maps;
 };
 struct BarrierOp {};
 struct ChunkOp {
@@ -429,7 +437,7 @@ int run_op(const Op& op, cudaStream_t s, bool pdl) {
   if (auto* o = std::get_if<QuantRowsOp>(&op)) return launch_quant_rows(o->d, s, pdl);
   if (auto* o = std::get_if<BlockNormOp>(&op)) return launch_block_norm(o->d, s, pdl);
   if (auto* o = std::get_if<RopeOp>(&op)) return launch_rope(o->d, s, pdl);
-  if (auto* o = std::get_if<LinearI8Op>(&op)) return launch_linear_i8(o->d, &o->x, &o->w, s, pdl);
+  if (auto* o = std::get_if<LinearI8Op>(&op)) return launch_linear_i8(o->d, o->maps, s, pdl);
   return set_error(RFX_E_STATE, "plan: unknown op");
 }
 // Launches every op in order; an op that follows a BarrierOp runs without PDL.
@@ -606,8 +614,8 @@ extern "C" int rfx_plan_add_rope(rfx_plan* plan, const rfx_rope_desc* desc) {
 }
 extern "C" int rfx_plan_add_linear_i8(rfx_plan* plan, const rfx_linear_i8_desc* desc) {
   PLAN_GUARD(plan);
-  LinearI8Op op{*desc, {}, {}};
-  const int rc = build_linear_i8_maps(op.d, &op.x, &op.w);
+  LinearI8Op op{*desc, {}};
+  const int rc = build_linear_i8_maps(op.d, &op.maps);
   if (rc) return rc;
   plan->ops.emplace_back(op);
   plan->launches += desc->T > 0 ? 1 : 0;
