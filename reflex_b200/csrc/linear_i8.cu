@@ -24,17 +24,19 @@ constexpr int kMaxK = 65536;  // 65536 * 128 * 128 = 2^30: an s32 sum cannot ove
 
 struct I8Params {
   int T, O, K;
-  int F;           // output columns: O, or O / 2 with GeGLU
-  int m_tiles;     // 128-token tiles (CTA pairs: 256)
-  int k_steps;
-  int splits;      // CTAs per cluster, each a part of K
-  int stages;
-  int n_tile;      // CTA pairs: weight rows per tile
-  int n_tail;      // of the tiles from units_a on
+  int F;            // output columns: O, or O / 2 with GeGLU
+  int k_steps;      // of 128
+  int splits;       // parts of K: pairs per cluster, or warps per pair of rows
+  int m_tiles;      // 256-token tiles
+  int n_tile;       // weight rows per tile,
+  int n_tail;       // of the tiles from units_a on
   int units_a, units;
-  int rows_a;      // token rows per copy: 128, or T rounded up to 8
-  int recv_off;    // receive buffer of the split sums
-  int small_off;
+  int stages;
+  int rows_a;       // token rows per copy: 128, or T rounded up to 8
+  const int8_t* x;
+  long ldx;
+  const int8_t* w;
+  long ldw;
   const float* x_scale;
   const float* w_scale;
   const float* bias;
@@ -64,258 +66,13 @@ __device__ __forceinline__ float activate(float v) {
   return v;
 }
 
-// Scales, bias and activation of 4 accumulators of token scale sx; for GeGLU
-// `up` are the 4 accumulators of the matching up rows.  o is the first output
-// column; columns past F read nothing.
-template <int ACT>
-__device__ __forceinline__ void finish4(const I8Params& p, const int (&acc)[4], const int (&up)[4], float sx, int o,
-                                        float (&v)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (o + j >= p.F) {
-      v[j] = 0.f;
-      continue;
-    }
-    float a = static_cast<float>(acc[j]) * sx * __ldg(p.w_scale + o + j);
-    if (p.bias) a += __ldg(p.bias + o + j);
-    if (ACT == kActGeglu) {
-      float u = static_cast<float>(up[j]) * sx * __ldg(p.w_scale + p.F + o + j);
-      if (p.bias) u += __ldg(p.bias + p.F + o + j);
-      v[j] = gelu_i8(a) * u;
-    } else {
-      v[j] = activate<ACT>(a);
-    }
-  }
-}
-
-__device__ __forceinline__ void put4(float* y, int n, bool wide, const float (&v)[4]) {
-  if (wide && n >= 4) {
-    *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) y[j] = v[j];
-  }
-}
-__device__ __forceinline__ void put4(__nv_bfloat16* y, int n, bool wide, const float (&v)[4]) {
-  if (wide && n >= 4) {
-    *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) y[j] = __float2bfloat16_rn(v[j]);
-  }
-}
-
 __device__ __forceinline__ void st_dsmem_i4(uint32_t addr, const int (&v)[4]) {
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                : "memory");
 }
 
-// One tile of 128 tokens x NT weight rows per cluster, K split over its CTAs.
-// Warp 0 issues the copies, warp 1 the MMAs, warps 2-5 read the accumulators.
-// With a split, every CTA pushes the s32 sums of the columns that CTA r owns
-// (1/splits of the tile) into r's receive buffer through DSMEM, and after a
-// cluster barrier r adds them and runs the epilogue of its columns.
-constexpr int kI8Threads = 192;
-constexpr int kI8MaxStages = 8;
-
-template <int NT, int ACT, typename Tout>
-__global__ void __launch_bounds__(kI8Threads, 1)
-    linear_i8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
-                     const I8Params p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr bool kGeglu = ACT == kActGeglu;
-  constexpr int kStage = (kTileM + NT) * kStepK;
-  constexpr int kOutCols = kGeglu ? NT / 2 : NT;  // output columns of a tile
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool clustered = p.splits > 1;
-  const int split = clustered ? static_cast<int>(cluster_ctarank()) : 0;
-  const int tile = blockIdx.x / p.splits;
-  const int t0 = tile % p.m_tiles * kTileM;
-  const int o0 = tile / p.m_tiles * kOutCols;
-  const int k0 = static_cast<int>(static_cast<long>(split) * p.k_steps / p.splits);
-  const int nk = static_cast<int>(static_cast<long>(split + 1) * p.k_steps / p.splits) - k0;
-
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.small_off);
-  uint64_t* empty = full + kI8MaxStages;
-  uint64_t* acc_bar = empty + kI8MaxStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_bar + 1);
-
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    mbar_init(acc_bar, 1);
-    fence_mbar_init();
-    tma_prefetch_desc(&tmX);
-    tma_prefetch_desc(&tmW);
-  }
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, NT);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  // the cluster's CTAs have all started before anyone writes into a peer
-  if (clustered)
-    cluster_sync();
-  else
-    __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  pdl_launch_dependents();
-  pdl_wait();
-
-  int issued = 0;
-  if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t bytes = static_cast<uint32_t>((p.rows_a + NT) * kStepK);
-      for (int i = 0; i < nk; ++i) {
-        const int s = i % p.stages;
-        if (i >= p.stages && !mbar_wait(&empty[s], ((i / p.stages) - 1) & 1, p.status, kDevTimeoutStageEmpty)) break;
-        uint8_t* st = smem + s * kStage;
-        const int kx = (k0 + i) * kStepK;
-        mbar_arrive_expect_tx(&full[s], bytes);
-        if (kGeglu) {
-          tma_load_2d(st + kTileM * kStepK, &tmW, &full[s], kx, o0);
-          tma_load_2d(st + (kTileM + NT / 2) * kStepK, &tmW, &full[s], kx, p.F + o0);
-        } else {
-          tma_load_2d(st + kTileM * kStepK, &tmW, &full[s], kx, o0);
-        }
-        tma_load_2d(st, &tmX, &full[s], kx, t0);
-        issued = i + 1;
-      }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // the whole warp walks the steps and one elected lane issues (uniform operands)
-    constexpr uint32_t idesc = make_idesc_i8(kTileM, NT);
-    const uint64_t a0 = make_sdesc_sw128(smem_u32(smem), 16, 1024);
-    const uint64_t b0 = make_sdesc_sw128(smem_u32(smem + kTileM * kStepK), 16, 1024);
-    for (int i = 0; i < nk; ++i) {
-      const int s = i % p.stages;
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (i / p.stages) & 1, p.status, kDevTimeoutTmaFull))) break;
-      tc_fence_after();
-      const uint64_t off = static_cast<uint64_t>((s * kStage) >> 4);
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < kStepK / 32; ++kk)
-          umma_i8_ss(tmem, a0 + off + kk * 2, b0 + off + kk * 2, idesc, (i > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&empty[s]);
-        if (i == nk - 1) umma_commit(acc_bar);
-      }
-      __syncwarp();
-    }
-  } else {
-    bool ok = true;
-    if (lane == 0) ok = mbar_wait(acc_bar, 0, p.status, kDevTimeoutMmaDone);
-    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-    const int quad = warp & 3;
-    const int row = quad * 32 + lane;
-    const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    if (ok) {
-      tc_fence_after();
-      if (!clustered) {
-        const int t = t0 + row;
-        const bool live = t < p.T;
-        const float sx = live ? p.x_scale[t] : 0.f;
-        Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy;
-        const bool wide = (p.ldy * sizeof(Tout)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
-#pragma unroll 1
-        for (int c = 0; c < kOutCols; c += 16) {
-          uint32_t r[16], u[16];
-          tmem_ld16(acc + c, r);
-          if (kGeglu) tmem_ld16(acc + NT / 2 + c, u);
-          tmem_wait_ld();
-          if (live) {
-#pragma unroll
-            for (int g = 0; g < 16; g += 4) {
-              const int o = o0 + c + g;
-              int a4[4], u4[4];
-              float v[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                a4[j] = static_cast<int>(r[g + j]);
-                u4[j] = kGeglu ? static_cast<int>(u[g + j]) : 0;
-              }
-              finish4<ACT>(p, a4, u4, sx, o, v);
-              if (o < p.F) put4(y + o, p.F - o, wide, v);
-            }
-          }
-          __syncwarp();
-        }
-      } else {
-        // groups of 4 accumulator columns; the output columns of owner r are
-        // r * own .. , the gate and up halves of a GeGLU tile alike
-        const int own = kOutCols / p.splits;       // output columns per owner
-        const int groups = NT / 4 / p.splits;      // accumulator groups per owner
-        const int ld = p.rows_a + 2;               // rows per group slot (+2: conflict-free reads)
-        const uint32_t base = smem_u32(smem + p.recv_off) + static_cast<uint32_t>(split * groups * ld + row) * 16u;
-#pragma unroll 1
-        for (int c = 0; c < NT; c += 16) {
-          uint32_t r[16];
-          tmem_ld16(acc + c, r);
-          tmem_wait_ld();
-          if (row < p.rows_a) {
-#pragma unroll
-            for (int g = 0; g < 16; g += 4) {
-              const int col = kGeglu ? (c + g) % (NT / 2) : c + g;
-              const int owner = col / own;
-              const int slot = (col - owner * own) / 4 + (kGeglu && c + g >= NT / 2 ? own / 4 : 0);
-              const int v[4] = {static_cast<int>(r[g]), static_cast<int>(r[g + 1]), static_cast<int>(r[g + 2]),
-                                static_cast<int>(r[g + 3])};
-              st_dsmem_i4(mapa_shared(base + static_cast<uint32_t>(slot * ld) * 16u, owner), v);
-            }
-          }
-          __syncwarp();
-        }
-      }
-    }
-  }
-  if (clustered) {
-    tc_fence_before();
-    cluster_sync();
-    const int own = kOutCols / p.splits;
-    const int groups = NT / 4 / p.splits;
-    const int ld = p.rows_a + 2;
-    const int4* recv = reinterpret_cast<const int4*>(smem + p.recv_off);
-    const int og = own / 4;  // output groups
-    const int rows = min(p.T - t0, kTileM);
-    const bool wide = (p.ldy * sizeof(Tout)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
-    for (int i = threadIdx.x; i < rows * og; i += kI8Threads) {
-      const int row = i / og, g = i - row * og;
-      int a4[4] = {0, 0, 0, 0}, u4[4] = {0, 0, 0, 0};
-#pragma unroll 4
-      for (int q = 0; q < p.splits; ++q) {
-        const int4 v = recv[(q * groups + g) * ld + row];
-        a4[0] += v.x; a4[1] += v.y; a4[2] += v.z; a4[3] += v.w;
-        if (kGeglu) {
-          const int4 w = recv[(q * groups + og + g) * ld + row];
-          u4[0] += w.x; u4[1] += w.y; u4[2] += w.z; u4[3] += w.w;
-        }
-      }
-      const int t = t0 + row, o = o0 + split * own + g * 4;
-      float v[4];
-      finish4<ACT>(p, a4, u4, p.x_scale[t], o, v);
-      if (o < p.F) put4(static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy + o, p.F - o, wide, v);
-    }
-  }
-  // a producer that stopped early waits (bounded) for its copies in flight
-  if (warp == 0 && lane == 0)
-    for (int i = (issued > p.stages ? issued - p.stages : 0); i < issued; ++i)
-      mbar_wait(&full[i % p.stages], (i / p.stages) & 1, p.status, kDevTimeoutTmaFull);
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, NT);
-  }
-}
-
 // ------------------------------------------------------- CTA-pair tiles ---
-// Many tokens: a pair of CTAs computes 256 tokens x N weight rows (N a
+// A pair of CTAs computes 256 tokens x N weight rows (N a
 // multiple of 32 up to 256) with cta_group::2 MMAs: each CTA stages its 128
 // tokens and half of the weight rows per K step, so a step moves 16 KB + 64 N
 // bytes into each SM for 2 N clocks of MMA, and with N = 256 the L2 -> SM
@@ -507,14 +264,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int t0 = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM;
       const int wrow = kGeglu ? (rank ? p.F + tile.o0 : tile.o0) : tile.o0 + static_cast<int>(rank) * (tile.N / 2);
       const CUtensorMap* tw = un < p.units_a ? &tmW : &tmW2;
-      const uint32_t bytes = 2u * (kTileM + tile.N / 2) * kStepK;  // both CTAs' copies count on the even CTA's barrier
+      // both CTAs' copies count on the even CTA's barrier; a half without
+      // tokens copies none (what its rows multiply is not stored)
+      const bool has_x = t0 < p.T;
+      const int x_rows = p.rows_a * (has_x && t0 + kTileM < p.T ? 2 : 1);
+      const uint32_t bytes = static_cast<uint32_t>(x_rows + tile.N) * kStepK;
       for (int i = 0; i < nk; ++i) {
         if (issued >= stages && !(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase ^ 1, p.status, kDevTimeoutStageEmpty))))
           break;
         if (elect_one()) {
           uint8_t* st = smem + s * stage;
           if (leader) mbar_arrive_expect_tx(&full[s], bytes);
-          tma_load_2d_pair(st, &tmX, full0 + 8u * s, (k0 + i) * kStepK, t0);
+          if (has_x) tma_load_2d_pair(st, &tmX, full0 + 8u * s, (k0 + i) * kStepK, t0);
           tma_load_2d_pair(st + kTileM * kStepK, tw, full0 + 8u * s, (k0 + i) * kStepK, wrow);
         }
         __syncwarp();
@@ -730,114 +491,241 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
 }
 
+// ------------------------------------------------------- few tokens ---
+// Up to 4 tokens: the weights are read once, 16 bytes per lane and load, and
+// multiplied on the integer units (4 products per instruction): no tiles, no
+// shared-memory round trip, nothing to set up, so a single token's call costs
+// little more than the memory's latency.  A warp takes two weight rows (GeGLU:
+// a gate row and its up row) over a 1/kw part of K; x comes through L1.
+constexpr int kFewTokens = 4;
+constexpr int kFewThreads = 256;
+
+__device__ __forceinline__ int4 ld_weights(const int8_t* p) {
+  int4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ int dot16(const int4& a, const int4& b, int acc) {
+  acc = __dp4a(a.x, b.x, acc);
+  acc = __dp4a(a.y, b.y, acc);
+  acc = __dp4a(a.z, b.z, acc);
+  return __dp4a(a.w, b.w, acc);
+}
+
+__device__ __forceinline__ void put1(float* y, float v) { *y = v; }
+__device__ __forceinline__ void put1(__nv_bfloat16* y, float v) { *y = __float2bfloat16_rn(v); }
+
+template <int TT, int ACT, typename Tout>
+__global__ void __launch_bounds__(kFewThreads) linear_i8_few_kernel(const I8Params p) {
+  constexpr bool kGeglu = ACT == kActGeglu;
+  constexpr int kUnroll = TT <= 2 ? 4 : 2;
+  __shared__ int part[8][2 * TT];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kw = p.splits;                        // warps that share a pair of rows
+  const int grp = (blockIdx.x * 8 + warp) / kw;   // pair of rows
+  const int part_k = warp % kw;
+  const int c0 = kGeglu ? grp : 2 * grp;          // output column
+  const int r0 = c0, r1 = kGeglu ? p.F + grp : min(2 * grp + 1, p.O - 1);
+  const bool live = c0 < p.F;
+  int acc[2][TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) acc[0][t] = acc[1][t] = 0;
+  if (live) {
+    const int8_t* w0 = p.w + static_cast<long>(r0) * p.ldw;
+    const int8_t* w1 = p.w + static_cast<long>(r1) * p.ldw;
+    const int vecs = p.K / 16;
+    const int v0 = static_cast<int>(static_cast<long>(part_k) * vecs / kw), v1 = static_cast<int>(static_cast<long>(part_k + 1) * vecs / kw);
+    for (int v = v0 + lane; v < v1; v += 32 * kUnroll) {
+      int4 a[kUnroll], b[kUnroll];
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) {
+        a[i] = b[i] = make_int4(0, 0, 0, 0);
+        if (v + 32 * i < v1) {
+          a[i] = ld_weights(w0 + static_cast<long>(v + 32 * i) * 16);
+          b[i] = ld_weights(w1 + static_cast<long>(v + 32 * i) * 16);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) {
+        if (v + 32 * i < v1) {
+#pragma unroll
+          for (int t = 0; t < TT; ++t) {
+            if (TT > 1 && t >= p.T) break;
+            const int4 x = __ldg(reinterpret_cast<const int4*>(p.x + t * p.ldx) + v + 32 * i);
+            acc[0][t] = dot16(a[i], x, acc[0][t]);
+            acc[1][t] = dot16(b[i], x, acc[1][t]);
+          }
+        }
+      }
+    }
+    // the last K % 16 elements, one per lane: nothing past a row's end is read
+    const int k = vecs * 16 + lane;
+    if (part_k == kw - 1 && k < p.K) {
+      const int a = w0[k], b = w1[k];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        if (t < p.T) {
+          const int x = p.x[t * p.ldx + k];
+          acc[0][t] += a * x;
+          acc[1][t] += b * x;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int s = __reduce_add_sync(0xffffffffu, acc[r][t]);
+      if (lane == 0) part[warp][2 * t + r] = s;
+    }
+  }
+  if (kw > 1)
+    __syncthreads();
+  else
+    __syncwarp();
+  // the outputs of this warp's rows: the first warp of those that share them
+  if (part_k == 0 && live && lane < (kGeglu ? TT : 2 * TT)) {
+    const int t = kGeglu ? lane : lane >> 1, r = kGeglu ? 0 : lane & 1;
+    const int o = c0 + r;
+    if (t < p.T && o < p.F) {
+      int s0 = 0, s1 = 0;
+      for (int q = 0; q < kw; ++q) {
+        s0 += part[warp + q][2 * t + r];
+        if (kGeglu) s1 += part[warp + q][2 * t + 1];
+      }
+      const float sx = p.x_scale[t];
+      float v = fmaf(static_cast<float>(s0) * sx, p.w_scale[o], p.bias ? p.bias[o] : 0.f);
+      if (kGeglu)
+        v = gelu_i8(v) * fmaf(static_cast<float>(s1) * sx, p.w_scale[p.F + o], p.bias ? p.bias[p.F + o] : 0.f);
+      else
+        v = activate<ACT>(v);
+      put1(static_cast<Tout*>(p.y) + t * p.ldy + o, v);
+    }
+  }
+}
+
 // ------------------------------------------------------------ host side ---
 struct I8Plan {
-  bool pair;
-  int nt, splits, stages, rows_a, recv_off, small_off, smem, m_tiles, n_tiles, clusters;
-  int nt2, n_tiles2;  // CTA pairs: the narrow last tiles' width and count per token tile
+  bool few;                  // few tokens: `clusters` CTAs, `splits` warps per pair of rows
+  int nt, n_tiles;           // CTA pairs: weight rows per tile, tiles per token tile
+  int nt2, n_tiles2;         // the narrower last tiles
+  int splits, stages, rows_a, m_tiles, clusters;
 };
 
 int out_cols(const rfx_linear_i8_desc& d) { return d.epilogue == RFX_EPI_GEGLU ? d.O / 2 : d.O; }
 
 template <int ACT>
-const void* i8_ptr(int out_dtype, bool pair) {
-  if (pair)
-    return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, __nv_bfloat16>)
-                                   : reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, float>);
-  return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_kernel<128, ACT, __nv_bfloat16>)
-                                 : reinterpret_cast<const void*>(linear_i8_kernel<128, ACT, float>);
+const void* few_ptr(int out_dtype, int T) {
+  if (out_dtype == kDtypeBF16) {
+    if (T == 1) return reinterpret_cast<const void*>(linear_i8_few_kernel<1, ACT, __nv_bfloat16>);
+    if (T == 2) return reinterpret_cast<const void*>(linear_i8_few_kernel<2, ACT, __nv_bfloat16>);
+    return reinterpret_cast<const void*>(linear_i8_few_kernel<4, ACT, __nv_bfloat16>);
+  }
+  if (T == 1) return reinterpret_cast<const void*>(linear_i8_few_kernel<1, ACT, float>);
+  if (T == 2) return reinterpret_cast<const void*>(linear_i8_few_kernel<2, ACT, float>);
+  return reinterpret_cast<const void*>(linear_i8_few_kernel<4, ACT, float>);
 }
-const void* i8_kernel(int epilogue, int out_dtype, bool pair) {
+template <int ACT>
+const void* i8_ptr(int out_dtype, bool few, int T) {
+  if (few) return few_ptr<ACT>(out_dtype, T);
+  return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, __nv_bfloat16>)
+                                 : reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, float>);
+}
+const void* i8_kernel(int epilogue, int out_dtype, bool few, int T) {
   switch (epilogue) {
-    case RFX_EPI_STORE: return i8_ptr<kActNone>(out_dtype, pair);
-    case RFX_EPI_SILU: return i8_ptr<kActSilu>(out_dtype, pair);
-    case RFX_EPI_GELU: return i8_ptr<kActGelu>(out_dtype, pair);
-    case RFX_EPI_GEGLU: return i8_ptr<kActGeglu>(out_dtype, pair);
+    case RFX_EPI_STORE: return i8_ptr<kActNone>(out_dtype, few, T);
+    case RFX_EPI_SILU: return i8_ptr<kActSilu>(out_dtype, few, T);
+    case RFX_EPI_GELU: return i8_ptr<kActGelu>(out_dtype, few, T);
+    case RFX_EPI_GEGLU: return i8_ptr<kActGeglu>(out_dtype, few, T);
   }
   return nullptr;
 }
 
+// How a call is cut up.  Up to 4 tokens go to the integer units: one token of
+// a 2048 x 2560 projection takes 3.1 us there and 7.0 as pair tiles, 4 tokens
+// 4.3, and of a 2048 x 32768 GeGLU 14.7 and 19.7 against 18.8; with 8 tokens
+// the products bound them (28.6 us).
+//
+// Pair tiles: the width N and the split of K that finish soonest by this
+// model, whose figures are fitted to measured times of these projections at
+// 16 to 4096 tokens.  A K step takes 150 ns + 0.45 ns per weight row while the
+// copies into the SM bound it, 1.12 ns per weight row once the MMAs do, and
+// 1.17 times that with every SM at work; a tile at least its epilogue's 10 ns
+// per weight row; the last epilogue is not hidden; adding up the splits costs
+// 0.9 us + 0.4 us per split.
 I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   I8Plan c{};
-  if (d.T > 128) {
-    const int m = (d.T + 2 * kTileM - 1) / (2 * kTileM);
-    const int k_steps = (d.K + kStepK - 1) / kStepK;
-    const void* fn = i8_kernel(d.epilogue, d.out_dtype, true);
-    const int div = d.epilogue == RFX_EPI_GEGLU ? 2 : 1;  // weight rows per output column
-    const int F = out_cols(d);
-    const int step = 32 * div;  // tiles of whole 64-byte pieces of output rows
-    auto tiles_of = [&](int cols, int nt) { return (cols * div + nt - 1) / nt; };
-    // A tile's time in ns: its K steps, each bound by the copies into the SM
-    // for narrow tiles and by the MMAs for wide ones, or its epilogue.
-    auto tile_ns = [&](int nt, int s) {
-      return std::max((k_steps + s - 1) / s * (100.0 + 0.95 * nt), 10.0 * nt);
-    };
-    double best = 0;
-    for (int s = 1; s <= std::min(kMaxSplits, k_steps); ++s) {
-      // clusters of 2s CTAs that are resident at once (GPCs hold whole clusters)
-      int slots = max_active_clusters(fn, kPairThreads, kPairSmem, 2 * s);
-      if (slots <= 0) slots = std::max(1, nsm / (2 * s) - (s > 1 ? 3 : 0));
-      for (int nt = 64; nt <= 256; nt += step) {
-        const int n = tiles_of(F, nt);
-        const long tiles = static_cast<long>(m) * n;
-        const long rounds = (tiles + slots - 1) / slots;
-        if (s > 1 && rounds > 1) continue;
-        auto consider = [&](double cost, int n_a, int nt2, int n_b) {
-          if (c.nt != 0 && cost >= best) return;
-          best = cost;
-          c.nt = nt;
-          c.splits = s;
-          c.n_tiles = n_a;
-          c.nt2 = nt2;
-          c.n_tiles2 = n_b;
-          c.clusters = static_cast<int>(std::min<long>(static_cast<long>(m) * (n_a + n_b), slots));
-        };
-        consider(rounds * tile_ns(nt, s) + 10.0 * nt + (s > 1 ? 1500.0 : 0.0), n, nt, 0);
-        if (s > 1 || rounds < 2) continue;
-        // the full rounds at this width, the rest in narrower tiles
-        const int n_a = static_cast<int>((rounds - 1) * slots / m);
-        if (n_a < 1 || n_a >= n) continue;
-        for (int nt2 = 64; nt2 < nt; nt2 += step) {
-          const int n_b = tiles_of(F - n_a * (nt / div), nt2);
-          const long ua = static_cast<long>(n_a) * m, ub = static_cast<long>(n_b) * m;
-          // the tiles go round the slots: the busiest slot's time
-          const double ta = tile_ns(nt, 1), tb = tile_ns(nt2, 1);
-          const long qa = ua / slots, ra = ua % slots, first = slots - ra;  // `first` slots have one tile less
-          double t;
-          if (ub <= first) {
-            t = std::max(qa * ta + tb, (qa + (ra ? 1 : 0)) * ta);
-          } else {
-            const long qb = (ub - first) / slots, rb = (ub - first) % slots;
-            t = std::max(ra ? (qa + 1) * ta + (qb + (rb ? 1 : 0)) * tb : 0.0, qa * ta + (1 + qb + (rb > ra ? 1 : 0)) * tb);
-          }
-          consider(t + 10.0 * nt2, n_a, nt2, n_b);
-        }
-      }
-    }
-    c.pair = true;
-    c.m_tiles = m;
-    c.rows_a = kTileM;
-    c.stages = std::min(kPairMaxStages, kPairRing / ((kTileM + c.nt / 2) * kStepK));
-    c.smem = kPairSmem;
+  const int div = d.epilogue == RFX_EPI_GEGLU ? 2 : 1;  // weight rows per output column
+  const int F = out_cols(d);
+  if (d.T <= kFewTokens) {
+    c.few = true;
+    // warps per pair of rows: enough of them for 16 per SM, with at least one
+    // 512-byte load per row each
+    const int pairs = d.epilogue == RFX_EPI_GEGLU ? F : (F + 1) / 2;
+    c.splits = 1;
+    while (c.splits < 8 && static_cast<long>(pairs) * c.splits < 16l * nsm && d.K >= 1024 * c.splits) c.splits *= 2;
+    c.clusters = static_cast<int>((static_cast<long>(pairs) * c.splits + 7) / 8);
     return c;
   }
-  c.nt = 128;
-  const int tile_cols = d.epilogue == RFX_EPI_GEGLU ? c.nt / 2 : c.nt;
-  c.m_tiles = (d.T + kTileM - 1) / kTileM;
-  c.n_tiles = (out_cols(d) + tile_cols - 1) / tile_cols;
-  c.rows_a = std::min(kTileM, (d.T + 7) / 8 * 8);
+  const int m = (d.T - 1) / (2 * kTileM) + 1;
   const int k_steps = (d.K + kStepK - 1) / kStepK;
-  c.splits = 1;
-  for (int s : {2, 4, 8})
-    if (s <= k_steps && static_cast<long>(c.m_tiles) * c.n_tiles * s <= nsm) c.splits = s;
-  const int stage = (kTileM + c.nt) * kStepK;
-  const int recv = c.splits > 1 ? c.nt / 4 * (c.rows_a + 2) * 16 : 0;
-  const int small = 256;
-  const int per = (k_steps + c.splits - 1) / c.splits;
-  c.stages = std::min({kI8MaxStages, per, (kSmemMax - 1024 - recv - small) / stage});
-  c.recv_off = c.stages * stage;
-  c.small_off = c.recv_off + recv;
-  c.smem = c.small_off + small + 1024;
+  const int step = 32 * div;  // tiles of whole 64-byte pieces of output rows
+  const void* fn = i8_kernel(d.epilogue, d.out_dtype, false, d.T);
+  auto tiles_of = [&](int cols, int nt) { return static_cast<int>((static_cast<long>(cols) * div + nt - 1) / nt); };
+  auto tile_ns = [&](int nt, int s) {
+    return std::max((k_steps + s - 1) / s * std::max(150.0 + 0.45 * nt, 1.12 * nt), 10.0 * nt);
+  };
+  double best = 0;
+  for (int s = 1; s <= std::min(kMaxSplits, k_steps); ++s) {
+    // clusters of 2s CTAs that are resident at once (GPCs hold whole clusters)
+    int slots = max_active_clusters(fn, kPairThreads, kPairSmem, 2 * s);
+    if (slots <= 0) slots = std::max(1, nsm / (2 * s) - (s > 1 ? 3 : 0));
+    for (int nt = 64; nt <= 256; nt += step) {
+      const int n = tiles_of(F, nt);
+      const long tiles = static_cast<long>(m) * n;
+      const long rounds = (tiles + slots - 1) / slots;
+      if (s > 1 && rounds > 1) continue;
+      auto consider = [&](double cost, int n_a, int nt2, int n_b) {
+        if (c.nt != 0 && cost >= best) return;
+        best = cost;
+        c.nt = nt;
+        c.splits = s;
+        c.n_tiles = n_a;
+        c.nt2 = nt2;
+        c.n_tiles2 = n_b;
+        c.clusters = static_cast<int>(std::min<long>(static_cast<long>(m) * (n_a + n_b), slots));
+      };
+      const double all = 1.17 * tiles / slots * tile_ns(nt, s);  // every SM at work
+      consider(std::max(rounds * tile_ns(nt, s), all) + 10.0 * nt + (s > 1 ? 900.0 + 400.0 * s : 0.0), n, nt, 0);
+      if (s > 1 || rounds < 2) continue;
+      // the full rounds at this width, the rest in narrower tiles
+      const int n_a = static_cast<int>((rounds - 1) * slots / m);
+      if (n_a < 1 || n_a >= n) continue;
+      for (int nt2 = 64; nt2 < nt; nt2 += step) {
+        const int n_b = tiles_of(F - n_a * (nt / div), nt2);
+        const long ua = static_cast<long>(n_a) * m, ub = static_cast<long>(n_b) * m;
+        // the tiles go round the slots: the busiest slot's time
+        const double ta = tile_ns(nt, 1), tb = tile_ns(nt2, 1);
+        const long qa = ua / slots, ra = ua % slots, first = slots - ra;  // `first` slots have one wide tile less
+        double t;
+        if (ub <= first) {
+          t = std::max(qa * ta + tb, (qa + (ra ? 1 : 0)) * ta);
+        } else {
+          const long qb = (ub - first) / slots, rb = (ub - first) % slots;
+          t = std::max(ra ? (qa + 1) * ta + (qb + (rb ? 1 : 0)) * tb : 0.0, qa * ta + (1 + qb + (rb > ra ? 1 : 0)) * tb);
+        }
+        consider(std::max(t, 1.17 * (ua * ta + ub * tb) / slots) + 10.0 * nt2, n_a, nt2, n_b);
+      }
+    }
+  }
+  c.m_tiles = m;
+  c.rows_a = d.T < kTileM ? (d.T + 7) / 8 * 8 : kTileM;
+  c.stages = std::min(kPairMaxStages, kPairRing / ((kTileM + c.nt / 2) * kStepK));
   return c;
 }
 
@@ -876,11 +764,11 @@ int build_linear_i8_maps(const rfx_linear_i8_desc& d, LinearI8Maps* maps) {
   int nsm = 148;
   rfx_num_sms(&nsm);
   const I8Plan c = plan_i8(d, nsm);
-  const bool geglu = d.epilogue == RFX_EPI_GEGLU;
+  if (c.few) return RFX_OK;
   rc = make_tmap_2d(&maps->x, d.x, 1, d.K, d.T, d.ldx, kStepK, c.rows_a, true);
   if (rc) return rc;
-  rc = make_tmap_2d(&maps->w, d.w, 1, d.K, d.O, d.ldw, kStepK, c.pair || geglu ? c.nt / 2 : c.nt, true);
-  if (rc || !c.pair) return rc;
+  rc = make_tmap_2d(&maps->w, d.w, 1, d.K, d.O, d.ldw, kStepK, c.nt / 2, true);
+  if (rc) return rc;
   maps->w2 = maps->w;
   if (c.n_tiles2 > 0) {
     rc = make_tmap_2d(&maps->w2, d.w, 1, d.K, d.O, d.ldw, kStepK, c.nt2 / 2, true);
@@ -898,9 +786,11 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cuda
   int nsm = 148;
   rfx_num_sms(&nsm);
   const I8Plan c = plan_i8(d, nsm);
-  const void* fn = i8_kernel(d.epilogue, d.out_dtype, c.pair);
-  const int rc = ensure_smem_attr(fn, c.smem);
-  if (rc) return rc;
+  const void* fn = i8_kernel(d.epilogue, d.out_dtype, c.few, d.T);
+  if (!c.few) {
+    const int rc = ensure_smem_attr(fn, kPairSmem);
+    if (rc) return rc;
+  }
   I8Params p{};
   p.T = d.T;
   p.O = d.O;
@@ -915,20 +805,20 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cuda
   p.units = p.units_a + c.m_tiles * c.n_tiles2;
   p.stages = c.stages;
   p.rows_a = c.rows_a;
-  p.recv_off = c.recv_off;
-  p.small_off = c.small_off;
+  p.x = static_cast<const int8_t*>(d.x);
+  p.ldx = d.ldx;
+  p.w = static_cast<const int8_t*>(d.w);
+  p.ldw = d.ldw;
   p.x_scale = d.x_scale;
   p.w_scale = d.w_scale;
   p.bias = d.bias;
   p.y = d.y;
   p.ldy = d.ldy;
   p.status = device_status_ptr();
+  if (c.few) return launch_kernel(fn, dim3(c.clusters), dim3(kFewThreads), 0, stream, pdl, 1, p);
   CUtensorMap x = maps.x, w = maps.w, w2 = maps.w2, y = maps.y;
-  if (c.pair)
-    return launch_kernel(fn, dim3(2 * c.splits * c.clusters), dim3(kPairThreads), static_cast<size_t>(c.smem), stream,
-                         pdl, 2 * c.splits, x, w, w2, y, p);
-  const unsigned grid = static_cast<unsigned>(c.m_tiles) * c.n_tiles * c.splits;
-  return launch_kernel(fn, dim3(grid), dim3(kI8Threads), static_cast<size_t>(c.smem), stream, pdl, c.splits, x, w, p);
+  return launch_kernel(fn, dim3(2 * c.splits * c.clusters), dim3(kPairThreads), static_cast<size_t>(kPairSmem), stream,
+                       pdl, 2 * c.splits, x, w, w2, y, p);
 }
 
 }  // namespace rfx
