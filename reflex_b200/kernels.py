@@ -353,6 +353,7 @@ def copy_rows(**kw) -> None:
 
 # -------------------------------------------------------- int8 layer path ---
 _CODES = {torch.bfloat16: L.RFX_DTYPE_BF16, torch.float32: L.RFX_DTYPE_F32}
+_F32 = torch.float32
 
 
 def _here(first: torch.Tensor, *rest) -> None:
@@ -368,11 +369,12 @@ def _here(first: torch.Tensor, *rest) -> None:
         raise ValueError(f"tensors on cuda:{dev}, current device cuda:{torch.cuda.current_device()}")
 
 
-def _rows(name: str, t: torch.Tensor, T: int, K: int, align: int = 1) -> int:
-    """Row stride of a [T, K] tensor with contiguous rows (a single row's
+def _rows(name: str, t: torch.Tensor, shape, align: int = 1) -> int:
+    """Row stride of a matrix of this shape with contiguous rows (a single row's
     stride is never used: the smallest that is a multiple of `align`)."""
-    if t.shape != (T, K):
-        raise ValueError(f"{name} must be [{T}, {K}], not {list(t.shape)}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
+    T, K = shape
     ld, step = t.stride()
     if step != 1 and K > 1:
         raise ValueError(f"{name} must have contiguous rows")
@@ -397,38 +399,40 @@ def _code(name: str, t: torch.Tensor) -> int:
 
 
 def _int8(name: str, t: torch.Tensor) -> None:
-    if t.dtype != torch.int8:
+    if t.dtype is not torch.int8:
         raise ValueError(f"{name} must be int8, not {t.dtype}")
 
 
-def _vector(name: str, t: torch.Tensor | None, K: int) -> int | None:
-    if t is None:
-        return None
-    if t.dtype != torch.float32 or t.shape != (K,) or not t.is_contiguous():
+def _vector(name: str, t: torch.Tensor, K: int) -> int:
+    if t.dtype is not _F32 or t.shape != (K,) or (K > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be a contiguous fp32 [{K}]")
     return t.data_ptr()
 
 
-def _per_batch(name: str, t: torch.Tensor | None, T: int, S: int, K: int) -> int:
+def _per_batch(name: str, t: torch.Tensor, T: int, S: int, K: int) -> int:
     """Batch stride of an fp32 vector per stream [B, K], or [K] for all of them."""
-    if t is None:
-        return 0
-    if t.dtype != torch.float32 or t.dim() not in (1, 2) or t.shape[-1] != K or (K > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{name} must be fp32 [B, {K}] or [{K}] with contiguous rows")
     if t.dim() == 1:
+        _vector(name, t, K)
         return 0
-    if t.shape[0] * S < T:
-        raise ValueError(f"{name} has {t.shape[0]} rows for {T} tokens of {S} per stream")
-    return t.stride(0)
+    if t.dtype is not _F32 or t.dim() != 2:
+        raise ValueError(f"{name} must be fp32 [B, {K}] or [{K}]")
+    B, n = t.shape
+    stride, step = t.stride()
+    if n != K or (step != 1 and K > 1):
+        raise ValueError(f"{name} must be fp32 [B, {K}] or [{K}] with contiguous rows")
+    if B * S < T:
+        raise ValueError(f"{name} has {B} rows for {T} tokens of {S} per stream")
+    return stride
 
 
 def quant_rows_desc(*, x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> L.QuantRowsDesc:
     """Rows x [T, K] (bf16 or fp32) to int8 q [T, K] and fp32 scale [T]."""
     _here(x, q, scale)
     _int8("q", q)
-    T, K = _rows_of("x", x)
-    return L.QuantRowsDesc(T, K, _code("x", x), x.data_ptr(), _rows("x", x, T, K), q.data_ptr(),
-                           _rows("q", q, T, K), _vector("scale", scale, T))
+    shape = _rows_of("x", x)
+    T, K = shape
+    return L.QuantRowsDesc(T, K, _code("x", x), x.data_ptr(), _rows("x", x, shape), q.data_ptr(),
+                           _rows("q", q, shape), _vector("scale", scale, T))
 
 
 def quant_rows(*, x, q, scale) -> None:
@@ -445,12 +449,13 @@ def linear_i8_desc(*, w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, x
     _here(w, w_scale, x, x_scale, y, bias)
     _int8("x", x)
     _int8("w", w)
-    T, K = _rows_of("x", x)
+    shape = _rows_of("x", x)
+    T, K = shape
     O = _rows_of("w", w)[0]
-    return L.LinearI8Desc(T, O, K, epilogue, _code("y", y), x.data_ptr(), _rows("x", x, T, K, 16),
-                          _vector("x_scale", x_scale, T), w.data_ptr(), _rows("w", w, O, K, 16),
-                          _vector("w_scale", w_scale, O), _vector("bias", bias, O), y.data_ptr(),
-                          _rows("y", y, T, O // 2 if epilogue == L.RFX_EPI_GEGLU else O))
+    return L.LinearI8Desc(T, O, K, epilogue, _code("y", y), x.data_ptr(), _rows("x", x, shape, 16),
+                          _vector("x_scale", x_scale, T), w.data_ptr(), _rows("w", w, (O, K), 16),
+                          _vector("w_scale", w_scale, O), None if bias is None else _vector("bias", bias, O),
+                          y.data_ptr(), _rows("y", y, (T, O // 2 if epilogue == L.RFX_EPI_GEGLU else O)))
 
 
 def linear_i8(*, w, w_scale, x, x_scale, y, epilogue=L.RFX_EPI_STORE, bias=None) -> None:
@@ -468,40 +473,32 @@ def block_norm_desc(*, h: torch.Tensor, S: int, y: torch.Tensor | None = None, p
     [B, K] or [K] (fp32).  h_out takes the updated stream (h for in place),
     z or z_q and z_scale the next norm's output."""
     _here(h, y, post_w, gate, h_out, norm_a1, norm_a2, norm_b2, z, z_q, z_scale)
-    T, K = _rows_of("h", h)
+    shape = _rows_of("h", h)
+    T, K = shape
     if S < 1:
         raise ValueError("S (tokens per stream) must be at least 1")
-    d = L.BlockNormDesc()
-    d.T, d.K, d.tokens_per_batch, d.dtype = T, K, min(S, 0x7FFFFFFF), _code("h", h)
-    d.h, d.ldh, d.residual_scale, d.eps = h.data_ptr(), _rows("h", h, T, K), residual_scale, eps
-    if (y is not None and y.dtype != h.dtype) or (h_out is not None and h_out.dtype != h.dtype) or (
-            z is not None and z.dtype != h.dtype):
+    dtype = h.dtype
+    if (y is not None and y.dtype is not dtype) or (h_out is not None and h_out.dtype is not dtype) or (
+            z is not None and z.dtype is not dtype):
         raise ValueError("h, y, h_out and z have one dtype")
-    if y is not None:
-        d.y, d.ldy = y.data_ptr(), _rows("y", y, T, K)
-    if post_w is not None:
-        d.post_w = _vector("post_w", post_w, K)
-    if gate is not None:
-        d.gate, d.gate_stride = gate.data_ptr(), _per_batch("gate", gate, T, S, K)
-    if h_out is not None:
-        d.h_out, d.ldho = h_out.data_ptr(), _rows("h_out", h_out, T, K)
-    if norm_a1 is not None:
-        d.norm_a1 = _vector("norm_a1", norm_a1, K)
-    if norm_a2 is not None:
-        d.norm_a2, d.norm_ab_stride = norm_a2.data_ptr(), _per_batch("norm_a2", norm_a2, T, S, K)
-    if norm_b2 is not None:
-        stride = _per_batch("norm_b2", norm_b2, T, S, K)
-        if norm_a2 is not None and stride != d.norm_ab_stride and T > S:
-            raise ValueError("norm_a2 and norm_b2 must have one batch stride")
-        d.norm_b2, d.norm_ab_stride = norm_b2.data_ptr(), stride
-    if z is not None:
-        d.z, d.ldz = z.data_ptr(), _rows("z", z, T, K)
     if z_q is not None:
         _int8("z_q", z_q)
-        d.z_q, d.ldzq = z_q.data_ptr(), _rows("z_q", z_q, T, K)
-    if z_scale is not None:
-        d.z_scale = _vector("z_scale", z_scale, T)
-    return d
+    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    ab = 0 if norm_a2 is None else _per_batch("norm_a2", norm_a2, T, S, K)
+    if norm_b2 is not None:
+        stride = _per_batch("norm_b2", norm_b2, T, S, K)
+        if norm_a2 is not None and stride != ab and T > S:
+            raise ValueError("norm_a2 and norm_b2 must have one batch stride")
+        ab = stride
+    return L.BlockNormDesc(
+        T, K, S if S <= 0x7FFFFFFF else 0x7FFFFFFF, _code("h", h), h.data_ptr(), _rows("h", h, shape),
+        at(y), 0 if y is None else _rows("y", y, shape),
+        0 if post_w is None else _vector("post_w", post_w, K),
+        at(gate), 0 if gate is None else _per_batch("gate", gate, T, S, K), residual_scale,
+        at(h_out), 0 if h_out is None else _rows("h_out", h_out, shape),
+        0 if norm_a1 is None else _vector("norm_a1", norm_a1, K), at(norm_a2), at(norm_b2), ab, eps,
+        at(z), 0 if z is None else _rows("z", z, shape), at(z_q), 0 if z_q is None else _rows("z_q", z_q, shape),
+        0 if z_scale is None else _vector("z_scale", z_scale, T))
 
 
 def block_norm(**kw) -> None:
@@ -549,14 +546,14 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, *, scaling: str = "no
 
 
 def _heads(name: str, t: torch.Tensor, x: torch.Tensor, shape: tuple) -> tuple:
-    """Strides (b, h, s) of an output of `rope`."""
-    if t.dtype != x.dtype or t.shape != shape:
+    """Address and strides (b, h, s) of an output of `rope`."""
+    if t.dtype is not x.dtype or t.shape != shape:
         raise ValueError(f"{name} must be {x.dtype} {list(shape)}")
     sb, sh, ss, sd = t.stride()
     B, H, S, D = shape
     if sd != 1 or (sb < D and B > 1) or (sh < D and H > 1) or (ss < D and S > 1):
         raise ValueError(f"{name}: heads must be contiguous and must not overlap (strides {t.stride()})")
-    return sb, sh, ss
+    return t.data_ptr(), sb, sh, ss
 
 
 def rope_desc(*, x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, q_out: torch.Tensor,
@@ -567,29 +564,30 @@ def rope_desc(*, x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
     with contiguous D (also over x itself); positions int32 [B*S]; inv_freq
     fp64 [rot_dim / 2]."""
     _here(x, positions, inv_freq, q_out, k_out, v_out)
-    code = _code("x", x)
     if q_out.dim() != 4:
         raise ValueError("q_out must be [B, Hq, S, D]")
-    B, Hq, S, D = q_out.shape
-    Hkv = k_out.shape[1] if k_out is not None else 0
-    heads = Hq + Hkv * (2 if v_out is not None else 1)
-    d = L.RopeDesc()
-    d.B, d.S, d.num_q_heads, d.num_kv_heads, d.head_dim, d.pairs, d.dtype = B, S, Hq, Hkv, D, pairs, code
-    d.x, d.ldx, d.magnitude = x.data_ptr(), _rows("x", x, B * S, heads * D, 8), magnitude
-    if positions.dtype != torch.int32 or positions.shape != (B * S,) or not positions.is_contiguous():
-        raise ValueError(f"positions must be a contiguous int32 [{B * S}]")
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+    shape = q_out.shape
+    B, Hq, S, D = shape
+    T = B * S
+    if positions.dtype is not torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
+        raise ValueError(f"positions must be a contiguous int32 [{T}]")
+    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous fp64 vector")
-    d.positions, d.inv_freq, d.rot_dim = positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0]
-    d.q_out = q_out.data_ptr()
-    d.qs_b, d.qs_h, d.qs_s = _heads("q_out", q_out, x, (B, Hq, S, D))
+    k = v = (0, 0, 0, 0)
+    heads, Hkv = Hq, 0
     if k_out is not None:
-        d.k_out = k_out.data_ptr()
-        d.ks_b, d.ks_h, d.ks_s = _heads("k_out", k_out, x, (B, Hkv, S, D))
-    if v_out is not None:
-        d.v_out = v_out.data_ptr()
-        d.vs_b, d.vs_h, d.vs_s = _heads("v_out", v_out, x, (B, Hkv, S, D))
-    return d
+        Hkv = k_out.shape[1]
+        kv = (B, Hkv, S, D)
+        k = _heads("k_out", k_out, x, kv)
+        heads += Hkv
+        if v_out is not None:
+            v = _heads("v_out", v_out, x, kv)
+            heads += Hkv
+    elif v_out is not None:
+        raise ValueError("v_out goes with k_out")
+    return L.RopeDesc(B, S, Hq, Hkv, D, 2 * inv_freq.shape[0], pairs, _code("x", x), x.data_ptr(),
+                      _rows("x", x, (T, heads * D), 8), positions.data_ptr(), inv_freq.data_ptr(), magnitude,
+                      *_heads("q_out", q_out, x, shape), *k, *v)
 
 
 def rope(**kw) -> None:
