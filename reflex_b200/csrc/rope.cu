@@ -17,8 +17,9 @@
 namespace rfx {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 512;  // at most
 constexpr int kMaxHeadDim = 256;
+constexpr int kMaxTokens = 16;  // per CTA
 
 struct RopeParams {
   int T, S;
@@ -78,83 +79,120 @@ struct Pack<float> {
 // or one dim past rot.  A thread owns every element of a pair, so the output
 // may lie over the input.
 template <typename T, bool HALF, bool VEC>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) {
-  extern __shared__ float2 cs[];  // [tokens][rot / 2] cos, sin
+struct Item {
+  float u[VEC ? 8 : 1], w[VEC ? 8 : 1];
+
+  // whether it has two parts (the halves of pairs), and where the first begins
+  static __device__ __forceinline__ bool two(int lane, int half) { return VEC ? HALF && lane * 8 < half : lane < half; }
+  static __device__ __forceinline__ int first(int lane, int half, int rot) {
+    if (VEC) return !HALF || lane * 8 < half ? lane * 8 : rot + (lane * 8 - half);
+    return lane < half ? (HALF ? lane : 2 * lane) : rot + (lane - half);
+  }
+  static __device__ __forceinline__ int second(int d, int half) { return HALF ? d + half : d + 1; }
+
+  __device__ __forceinline__ void load(const T* src, int d, bool pair, int half) {
+    if constexpr (VEC) {
+      Pack<T>::load(src + d, u);
+      if (pair) Pack<T>::load(src + second(d, half), w);
+    } else {
+      u[0] = Pack<T>::get(src + d);
+      if (pair) w[0] = Pack<T>::get(src + second(d, half));
+    }
+  }
+  // cs: cos, sin of the token's pairs
+  __device__ __forceinline__ void turn(const float2* cs, int d, bool pair, int rot) {
+    if constexpr (VEC && !HALF) {
+      if (d < rot) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float2 r = cs[(d + e) >> 1];
+          const float x = u[e], y = u[e + 1];
+          u[e] = x * r.x - y * r.y;
+          u[e + 1] = y * r.x + x * r.y;
+        }
+      }
+    } else if (pair) {
+#pragma unroll
+      for (int e = 0; e < (VEC ? 8 : 1); ++e) {
+        const float2 r = cs[HALF ? d + e : d >> 1];
+        const float x = u[e], y = w[e];
+        u[e] = x * r.x - y * r.y;
+        w[e] = y * r.x + x * r.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* dst, int d, bool pair, int half) const {
+    if constexpr (VEC) {
+      Pack<T>::store(dst + d, u);
+      if (pair) Pack<T>::store(dst + second(d, half), w);
+    } else {
+      Pack<T>::put(dst + d, u[0]);
+      if (pair) Pack<T>::put(dst + second(d, half), w[0]);
+    }
+  }
+};
+
+// Threads on an SM, and tokens whose loads a thread has in flight: a half-split
+// item is two loads, an interleaved one is one.
+template <bool TWO_LOADS>
+constexpr int resident_threads() {
+  return TWO_LOADS ? 1024 : 1536;
+}
+
+// A CTA takes a few neighbouring tokens.  A thread keeps its (head, item) and
+// walks the tokens, so that what it adds per 16 bytes is one row stride.
+template <typename T, bool HALF, bool VEC>
+__global__ void __launch_bounds__(kRopeThreads, resident_threads<HALF && VEC>() / kRopeThreads) rope_kernel(const RopeParams p) {
+  constexpr int kBatch = 2;
+  extern __shared__ float2 cs[];               // [tokens][rot / 2] cos, sin
+  __shared__ long at[3][kMaxTokens];           // where a token's q, k and v begin
   pdl_wait();
   pdl_launch_dependents();
   const int half = p.rot >> 1;
   const int t0 = blockIdx.x * p.tokens;
   const int nt = min(p.tokens, p.T - t0);
-  for (int i = threadIdx.x; i < nt * half; i += kRopeThreads) {
-    const int tt = i / half, pair = i - tt * half;
-    const double turns = static_cast<double>(p.pos[t0 + tt]) * (p.freq[pair] * 0.15915494309189533577);
-    const float frac = static_cast<float>(turns - rint(turns));
-    float s, c;
-    sincospif(2.f * frac, &s, &c);
-    cs[i] = make_float2(p.mag * c, p.mag * s);
+  for (int i = threadIdx.x; i < nt; i += blockDim.x) {
+    const int t = t0 + i, b = t / p.S, s = t - b * p.S;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) at[j][i] = b * p.sb[j] + s * p.ss[j];
+  }
+  // a thread keeps its pair: its frequency in turns per position is formed once
+  const int width = min(half, static_cast<int>(blockDim.x)), rows = blockDim.x / width;
+  for (int pair = threadIdx.x % width; pair < half; pair += width) {
+    const double f = p.freq[pair] * 0.15915494309189533577;
+    for (int tt = threadIdx.x / width; tt < nt && threadIdx.x < rows * width; tt += rows) {
+      const double turns = static_cast<double>(p.pos[t0 + tt]) * f;
+      // to the nearest whole turn: |turns| < 2^31, so adding 1.5 * 2^52 rounds it
+      const double whole = __dadd_rn(__dadd_rn(turns, 0x1.8p52), -0x1.8p52);
+      float s, c;
+      sincospif(2.f * static_cast<float>(turns - whole), &s, &c);
+      cs[tt * half + pair] = make_float2(p.mag * c, p.mag * s);
+    }
   }
   __syncthreads();
-  const int per = kRopeThreads / p.items;  // head rows per sweep of the CTA
-  const int lane = threadIdx.x % p.items;
-  int row = threadIdx.x / p.items;  // (token, head) of this CTA
-  if (row >= per) return;
-  const int rows = nt * p.ha;
-  for (; row < rows; row += per) {
-    const int tt = row / p.ha, head = row - tt * p.ha;
-    const int t = t0 + tt;
-    const int b = t / p.S, s = t - b * p.S;
+  for (int slot = threadIdx.x; slot < p.items * p.ha; slot += blockDim.x) {
+    const int head = slot / p.items, lane = slot - head * p.items;
     const int part = head < p.hq ? 0 : head < p.hr ? 1 : 2;
-    const int ph = head - (part == 0 ? 0 : part == 1 ? p.hq : p.hr);
-    const T* src = static_cast<const T*>(p.x) + t * p.ldx + static_cast<long>(head) * p.D;
-    T* dst = static_cast<T*>(p.out[part]) + b * p.sb[part] + ph * p.sh[part] + s * p.ss[part];
-    const bool turn = part < 2;
-    const float2* a = cs + tt * half;
-    if (VEC) {
-      if (HALF && lane * 8 < half) {
-        float u[8], w[8];
-        const int d = lane * 8;
-        Pack<T>::load(src + d, u);
-        Pack<T>::load(src + half + d, w);
-        if (turn) {
+    const bool pair = Item<T, HALF, VEC>::two(lane, half);
+    const int d = Item<T, HALF, VEC>::first(lane, half, p.rot);
+    const T* src = static_cast<const T*>(p.x) + t0 * p.ldx + head * p.D;
+    T* dst = static_cast<T*>(part == 0 ? p.out[0] : part == 1 ? p.out[1] : p.out[2]) +
+             (part == 0 ? head * p.sh[0] : part == 1 ? (head - p.hq) * p.sh[1] : (head - p.hr) * p.sh[2]);
+    const long* to = at[part];
+    for (int tt = 0; tt < nt; tt += kBatch) {
+      Item<T, HALF, VEC> it[kBatch];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float2 r = a[d + e];
-            const float x = u[e], y = w[e];
-            u[e] = x * r.x - y * r.y;
-            w[e] = y * r.x + x * r.y;
-          }
-        }
-        Pack<T>::store(dst + d, u);
-        Pack<T>::store(dst + half + d, w);
-      } else {
-        const int d = HALF ? p.rot + (lane * 8 - half) : lane * 8;
-        float u[8];
-        Pack<T>::load(src + d, u);
-        if (!HALF && turn && d < p.rot) {
+      for (int i = 0; i < kBatch; ++i) {
+        if (tt + i < nt) it[i].load(src, d, pair, half);
+        src += p.ldx;
+      }
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float2 r = a[(d + e) >> 1];
-            const float x = u[e], y = u[e + 1];
-            u[e] = x * r.x - y * r.y;
-            u[e + 1] = y * r.x + x * r.y;
-          }
+      for (int i = 0; i < kBatch; ++i) {
+        if (tt + i < nt) {
+          if (part < 2) it[i].turn(cs + (tt + i) * half, d, pair, p.rot);
+          it[i].store(dst + to[tt + i], d, pair, half);
         }
-        Pack<T>::store(dst + d, u);
       }
-    } else if (lane < half) {
-      const int d0 = HALF ? lane : 2 * lane, d1 = HALF ? lane + half : 2 * lane + 1;
-      float x = Pack<T>::get(src + d0), y = Pack<T>::get(src + d1);
-      if (turn) {
-        const float2 r = a[lane];
-        const float u = x * r.x - y * r.y;
-        y = y * r.x + x * r.y;
-        x = u;
-      }
-      Pack<T>::put(dst + d0, x);
-      Pack<T>::put(dst + d1, y);
-    } else {
-      const int d = p.rot + (lane - half);
-      Pack<T>::put(dst + d, Pack<T>::get(src + d));
     }
   }
 }
@@ -225,13 +263,15 @@ int launch_rope(const rfx_rope_desc& d, cudaStream_t stream, bool pdl) {
                 : d.rot_dim / 2 + (d.head_dim - d.rot_dim);
   int nsm = 148;
   rfx_num_sms(&nsm);
-  // enough tokens per CTA for a few sweeps over its rows, while every SM still
-  // has some CTAs; their cos / sin stay within 32 KB of shared memory
+  const int threads = std::min(kRopeThreads, (p.items * p.ha + 31) / 32 * 32);
+  // tokens per CTA: one wave of CTAs over all tokens, their cos / sin within
+  // 16 KB of shared memory
   const int half_rot = d.rot_dim / 2;
-  p.tokens = std::max(1, std::min({p.T / (8 * nsm), 8, 32 * 1024 / (8 * half_rot)}));
-  const unsigned grid = static_cast<unsigned>((p.T + p.tokens - 1) / p.tokens);
+  const int slots = nsm * std::min(16, (half && vec ? resident_threads<true>() : resident_threads<false>()) / threads);
+  p.tokens = std::max(1, std::min({(p.T - 1) / slots + 1, kMaxTokens, 16 * 1024 / (8 * half_rot)}));
+  const unsigned grid = static_cast<unsigned>((p.T - 1) / p.tokens + 1);
   const void* fn = d.dtype == kDtypeBF16 ? rope_ptr<__nv_bfloat16>(half, vec) : rope_ptr<float>(half, vec);
-  return launch_kernel(fn, dim3(grid), dim3(kRopeThreads), static_cast<size_t>(p.tokens) * half_rot * sizeof(float2),
+  return launch_kernel(fn, dim3(grid), dim3(threads), static_cast<size_t>(p.tokens) * half_rot * sizeof(float2),
                        stream, pdl, 1, p);
 }
 
