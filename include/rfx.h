@@ -510,7 +510,7 @@ int rfx_quant_rows(const rfx_quant_rows_desc* desc, void* stream);
 
 /* y[t][o] = act(x_scale[t] * w_scale[o] * sum_k x[t][k] * w[o][k] + bias[o]).
  * The integer sum is exact (s32; K <= 65536); scales, bias and activation are
- * fp32, rounded once to the output type.  epilogue: RFX_EPI_STORE, RFX_EPI_SILU,
+ * fp32, rounded once to the output type.  T and O up to 2^30.  epilogue: RFX_EPI_STORE, RFX_EPI_SILU,
  * RFX_EPI_GELU (tanh form), or RFX_EPI_GEGLU: w holds O/2 gate rows and then
  * O/2 up rows as they are ([Wgate; Wup], no repacking) and
  * y[t][f] = gelu_tanh(gate_f) * up_f, O/2 columns.  Any T, O and K; rows of x
@@ -569,12 +569,13 @@ int rfx_block_norm(const rfx_block_norm_desc* desc, void* stream);
 
 /* Rotary positions on QKV rows x[b*S + s] = [num_q_heads q heads | num_kv_heads
  * k heads | num_kv_heads v heads (with v_out)], split into q, k and v, element
- * (b, h, s, d) at b * stride_b + h * stride_h + s * stride_s + d (so head-major
- * and token-major outputs, and an output over x itself, are all strides).
+ * (b, h, s, d) at b * stride_b + h * stride_h + s * stride_s + d (head-major,
+ * token-major, or over x itself).
  * Pair i < rot_dim/2 of a q or k head is dims (i, i + rot_dim/2)
  * (RFX_ROPE_HALF) or (2i, 2i + 1) (RFX_ROPE_INTERLEAVED) and turns by
  * positions[b*S + s] * inv_freq[i] radians, times `magnitude`; dims past
- * rot_dim and v are copied.  inv_freq is fp64 on the device (positions far
+ * rot_dim and v are copied.  An output lies over x exactly (each element at its
+ * own input's address) or apart from it.  inv_freq is fp64 on the device (positions far
  * beyond fp32's reach keep their angle), scaled by the caller for long
  * contexts.  head_dim <= 256, rot_dim even. */
 #define RFX_ROPE_HALF 0

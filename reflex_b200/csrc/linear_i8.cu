@@ -20,6 +20,7 @@ namespace {
 constexpr int kTileM = 128;
 constexpr int kStepK = 128;  // int8 elements (bytes) of K per stage
 constexpr int kSmemMax = 227 * 1024;
+constexpr int kMaxRows = 1 << 30;  // of x and of w
 constexpr int kMaxK = 65536;  // 65536 * 128 * 128 = 2^30: an s32 sum cannot overflow
 
 struct I8Params {
@@ -734,8 +735,9 @@ bool al(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) 
 }  // namespace
 
 int validate_linear_i8(const rfx_linear_i8_desc& d) {
-  if (d.T < 0 || d.O < 1 || d.K < 1 || d.K > kMaxK)
-    return set_error(RFX_E_INVAL, "rfx_linear_i8: need T>=0, O>=1, 1<=K<=%d (T=%d O=%d K=%d)", kMaxK, d.T, d.O, d.K);
+  if (d.T < 0 || d.T > kMaxRows || d.O < 1 || d.O > kMaxRows || d.K < 1 || d.K > kMaxK)
+    return set_error(RFX_E_INVAL, "rfx_linear_i8: need 0<=T<=2^30, 1<=O<=2^30, 1<=K<=%d (T=%d O=%d K=%d)", kMaxK, d.T,
+                     d.O, d.K);
   if (d.epilogue != RFX_EPI_STORE && d.epilogue != RFX_EPI_SILU && d.epilogue != RFX_EPI_GELU &&
       d.epilogue != RFX_EPI_GEGLU)
     return set_error(RFX_E_INVAL, "rfx_linear_i8: epilogue must be STORE, SILU, GELU or GEGLU");

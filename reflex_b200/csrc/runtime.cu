@@ -5,10 +5,8 @@
 
 #include <atomic>
 #include <cstdarg>
-#include <map>
 #include <memory>
 #include <mutex>
-#include <tuple>
 #include <unordered_map>
 #include <variant>
 #include <vector>
@@ -158,17 +156,22 @@ bool cluster_fits(const void* func, dim3 grid, int threads, int smem, int cluste
 }
 
 int max_active_clusters(const void* func, int threads, int smem, int cluster_x) {
+  struct Entry {
+    const void* func;
+    int smem, cluster, dev, n;
+  };
   static std::mutex mu;
-  static std::map<std::tuple<const void*, int, int, int>, int> memo;
+  static Entry memo[128];  // a few kernels x cluster sizes x devices; the rest is asked again
+  static int used = 0;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
-  const auto key = std::make_tuple(func, smem, cluster_x, dev);
   std::lock_guard<std::mutex> lk(mu);
-  auto it = memo.find(key);
-  if (it != memo.end()) return it->second;
+  for (int i = 0; i < used; ++i)
+    if (memo[i].func == func && memo[i].smem == smem && memo[i].cluster == cluster_x && memo[i].dev == dev)
+      return memo[i].n;
   int n = 0;
   if (ensure_smem_attr(func, smem) == RFX_OK) {
     cudaLaunchConfig_t cfg{};
@@ -185,7 +188,7 @@ int max_active_clusters(const void* func, int threads, int smem, int cluster_x) 
     if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess) n = 0;
     cudaGetLastError();
   }
-  memo[key] = n;
+  if (used < 128) memo[used++] = Entry{func, smem, cluster_x, dev, n};
   return n;
 }
 
@@ -588,38 +591,44 @@ extern "C" int rfx_plan_add_vit_attention(rfx_plan* plan, const rfx_vit_attn_des
   return RFX_OK;
 }
 
+namespace {
+// Appends an op of one launch (none if it has no rows); no exception leaves a C entry.
+template <typename T>
+int plan_push(rfx_plan* plan, T&& op, bool launches) {
+  try {
+    plan->ops.emplace_back(std::forward<T>(op));
+  } catch (...) {
+    return set_error(RFX_E_INVAL, "plan: out of host memory");
+  }
+  plan->launches += launches ? 1 : 0;
+  return RFX_OK;
+}
+}  // namespace
+
 extern "C" int rfx_plan_add_quant_rows(rfx_plan* plan, const rfx_quant_rows_desc* desc) {
   PLAN_GUARD(plan);
   const int rc = validate_quant_rows(*desc);
   if (rc) return rc;
-  plan->ops.emplace_back(QuantRowsOp{*desc});
-  plan->launches += desc->T > 0 ? 1 : 0;
-  return RFX_OK;
+  return plan_push(plan, QuantRowsOp{*desc}, desc->T > 0);
 }
 extern "C" int rfx_plan_add_block_norm(rfx_plan* plan, const rfx_block_norm_desc* desc) {
   PLAN_GUARD(plan);
   const int rc = validate_block_norm(*desc);
   if (rc) return rc;
-  plan->ops.emplace_back(BlockNormOp{*desc});
-  plan->launches += desc->T > 0 ? 1 : 0;
-  return RFX_OK;
+  return plan_push(plan, BlockNormOp{*desc}, desc->T > 0);
 }
 extern "C" int rfx_plan_add_rope(rfx_plan* plan, const rfx_rope_desc* desc) {
   PLAN_GUARD(plan);
   const int rc = validate_rope(*desc);
   if (rc) return rc;
-  plan->ops.emplace_back(RopeOp{*desc});
-  plan->launches += desc->B > 0 && desc->S > 0 ? 1 : 0;
-  return RFX_OK;
+  return plan_push(plan, RopeOp{*desc}, desc->B > 0 && desc->S > 0);
 }
 extern "C" int rfx_plan_add_linear_i8(rfx_plan* plan, const rfx_linear_i8_desc* desc) {
   PLAN_GUARD(plan);
   LinearI8Op op{*desc, {}};
   const int rc = build_linear_i8_maps(op.d, &op.maps);
   if (rc) return rc;
-  plan->ops.emplace_back(op);
-  plan->launches += desc->T > 0 ? 1 : 0;
-  return RFX_OK;
+  return plan_push(plan, op, desc->T > 0);
 }
 
 extern "C" int rfx_plan_add_chunk(rfx_plan* plan, rfx_chunk* chunk) {
