@@ -146,9 +146,11 @@ __device__ __forceinline__ void pack16(const float (&v)[16], uint32_t* w, const 
 }
 
 // A warp's 32 rows x 64 bytes of outputs (lane = row) to memory through its own
-// 2 KB of shared memory: one TMA store, which also clips rows past T and
-// columns past F, where y's rows begin on 16-byte boundaries (`tma`), else
-// coalesced elements.  `rows` and `n` are the live rows and columns from (t, o).
+// 2 KB of shared memory: one TMA store where y's rows begin on 16-byte
+// boundaries (`tma`), else coalesced elements.  The copy clips rows past T, and
+// columns past F only in units of 16 bytes, so a last piece that ends inside
+// such a unit goes out by elements.  `rows` and `n` are the live rows and
+// columns from (t, o).
 template <typename Tout>
 __device__ __forceinline__ void store_part(const I8Params& p, const CUtensorMap* tmY, uint8_t* st,
                                            const uint32_t (&w)[16], int t, int o, int rows, int n, bool tma, int lane) {
@@ -157,6 +159,7 @@ __device__ __forceinline__ void store_part(const I8Params& p, const CUtensorMap*
   if (tma) {
     if (lane == 0) bulk_wait_read();  // the previous store has left the buffer
     __syncwarp();
+    tma = n >= kCols || n * sizeof(Tout) % 16 == 0;
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j)

@@ -164,6 +164,7 @@ def check_linear(T, O, Kc, epi, dtype, bias, ldy_pad=0, seed=0):
     (1, 1, 1), (1, 2560, 2048), (2, 8, 16), (3, 31, 33), (7, 129, 127), (8, 128, 128), (16, 256, 129), (50, 8192, 1024),
     (50, 1024, 4096), (64, 100, 200), (65, 2048, 640), (127, 300, 1152), (128, 1152, 4304), (129, 130, 255),
     (200, 4304, 1152), (256, 512, 16384), (300, 2050, 511), (768, 2560, 2048), (771, 1153, 4304), (1600, 1024, 128),
+    (4, 260, 1040), (5, 260, 1040), (9, 3000, 48), (2000, 6000, 128), (2047, 5001, 64),
 ])
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_linear_i8_store(T, O, Kc, dtype):
@@ -174,10 +175,20 @@ def test_linear_i8_store(T, O, Kc, dtype):
 
 @pytest.mark.parametrize("epi", [L.RFX_EPI_SILU, L.RFX_EPI_GELU, L.RFX_EPI_GEGLU])
 @pytest.mark.parametrize("T,O,Kc", [(1, 2, 16), (1, 8192, 1024), (5, 66, 100), (50, 8192, 1024), (130, 258, 700),
-                                    (513, 1154, 1152), (768, 4608, 2048), (1000, 300, 64)])
+                                    (513, 1154, 1152), (768, 4608, 2048), (1000, 300, 64), (4, 66, 272), (2000, 9002, 64)])
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_linear_i8_activations(epi, T, O, Kc, dtype):
     check_linear(T, O, Kc, epi, dtype, bias=T % 2 == 1, seed=epi * 100 + T)
+
+
+@pytest.mark.parametrize("epi", [L.RFX_EPI_STORE, L.RFX_EPI_GEGLU])
+@pytest.mark.parametrize("T,O,Kc", [(50, 74, 256), (333, 1178, 300), (129, 526, 8192)])
+def test_linear_i8_aligned_rows_of_odd_length(epi, T, O, Kc):
+    """Outputs of 37, 589, 263 or twice as many columns in rows of a multiple
+    of 16 bytes: the wide stores stop at the last column and the last row."""
+    for dtype in (BF, F32):
+        cols = O // 2 if epi == L.RFX_EPI_GEGLU else O
+        check_linear(T, O, Kc, epi, dtype, bias=False, ldy_pad=-cols % 8 + 8, seed=3)
 
 
 def test_linear_i8_largest_sums():
@@ -313,6 +324,45 @@ def test_block_norm_without_block_output(Kc):
 def test_block_norm_shared_vectors():
     """One gate, scale and shift for all streams ([K] instead of [B, K])."""
     check_norm(20, 5, 512, F32, True, True, True, "z", shared=True)
+
+
+@pytest.mark.parametrize("Kc", [200, 1024, 1031])
+def test_block_norm_nonfinite_rows_show(Kc):
+    """A NaN or an infinity in the stream or the block's output leaves its row's
+    scale not finite and its int8 values 0; the other rows are not touched."""
+    r = gen(Kc)
+    h, y = r(6, Kc).cuda(), r(6, Kc).cuda()
+    a1 = torch.ones(Kc, device="cuda")
+    out = []
+    for bad in (False, True):
+        hb, yb = h.clone(), y.clone()
+        if bad:
+            hb[1, 3], yb[4, Kc - 1] = float("nan"), float("inf")
+        q, s = torch.full((6, Kc), 5, dtype=torch.int8, device="cuda"), torch.empty(6, device="cuda")
+        K.block_norm(h=hb, y=yb, S=3, h_out=hb, norm_a1=a1, z_q=q, z_scale=s)
+        out.append((hb, q, s))
+    done()
+    (h0, q0, s0), (h1, q1, s1) = out
+    keep, bad = [0, 2, 3, 5], [1, 4]
+    assert torch.equal(h0[keep], h1[keep]) and torch.equal(q0[keep], q1[keep]) and torch.equal(s0[keep], s1[keep])
+    assert not torch.isfinite(s1[bad]).any() and (q1[bad] == 0).all()
+
+
+@pytest.mark.parametrize("Kc", [1024, 1027, 6000])
+def test_block_norm_output_over_an_input(Kc):
+    """z over y, or over h (with the stream written elsewhere): the same as apart."""
+    r = gen(Kc + 1)
+    h, y = r(40, Kc).to(BF).cuda(), r(40, Kc).to(BF).cuda()
+    w = (1 + 0.1 * r(Kc)).cuda()
+    kw = dict(S=8, post_w=w, norm_a1=w)
+    h0, z0 = torch.empty_like(h), torch.empty_like(h)
+    K.block_norm(h=h, y=y, h_out=h0, z=z0, **kw)
+    y1, h1 = y.clone(), h.clone()
+    K.block_norm(h=h1, y=y1, h_out=h1, z=y1, **kw)
+    h2, hz = torch.empty_like(h), h.clone()
+    K.block_norm(h=hz, y=y, h_out=h2, z=hz, **kw)
+    done()
+    assert torch.equal(h1, h0) and torch.equal(y1, z0) and torch.equal(h2, h0) and torch.equal(hz, z0)
 
 
 def test_block_norm_matches_rms_norm():
@@ -597,3 +647,84 @@ def test_calls_on_two_streams_at_once():
     done()
     for *_, want, y, st in cases:
         assert torch.equal(want, y)
+
+
+def test_offsets_past_32_bits():
+    """Rows so far apart that an element's offset passes 2^31: every operator's
+    outputs land where the stride says."""
+    big = torch.empty((1 << 31) + (1 << 20), dtype=BF, device="cuda")  # 4.3 GB
+    r = gen(8)
+    x = r(2, 64).cuda()
+    q = big.view(torch.int8).as_strided((2, 64), ((1 << 32) + 64, 1))
+    s = torch.empty(2, device="cuda")
+    K.quant_rows(x=x, q=q, scale=s)
+    done()
+    assert np.array_equal(q.cpu().numpy(), ref_quant(x)[0])
+    for T in (2, 5):
+        ld = (1 << 31) // (T - 1) + 64
+        xq, xd = ints(1, T, 256)
+        w, wd = ints(2, 96, 256)
+        y = big.as_strided((T, 96), (ld, 1))
+        K.linear_i8(w=wd, w_scale=torch.ones(96, device="cuda"), x=xd, x_scale=torch.ones(T, device="cuda"), y=y)
+        done()
+        want = xq.double() @ w.double().t()
+        assert ((y.double().cpu() - want).abs() <= HALF[BF] * want.abs()).all()
+    far = (1 << 31) + 64
+    h = big.as_strided((2, 64), (far, 1))
+    h.copy_(x)
+    z = torch.empty(2, 64, dtype=BF, device="cuda")
+    K.block_norm(h=h, S=2, z=z)
+    want = x.to(BF).double()
+    want = (want / torch.sqrt((want * want).mean(1, keepdim=True) + 1e-6)).cpu()
+    done()
+    assert ((z.double().cpu() - want).abs() <= 1.1 * HALF[BF] * want.abs()).all()
+    x1 = torch.empty(2, 64, dtype=BF, device="cuda")
+    x1.copy_(x)
+    out = big.as_strided((1, 1, 2, 64), (far, far, far, 1))
+    K.rope(x=x1, positions=torch.zeros(2, dtype=torch.int32, device="cuda"),
+           inv_freq=torch.ones(32, dtype=torch.float64, device="cuda"), q_out=out)
+    done()
+    assert torch.equal(out[0, 0], x1)  # position 0 turns nothing
+
+
+def test_captured_direct_calls_follow_their_inputs():
+    """The four calls captured into a torch CUDA graph (after one eager run)
+    and replayed over changed inputs give what the eager calls give."""
+    r = gen(12)
+    T, W, O = 50, 1024, 1536
+    h, y = r(T, W).to(BF).cuda(), r(T, W).to(BF).cuda()
+    w = torch.empty(O, W, dtype=torch.int8, device="cuda")
+    ws = torch.empty(O, device="cuda")
+    K.quant_rows(x=r(O, W).cuda(), q=w, scale=ws)
+    a1 = (1 + 0.1 * r(W)).cuda()
+    zq, zs = torch.empty(T, W, dtype=torch.int8, device="cuda"), torch.empty(T, device="cuda")
+    h_out, qkv = torch.empty_like(h), torch.empty(T, O, dtype=BF, device="cuda")
+    aq, as_ = torch.empty(T, O, dtype=torch.int8, device="cuda"), torch.empty(T, device="cuda")
+    q = torch.empty(1, 4, T, 256, dtype=BF, device="cuda")
+    k, v = torch.empty(1, 1, T, 256, dtype=BF, device="cuda"), torch.empty(1, 1, T, 256, dtype=BF, device="cuda")
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    freq, _ = K.rope_frequencies(256)
+
+    def step():
+        K.block_norm(h=h, y=y, S=T, h_out=h_out, norm_a1=a1, z_q=zq, z_scale=zs)
+        K.linear_i8(w=w, w_scale=ws, x=zq, x_scale=zs, y=qkv)
+        K.quant_rows(x=qkv, q=aq, scale=as_)
+        K.rope(x=qkv, positions=pos, inv_freq=freq, q_out=q, k_out=k, v_out=v)
+        return [t.clone() for t in (h_out, zq, zs, qkv, aq, as_, q, k, v)]
+
+    step()
+    done()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = step()
+    for seed in (1, 2):
+        r = gen(seed)
+        h.copy_(r(T, W))
+        y.copy_(r(T, W))
+        pos.add_(100)
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        want = step()
+        done()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -87,6 +87,8 @@ BAD = [
     ("rfx_linear_i8", linear, dict(ldy=63)), ("rfx_linear_i8", linear, dict(y=None)),
     ("rfx_linear_i8", linear, dict(x_scale=None)), ("rfx_linear_i8", linear, dict(w_scale=A + 2)),
     ("rfx_linear_i8", linear, dict(T=2147483647, O=2147483646, ldy=2147483646)),
+    ("rfx_linear_i8", linear, dict(T=(1 << 30) + 1)), ("rfx_linear_i8", linear, dict(O=(1 << 30) + 1, ldy=1 << 31)),
+    ("rfx_linear_i8", linear, dict(T=1 << 30, O=1 << 20, ldy=1 << 20)),
     ("rfx_block_norm", norm, dict(T=-1)), ("rfx_block_norm", norm, dict(K=16385)),
     ("rfx_block_norm", norm, dict(tokens_per_batch=0)), ("rfx_block_norm", norm, dict(dtype=3)),
     ("rfx_block_norm", norm, dict(h=None)), ("rfx_block_norm", norm, dict(h_out=None)),
