@@ -557,7 +557,7 @@ int launch_quant_rows(const rfx_quant_rows_desc& d, cudaStream_t stream, bool pd
   const void* fn = d.in_dtype == kDtypeBF16
                        ? (vec ? quant_rows_ptr<__nv_bfloat16, true>(s) : quant_rows_ptr<__nv_bfloat16, false>(s))
                        : (vec ? quant_rows_ptr<float, true>(s) : quant_rows_ptr<float, false>(s));
-  return launch_kernel(fn, dim3(row_grid(d.T, s.tpr, 1536)), dim3(s.tpr == 32 ? 128 : s.tpr), 0, stream, pdl, 1, p);
+  return launch_kernel(fn, dim3(row_grid(d.T, s.tpr, s.nv == 1 ? 1536 : 1024)), dim3(s.tpr == 32 ? 128 : s.tpr), 0, stream, pdl, 1, p);
 }
 
 int validate_block_norm(const rfx_block_norm_desc& d) {
