@@ -422,7 +422,7 @@ def check_rope(B, S, Hq, Hkv, D, rot, pairs, dtype, first, v=True, pad=0, head_m
 @pytest.mark.parametrize("B,S,Hq,Hkv,D,rot", [
     (1, 1, 1, 0, 2, 2), (1, 1, 8, 1, 256, 256), (1, 50, 8, 1, 256, 256), (3, 17, 4, 2, 64, 32), (2, 5, 3, 1, 72, 72),
     (1, 300, 8, 1, 256, 64), (2, 9, 2, 2, 72, 40), (1, 7, 5, 1, 250, 10), (1, 3, 2, 1, 256, 2), (4, 700, 1, 1, 128, 128),
-    (2, 3, 16, 4, 128, 96),
+    (2, 3, 16, 4, 128, 96), (2, 700, 16, 4, 128, 74), (1, 60, 4, 1, 256, 250), (1, 2, 64, 16, 256, 74),
 ])
 def test_rope(pairs, dtype, B, S, Hq, Hkv, D, rot):
     """Both layouts, part of the head and all of it, head dims off the vector
@@ -430,12 +430,14 @@ def test_rope(pairs, dtype, B, S, Hq, Hkv, D, rot):
     check_rope(B, S, Hq, Hkv, D, rot, pairs, dtype, first=818, v=Hkv > 0)
 
 
+@pytest.mark.parametrize("rot", [48, 44])
 @pytest.mark.parametrize("pairs", [L.RFX_ROPE_HALF, L.RFX_ROPE_INTERLEAVED])
 @pytest.mark.parametrize("in_place,head_major,pad,v", [(True, True, 0, True), (True, True, 5, True), (False, False, 0, True),
                                                        (False, True, 8, False), (False, False, 1, False)])
-def test_rope_layouts(pairs, in_place, head_major, pad, v):
-    """Over its own input, token-major outputs, wider rows, no v heads."""
-    check_rope(2, 33, 4, 2, 64, 48, pairs, BF, first=0, v=v, pad=pad, head_major=head_major, in_place=in_place)
+def test_rope_layouts(pairs, in_place, head_major, pad, v, rot):
+    """Over its own input, token-major outputs, wider rows, no v heads; halves
+    on and off 16-byte boundaries."""
+    check_rope(2, 33, 4, 2, 64, rot, pairs, BF, first=0, v=v, pad=pad, head_major=head_major, in_place=in_place)
 
 
 def test_rope_far_and_negative_positions():
