@@ -659,7 +659,7 @@ const void* i8_kernel(int epilogue, int out_dtype, bool few, int T) {
 // model, whose figures are fitted to measured times of these projections at
 // 16 to 4096 tokens.  A K step takes 150 ns + 0.45 ns per weight row while the
 // copies into the SM bound it, 1.12 ns per weight row once the MMAs do, and
-// 1.17 times that with every SM at work; a tile at least its epilogue's 10 ns
+// 1.17 times that over several rounds of tiles; a tile at least its epilogue's 10 ns
 // per weight row; the last epilogue is not hidden; adding up the splits costs
 // 0.9 us + 0.4 us per split.
 I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
@@ -704,7 +704,8 @@ I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
         c.n_tiles2 = n_b;
         c.clusters = static_cast<int>(std::min<long>(static_cast<long>(m) * (n_a + n_b), slots));
       };
-      const double all = 1.17 * tiles / slots * tile_ns(nt, s);  // every SM at work
+      // several rounds: every SM at work
+      const double all = rounds > 1 ? 1.17 * tiles / slots * tile_ns(nt, s) : 0.0;
       consider(std::max(rounds * tile_ns(nt, s), all) + 10.0 * nt + (s > 1 ? 900.0 + 400.0 * s : 0.0), n, nt, 0);
       if (s > 1 || rounds < 2) continue;
       // the full rounds at this width, the rest in narrower tiles
@@ -723,7 +724,8 @@ I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
           const long qb = (ub - first) / slots, rb = (ub - first) % slots;
           t = std::max(ra ? (qa + 1) * ta + (qb + (rb ? 1 : 0)) * tb : 0.0, qa * ta + (1 + qb + (rb > ra ? 1 : 0)) * tb);
         }
-        consider(std::max(t, 1.17 * (ua * ta + ub * tb) / slots) + 10.0 * nt2, n_a, nt2, n_b);
+        // (a gain of a hundredth by this model is none by the clock)
+        consider(1.01 * (std::max(t, 1.17 * (ua * ta + ub * tb) / slots) + 10.0 * nt2), n_a, nt2, n_b);
       }
     }
   }
