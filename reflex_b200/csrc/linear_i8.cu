@@ -174,14 +174,14 @@ __device__ __forceinline__ void store_part(const I8Params& p, const CUtensorMap*
     }
   } else {
     __syncwarp();
-    Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t) * p.ldy + o;
-    for (int i = lane; i < 32 * kCols; i += 32) {
-      const int r = i / kCols, c = i % kCols;
-      const int byte = c * static_cast<int>(sizeof(Tout));
-      if (r < rows && c < n)
-        y[r * p.ldy + c] =
-            *reinterpret_cast<const Tout*>(st + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
-    }
+    // a lane keeps its column and walks the rows
+    constexpr int kRowsPer = 32 / kCols;
+    const int c = lane % kCols, byte = c * static_cast<int>(sizeof(Tout));
+    Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t + lane / kCols) * p.ldy + o + c;
+    const int end = c < n ? min(rows, 32) : 0;
+#pragma unroll 4
+    for (int r = lane / kCols; r < end; r += kRowsPer, y += kRowsPer * p.ldy)
+      *y = *reinterpret_cast<const Tout*>(st + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
     __syncwarp();
   }
 }
@@ -496,12 +496,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 }
 
 // ------------------------------------------------------- few tokens ---
-// Up to 4 tokens: the weights are read once, 16 bytes per lane and load, and
+// Up to 4 tokens, or 8 of a small layer: the weights are read once, 16 bytes per lane and load, and
 // multiplied on the integer units (4 products per instruction): no tiles, no
 // shared-memory round trip, nothing to set up, so a single token's call costs
 // little more than the memory's latency.  A warp takes two weight rows (GeGLU:
 // a gate row and its up row) over a 1/kw part of K; x comes through L1.
-constexpr int kFewTokens = 4;
+constexpr int kFewTokens = 4, kFewTokensSmall = 8;
+constexpr long kFewSmall = 6 << 20;  // bytes of weights
 constexpr int kFewThreads = 256;
 
 __device__ __forceinline__ int4 ld_weights(const int8_t* p) {
@@ -628,11 +629,13 @@ const void* few_ptr(int out_dtype, int T) {
   if (out_dtype == kDtypeBF16) {
     if (T == 1) return reinterpret_cast<const void*>(linear_i8_few_kernel<1, ACT, __nv_bfloat16>);
     if (T == 2) return reinterpret_cast<const void*>(linear_i8_few_kernel<2, ACT, __nv_bfloat16>);
-    return reinterpret_cast<const void*>(linear_i8_few_kernel<4, ACT, __nv_bfloat16>);
+    if (T <= 4) return reinterpret_cast<const void*>(linear_i8_few_kernel<4, ACT, __nv_bfloat16>);
+    return reinterpret_cast<const void*>(linear_i8_few_kernel<8, ACT, __nv_bfloat16>);
   }
   if (T == 1) return reinterpret_cast<const void*>(linear_i8_few_kernel<1, ACT, float>);
   if (T == 2) return reinterpret_cast<const void*>(linear_i8_few_kernel<2, ACT, float>);
-  return reinterpret_cast<const void*>(linear_i8_few_kernel<4, ACT, float>);
+  if (T <= 4) return reinterpret_cast<const void*>(linear_i8_few_kernel<4, ACT, float>);
+  return reinterpret_cast<const void*>(linear_i8_few_kernel<8, ACT, float>);
 }
 template <int ACT>
 const void* i8_ptr(int out_dtype, bool few, int T) {
@@ -652,8 +655,9 @@ const void* i8_kernel(int epilogue, int out_dtype, bool few, int T) {
 
 // How a call is cut up.  Up to 4 tokens go to the integer units: one token of
 // a 2048 x 2560 projection takes 3.1 us there and 7.0 as pair tiles, 4 tokens
-// 4.3, and of a 2048 x 32768 GeGLU 14.7 and 19.7 against 18.8; with 8 tokens
-// the products bound them (28.6 us).
+// 4.3, and of a 2048 x 32768 GeGLU 14.7 and 19.7 against 18.8.  With 8 tokens
+// the products bound them: a 2048 x 2560 projection (5 MB of weights) takes
+// 5.9 us against 7.3, a 1024 x 8192 one (8 MB) 9.3 against 7.2.
 //
 // Pair tiles: the width N and the split of K that finish soonest by this
 // model, whose figures are fitted to measured times of these projections at
@@ -666,7 +670,7 @@ I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   I8Plan c{};
   const int div = d.epilogue == RFX_EPI_GEGLU ? 2 : 1;  // weight rows per output column
   const int F = out_cols(d);
-  if (d.T <= kFewTokens) {
+  if (d.T <= kFewTokens || (d.T <= kFewTokensSmall && static_cast<long>(d.O) * d.K <= kFewSmall)) {
     c.few = true;
     // warps per pair of rows: enough of them for 16 per SM, with at least one
     // 512-byte load per row each

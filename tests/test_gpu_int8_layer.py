@@ -164,7 +164,7 @@ def check_linear(T, O, Kc, epi, dtype, bias, ldy_pad=0, seed=0):
     (1, 1, 1), (1, 2560, 2048), (2, 8, 16), (3, 31, 33), (7, 129, 127), (8, 128, 128), (16, 256, 129), (50, 8192, 1024),
     (50, 1024, 4096), (64, 100, 200), (65, 2048, 640), (127, 300, 1152), (128, 1152, 4304), (129, 130, 255),
     (200, 4304, 1152), (256, 512, 16384), (300, 2050, 511), (768, 2560, 2048), (771, 1153, 4304), (1600, 1024, 128),
-    (4, 260, 1040), (5, 260, 1040), (9, 3000, 48), (2000, 6000, 128), (2047, 5001, 64),
+    (4, 260, 1040), (5, 260, 1040), (8, 3000, 2100), (9, 3000, 48), (2000, 6000, 128), (2047, 5001, 64),
 ])
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_linear_i8_store(T, O, Kc, dtype):
