@@ -510,11 +510,14 @@ int rfx_quant_rows(const rfx_quant_rows_desc* desc, void* stream);
 
 /* y[t][o] = act(x_scale[t] * w_scale[o] * sum_k x[t][k] * w[o][k] + bias[o]).
  * The integer sum is exact (s32; K <= 65536); scales, bias and activation are
- * fp32, rounded once to the output type.  T and O up to 2^30.  epilogue: RFX_EPI_STORE, RFX_EPI_SILU,
- * RFX_EPI_GELU (tanh form), or RFX_EPI_GEGLU: w holds O/2 gate rows and then
- * O/2 up rows as they are ([Wgate; Wup], no repacking) and
- * y[t][f] = gelu_tanh(gate_f) * up_f, O/2 columns.  Any T, O and K; rows of x
- * and w begin on 16-byte boundaries (pad ldx / ldw; the padding is not read). */
+ * fp32, rounded once to the output type.  epilogue: RFX_EPI_STORE,
+ * RFX_EPI_SILU, RFX_EPI_GELU (tanh form), or RFX_EPI_GEGLU: w holds O/2 gate
+ * rows and then O/2 up rows as they are ([Wgate; Wup], no repacking) and
+ * y[t][f] = gelu_tanh(gate_f) * up_f, O/2 columns.  Any T and O up to 2^30;
+ * rows of x and w begin on 16-byte boundaries (pad ldx / ldw; the padding is
+ * not read).  No workspace; calls on several streams do not disturb each other.
+ * Run a shape once before capturing it (the first call sets the kernel's
+ * shared-memory size). */
 typedef struct rfx_linear_i8_desc {
   int T, O, K;
   int epilogue;
