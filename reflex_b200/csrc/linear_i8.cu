@@ -73,11 +73,11 @@ __device__ __forceinline__ void st_dsmem_i4(uint32_t addr, const int (&v)[4]) {
 }
 
 // ------------------------------------------------------- CTA-pair tiles ---
-// A pair of CTAs computes 256 tokens x N weight rows (N a
-// multiple of 32 up to 256) with cta_group::2 MMAs: each CTA stages its 128
-// tokens and half of the weight rows per K step, so a step moves 16 KB + 64 N
-// bytes into each SM for 2 N clocks of MMA, and with N = 256 the L2 -> SM
-// stream (64 B/clk) just keeps up.  With GeGLU the even CTA stages the gate
+// A pair of CTAs computes 256 tokens x N weight rows (N a multiple of 32 up to
+// 256) with cta_group::2 MMAs: each CTA stages its 128 tokens and half of the
+// weight rows per K step, so a step moves 16 KB + 64 N bytes into each SM for
+// 2 N clocks of MMA, and with N = 256 the L2 -> SM stream (64 B/clk) just keeps
+// up.  With GeGLU the even CTA stages the gate
 // rows and the odd one the up rows, and a thread of either finds both halves of
 // its outputs in its own TMEM lane.
 //
@@ -361,10 +361,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const int c = kGeglu ? (et < nh ? et : et - nh) : et;
         const bool in = o0 + c < p.F;
         const int o = o0 + c + (kGeglu && et >= nh ? p.F : 0);
-        ws[et] = in ? __ldg(p.w_scale + o) : 0.f;
-        bs[et] = in && p.bias ? __ldg(p.bias + o) : 0.f;
+        ws[et] = in ? p.w_scale[o] : 0.f;
+        bs[et] = in && p.bias ? p.bias[o] : 0.f;
       }
-      const float sx = t < p.T ? __ldg(p.x_scale + t) : 0.f;
+      const float sx = t < p.T ? p.x_scale[t] : 0.f;
       // every epilogue warp agrees before anyone leaves the loop
       if (!epi_agree(mbar_wait(&acc_full[buf], (tl >> 1) & 1, p.status, kDevTimeoutMmaDone))) {
         failed = true;
@@ -419,6 +419,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     constexpr int kParts = kGeglu ? 2 : 1;
     constexpr int kSlot = kGroup / 4 * kTileM * 16;  // bytes of one part of one group
     const int groups = (oc + kGroup - 1) / kGroup, others = p.splits - 1;
+    __syncwarp();
     cluster_sync();
     if (warp >= 2 && !failed) {
       const uint32_t base = smem_u32(smem) + static_cast<uint32_t>(rowt) * 16u;
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (warp >= 2 && !failed) {
       const int tw = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32;
       const int o0 = tile.o0;
-      const float sx = tw + lane < p.T ? __ldg(p.x_scale + tw + lane) : 0.f;
+      const float sx = tw + lane < p.T ? p.x_scale[tw + lane] : 0.f;
 #pragma unroll 1
       for (int lg = 0; lg * p.splits + split < groups; ++lg) {
         const int g0 = (lg * p.splits + split) * kGroup;
@@ -505,19 +506,22 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 }
 
 // ------------------------------------------------------- few tokens ---
-// Up to 4 tokens, or 8 of a small layer: the weights are read once, 16 bytes per lane and load, and
-// multiplied on the integer units (4 products per instruction): no tiles, no
-// shared-memory round trip, nothing to set up, so a single token's call costs
-// little more than the memory's latency (3.0 us for 2048 x 2560, 14.7 us or
-// 4.6 TB/s for the 67 MB of a 2048 x 32768 GeGLU).  A warp takes two weight rows (GeGLU:
-// a gate row and its up row) over a 1/kw part of K; x comes through L1.
+// Up to 4 tokens, or 8 of a small layer: the weights are read once, 16 bytes
+// per lane and load, and multiplied on the integer units (4 products per
+// instruction): no tiles, no shared-memory round trip, nothing to set up, so a
+// single token's call costs little more than the memory's latency (3.0 us for
+// 2048 x 2560, 15.4 us or 4.4 TB/s for the 67 MB of a 2048 x 32768 GeGLU).  A
+// warp takes two weight rows (GeGLU: a gate row and its up row) over a 1/kw
+// part of K; x comes through L1.
 constexpr int kFewTokens = 4, kFewTokensSmall = 8;
 constexpr long kFewSmall = 6 << 20;  // bytes of weights
 constexpr int kFewThreads = 256;
 
+// (Not the read-only path: under programmatic launch this grid may start before
+// the one that writes its operands has ended.)
 __device__ __forceinline__ int4 ld_weights(const int8_t* p) {
   int4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
@@ -570,7 +574,7 @@ __global__ void __launch_bounds__(kFewThreads) linear_i8_few_kernel(const I8Para
 #pragma unroll
           for (int t = 0; t < TT; ++t) {
             if (TT > 1 && t >= p.T) break;
-            const int4 x = __ldg(reinterpret_cast<const int4*>(p.x + t * p.ldx) + v + 32 * i);
+            const int4 x = reinterpret_cast<const int4*>(p.x + t * p.ldx)[v + 32 * i];
             acc[0][t] = dot16(a[i], x, acc[0][t]);
             acc[1][t] = dot16(b[i], x, acc[1][t]);
           }
@@ -625,13 +629,6 @@ __global__ void __launch_bounds__(kFewThreads) linear_i8_few_kernel(const I8Para
 }
 
 // ------------------------------------------------------------ host side ---
-struct I8Plan {
-  bool few;                  // few tokens: `clusters` CTAs, `splits` warps per pair of rows
-  int nt, n_tiles;           // CTA pairs: weight rows per tile, tiles per token tile
-  int nt2, n_tiles2;         // the narrower last tiles
-  int splits, stages, rows_a, m_tiles, clusters;
-};
-
 int out_cols(const rfx_linear_i8_desc& d) { return d.epilogue == RFX_EPI_GEGLU ? d.O / 2 : d.O; }
 
 template <int ACT>
@@ -665,19 +662,19 @@ const void* i8_kernel(int epilogue, int out_dtype, bool few, int T) {
 
 // How a call is cut up.  Up to 4 tokens go to the integer units: one token of
 // a 2048 x 2560 projection takes 3.1 us there and 7.0 as pair tiles, 4 tokens
-// 4.3, and of a 2048 x 32768 GeGLU 14.7 and 19.7 against 18.8.  With 8 tokens
+// 4.4, and of a 2048 x 32768 GeGLU 15.4 and 19.7 against 18.8.  With 8 tokens
 // the products bound them: a 2048 x 2560 projection (5 MB of weights) takes
-// 5.9 us against 7.3, a 1024 x 8192 one (8 MB) 9.3 against 7.2.
+// 6.7 us against 7.3, a 1024 x 8192 one (8 MB) 9.3 against 7.2.
 //
 // Pair tiles: the width N and the split of K that finish soonest by this
 // model, whose figures are fitted to measured times of these projections at
 // 16 to 4096 tokens.  A K step takes 150 ns + 0.45 ns per weight row while the
 // copies into the SM bound it, 1.12 ns per weight row once the MMAs do, and
-// 1.17 times that over several rounds of tiles; a tile at least its epilogue's 10 ns
-// per weight row; the last epilogue is not hidden; adding up the splits costs
-// 0.9 us + 0.4 us per split.
-I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
-  I8Plan c{};
+// 1.17 times that over several rounds of tiles; a tile at least its epilogue's
+// 10 ns per weight row; the last epilogue is not hidden; adding up the splits
+// costs 0.9 us + 0.4 us per split.
+LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
+  LinearI8Plan c{};
   const int div = d.epilogue == RFX_EPI_GEGLU ? 2 : 1;  // weight rows per output column
   const int F = out_cols(d);
   if (d.T <= kFewTokens || (d.T <= kFewTokensSmall && static_cast<long>(d.O) * d.K <= kFewSmall)) {
@@ -702,7 +699,10 @@ I8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   for (int s = 1; s <= std::min(kMaxSplits, k_steps); ++s) {
     // clusters of 2s CTAs that are resident at once (GPCs hold whole clusters)
     int slots = max_active_clusters(fn, kPairThreads, kPairSmem, 2 * s);
-    if (slots <= 0) slots = std::max(1, nsm / (2 * s) - (s > 1 ? 3 : 0));
+    if (slots <= 0) {
+      if (s > 1) break;
+      slots = std::max(1, nsm / 2);
+    }
     for (int nt = 64; nt <= 256; nt += step) {
       const int n = tiles_of(F, nt);
       const long tiles = static_cast<long>(m) * n;
@@ -784,7 +784,8 @@ int build_linear_i8_maps(const rfx_linear_i8_desc& d, LinearI8Maps* maps) {
   if (rc || d.T == 0) return rc;
   int nsm = 148;
   rfx_num_sms(&nsm);
-  const I8Plan c = plan_i8(d, nsm);
+  maps->plan = plan_i8(d, nsm);
+  const LinearI8Plan& c = maps->plan;
   if (c.few) return RFX_OK;
   rc = make_tmap_2d(&maps->x, d.x, 1, d.K, d.T, d.ldx, kStepK, c.rows_a, true);
   if (rc) return rc;
@@ -804,9 +805,7 @@ int build_linear_i8_maps(const rfx_linear_i8_desc& d, LinearI8Maps* maps) {
 
 int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cudaStream_t stream, bool pdl) {
   if (d.T == 0) return RFX_OK;
-  int nsm = 148;
-  rfx_num_sms(&nsm);
-  const I8Plan c = plan_i8(d, nsm);
+  const LinearI8Plan& c = maps.plan;
   const void* fn = i8_kernel(d.epilogue, d.out_dtype, c.few, d.T);
   if (!c.few) {
     const int rc = ensure_smem_attr(fn, kPairSmem);

@@ -126,8 +126,16 @@ int launch_vit_attention(const rfx_vit_attn_desc& d, cudaStream_t stream, bool p
 int launch_quant_rows(const rfx_quant_rows_desc& d, cudaStream_t stream, bool pdl);
 int launch_block_norm(const rfx_block_norm_desc& d, cudaStream_t stream, bool pdl);
 int launch_rope(const rfx_rope_desc& d, cudaStream_t stream, bool pdl);
+// How rfx_linear_i8 cuts a call up; its tensor maps are made for it.
+struct LinearI8Plan {
+  bool few;         // few tokens: `clusters` CTAs, `splits` warps per pair of rows
+  int nt, n_tiles;  // CTA pairs: weight rows per tile, tiles per token tile
+  int nt2, n_tiles2;  // the narrower last tiles
+  int splits, stages, rows_a, m_tiles, clusters;
+};
 struct LinearI8Maps {
   CUtensorMap x, w, w2, y;
+  LinearI8Plan plan;
 };
 int build_linear_i8_maps(const rfx_linear_i8_desc& d, LinearI8Maps* maps);
 int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cudaStream_t stream, bool pdl);
