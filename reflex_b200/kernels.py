@@ -352,43 +352,59 @@ def copy_rows(**kw) -> None:
 
 
 # -------------------------------------------------------- int8 layer path ---
+# These wrappers run once per launch and a launch takes 2.5 us, so they look at
+# each tensor as seldom as they can.
 _CODES = {torch.bfloat16: L.RFX_DTYPE_BF16, torch.float32: L.RFX_DTYPE_F32}
-_F32 = torch.float32
+_F32, _I8 = torch.float32, torch.int8
+_ENTRIES: dict = {}
 
 
-def _here(first: torch.Tensor, *rest) -> None:
-    """Every tensor lies on the current CUDA device (whose stream is used).
-    These checks run on every call: they look at each tensor as seldom as they can."""
-    dev = first.get_device()
-    for t in rest:
-        if t is not None and t.get_device() != dev:
-            raise ValueError("rfx kernels take CUDA tensors of one device")
+def _launch(name: str, desc, dev: int) -> None:
+    """Calls a C entry on the current stream of device `dev`."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = _ENTRIES[name] = getattr(L.load(), name)
+    rc = fn(ctypes.byref(desc), torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        L.check(rc)
+
+
+def _current(dev: int) -> int:
+    """`dev`, the device of a call's tensors, if it is the current one."""
     if dev < 0:
         raise ValueError("rfx kernels take CUDA tensors only (there is no CPU fallback)")
-    if dev != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         raise ValueError(f"tensors on cuda:{dev}, current device cuda:{torch.cuda.current_device()}")
+    return dev
 
 
-def _rows(name: str, t: torch.Tensor, shape, align: int = 1) -> int:
-    """Row stride of a matrix of this shape with contiguous rows (a single row's
+def _apart(*ts) -> ValueError:
+    where = sorted({str(t.device) for t in ts if t is not None})
+    return ValueError(f"rfx kernels take CUDA tensors of one device, not of {', '.join(where)}")
+
+
+def _matrix(name: str, t: torch.Tensor):
+    try:
+        T, K = t.shape
+    except ValueError:
+        raise ValueError(f"{name} must be a matrix, not {list(t.shape)}") from None
+    return T, K
+
+
+def _rows(name: str, t: torch.Tensor, T: int, K: int, align: int = 1) -> int:
+    """Row stride of a [T, K] matrix with contiguous rows (a single row's
     stride is never used: the smallest that is a multiple of `align`)."""
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
-    T, K = shape
-    ld, step = t.stride()
-    if step != 1 and K > 1:
-        raise ValueError(f"{name} must have contiguous rows")
+    try:
+        (rows, cols), (ld, step) = t.shape, t.stride()
+    except ValueError:
+        raise ValueError(f"{name} must be [{T}, {K}], not {list(t.shape)}") from None
+    if rows != T or cols != K or (step != 1 and K > 1):
+        raise ValueError(f"{name} must be [{T}, {K}] with contiguous rows, not {list(t.shape)} (strides {t.stride()})")
     if T < 2:
         return -(-K // align) * align
     if ld < K or T > 0x7FFFFFFF:
         raise ValueError(f"{name}: rows overlap (stride {ld}, length {K}), or more than 2^31 - 1 of them")
     return ld
-
-
-def _rows_of(name: str, t: torch.Tensor) -> torch.Size:
-    if t.dim() != 2:
-        raise ValueError(f"{name} must be a matrix, not {list(t.shape)}")
-    return t.shape
 
 
 def _code(name: str, t: torch.Tensor) -> int:
@@ -398,13 +414,8 @@ def _code(name: str, t: torch.Tensor) -> int:
     return code
 
 
-def _int8(name: str, t: torch.Tensor) -> None:
-    if t.dtype is not torch.int8:
-        raise ValueError(f"{name} must be int8, not {t.dtype}")
-
-
 def _vector(name: str, t: torch.Tensor, K: int) -> int:
-    if t.dtype is not _F32 or t.shape != (K,) or (K > 1 and t.stride(0) != 1):
+    if t.dtype is not _F32 or t.shape != (K,) or (t.stride(0) != 1 and K > 1):
         raise ValueError(f"{name} must be a contiguous fp32 [{K}]")
     return t.data_ptr()
 
@@ -414,31 +425,54 @@ def _per_batch(name: str, t: torch.Tensor, T: int, S: int, K: int) -> int:
     if t.dim() == 1:
         _vector(name, t, K)
         return 0
-    if t.dtype is not _F32 or t.dim() != 2:
-        raise ValueError(f"{name} must be fp32 [B, {K}] or [{K}]")
-    B, n = t.shape
-    stride, step = t.stride()
-    if n != K or (step != 1 and K > 1):
+    try:
+        (B, n), (stride, step) = t.shape, t.stride()
+    except ValueError:
+        raise ValueError(f"{name} must be fp32 [B, {K}] or [{K}]") from None
+    if t.dtype is not _F32 or n != K or (step != 1 and K > 1):
         raise ValueError(f"{name} must be fp32 [B, {K}] or [{K}] with contiguous rows")
     if B * S < T:
         raise ValueError(f"{name} has {B} rows for {T} tokens of {S} per stream")
     return stride
 
 
+def _quant_rows(x, q, scale):
+    dev = x.get_device()
+    if q.get_device() != dev or scale.get_device() != dev:
+        raise _apart(x, q, scale)
+    _current(dev)
+    if q.dtype is not _I8:
+        raise ValueError(f"q must be int8, not {q.dtype}")
+    T, K = _matrix("x", x)
+    return L.QuantRowsDesc(T, K, _code("x", x), x.data_ptr(), _rows("x", x, T, K), q.data_ptr(),
+                           _rows("q", q, T, K), _vector("scale", scale, T)), dev
+
+
 def quant_rows_desc(*, x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> L.QuantRowsDesc:
     """Rows x [T, K] (bf16 or fp32) to int8 q [T, K] and fp32 scale [T]."""
-    _here(x, q, scale)
-    _int8("q", q)
-    shape = _rows_of("x", x)
-    T, K = shape
-    return L.QuantRowsDesc(T, K, _code("x", x), x.data_ptr(), _rows("x", x, shape), q.data_ptr(),
-                           _rows("q", q, shape), _vector("scale", scale, T))
+    return _quant_rows(x, q, scale)[0]
 
 
 def quant_rows(*, x, q, scale) -> None:
     """int8 rows with one scale per row: scale = absmax / 127, q = rne(x / scale)."""
-    d = quant_rows_desc(x=x, q=q, scale=scale)
-    L.call("rfx_quant_rows", ctypes.byref(d), _stream())
+    _launch("rfx_quant_rows", *_quant_rows(x, q, scale))
+
+
+def _linear_i8(w, w_scale, x, x_scale, y, epilogue, bias):
+    dev = x.get_device()
+    if w.get_device() != dev or y.get_device() != dev or x_scale.get_device() != dev or (
+            w_scale.get_device() != dev) or (bias is not None and bias.get_device() != dev):
+        raise _apart(w, w_scale, x, x_scale, y, bias)
+    _current(dev)
+    if x.dtype is not _I8 or w.dtype is not _I8:
+        raise ValueError(f"x and w must be int8, not {x.dtype} and {w.dtype}")
+    T, K = _matrix("x", x)
+    O = _matrix("w", w)[0]
+    F = O // 2 if epilogue == L.RFX_EPI_GEGLU else O
+    return L.LinearI8Desc(T, O, K, epilogue, _code("y", y), x.data_ptr(), _rows("x", x, T, K, 16),
+                          _vector("x_scale", x_scale, T), w.data_ptr(), _rows("w", w, O, K, 16),
+                          _vector("w_scale", w_scale, O), None if bias is None else _vector("bias", bias, O),
+                          y.data_ptr(), _rows("y", y, T, F)), dev
 
 
 def linear_i8_desc(*, w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, y: torch.Tensor,
@@ -446,22 +480,60 @@ def linear_i8_desc(*, w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, x
     """y = act((x_scale * w_scale) * (x @ w^T) + bias): int8 x [T, K] and
     w [O, K] whose rows begin on 16-byte boundaries, fp32 scales [T] and [O],
     y [T, O] bf16 or fp32 ([T, O/2] with RFX_EPI_GEGLU, w = [Wgate; Wup])."""
-    _here(w, w_scale, x, x_scale, y, bias)
-    _int8("x", x)
-    _int8("w", w)
-    shape = _rows_of("x", x)
-    T, K = shape
-    O = _rows_of("w", w)[0]
-    return L.LinearI8Desc(T, O, K, epilogue, _code("y", y), x.data_ptr(), _rows("x", x, shape, 16),
-                          _vector("x_scale", x_scale, T), w.data_ptr(), _rows("w", w, (O, K), 16),
-                          _vector("w_scale", w_scale, O), None if bias is None else _vector("bias", bias, O),
-                          y.data_ptr(), _rows("y", y, (T, O // 2 if epilogue == L.RFX_EPI_GEGLU else O)))
+    return _linear_i8(w, w_scale, x, x_scale, y, epilogue, bias)[0]
 
 
 def linear_i8(*, w, w_scale, x, x_scale, y, epilogue=L.RFX_EPI_STORE, bias=None) -> None:
     """Linear layer in 8-bit integers with a scale per token and per output channel."""
-    d = linear_i8_desc(w=w, w_scale=w_scale, x=x, x_scale=x_scale, y=y, epilogue=epilogue, bias=bias)
-    L.call("rfx_linear_i8", ctypes.byref(d), _stream())
+    _launch("rfx_linear_i8", *_linear_i8(w, w_scale, x, x_scale, y, epilogue, bias))
+
+
+def _block_norm(h, S, y, post_w, gate, residual_scale, h_out, norm_a1, norm_a2, norm_b2, eps, z, z_q, z_scale):
+    dev = _current(h.get_device())
+    T, K = _matrix("h", h)
+    if S < 1:
+        raise ValueError("S (tokens per stream) must be at least 1")
+    dtype = h.dtype
+    y_at = ldy = post_at = gate_at = gate_ld = ho_at = ldho = a1_at = a2_at = b2_at = ab = 0
+    z_at = ldz = q_at = ldq = s_at = 0
+    apart = wrong = False
+    if y is not None:
+        apart, wrong = y.get_device() != dev, y.dtype is not dtype
+        y_at, ldy = y.data_ptr(), _rows("y", y, T, K)
+    if h_out is not None:
+        apart, wrong = apart or h_out.get_device() != dev, wrong or h_out.dtype is not dtype
+        ho_at, ldho = h_out.data_ptr(), _rows("h_out", h_out, T, K)
+    if z is not None:
+        apart, wrong = apart or z.get_device() != dev, wrong or z.dtype is not dtype
+        z_at, ldz = z.data_ptr(), _rows("z", z, T, K)
+    if wrong:
+        raise ValueError("h, y, h_out and z have one dtype")
+    if post_w is not None:
+        apart, post_at = apart or post_w.get_device() != dev, _vector("post_w", post_w, K)
+    if gate is not None:
+        apart, gate_at, gate_ld = apart or gate.get_device() != dev, gate.data_ptr(), _per_batch("gate", gate, T, S, K)
+    if norm_a1 is not None:
+        apart, a1_at = apart or norm_a1.get_device() != dev, _vector("norm_a1", norm_a1, K)
+    if norm_a2 is not None:
+        apart, a2_at = apart or norm_a2.get_device() != dev, norm_a2.data_ptr()
+        ab = _per_batch("norm_a2", norm_a2, T, S, K)
+    if norm_b2 is not None:
+        apart, b2_at = apart or norm_b2.get_device() != dev, norm_b2.data_ptr()
+        stride = _per_batch("norm_b2", norm_b2, T, S, K)
+        if norm_a2 is not None and stride != ab and T > S:
+            raise ValueError("norm_a2 and norm_b2 must have one batch stride")
+        ab = stride
+    if z_q is not None:
+        if z_q.dtype is not _I8:
+            raise ValueError(f"z_q must be int8, not {z_q.dtype}")
+        apart, q_at, ldq = apart or z_q.get_device() != dev, z_q.data_ptr(), _rows("z_q", z_q, T, K)
+    if z_scale is not None:
+        apart, s_at = apart or z_scale.get_device() != dev, _vector("z_scale", z_scale, T)
+    if apart:
+        raise _apart(h, y, post_w, gate, h_out, norm_a1, norm_a2, norm_b2, z, z_q, z_scale)
+    return L.BlockNormDesc(T, K, S if S <= 0x7FFFFFFF else 0x7FFFFFFF, _code("h", h), h.data_ptr(),
+                           _rows("h", h, T, K), y_at, ldy, post_at, gate_at, gate_ld, residual_scale, ho_at, ldho,
+                           a1_at, a2_at, b2_at, ab, eps, z_at, ldz, q_at, ldq, s_at), dev
 
 
 def block_norm_desc(*, h: torch.Tensor, S: int, y: torch.Tensor | None = None, post_w=None, gate=None,
@@ -472,40 +544,16 @@ def block_norm_desc(*, h: torch.Tensor, S: int, y: torch.Tensor | None = None, p
     tokens per stream; post_w and norm_a1 [K], gate, norm_a2 and norm_b2
     [B, K] or [K] (fp32).  h_out takes the updated stream (h for in place),
     z or z_q and z_scale the next norm's output."""
-    _here(h, y, post_w, gate, h_out, norm_a1, norm_a2, norm_b2, z, z_q, z_scale)
-    shape = _rows_of("h", h)
-    T, K = shape
-    if S < 1:
-        raise ValueError("S (tokens per stream) must be at least 1")
-    dtype = h.dtype
-    if (y is not None and y.dtype is not dtype) or (h_out is not None and h_out.dtype is not dtype) or (
-            z is not None and z.dtype is not dtype):
-        raise ValueError("h, y, h_out and z have one dtype")
-    if z_q is not None:
-        _int8("z_q", z_q)
-    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    ab = 0 if norm_a2 is None else _per_batch("norm_a2", norm_a2, T, S, K)
-    if norm_b2 is not None:
-        stride = _per_batch("norm_b2", norm_b2, T, S, K)
-        if norm_a2 is not None and stride != ab and T > S:
-            raise ValueError("norm_a2 and norm_b2 must have one batch stride")
-        ab = stride
-    return L.BlockNormDesc(
-        T, K, S if S <= 0x7FFFFFFF else 0x7FFFFFFF, _code("h", h), h.data_ptr(), _rows("h", h, shape),
-        at(y), 0 if y is None else _rows("y", y, shape),
-        0 if post_w is None else _vector("post_w", post_w, K),
-        at(gate), 0 if gate is None else _per_batch("gate", gate, T, S, K), residual_scale,
-        at(h_out), 0 if h_out is None else _rows("h_out", h_out, shape),
-        0 if norm_a1 is None else _vector("norm_a1", norm_a1, K), at(norm_a2), at(norm_b2), ab, eps,
-        at(z), 0 if z is None else _rows("z", z, shape), at(z_q), 0 if z_q is None else _rows("z_q", z_q, shape),
-        0 if z_scale is None else _vector("z_scale", z_scale, T))
+    return _block_norm(h, S, y, post_w, gate, residual_scale, h_out, norm_a1, norm_a2, norm_b2, eps, z, z_q,
+                       z_scale)[0]
 
 
-def block_norm(**kw) -> None:
+def block_norm(*, h, S, y=None, post_w=None, gate=None, residual_scale=1.0, h_out=None, norm_a1=None, norm_a2=None,
+               norm_b2=None, eps=1e-6, z=None, z_q=None, z_scale=None) -> None:
     """The norm of a block's output, its gate and residual scale, the residual
     add and the next block's norm (as it is, or as int8 rows), in one pass."""
-    d = block_norm_desc(**kw)
-    L.call("rfx_block_norm", ctypes.byref(d), _stream())
+    _launch("rfx_block_norm", *_block_norm(h, S, y, post_w, gate, residual_scale, h_out, norm_a1, norm_a2, norm_b2,
+                                           eps, z, z_q, z_scale))
 
 
 def rope_frequencies(rot_dim: int, theta: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
@@ -548,7 +596,7 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, *, scaling: str = "no
 def _heads(name: str, t: torch.Tensor, x: torch.Tensor, shape: tuple) -> tuple:
     """Address and strides (b, h, s) of an output of `rope`."""
     if t.dtype is not x.dtype or t.shape != shape:
-        raise ValueError(f"{name} must be {x.dtype} {list(shape)}")
+        raise ValueError(f"{name} must be {x.dtype} {list(shape)}, not {t.dtype} {list(t.shape)}")
     sb, sh, ss, sd = t.stride()
     B, H, S, D = shape
     if sd != 1 or (sb < D and B > 1) or (sh < D and H > 1) or (ss < D and S > 1):
@@ -556,18 +604,16 @@ def _heads(name: str, t: torch.Tensor, x: torch.Tensor, shape: tuple) -> tuple:
     return t.data_ptr(), sb, sh, ss
 
 
-def rope_desc(*, x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, q_out: torch.Tensor,
-              k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None, pairs: int = L.RFX_ROPE_HALF,
-              magnitude: float = 1.0) -> L.RopeDesc:
-    """x [B*S, (Hq + Hkv + Hkv) * D] QKV rows (Hkv once less without v_out);
-    q_out [B, Hq, S, D], k_out and v_out [B, Hkv, S, D] views of any strides
-    with contiguous D (also over x itself); positions int32 [B*S]; inv_freq
-    fp64 [rot_dim / 2]."""
-    _here(x, positions, inv_freq, q_out, k_out, v_out)
-    if q_out.dim() != 4:
-        raise ValueError("q_out must be [B, Hq, S, D]")
-    shape = q_out.shape
-    B, Hq, S, D = shape
+def _rope(x, positions, inv_freq, q_out, k_out, v_out, pairs, magnitude):
+    dev = x.get_device()
+    if positions.get_device() != dev or inv_freq.get_device() != dev or q_out.get_device() != dev or (
+            k_out is not None and k_out.get_device() != dev) or (v_out is not None and v_out.get_device() != dev):
+        raise _apart(x, positions, inv_freq, q_out, k_out, v_out)
+    _current(dev)
+    try:
+        shape = B, Hq, S, D = q_out.shape
+    except ValueError:
+        raise ValueError(f"q_out must be [B, Hq, S, D], not {list(q_out.shape)}") from None
     T = B * S
     if positions.dtype is not torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
         raise ValueError(f"positions must be a contiguous int32 [{T}]")
@@ -576,7 +622,7 @@ def rope_desc(*, x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
     k = v = (0, 0, 0, 0)
     heads, Hkv = Hq, 0
     if k_out is not None:
-        Hkv = k_out.shape[1]
+        Hkv = k_out.shape[1] if k_out.dim() == 4 else 0
         kv = (B, Hkv, S, D)
         k = _heads("k_out", k_out, x, kv)
         heads += Hkv
@@ -586,14 +632,23 @@ def rope_desc(*, x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
     elif v_out is not None:
         raise ValueError("v_out goes with k_out")
     return L.RopeDesc(B, S, Hq, Hkv, D, 2 * inv_freq.shape[0], pairs, _code("x", x), x.data_ptr(),
-                      _rows("x", x, (T, heads * D), 8), positions.data_ptr(), inv_freq.data_ptr(), magnitude,
-                      *_heads("q_out", q_out, x, shape), *k, *v)
+                      _rows("x", x, T, heads * D, 8), positions.data_ptr(), inv_freq.data_ptr(), magnitude,
+                      *_heads("q_out", q_out, x, shape), *k, *v), dev
 
 
-def rope(**kw) -> None:
+def rope_desc(*, x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, q_out: torch.Tensor,
+              k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None, pairs: int = L.RFX_ROPE_HALF,
+              magnitude: float = 1.0) -> L.RopeDesc:
+    """x [B*S, (Hq + Hkv + Hkv) * D] QKV rows (Hkv once less without v_out);
+    q_out [B, Hq, S, D], k_out and v_out [B, Hkv, S, D] views of any strides
+    with contiguous D (also over x itself); positions int32 [B*S]; inv_freq
+    fp64 [rot_dim / 2]."""
+    return _rope(x, positions, inv_freq, q_out, k_out, v_out, pairs, magnitude)[0]
+
+
+def rope(*, x, positions, inv_freq, q_out, k_out=None, v_out=None, pairs=L.RFX_ROPE_HALF, magnitude=1.0) -> None:
     """Rotary positions on QKV rows, split into q, k and v on the way."""
-    d = rope_desc(**kw)
-    L.call("rfx_rope", ctypes.byref(d), _stream())
+    _launch("rfx_rope", *_rope(x, positions, inv_freq, q_out, k_out, v_out, pairs, magnitude))
 
 
 def device_status() -> int:
