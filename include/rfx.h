@@ -496,7 +496,7 @@ int rfx_vit_attention(const rfx_vit_attn_desc* desc, void* stream);
  * that holds a NaN or an infinity gets that as its scale and q = 0, so that
  * what is computed from it is NaN.  1 <= K <= 16384, any alignment of
  * elements; 16-byte aligned rows (8-byte for q) with K % 8 == 0 take wide
- * accesses. */
+ * accesses.  x, q and scale must not share memory (refused). */
 typedef struct rfx_quant_rows_desc {
   int T, K;
   int in_dtype;  /* RFX_DTYPE_BF16 or RFX_DTYPE_F32 */
@@ -515,7 +515,7 @@ int rfx_quant_rows(const rfx_quant_rows_desc* desc, void* stream);
  * rows and then O/2 up rows as they are ([Wgate; Wup], no repacking) and
  * y[t][f] = gelu_tanh(gate_f) * up_f, O/2 columns.  Any T and O up to 2^30;
  * rows of x and w begin on 16-byte boundaries (pad ldx / ldw; the padding is
- * not read).  No workspace; calls on several streams do not disturb each other.
+ * not read).  y shares no memory with an input (refused).  No workspace; calls on several streams do not disturb each other.
  * Run a shape once before capturing it (the first call sets the kernel's
  * shared-memory size). */
 typedef struct rfx_linear_i8_desc {
@@ -543,7 +543,8 @@ int rfx_linear_i8(const rfx_linear_i8_desc* desc, void* stream);
  * The next norm reads h' as rounded.  z goes to `z` (dtype) or, as int8 rows
  * with the scheme of rfx_quant_rows, to z_q / z_scale; with neither, only the
  * stream is updated; with y == NULL only the norm is computed (h' = h).
- * h_out may be h and z may be h or y (same stride).  1 <= K <= 16384. */
+ * h_out may be h and z may be h or y (same stride); any other overlap of h, y
+ * and the outputs is refused.  1 <= K <= 16384. */
 typedef struct rfx_block_norm_desc {
   int T, K, tokens_per_batch;
   int dtype;     /* of h, y, h_out and z: RFX_DTYPE_BF16 or RFX_DTYPE_F32 */
@@ -578,7 +579,7 @@ int rfx_block_norm(const rfx_block_norm_desc* desc, void* stream);
  * (RFX_ROPE_HALF) or (2i, 2i + 1) (RFX_ROPE_INTERLEAVED) and turns by
  * positions[b*S + s] * inv_freq[i] radians, times `magnitude`; dims past
  * rot_dim and v are copied.  An output lies over x exactly (each element at its
- * own input's address) or apart from it.  inv_freq is fp64 on the device (positions far
+ * own input's address) or apart from it; else it is refused.  inv_freq is fp64 on the device (positions far
  * beyond fp32's reach keep their angle), scaled by the caller for long
  * contexts.  head_dim <= 256, rot_dim even. */
 #define RFX_ROPE_HALF 0

@@ -774,6 +774,12 @@ int validate_linear_i8(const rfx_linear_i8_desc& d) {
   if (d.ldy < out_cols(d) || !al(d.y, d.out_dtype == kDtypeBF16 ? 2 : 4) || !al(d.x_scale, 4) || !al(d.w_scale, 4) ||
       !al(d.bias, 4))
     return set_error(RFX_E_INVAL, "rfx_linear_i8: ldy below the output's columns, or a misaligned pointer");
+  const long esz = d.out_dtype == kDtypeBF16 ? 2 : 4;
+  const Rows y{d.y, d.T, d.ldy * esz, out_cols(d) * esz};
+  if (rows_shared(y, {d.x, d.T, d.ldx, d.K}) || rows_shared(y, {d.w, d.O, d.ldw, d.K}) ||
+      rows_shared(y, {d.x_scale, 1, 0, d.T * 4l}) || rows_shared(y, {d.w_scale, 1, 0, d.O * 4l}) ||
+      rows_shared(y, {d.bias, 1, 0, d.O * 4l}))
+    return set_error(RFX_E_INVAL, "rfx_linear_i8: y shares memory with an input");
   if ((static_cast<long>(d.T) / kTileM + 1) * (d.O / 32 + 1) > 0x7fffffffL / 8)
     return set_error(RFX_E_INVAL, "rfx_linear_i8: too many output tiles (T=%d O=%d)", d.T, d.O);
   return RFX_OK;

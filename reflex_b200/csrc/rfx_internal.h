@@ -54,6 +54,17 @@ int launch_kernel_cluster(const void* func, dim3 grid, dim3 block, size_t smem, 
 // Whether a cluster of cluster_x CTAs of this kernel can be resident at once.
 bool cluster_fits(const void* func, dim3 grid, int threads, int smem, int cluster_x);
 
+// Rows in memory, in bytes: where they begin, how many, from row to row, of one.
+struct Rows {
+  const void* p;
+  long n, pitch, width;
+};
+// Whether two matrices share memory (false with a null pointer).  Columns of one
+// wider buffer do not; rows of different pitches that interleave count as shared.
+bool rows_shared(Rows a, Rows b);
+// Whether b is a, element for element: what an operator in place may be given.
+bool rows_same(const Rows& a, const Rows& b);
+
 // Clusters of cluster_x CTAs of this kernel that can be resident at once (memoised; 0 when no device answers).
 int max_active_clusters(const void* func, int threads, int smem, int cluster_x);
 

@@ -290,6 +290,23 @@ const void* rope_ptr(bool half, bool vec) {
 
 }  // namespace
 
+// Whether an output whose first head is head `at` of x may be written: over x
+// element for element, or apart from it.
+static bool rope_place_ok(const rfx_rope_desc& d, const void* out, long heads, long at, int H, long sb, long sh, long ss) {
+  if (!out) return true;
+  const long esz = d.dtype == kDtypeBF16 ? 2 : 4;
+  const bool rows = (d.S == 1 || ss == d.ldx) && (d.B == 1 || sb == d.S * d.ldx);  // token rows at x's pitch
+  const uintptr_t x = reinterpret_cast<uintptr_t>(d.x), o = reinterpret_cast<uintptr_t>(out);
+  if (rows && (H == 1 || sh == d.head_dim) && o == x + at * d.head_dim * esz) return true;
+  const long T = static_cast<long>(d.B) * d.S;
+  const Rows in{d.x, T, d.ldx * esz, heads * d.head_dim * esz};
+  if (rows && sh >= 0) return !rows_shared(in, {out, T, d.ldx * esz, ((H - 1) * sh + d.head_dim) * esz});
+  __int128 lo = o, hi = o + static_cast<__int128>(d.head_dim) * esz;
+  const long n[3] = {d.B, H, d.S}, stride[3] = {sb, sh, ss};
+  for (int i = 0; i < 3; ++i) (stride[i] < 0 ? lo : hi) += static_cast<__int128>(n[i] - 1) * stride[i] * esz;
+  return hi <= x || lo >= x + (static_cast<__int128>(T - 1) * d.ldx + heads * d.head_dim) * esz;
+}
+
 int validate_rope(const rfx_rope_desc& d) {
   if (d.B < 0 || d.S < 0 || static_cast<long>(d.B) * d.S > 0x7fffffffL - 1024)
     return set_error(RFX_E_INVAL, "rfx_rope: bad B/S (B=%d S=%d)", d.B, d.S);
@@ -311,6 +328,10 @@ int validate_rope(const rfx_rope_desc& d) {
   if (!al(d.x, esz) || !al(d.q_out, esz) || !al(d.k_out, esz) || !al(d.v_out, esz) || !al(d.positions, 4) ||
       !al(d.inv_freq, 8))
     return set_error(RFX_E_INVAL, "rfx_rope: misaligned pointer");
+  if (!rope_place_ok(d, d.q_out, heads, 0, d.num_q_heads, d.qs_b, d.qs_h, d.qs_s) ||
+      !rope_place_ok(d, d.k_out, heads, d.num_q_heads, d.num_kv_heads, d.ks_b, d.ks_h, d.ks_s) ||
+      !rope_place_ok(d, d.v_out, heads, d.num_q_heads + d.num_kv_heads, d.num_kv_heads, d.vs_b, d.vs_h, d.vs_s))
+    return set_error(RFX_E_INVAL, "rfx_rope: an output lies across x (over its own heads exactly, or apart from x)");
   return RFX_OK;
 }
 

@@ -556,6 +556,10 @@ int validate_quant_rows(const rfx_quant_rows_desc& d) {
     return set_error(RFX_E_INVAL, "rfx_quant_rows: null pointer or a row stride below K");
   if (!aligned(d.x, elem_size(d.in_dtype)) || !aligned(d.scale, 4))
     return set_error(RFX_E_INVAL, "rfx_quant_rows: misaligned pointer");
+  const long esz = elem_size(d.in_dtype);
+  const Rows x{d.x, d.T, d.ldx * esz, d.K * esz}, q{d.q, d.T, d.ldq, d.K}, scale{d.scale, 1, 0, d.T * 4l};
+  if (rows_shared(q, x) || rows_shared(scale, x) || rows_shared(scale, q))
+    return set_error(RFX_E_INVAL, "rfx_quant_rows: x, q and scale share memory");
   return RFX_OK;
 }
 
@@ -578,7 +582,7 @@ int validate_block_norm(const rfx_block_norm_desc& d) {
   if (d.dtype != kDtypeBF16 && d.dtype != kDtypeF32)
     return set_error(RFX_E_INVAL, "rfx_block_norm: dtype must be bf16 or f32");
   if (d.T == 0) return RFX_OK;
-  const int esz = elem_size(d.dtype);
+  const long esz = elem_size(d.dtype);
   if (!d.h || d.ldh < d.K || (d.y && d.ldy < d.K) || (d.h_out && d.ldho < d.K) || (d.z && d.ldz < d.K) ||
       (d.z_q && d.ldzq < d.K))
     return set_error(RFX_E_INVAL, "rfx_block_norm: null h or a row stride below K");
@@ -589,12 +593,17 @@ int validate_block_norm(const rfx_block_norm_desc& d) {
   if (!d.y && !d.z && !d.z_q)
     return set_error(RFX_E_INVAL, "rfx_block_norm: nothing to compute (no y and no norm output)");
   if (!d.z_q != !d.z_scale) return set_error(RFX_E_INVAL, "rfx_block_norm: z_q and z_scale come together");
-  if ((d.h_out == d.h && d.h_out && d.ldho != d.ldh) || (d.z && d.z == d.h_out) || (d.z == d.h && d.z && d.ldz != d.ldh) ||
-      (d.z && d.z == d.y && d.ldz != d.ldy) || (d.h_out && d.h_out == d.y))
-    return set_error(RFX_E_INVAL, "rfx_block_norm: outputs overlap (in place only over h, or z over y, at the same stride)");
+  const long w = static_cast<long>(d.K) * esz;
+  const Rows h{d.h, d.T, d.ldh * esz, w}, y{d.y, d.T, d.ldy * esz, w}, ho{d.h_out, d.T, d.ldho * esz, w};
+  const Rows z{d.z, d.T, d.ldz * esz, w}, q{d.z_q, d.T, d.ldzq, d.K}, zs{d.z_scale, 1, 0, d.T * 4l};
+  if ((!rows_same(ho, h) && rows_shared(ho, h)) || rows_shared(ho, y) || (!rows_same(z, h) && rows_shared(z, h)) ||
+      (!rows_same(z, y) && rows_shared(z, y)) || rows_shared(z, ho) || rows_shared(q, h) || rows_shared(q, y) ||
+      rows_shared(q, ho) || rows_shared(zs, h) || rows_shared(zs, y) || rows_shared(zs, ho) || rows_shared(zs, q))
+    return set_error(RFX_E_INVAL, "rfx_block_norm: outputs overlap (in place only h_out or z over h, or z over y, at the same stride)");
   if (!d.z && !d.z_q && (d.norm_a1 || d.norm_a2 || d.norm_b2))
     return set_error(RFX_E_INVAL, "rfx_block_norm: norm vectors without a norm output");
-  if (!aligned(d.h, esz) || !aligned(d.y, esz) || !aligned(d.h_out, esz) || !aligned(d.z, esz) ||
+  if (!aligned(d.h, elem_size(d.dtype)) || !aligned(d.y, elem_size(d.dtype)) || !aligned(d.h_out, elem_size(d.dtype)) ||
+      !aligned(d.z, elem_size(d.dtype)) ||
       !aligned(d.post_w, 4) || !aligned(d.gate, 4) || !aligned(d.norm_a1, 4) || !aligned(d.norm_a2, 4) ||
       !aligned(d.norm_b2, 4) || !aligned(d.z_scale, 4))
     return set_error(RFX_E_INVAL, "rfx_block_norm: misaligned pointer");

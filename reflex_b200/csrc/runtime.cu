@@ -155,6 +155,23 @@ bool cluster_fits(const void* func, dim3 grid, int threads, int smem, int cluste
   return ok;
 }
 
+bool rows_shared(Rows a, Rows b) {
+  if (!a.p || !b.p) return false;
+  using wide = __int128;
+  const wide pa = static_cast<wide>(reinterpret_cast<uintptr_t>(a.p)), pb = static_cast<wide>(reinterpret_cast<uintptr_t>(b.p));
+  const wide ea = pa + static_cast<wide>(a.n - 1) * a.pitch + a.width, eb = pb + static_cast<wide>(b.n - 1) * b.pitch + b.width;
+  if (ea <= pb || eb <= pa) return false;
+  if (a.n == 1) a.pitch = b.pitch;
+  if (b.n == 1) b.pitch = a.pitch;
+  if (a.pitch != b.pitch || a.pitch <= 0) return true;
+  const wide off = ((pb - pa) % a.pitch + a.pitch) % a.pitch;
+  return off < a.width || off + b.width > a.pitch;
+}
+
+bool rows_same(const Rows& a, const Rows& b) {
+  return a.p == b.p && a.n == b.n && a.width == b.width && (a.pitch == b.pitch || a.n == 1);
+}
+
 int max_active_clusters(const void* func, int threads, int smem, int cluster_x) {
   struct Entry {
     const void* func;

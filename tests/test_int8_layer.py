@@ -45,11 +45,12 @@ def test_null_descriptor_is_rejected(name):
 
 
 def quant():
-    return _lib.QuantRowsDesc(4, 64, _lib.RFX_DTYPE_BF16, A, 64, A, 64, A)
+    return _lib.QuantRowsDesc(4, 64, _lib.RFX_DTYPE_BF16, A, 64, 2 * A, 64, 3 * A)
 
 
 def linear():
-    return _lib.LinearI8Desc(4, 64, 64, _lib.RFX_EPI_STORE, _lib.RFX_DTYPE_BF16, A, 64, A, A, 64, A, None, A, 64)
+    return _lib.LinearI8Desc(4, 64, 64, _lib.RFX_EPI_STORE, _lib.RFX_DTYPE_BF16, A, 64, 2 * A, 3 * A, 64, 4 * A, None,
+                             5 * A, 64)
 
 
 def norm():
@@ -65,7 +66,7 @@ def rope():
     d = _lib.RopeDesc()
     d.B, d.S, d.num_q_heads, d.num_kv_heads, d.head_dim, d.rot_dim = 1, 4, 2, 1, 64, 64
     d.pairs, d.dtype, d.magnitude = _lib.RFX_ROPE_HALF, _lib.RFX_DTYPE_BF16, 1.0
-    d.x = d.positions = d.inv_freq = d.q_out = d.k_out = d.v_out = A
+    d.x, d.positions, d.inv_freq, d.q_out, d.k_out, d.v_out = A, 2 * A, 3 * A, 4 * A, 5 * A, 6 * A
     d.ldx = 4 * 64
     return d
 
@@ -146,6 +147,69 @@ def test_no_rows_is_a_no_op(entry, make, change):
         assert getattr(lib, "rfx_plan_add_" + ENTRIES[entry])(plan, ctypes.byref(d)) == _lib.RFX_OK
         n = ctypes.c_int(-1)
         assert lib.rfx_plan_num_launches(plan, ctypes.byref(n)) == _lib.RFX_OK and n.value == 0
+    finally:
+        lib.rfx_plan_destroy(plan)
+
+
+ROW = 4 * 64 * 2  # bytes of a row of rope()'s x: 2 q heads, one k, one v
+OVER_X = dict(q_out=A, qs_b=4 * 256, qs_h=64, qs_s=256, k_out=A + 256, ks_b=4 * 256, ks_h=64, ks_s=256,
+              v_out=A + 384, vs_b=4 * 256, vs_h=64, vs_s=256)
+PLACES = [  # which memory outputs and inputs may share
+    (quant, {}, True),
+    (quant, dict(q=A), False),                                        # rows of half the pitch over x
+    (quant, dict(q=A + 511), False), (quant, dict(q=A + 512), True),  # its last byte; right behind it
+    (quant, dict(q=A - 255), False), (quant, dict(q=A - 256), True),
+    (quant, dict(scale=A + 256), False), (quant, dict(scale=2 * A + 252), False),
+    (quant, dict(ldx=96, q=A + 128, ldq=192), True),                  # the free columns of x's own rows
+    (quant, dict(ldx=95, q=A + 128, ldq=190), False),                 # two bytes too few of them
+    (quant, dict(ldx=96, q=A + 127, ldq=192), False), (quant, dict(ldx=96, q=A + 128, ldq=191), False),
+    (quant, dict(T=1, q=A + 128), True), (quant, dict(T=1, q=A + 127), False),
+    (linear, {}, True),
+    (linear, dict(y=A), False), (linear, dict(y=3 * A + 64), False), (linear, dict(y=2 * A), False),
+    (linear, dict(y=4 * A + 252), False), (linear, dict(y=4 * A + 256), True), (linear, dict(bias=5 * A), False),
+    (linear, dict(bias=5 * A + 512), True), (linear, dict(ldx=192, y=A + 64, ldy=96), True),
+    (norm, {}, True),
+    (norm, dict(h_out=A), True), (norm, dict(z=A), True), (norm, dict(z=2 * A), True),
+    (norm, dict(h_out=A, z=A), False), (norm, dict(h_out=2 * A), False), (norm, dict(h_out=A + 128), False),
+    (norm, dict(z=A, ldz=72), False), (norm, dict(z=2 * A + 128), False), (norm, dict(z=3 * A + 2), False),
+    (norm, dict(z=None, z_q=5 * A, z_scale=6 * A), True), (norm, dict(z=None, z_q=A, z_scale=6 * A), False),
+    (norm, dict(z=None, z_q=2 * A + 511, z_scale=6 * A), False), (norm, dict(z=None, z_q=3 * A, z_scale=6 * A), False),
+    (norm, dict(z=None, z_q=5 * A, z_scale=5 * A), False), (norm, dict(z=None, z_q=5 * A, z_scale=3 * A), False),
+    (rope, {}, True),
+    (rope, OVER_X, True),
+    (rope, dict(OVER_X, k_out=A), False),                             # k over the q heads
+    (rope, dict(OVER_X, q_out=A + 128), False), (rope, dict(OVER_X, qs_h=128), False),
+    (rope, dict(OVER_X, qs_s=128), False), (rope, dict(OVER_X, vs_s=264), False),
+    (rope, dict(q_out=A, qs_b=512, qs_h=256, qs_s=64), False),        # head-major over x
+    (rope, dict(q_out=A + 4 * ROW, qs_b=512, qs_h=256, qs_s=64), True),
+    (rope, dict(q_out=A + 4 * ROW - 2, qs_b=512, qs_h=256, qs_s=64), False),
+    (rope, dict(q_out=A - 1024, qs_b=512, qs_h=256, qs_s=64), True),
+    (rope, dict(q_out=A - 1022, qs_b=512, qs_h=256, qs_s=64), False),
+    (rope, dict(ldx=384, q_out=A + 512, qs_b=4 * 384, qs_h=64, qs_s=384), True),  # the free columns of x's rows
+    (rope, dict(ldx=384, q_out=A + 510, qs_b=4 * 384, qs_h=64, qs_s=384), False),
+    (rope, dict(q_out=A + 4 * ROW, qs_h=-256, qs_s=64), False),       # strides that lead back into x
+]
+
+
+@pytest.mark.parametrize("make,change,fine", PLACES)
+def test_shared_memory_is_in_place_or_refused(make, change, fine):
+    """An output lies over an input exactly where the operator may work in
+    place, or apart from it; what reads and writes across rows is refused."""
+    lib = _lib.load()
+    d = make()
+    for k, v in change.items():
+        setattr(d, k, v)
+    name = {"quant": "quant_rows", "linear": "linear_i8", "norm": "block_norm", "rope": "rope"}[make.__name__]
+    plan = ctypes.c_void_p()
+    assert lib.rfx_plan_create(ctypes.byref(plan)) == _lib.RFX_OK
+    try:
+        rc = getattr(lib, "rfx_plan_add_" + name)(plan, ctypes.byref(d))
+        if name == "linear_i8" and fine:  # without a driver its tensor maps cannot be made
+            assert rc != _lib.RFX_E_INVAL or b"shares memory" not in lib.rfx_last_error()
+        else:
+            assert rc == (_lib.RFX_OK if fine else _lib.RFX_E_INVAL)
+        if not fine:
+            assert any(w in lib.rfx_last_error() for w in (b"share", b"overlap", b"lies across"))
     finally:
         lib.rfx_plan_destroy(plan)
 
