@@ -5,14 +5,18 @@
 // changes a result: the only roundings are the int -> fp32 conversion, the two
 // scales, bias and activation in fp32, and one rounding to the output type.
 //
-// Tokens are the MMA's M (a TMEM lane is a token, so a thread of the epilogue
-// holds consecutive outputs of one row) and weight rows its N.  Operands are
-// K-major rows of 128 bytes per K step, staged by TMA with 128-byte swizzle;
-// what lies past T, O or K is filled with zeros by the copy and not stored.
-// For GeGLU a tile's N is half gate rows and half up rows of [Wgate; Wup].
+// Three forms, whose results are the same bits: CTA-pair tiles of 256 tokens
+// (tokens on the MMA's M side: a TMEM lane is a token, and a thread of the
+// epilogue holds consecutive outputs of one row), tiles of 128 weight rows (the
+// weights on the M side) for up to 128 tokens, and the integer units for up to
+// 4.  The tiles' operands are K-major rows of 128 bytes per K step, staged by TMA
+// with 128-byte swizzle; what lies past T, O or K is filled with zeros by the
+// copy or not copied, and not stored.  For GeGLU half of a tile's weight rows
+// are gate rows and half up rows of [Wgate; Wup].
 #include "rfx_internal.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace rfx {
 namespace {
@@ -66,6 +70,9 @@ __device__ __forceinline__ float activate(float v) {
   if (ACT == kActGelu) return gelu_i8(v);
   return v;
 }
+
+__device__ __forceinline__ void put1(float* y, float v) { *y = v; }
+__device__ __forceinline__ void put1(__nv_bfloat16* y, float v) { *y = __float2bfloat16_rn(v); }
 
 __device__ __forceinline__ void st_dsmem_i4(uint32_t addr, const int (&v)[4]) {
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
@@ -505,16 +512,249 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
 }
 
+// ------------------------------------------- weights on the MMA's M side ---
+// Few tokens leave most of a 256-token tile's TMEM lanes empty and its epilogue
+// to one or two of a pair's eight quadrants.  Here 128 weight rows are the
+// MMA's M (with GeGLU 64 gate rows and their 64 up rows) and the tokens, a
+// multiple of 16 up to kSideTokens, its N: every lane of the accumulator holds
+// outputs, lanes lie along a row of y, and the tokens are copied once per
+// weight row tile at their own size.
+//
+// One CTA per tile and part of K; a cluster of `splits` CTAs computes a tile.
+// A CTA gives the sums of 4 tokens x 128 rows (group g: CTA g % splits) to the
+// CTA that finishes them, as [source][group][row][4], through DSMEM into memory
+// of their own (not the ring: no CTA has to wait for another's products before
+// it sends).  GeGLU goes the same way with one CTA, through its idle ring: a
+// gate's lane and its up's differ.
+//
+// Bound by what an SM takes in, 16 KB of weights and T x 128 bytes of tokens per
+// K step, about 75 GB/s of the former, and by 3 to 4 us around the product.
+// Measured (captured; in brackets as pair tiles): 50 x 1024 x 8192 GeGLU 6.5 us
+// (7.5), 50 x 4096 x 1024 5.7 (9.4), 16 x 1024 x 2560 3.5 (5.4), 50 x 2048 x
+// 32768 GeGLU 16.0, 4.2 TB/s of weights (19.7), 16 x 16384 x 2048 10.4 (16.3).
+constexpr int kSideTokens = 128;
+constexpr int kSideThreads = 320;
+constexpr int kSideMaxSplits = 8;
+constexpr int kSideMaxStages = 16;
+
+int side_groups(int N, int splits) { return (N / 4 + splits - 1) / splits; }
+int side_ring(int N, int splits, bool geglu, int stages) {
+  const int ring = stages * (kTileM + N) * kStepK;
+  return splits == 1 && geglu ? std::max(ring, N * kTileM * 4) : ring;
+}
+int side_smem(int N, int splits, bool geglu, int stages) {
+  return side_ring(N, splits, geglu, stages) + (splits > 1 ? splits * side_groups(N, splits) * kTileM * 16 : 0) + N * 4 +
+         (2 * stages + 2) * 8 + 1024;
+}
+
+template <int ACT, typename Tout>
+__global__ void __launch_bounds__(kSideThreads, 3)
+    linear_i8_side_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const I8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr bool kGeglu = ACT == kActGeglu;
+  constexpr int kRows = kGeglu ? kTileM / 2 : kTileM;  // output columns of a tile
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int N = p.n_tile, splits = p.splits, stages = p.stages;
+  const int stage = (kTileM + N) * kStepK;
+  const int mine = (N / 4 + splits - 1) / splits;  // groups of 4 tokens per CTA, at most
+  const bool joined = kGeglu || splits > 1;
+  // one CTA's own sums go where its ring was
+  const int ring = splits == 1 && kGeglu ? max(stages * stage, N * kTileM * 4) : stages * stage;
+  uint8_t* red = splits == 1 ? smem : smem + ring;
+  float* sx = reinterpret_cast<float*>(smem + ring + (splits > 1 ? splits * mine * kTileM * 16 : 0));
+  uint64_t* full = reinterpret_cast<uint64_t*>(sx + N);
+  uint64_t* empty = full + stages;
+  uint64_t* acc_full = empty + stages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  const int rank = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int o0 = static_cast<int>(blockIdx.x) / splits * kRows;
+  const int k0 = static_cast<int>(static_cast<long>(rank) * p.k_steps / splits);
+  const int nk = static_cast<int>(static_cast<long>(rank + 1) * p.k_steps / splits) - k0;
+  const uint32_t cols = N <= 32 ? 32 : N <= 64 ? 64 : 128;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(acc_full, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmW);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (splits > 1) cluster_arrive_release();  // waited for before the first store into a peer
+  pdl_launch_dependents();
+  pdl_wait();
+
+  const int et = threadIdx.x - 64, quad = warp & 3, hw = (warp - 2) >> 2;
+  const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+  const int rowt = quad * 32 + lane;
+  float ws = 0.f, bs = 0.f, wu = 0.f, bu = 0.f;  // of the row that this thread finishes
+  int o = 0;
+  bool summed = false;
+  int issued = 0;
+  if (warp == 0) {
+    bool ok = true;
+    int s = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < nk; ++i) {
+      if (issued >= stages && !(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase ^ 1, p.status, kDevTimeoutStageEmpty))))
+        break;
+      if (elect_one()) {
+        uint8_t* st = smem + s * stage;
+        const int k = (k0 + i) * kStepK;
+        mbar_arrive_expect_tx(&full[s], static_cast<uint32_t>((kTileM + p.T) * kStepK));
+        tma_load_2d(st, &tmW, &full[s], k, o0);
+        if (kGeglu) tma_load_2d(st + kRows * kStepK, &tmW, &full[s], k, p.F + o0);
+        tma_load_2d(st + kTileM * kStepK, &tmX, &full[s], k, 0);
+      }
+      __syncwarp();
+      ++issued;
+      if (++s == stages) {
+        s = 0;
+        phase ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    const uint64_t a0 = make_sdesc_sw128(smem_u32(smem), 16, 1024);
+    const uint64_t b0 = make_sdesc_sw128(smem_u32(smem + kTileM * kStepK), 16, 1024);
+    const uint32_t idesc = make_idesc_i8(kTileM, N);
+    int s = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < nk; ++i) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], phase, p.status, kDevTimeoutTmaFull))) break;
+      tc_fence_after();
+      const uint64_t off = static_cast<uint64_t>((s * stage) >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kStepK / 32; ++kk)
+          umma_i8_ss(tmem, a0 + off + kk * 2, b0 + off + kk * 2, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&empty[s]);
+        if (i == nk - 1) umma_commit(acc_full);
+      }
+      __syncwarp();
+      if (++s == stages) {
+        s = 0;
+        phase ^= 1;
+      }
+    }
+  } else {
+    if (et < N) sx[et] = et < p.T ? p.x_scale[et] : 0.f;
+    o = o0 + (joined ? et % kRows : rowt);
+    if (o < p.F) {
+      ws = p.w_scale[o];
+      if (p.bias) bs = p.bias[o];
+      if (kGeglu) {
+        wu = p.w_scale[p.F + o];
+        if (p.bias) bu = p.bias[p.F + o];
+      }
+    }
+    epi_agree(true);  // the scales are in shared memory
+    summed = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, p.status, kDevTimeoutMmaDone));
+    tc_fence_after();
+    if (!joined && summed) {
+      for (int j = hw; j < N / 16; j += 2) {
+        uint32_t r[16];
+        tmem_ld16(acc + 16 * j, r);
+        tmem_wait_ld();
+        if (o < p.F) {
+          Tout* y = static_cast<Tout*>(p.y) + 16l * j * p.ldy + o;
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            if (16 * j + q < p.T)
+              put1(y + q * p.ldy, activate<ACT>(fmaf(static_cast<float>(static_cast<int>(r[q])) * sx[16 * j + q], ws, bs)));
+          }
+        }
+      }
+    }
+  }
+  if (joined) {
+    __syncwarp();
+    if (splits > 1) cluster_wait_acquire();
+    if (warp >= 2 && summed) {
+      for (int j = hw; j < N / 16; j += 2) {
+        uint32_t r[16];
+        tmem_ld16(acc + 16 * j, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int g = 4 * j + q;
+          const int v[4] = {static_cast<int>(r[4 * q]), static_cast<int>(r[4 * q + 1]), static_cast<int>(r[4 * q + 2]),
+                            static_cast<int>(r[4 * q + 3])};
+          if (splits == 1) {
+            reinterpret_cast<int4*>(red)[g * kTileM + rowt] = make_int4(v[0], v[1], v[2], v[3]);
+          } else {
+            const int owner = g % splits, slot = (rank * mine + g / splits) * kTileM + rowt;
+            st_dsmem_i4(mapa_shared(smem_u32(red), static_cast<uint32_t>(owner)) + static_cast<uint32_t>(slot) * 16u, v);
+          }
+        }
+      }
+    }
+    if (splits > 1)
+      cluster_sync();
+    else
+      __syncthreads();
+    if (warp >= 2 && summed && o < p.F) {
+      const int4* in = reinterpret_cast<const int4*>(red) + et % kRows;
+      for (int it = et / kRows; it < mine; it += 256 / kRows) {
+        const int t = (it * splits + rank) * 4;
+        if (t >= p.T) break;
+        int4 a = make_int4(0, 0, 0, 0), b = a;
+        for (int src = 0; src < splits; ++src) {
+          const int4 v = in[(src * mine + it) * kTileM];
+          a = make_int4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
+          if (kGeglu) {
+            const int4 u = in[(src * mine + it) * kTileM + kRows];
+            b = make_int4(b.x + u.x, b.y + u.y, b.z + u.z, b.w + u.w);
+          }
+        }
+        const int av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+        Tout* y = static_cast<Tout*>(p.y) + t * p.ldy + o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (t + q < p.T) {
+            float v = fmaf(static_cast<float>(av[q]) * sx[t + q], ws, bs);
+            if (kGeglu)
+              v = gelu_i8(v) * fmaf(static_cast<float>(bv[q]) * sx[t + q], wu, bu);
+            else
+              v = activate<ACT>(v);
+            put1(y + q * p.ldy, v);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  // a producer that stopped early waits (bounded) for its copies in flight
+  if (warp == 0 && lane == 0)
+    for (int i = (issued > stages ? issued - stages : 0); i < issued; ++i)
+      mbar_wait(&full[i % stages], (i / stages) & 1, p.status, kDevTimeoutTmaFull);
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, cols);
+  }
+}
+
 // ------------------------------------------------------- few tokens ---
-// Up to 4 tokens, or 8 of a small layer: the weights are read once, 16 bytes
-// per lane and load, and multiplied on the integer units (4 products per
-// instruction): no tiles, no shared-memory round trip, nothing to set up, so a
-// single token's call costs little more than the memory's latency (3.0 us for
-// 2048 x 2560, 15.4 us or 4.4 TB/s for the 67 MB of a 2048 x 32768 GeGLU).  A
+// Up to 4 tokens: the weights are read once, 16 bytes per lane and load, and
+// multiplied on the integer units (4 products per instruction): no tiles, no
+// shared-memory round trip, nothing to set up, so a single token's call costs
+// little more than the memory's latency (3.0 us for 2048 x 2560, 14.6 us or
+// 4.6 TB/s for the 67 MB of a 2048 x 32768 GeGLU).  A
 // warp takes two weight rows (GeGLU: a gate row and its up row) over a 1/kw
 // part of K; x comes through L1.
-constexpr int kFewTokens = 4, kFewTokensSmall = 8;
-constexpr long kFewSmall = 6 << 20;  // bytes of weights
+constexpr int kFewTokens = 4;
+constexpr long kFewSmall = 16 << 20;  // bytes of weights for 3 and 4 tokens
 constexpr int kFewThreads = 256;
 
 // (Not the read-only path: under programmatic launch this grid may start before
@@ -532,9 +772,6 @@ __device__ __forceinline__ int dot16(const int4& a, const int4& b, int acc) {
   acc = __dp4a(a.z, b.z, acc);
   return __dp4a(a.w, b.w, acc);
 }
-
-__device__ __forceinline__ void put1(float* y, float v) { *y = v; }
-__device__ __forceinline__ void put1(__nv_bfloat16* y, float v) { *y = __float2bfloat16_rn(v); }
 
 template <int TT, int ACT, typename Tout>
 __global__ void __launch_bounds__(kFewThreads) linear_i8_few_kernel(const I8Params p) {
@@ -636,35 +873,91 @@ const void* few_ptr(int out_dtype, int T) {
   if (out_dtype == kDtypeBF16) {
     if (T == 1) return reinterpret_cast<const void*>(linear_i8_few_kernel<1, ACT, __nv_bfloat16>);
     if (T == 2) return reinterpret_cast<const void*>(linear_i8_few_kernel<2, ACT, __nv_bfloat16>);
-    if (T <= 4) return reinterpret_cast<const void*>(linear_i8_few_kernel<4, ACT, __nv_bfloat16>);
-    return reinterpret_cast<const void*>(linear_i8_few_kernel<8, ACT, __nv_bfloat16>);
+    return reinterpret_cast<const void*>(linear_i8_few_kernel<4, ACT, __nv_bfloat16>);
   }
   if (T == 1) return reinterpret_cast<const void*>(linear_i8_few_kernel<1, ACT, float>);
   if (T == 2) return reinterpret_cast<const void*>(linear_i8_few_kernel<2, ACT, float>);
-  if (T <= 4) return reinterpret_cast<const void*>(linear_i8_few_kernel<4, ACT, float>);
-  return reinterpret_cast<const void*>(linear_i8_few_kernel<8, ACT, float>);
+  return reinterpret_cast<const void*>(linear_i8_few_kernel<4, ACT, float>);
 }
 template <int ACT>
-const void* i8_ptr(int out_dtype, bool few, int T) {
-  if (few) return few_ptr<ACT>(out_dtype, T);
+const void* i8_ptr(int out_dtype, int form, int T) {
+  if (form == kI8Few) return few_ptr<ACT>(out_dtype, T);
+  if (form == kI8Side)
+    return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_side_kernel<ACT, __nv_bfloat16>)
+                                   : reinterpret_cast<const void*>(linear_i8_side_kernel<ACT, float>);
   return out_dtype == kDtypeBF16 ? reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, __nv_bfloat16>)
                                  : reinterpret_cast<const void*>(linear_i8_pair_kernel<ACT, float>);
 }
-const void* i8_kernel(int epilogue, int out_dtype, bool few, int T) {
+const void* i8_kernel(int epilogue, int out_dtype, int form, int T) {
   switch (epilogue) {
-    case RFX_EPI_STORE: return i8_ptr<kActNone>(out_dtype, few, T);
-    case RFX_EPI_SILU: return i8_ptr<kActSilu>(out_dtype, few, T);
-    case RFX_EPI_GELU: return i8_ptr<kActGelu>(out_dtype, few, T);
-    case RFX_EPI_GEGLU: return i8_ptr<kActGeglu>(out_dtype, few, T);
+    case RFX_EPI_STORE: return i8_ptr<kActNone>(out_dtype, form, T);
+    case RFX_EPI_SILU: return i8_ptr<kActSilu>(out_dtype, form, T);
+    case RFX_EPI_GELU: return i8_ptr<kActGelu>(out_dtype, form, T);
+    case RFX_EPI_GEGLU: return i8_ptr<kActGeglu>(out_dtype, form, T);
   }
   return nullptr;
 }
 
-// How a call is cut up.  Up to 4 tokens go to the integer units: one token of
-// a 2048 x 2560 projection takes 3.1 us there and 7.0 as pair tiles, 4 tokens
-// 4.4, and of a 2048 x 32768 GeGLU 15.4 and 19.7 against 18.8.  With 8 tokens
-// the products bound them: a 2048 x 2560 projection (5 MB of weights) takes
-// 6.7 us against 7.3, a 1024 x 8192 one (8 MB) 9.3 against 7.2.
+// Tiles with the weights on the M side: the split of K and the CTAs meant to
+// share an SM (fewer stages each) that finish soonest by this model, in us,
+// fitted to measured times of seven projections at 8 to 128 tokens.  A K step
+// takes an SM 0.215 + 0.00035 per token; the weights come at 6.2 TB/s at best; a
+// ring that does not hold a CTA's whole part costs 0.5 and up to 1.1 per turn;
+// joining a split 0.8 + 0.006 per token + 0.1 per part; a further round of CTAs
+// 1.4 where each has the SM to itself, else 0.3; and a CTA that leaves room lets
+// the next launch set up beside it.
+void plan_side(const rfx_linear_i8_desc& d, int nsm, int k_steps, LinearI8Plan* c) {
+  const bool geglu = d.epilogue == RFX_EPI_GEGLU;
+  const void* fn = i8_kernel(d.epilogue, d.out_dtype, kI8Side, d.T);
+  const int rows = geglu ? kTileM / 2 : kTileM;
+  const int N = (d.T + 15) / 16 * 16;
+  const long tiles = (out_cols(d) - 1) / rows + 1;
+  const double step = 0.215 + 0.00035 * d.T, memory = static_cast<double>(d.O) * d.K / 6.2e6;
+  double best = 0;
+  for (int s = 1; s <= std::min(kSideMaxSplits, k_steps); s *= 2) {
+    const int n = (k_steps + s - 1) / s;
+    const long ctas = tiles * s;
+    if (s > 1 && ctas > 2l * nsm) break;
+    for (int share = 1; share <= 3; ++share) {
+      const int room = share == 1 ? kSmemMax : 228 * 1024 / share - 1024;
+      int stages = std::min(kSideMaxStages, n);
+      while (stages > 1 && side_smem(N, s, geglu, stages) > room) --stages;
+      if (side_smem(N, s, geglu, stages) > room || stages < std::min(n, 2)) continue;
+      const long slots = s == 1 ? static_cast<long>(nsm) * share : static_cast<long>(max_active_clusters(fn, kSideThreads, kSmemMax, s)) * s * share;
+      if (slots <= 0) continue;
+      const long waves = (ctas + slots - 1) / slots;
+      const double even = static_cast<double>(ctas) / nsm;
+      const double per_sm = share == 1 ? std::max<double>(waves, std::ceil(even)) : waves == 1 ? std::ceil(even) : even;
+      const double turns = static_cast<double>(n) / stages - 1.0;  // of the ring, after the first
+      double cost = std::max({per_sm * n * step, waves * turns * 1.1, memory}) + (turns > 0 ? 0.5 + 0.3 * turns : 0.0);
+      cost += (waves - 1) * (share == 1 ? 1.4 : 0.3) + (s > 1 ? 0.8 + 0.006 * d.T + 0.1 * s : 0.0);
+      cost -= 0.15 * (share - 1);
+      if (c->form == kI8Side && cost >= best) continue;
+      best = cost;
+      c->form = kI8Side;
+      c->splits = s;
+      c->stages = stages;
+    }
+  }
+  c->nt = N;
+  c->rows_a = d.T;
+  c->clusters = static_cast<int>(tiles);
+}
+
+// How a call is cut up.
+//
+// Up to 4 tokens go to the integer units, unless the layer is wide and short
+// (16 output rows and more per column of K: a warp's part is then too small) or,
+// with 3 or 4 tokens, large (the products bound them).  Measured there and with
+// the weights on the M side: 1 token of 1024 x 2560 2.8 and 3.1 us, of 1024 x
+// 8000 3.3 and 4.8, of 256 x 21953 5.8 and 3.8; 4 tokens of 1024 x 8000 4.7 and
+// 4.8, of 16384 x 2048 12.3 and 10.1.
+//
+// The weights lie on the M side up to 64 tokens and, but for K from 768 to 2048,
+// up to 128.  Measured there and as pair tiles: 50 tokens of 1024 x 8192 GeGLU
+// 6.5 and 7.5 us, of 4096 x 1024 5.7 and 9.4, of 2048 x 32768 GeGLU 16.0 and
+// 19.7, of 72 x 21953 7.7 and 19.9; 96 tokens of 1152 x 4304 8.0 and 7.3, 128 of
+// 1024 x 8192 GeGLU 8.8 and 7.8, of 4096 x 1024 6.9 and 9.5.
 //
 // Pair tiles: the width N and the split of K that finish soonest by this
 // model, whose figures are fitted to measured times of these projections at
@@ -677,8 +970,8 @@ LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   LinearI8Plan c{};
   const int div = d.epilogue == RFX_EPI_GEGLU ? 2 : 1;  // weight rows per output column
   const int F = out_cols(d);
-  if (d.T <= kFewTokens || (d.T <= kFewTokensSmall && static_cast<long>(d.O) * d.K <= kFewSmall)) {
-    c.few = true;
+  if (d.T <= kFewTokens && d.O <= 16l * d.K && (d.T <= 2 || static_cast<long>(d.O) * d.K <= kFewSmall)) {
+    c.form = kI8Few;
     // warps per pair of rows: enough of them for 16 per SM, with at least one
     // 512-byte load per row each
     const int pairs = d.epilogue == RFX_EPI_GEGLU ? F : (F + 1) / 2;
@@ -687,10 +980,14 @@ LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
     c.clusters = static_cast<int>((static_cast<long>(pairs) * c.splits + 7) / 8);
     return c;
   }
-  const int m = (d.T - 1) / (2 * kTileM) + 1;
   const int k_steps = (d.K + kStepK - 1) / kStepK;
+  if (d.T <= 64 || (d.T <= kSideTokens && (d.K <= 768 || d.K >= 2048))) {
+    plan_side(d, nsm, k_steps, &c);
+    return c;
+  }
+  const int m = (d.T - 1) / (2 * kTileM) + 1;
   const int step = 32 * div;  // tiles of whole 64-byte pieces of output rows
-  const void* fn = i8_kernel(d.epilogue, d.out_dtype, false, d.T);
+  const void* fn = i8_kernel(d.epilogue, d.out_dtype, kI8Pair, d.T);
   auto tiles_of = [&](int cols, int nt) { return static_cast<int>((static_cast<long>(cols) * div + nt - 1) / nt); };
   auto tile_ns = [&](int nt, int s) {
     return std::max((k_steps + s - 1) / s * std::max(150.0 + 0.45 * nt, 1.12 * nt), 10.0 * nt);
@@ -792,9 +1089,11 @@ int build_linear_i8_maps(const rfx_linear_i8_desc& d, LinearI8Maps* maps) {
   rfx_num_sms(&nsm);
   maps->plan = plan_i8(d, nsm);
   const LinearI8Plan& c = maps->plan;
-  if (c.few) return RFX_OK;
+  if (c.form == kI8Few) return RFX_OK;
   rc = make_tmap_2d(&maps->x, d.x, 1, d.K, d.T, d.ldx, kStepK, c.rows_a, true);
   if (rc) return rc;
+  if (c.form == kI8Side)
+    return make_tmap_2d(&maps->w, d.w, 1, d.K, d.O, d.ldw, kStepK, d.epilogue == RFX_EPI_GEGLU ? kTileM / 2 : kTileM, true);
   rc = make_tmap_2d(&maps->w, d.w, 1, d.K, d.O, d.ldw, kStepK, c.nt / 2, true);
   if (rc) return rc;
   maps->w2 = maps->w;
@@ -812,9 +1111,9 @@ int build_linear_i8_maps(const rfx_linear_i8_desc& d, LinearI8Maps* maps) {
 int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cudaStream_t stream, bool pdl) {
   if (d.T == 0) return RFX_OK;
   const LinearI8Plan& c = maps.plan;
-  const void* fn = i8_kernel(d.epilogue, d.out_dtype, c.few, d.T);
-  if (!c.few) {
-    const int rc = ensure_smem_attr(fn, kPairSmem);
+  const void* fn = i8_kernel(d.epilogue, d.out_dtype, c.form, d.T);
+  if (c.form != kI8Few) {
+    const int rc = ensure_smem_attr(fn, kSmemMax);
     if (rc) return rc;
   }
   I8Params p{};
@@ -841,8 +1140,12 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cuda
   p.y = d.y;
   p.ldy = d.ldy;
   p.status = device_status_ptr();
-  if (c.few) return launch_kernel(fn, dim3(c.clusters), dim3(kFewThreads), 0, stream, pdl, 1, p);
+  if (c.form == kI8Few) return launch_kernel(fn, dim3(c.clusters), dim3(kFewThreads), 0, stream, pdl, 1, p);
   CUtensorMap x = maps.x, w = maps.w, w2 = maps.w2, y = maps.y;
+  if (c.form == kI8Side)
+    return launch_kernel(fn, dim3(c.clusters * c.splits), dim3(kSideThreads),
+                         static_cast<size_t>(side_smem(c.nt, c.splits, d.epilogue == RFX_EPI_GEGLU, c.stages)), stream, pdl,
+                         c.splits, x, w, p);
   return launch_kernel(fn, dim3(2 * c.splits * c.clusters), dim3(kPairThreads), static_cast<size_t>(kPairSmem), stream,
                        pdl, 2 * c.splits, x, w, w2, y, p);
 }

@@ -138,8 +138,9 @@ int launch_quant_rows(const rfx_quant_rows_desc& d, cudaStream_t stream, bool pd
 int launch_block_norm(const rfx_block_norm_desc& d, cudaStream_t stream, bool pdl);
 int launch_rope(const rfx_rope_desc& d, cudaStream_t stream, bool pdl);
 // How rfx_linear_i8 cuts a call up; its tensor maps are made for it.
+enum { kI8Pair, kI8Side, kI8Few };
 struct LinearI8Plan {
-  bool few;         // few tokens: `clusters` CTAs, `splits` warps per pair of rows
+  int form;         // kI8Few: `clusters` CTAs, `splits` warps per pair of rows
   int nt, n_tiles;  // CTA pairs: weight rows per tile, tiles per token tile
   int nt2, n_tiles2;  // the narrower last tiles
   int splits, stages, rows_a, m_tiles, clusters;

@@ -178,7 +178,7 @@ int max_active_clusters(const void* func, int threads, int smem, int cluster_x) 
     int smem, cluster, dev, n;
   };
   static std::mutex mu;
-  static Entry memo[128];  // a few kernels x cluster sizes x devices; the rest is asked again
+  static Entry memo[256];  // a few kernels x cluster sizes x devices; the rest is asked again
   static int used = 0;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
@@ -205,7 +205,7 @@ int max_active_clusters(const void* func, int threads, int smem, int cluster_x) 
     if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess) n = 0;
     cudaGetLastError();
   }
-  if (used < 128) memo[used++] = Entry{func, smem, cluster_x, dev, n};
+  if (used < static_cast<int>(sizeof(memo) / sizeof(memo[0]))) memo[used++] = Entry{func, smem, cluster_x, dev, n};
   return n;
 }
 

@@ -191,6 +191,50 @@ def test_linear_i8_aligned_rows_of_odd_length(epi, T, O, Kc):
         check_linear(T, O, Kc, epi, dtype, bias=False, ldy_pad=-cols % 8 + 8, seed=3)
 
 
+@pytest.mark.parametrize("epi", [L.RFX_EPI_STORE, L.RFX_EPI_GELU, L.RFX_EPI_GEGLU])
+@pytest.mark.parametrize("T,O,Kc", [
+    (1, 20002, 64), (2, 9000, 333), (3, 2050, 9000), (5, 128, 128), (6, 130, 129), (15, 1026, 4096), (16, 256, 1100),
+    (17, 2560, 1024), (31, 126, 2000), (33, 2050, 3333), (48, 60002, 100), (49, 1152, 4304), (63, 514, 16384),
+    (64, 40000, 200), (65, 700, 512), (80, 300, 2049), (96, 5002, 700), (97, 64, 30000), (112, 4096, 2048),
+    (113, 2, 2048), (127, 20000, 72), (128, 2050, 5000),
+])
+def test_linear_i8_up_to_128_tokens(epi, T, O, Kc):
+    """One and several parts of K and rounds of tiles, tiles of one row and of
+    all but one, tokens at and around the multiples of 16."""
+    check_linear(T, O, Kc, epi, BF if (T + O) % 4 else F32, bias=T % 2 == 0, ldy_pad=T % 3, seed=T + 7)
+
+
+@pytest.mark.parametrize("T", [8, 100])
+def test_linear_i8_largest_sums_of_some_tokens(T):
+    """As the test below, with K in parts that are joined."""
+    Kc = 65536
+    x = torch.full((T, Kc), -128, dtype=torch.int8, device="cuda")
+    w = torch.full((40, Kc), -128, dtype=torch.int8, device="cuda")
+    w[1] = 127
+    y = torch.empty(T, 40, device="cuda")
+    K.linear_i8(w=w, w_scale=torch.ones(40, device="cuda"), x=x, x_scale=torch.ones(T, device="cuda"), y=y)
+    done()
+    assert (y[:, 0] == 2.0 ** 30).all() and (y[:, 2:] == 2.0 ** 30).all()
+    assert (y[:, 1] == float(-128 * 127 * Kc)).all()
+
+
+def test_linear_i8_rows_do_not_depend_on_the_others():
+    """A token's outputs are the same bits in any batch: the forms that a call
+    may take differ in no rounding."""
+    q, x = ints(8, 300, 2304)
+    w, wd = ints(9, 1536, 2304)
+    sx, sw, b = torch.rand(300).cuda(), torch.rand(1536).cuda() * 1e-4, torch.randn(1536).cuda()
+    for epi in (L.RFX_EPI_STORE, L.RFX_EPI_SILU, L.RFX_EPI_GELU, L.RFX_EPI_GEGLU):
+        F = 768 if epi == L.RFX_EPI_GEGLU else 1536
+        whole = None
+        for T in (300, 128, 64, 50, 16, 5, 4, 2, 1):
+            y = torch.empty(T, F, device="cuda")
+            K.linear_i8(w=wd, w_scale=sw, x=x[:T], x_scale=sx[:T], y=y, epilogue=epi, bias=b)
+            done()
+            whole = y if whole is None else whole
+            assert torch.equal(y, whole[:T]), (epi, T)
+
+
 def test_linear_i8_largest_sums():
     """Every product at its extreme (-128 * -128 over K = 65536, a sum of
     2^30): the s32 accumulators hold it."""
