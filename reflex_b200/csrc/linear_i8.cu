@@ -866,6 +866,8 @@ __global__ void __launch_bounds__(kFewThreads) linear_i8_few_kernel(const I8Para
 }
 
 // ------------------------------------------------------------ host side ---
+bool al(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
 int out_cols(const rfx_linear_i8_desc& d) { return d.epilogue == RFX_EPI_GEGLU ? d.O / 2 : d.O; }
 
 template <int ACT>
@@ -963,9 +965,11 @@ void plan_side(const rfx_linear_i8_desc& d, int nsm, int k_steps, LinearI8Plan* 
 // model, whose figures are fitted to measured times of these projections at
 // 16 to 4096 tokens.  A K step takes 150 ns + 0.45 ns per weight row while the
 // copies into the SM bound it, 1.12 ns per weight row once the MMAs do, and
-// 1.17 times that over several rounds of tiles; a tile at least its epilogue's
-// 10 ns per weight row; the last epilogue is not hidden; adding up the splits
-// costs 0.9 us + 0.4 us per split.
+// 1.17 times that over several rounds of tiles, each at least its epilogue's
+// 1.7 us + 10.5 ns per weight row (14.5 with GeGLU, 18.5 with an activation, 4
+// more for fp32 and 16 more where output rows are off the 16-byte grid); the
+// last epilogue is not hidden, and where K is split adding up costs 0.9 us + 0.4
+// us per split.  (1600 x 72 x 21952: 86 us in tiles of 64 rows, 43 in tiles of 256.)
 LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   LinearI8Plan c{};
   const int div = d.epilogue == RFX_EPI_GEGLU ? 2 : 1;  // weight rows per output column
@@ -989,9 +993,12 @@ LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   const int step = 32 * div;  // tiles of whole 64-byte pieces of output rows
   const void* fn = i8_kernel(d.epilogue, d.out_dtype, kI8Pair, d.T);
   auto tiles_of = [&](int cols, int nt) { return static_cast<int>((static_cast<long>(cols) * div + nt - 1) / nt); };
-  auto tile_ns = [&](int nt, int s) {
-    return std::max((k_steps + s - 1) / s * std::max(150.0 + 0.45 * nt, 1.12 * nt), 10.0 * nt);
-  };
+  const int esz = d.out_dtype == kDtypeBF16 ? 2 : 4;
+  double row_ns = d.epilogue == RFX_EPI_STORE ? 10.5 : d.epilogue == RFX_EPI_GEGLU ? 14.5 : 18.5;
+  if (esz == 4) row_ns += 4.0;
+  if (!al(d.y, 16) || (d.ldy * esz) % 16 != 0) row_ns += 16.0 / div;
+  auto sum_ns = [&](int nt, int s) { return (k_steps + s - 1) / s * std::max(150.0 + 0.45 * nt, 1.12 * nt); };
+  auto tile_ns = [&](int nt, int rounds) { return rounds > 1 ? std::max(sum_ns(nt, 1), 1700.0 + row_ns * nt) : sum_ns(nt, 1); };
   double best = 0;
   for (int s = 1; s <= std::min(kMaxSplits, k_steps); ++s) {
     // clusters of 2s CTAs that are resident at once (GPCs hold whole clusters)
@@ -1016,9 +1023,13 @@ LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
         c.clusters = static_cast<int>(std::min<long>(static_cast<long>(m) * (n_a + n_b), slots));
       };
       // several rounds: every SM at work
-      const double all = rounds > 1 ? 1.17 * tiles / slots * tile_ns(nt, s) : 0.0;
-      consider(std::max(rounds * tile_ns(nt, s), all) + 10.0 * nt + (s > 1 ? 900.0 + 400.0 * s : 0.0), n, nt, 0);
-      if (s > 1 || rounds < 2) continue;
+      const double all = rounds > 1 ? 1.17 * tiles / slots * tile_ns(nt, 2) : 0.0;
+      if (s > 1) {
+        consider(sum_ns(nt, s) + 10.0 * nt + 900.0 + 400.0 * s, n, nt, 0);
+        continue;
+      }
+      consider(std::max(rounds * tile_ns(nt, static_cast<int>(rounds)), all) + 10.0 * nt, n, nt, 0);
+      if (rounds < 2) continue;
       // the full rounds at this width, the rest in narrower tiles
       const int n_a = static_cast<int>((rounds - 1) * slots / m);
       if (n_a < 1 || n_a >= n) continue;
@@ -1026,7 +1037,7 @@ LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
         const int n_b = tiles_of(F - n_a * (nt / div), nt2);
         const long ua = static_cast<long>(n_a) * m, ub = static_cast<long>(n_b) * m;
         // the tiles go round the slots: the busiest slot's time
-        const double ta = tile_ns(nt, 1), tb = tile_ns(nt2, 1);
+        const double ta = tile_ns(nt, 2), tb = tile_ns(nt2, 2);
         const long qa = ua / slots, ra = ua % slots, first = slots - ra;  // `first` slots have one wide tile less
         double t;
         if (ub <= first) {
@@ -1045,8 +1056,6 @@ LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   c.stages = std::min(kPairMaxStages, kPairRing / ((kTileM + c.nt / 2) * kStepK));
   return c;
 }
-
-bool al(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 }  // namespace
 
