@@ -34,8 +34,8 @@ struct I8Params {
   int splits;       // parts of K: pairs per cluster, or warps per pair of rows
   int m_tiles;      // 256-token tiles
   int n_tile;       // weight rows per tile,
-  int n_tail;       // of the tiles from units_a on
-  int units_a, units;
+  int n_tail;       // of the tiles from column cols_a on
+  int cols_a, units;
   int stages;
   int rows_a;       // token rows per copy: 128, or T rounded up to 8
   const int8_t* x;
@@ -221,25 +221,39 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t rank = crank & 1u;  // in the pair
   const bool leader = rank == 0;
   const int split = static_cast<int>(crank >> 1);
-  // Units: first `units_a` tiles of N = n_tile, then tiles of N = n_tail over
-  // the remaining columns, so that the last round of tiles is a narrow one.
+  // Units, m_tiles to a column of tiles: first tiles of N = n_tile, then, from
+  // column cols_a on, of N = n_tail, so that the last round of tiles is a narrow
+  // one.  A walker keeps its place (tile row, column) and steps without dividing.
+  const int ustep = gridDim.x / (2 * p.splits), unit0 = blockIdx.x / (2 * p.splits);
   struct Unit {
     int m, o0, N;
+    bool tail;
   };
-  auto unit_of = [&](int un) {
-    const bool tail = un >= p.units_a;
-    const int v = tail ? un - p.units_a : un;
-    const int n = v / p.m_tiles;
-    const int w = kGeglu ? p.n_tile / 2 : p.n_tile;
+  struct Walk {
+    int un, n, m;
+  };
+  const int step_n = ustep / p.m_tiles, step_m = ustep - step_n * p.m_tiles;
+  const int first_n = unit0 / p.m_tiles;
+  const Walk first{unit0, first_n, unit0 - first_n * p.m_tiles};
+  auto next = [&](Walk& k) {
+    k.un += ustep;
+    k.n += step_n;
+    k.m += step_m;
+    if (k.m >= p.m_tiles) {
+      k.m -= p.m_tiles;
+      ++k.n;
+    }
+  };
+  auto unit_of = [&](const Walk& k) {
+    const int w = kGeglu ? p.n_tile / 2 : p.n_tile, w2 = kGeglu ? p.n_tail / 2 : p.n_tail;
     Unit u;
-    u.m = v - n * p.m_tiles;
-    u.N = tail ? p.n_tail : p.n_tile;
-    u.o0 = tail ? p.units_a / p.m_tiles * w + n * (kGeglu ? u.N / 2 : u.N) : n * w;
+    u.m = k.m;
+    u.tail = k.n >= p.cols_a;
+    u.N = u.tail ? p.n_tail : p.n_tile;
+    u.o0 = u.tail ? p.cols_a * w + (k.n - p.cols_a) * w2 : k.n * w;
     return u;
   };
   const int stages = p.stages, stage = (kTileM + p.n_tile / 2) * kStepK;
-  const int csize = 2 * p.splits;
-  const int unit0 = blockIdx.x / csize, ustep = gridDim.x / csize;
   const int k0 = static_cast<int>(static_cast<long>(split) * p.k_steps / p.splits);
   const int nk = static_cast<int>(static_cast<long>(split + 1) * p.k_steps / p.splits) - k0;
 
@@ -279,11 +293,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     int s = 0;
     uint32_t phase = 0;
     const uint32_t full0 = mapa_shared(smem_u32(full), crank & ~1u);
-    for (int un = unit0; un < p.units && ok; un += ustep) {
-      const Unit tile = unit_of(un);
+    for (Walk k = first; k.un < p.units && ok; next(k)) {
+      const Unit tile = unit_of(k);
       const int t0 = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM;
       const int wrow = kGeglu ? (rank ? p.F + tile.o0 : tile.o0) : tile.o0 + static_cast<int>(rank) * (tile.N / 2);
-      const CUtensorMap* tw = un < p.units_a ? &tmW : &tmW2;
+      const CUtensorMap* tw = tile.tail ? &tmW2 : &tmW;
       // both CTAs' copies count on the even CTA's barrier; a half without
       // tokens copies none (what its rows multiply is not stored)
       const bool has_x = t0 < p.T;
@@ -316,9 +330,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       bool ok = true;
       int s = 0, tl = 0;
       uint32_t phase = 0;
-      for (int un = unit0; un < p.units && ok; un += ustep, ++tl) {
+      for (Walk k = first; k.un < p.units && ok; next(k), ++tl) {
         const int buf = tl & 1;
-        const uint32_t idesc = make_idesc_i8(2 * kTileM, un < p.units_a ? p.n_tile : p.n_tail);
+        const uint32_t idesc = make_idesc_i8(2 * kTileM, k.n < p.cols_a ? p.n_tile : p.n_tail);
         if (tl >= 2 &&
             !(ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[buf], ((tl >> 1) - 1) & 1, p.status, kDevTimeoutMmaDone))))
           break;
@@ -354,24 +368,41 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t free_bar = mapa_shared(smem_u32(&acc_free[0]), crank & ~1u);
     int tl = 0;
-    for (int un = unit0; un < p.units; un += ustep, ++tl) {
+    // a tile's scales and bias come asynchronously while the tile before it is
+    // finished (a short K's products are there at once: the loads would be
+    // waited for at every tile's start)
+    float sx_next = 0.f;
+    auto request = [&](const Unit& tile, int b) {
+      if (et < tile.N) {
+        const int nh = tile.N / 2;
+        const int c = kGeglu ? (et < nh ? et : et - nh) : et;
+        const bool in = tile.o0 + c < p.F;
+        const int o = tile.o0 + c + (kGeglu && et >= nh ? p.F : 0);
+        float* ws = vec + b * 512 + et;
+        if (in)
+          cp_async4(ws, p.w_scale + o);
+        else
+          *ws = 0.f;
+        if (in && p.bias)
+          cp_async4(ws + 256, p.bias + o);
+        else
+          ws[256] = 0.f;
+      }
+      cp_async_commit();
+      const int t = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32 + lane;
+      sx_next = t < p.T ? p.x_scale[t] : 0.f;
+    };
+    if (first.un < p.units) request(unit_of(first), 0);
+    for (Walk k = first; k.un < p.units; next(k), ++tl) {
       const int buf = tl & 1;
-      const Unit tile = unit_of(un);
+      const Unit tile = unit_of(k);
       const int N = tile.N, nh = N / 2, oc = kGeglu ? nh : N;  // oc output columns
       const int tw = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32;  // the warp's first token
-      const int t = tw + lane;
       const int o0 = tile.o0;
-      // this tile's scales and bias, while its products are still computed
-      float* ws = vec + buf * 512;
-      float* bs = ws + 256;
-      if (et < N) {
-        const int c = kGeglu ? (et < nh ? et : et - nh) : et;
-        const bool in = o0 + c < p.F;
-        const int o = o0 + c + (kGeglu && et >= nh ? p.F : 0);
-        ws[et] = in ? p.w_scale[o] : 0.f;
-        bs[et] = in && p.bias ? p.bias[o] : 0.f;
-      }
-      const float sx = t < p.T ? p.x_scale[t] : 0.f;
+      const float* ws = vec + buf * 512;
+      const float* bs = ws + 256;
+      const float sx = sx_next;
+      cp_async_wait_all();
       // every epilogue warp agrees before anyone leaves the loop
       if (!epi_agree(mbar_wait(&acc_full[buf], (tl >> 1) & 1, p.status, kDevTimeoutMmaDone))) {
         failed = true;
@@ -380,6 +411,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       tc_fence_after();
       const uint32_t acc = tmem + buf * 256 + lane_base;
       if (p.splits > 1) break;  // one tile per cluster: summed below
+      Walk ahead = k;
+      next(ahead);
+      if (ahead.un < p.units) request(unit_of(ahead), buf ^ 1);
       // groups of 128 output bytes, of which each warp of the quadrant finishes
       // and stores 64
 #pragma unroll 1
@@ -397,7 +431,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (g + kGroup >= oc) {  // this warp's last read of the accumulator
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(free_bar + 8u * buf);
+          if (lane == 0) mbar_arrive_cluster_relaxed(free_bar + 8u * buf);  // (a releasing one: 1400 clocks a tile)
         }
 #pragma unroll
         for (int q = 0; q < kHalf / 16; ++q) {
@@ -409,7 +443,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         store_part<Tout>(p, &tmY, out_st, w, tw, o0 + g, p.T - tw, min(min(kHalf, oc - g), p.F - o0 - g), tma_y, lane);
       }
-      if (hw * kHalf >= oc && lane == 0) mbar_arrive_cluster(free_bar + 8u * buf);  // a warp without columns
+      if (hw * kHalf >= oc && lane == 0) mbar_arrive_cluster_relaxed(free_bar + 8u * buf);  // a warp without columns
     }
   }
   if (p.splits > 1) {
@@ -418,7 +452,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     // j % splits) to the CTA of the same token half there, as
     // [group][source][gate | up][4 columns][token], and adds what it receives
     // to its own.  s32 sums: any order is exact.
-    const Unit tile = unit_of(unit0);
+    const Unit tile = unit_of(first);
     const int nh = tile.N / 2, oc = kGeglu ? nh : tile.N;
     const int quad = warp & 3, hw = (warp - 2) >> 2;
     const int rowt = quad * 32 + lane;
@@ -1135,8 +1169,8 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cuda
   p.splits = c.splits;
   p.n_tile = c.nt;
   p.n_tail = c.nt2;
-  p.units_a = c.m_tiles * c.n_tiles;
-  p.units = p.units_a + c.m_tiles * c.n_tiles2;
+  p.cols_a = c.n_tiles;
+  p.units = c.m_tiles * (c.n_tiles + c.n_tiles2);
   p.stages = c.stages;
   p.rows_a = c.rows_a;
   p.x = static_cast<const int8_t*>(d.x);

@@ -328,9 +328,11 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 // Arrives once on an mbarrier given by its shared::cluster address (this
-// CTA's or another CTA's of the cluster), release at cluster scope.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+// CTA's or another CTA's of the cluster).  Relaxed: it does not wait for the
+// thread's other memory operations, and stands for what is complete by itself,
+// as TMEM reads are after tcgen05.wait::ld.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
 
 // TMEM -> registers: 32 lanes x 32-bit, 16 consecutive columns per thread.
