@@ -98,7 +98,7 @@ __device__ __forceinline__ void st_dsmem_i4(uint32_t addr, const int (&v)[4]) {
 //
 // Measured: 4096 x 4096 x 4096 47 us, 2.9 POP/s (87 % of twice the measured
 // bf16 burst rate; 55 us, 89 % of twice the sustained one, in a loop under the
-// power cap); 768 x 32768 x 2048 GeGLU 41 us (2.5 POP/s); 768 x 2048 x 16384
+// power cap); 768 x 32768 x 2048 GeGLU 40 us (2.6 POP/s); 768 x 2048 x 16384
 // 24 us (2.2 POP/s, two splits).  With the MMAs left out the first takes 34 us
 // and with the copies left out 39: both streams are near their limit, and they
 // share the SM's shared memory.  Calls of one tile per pair spend about 7 us
@@ -161,11 +161,34 @@ __device__ __forceinline__ void pack16(const float (&v)[16], uint32_t* w, const 
   for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i]);
 }
 
+// 32 staged rows of 64 bytes to global rows of `pitch` bytes, in units of U: a
+// lane keeps its column of units and walks the rows, several of them on their way.
+template <typename U>
+__device__ __forceinline__ void store_units(const uint8_t* st, uint8_t* y, long pitch, int rows, int bytes, int lane) {
+  constexpr int kCols = 64 / static_cast<int>(sizeof(U)), kRowsPer = 32 / kCols, kBatch = sizeof(U) == 8 ? 4 : 8;
+  const int byte = lane % kCols * static_cast<int>(sizeof(U)), r0 = lane / kCols;
+  const int end = byte < bytes ? min(rows, 32) : 0;
+  y += r0 * pitch + byte;
+#pragma unroll 1
+  for (int r = r0; r < 32; r += kBatch * kRowsPer, y += kBatch * kRowsPer * pitch) {
+    U v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int q = r + i * kRowsPer;
+      v[i] = *reinterpret_cast<const U*>(st + q * 64 + (((byte >> 4) ^ ((q >> 1) & 3)) << 4) + (byte & 15));
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (r + i * kRowsPer < end) *reinterpret_cast<U*>(y + i * kRowsPer * pitch) = v[i];
+  }
+}
+
 // A warp's 32 rows x 64 bytes of outputs (lane = row) to memory through its own
 // 2 KB of shared memory: one TMA store where y's rows begin on 16-byte
-// boundaries (`tma`), else coalesced elements.  The copy clips rows past T, and
-// columns past F only in units of 16 bytes, so a last piece that ends inside
-// such a unit goes out by elements.  `rows` and `n` are the live rows and
+// boundaries (`tma`), else in coalesced units of the 2, 4 or 8 bytes that the
+// rows allow.  The copy clips rows past T, and columns past F only in units of 16
+// bytes, so a last piece that ends inside such a unit goes out that way too.
+// `rows` and `n` are the live rows and
 // columns from (t, o).
 template <typename Tout>
 __device__ __forceinline__ void store_part(const I8Params& p, const CUtensorMap* tmY, uint8_t* st,
@@ -190,14 +213,17 @@ __device__ __forceinline__ void store_part(const I8Params& p, const CUtensorMap*
     }
   } else {
     __syncwarp();
-    // a lane keeps its column and walks the rows
-    constexpr int kRowsPer = 32 / kCols;
-    const int c = lane % kCols, byte = c * static_cast<int>(sizeof(Tout));
-    Tout* y = static_cast<Tout*>(p.y) + static_cast<long>(t + lane / kCols) * p.ldy + o + c;
-    const int end = c < n ? min(rows, 32) : 0;
-#pragma unroll 4
-    for (int r = lane / kCols; r < end; r += kRowsPer, y += kRowsPer * p.ldy)
-      *y = *reinterpret_cast<const Tout*>(st + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
+    const long pitch = p.ldy * static_cast<long>(sizeof(Tout));
+    uint8_t* y = reinterpret_cast<uint8_t*>(static_cast<Tout*>(p.y) + t * p.ldy + o);
+    const int bytes = min(n, kCols) * static_cast<int>(sizeof(Tout));
+    const uint32_t odd = static_cast<uint32_t>(pitch) | static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p.y)) |
+                         static_cast<uint32_t>(bytes);
+    if (odd % 8 == 0)
+      store_units<uint2>(st, y, pitch, rows, bytes, lane);
+    else if (sizeof(Tout) == 4 || odd % 4 == 0)
+      store_units<uint32_t>(st, y, pitch, rows, bytes, lane);
+    else
+      store_units<uint16_t>(st, y, pitch, rows, bytes, lane);
     __syncwarp();
   }
 }
@@ -1003,7 +1029,9 @@ void plan_side(const rfx_linear_i8_desc& d, int nsm, int k_steps, LinearI8Plan* 
 // 1.7 us + 10.5 ns per weight row (14.5 with GeGLU, 18.5 with an activation, 4
 // more for fp32 and 16 more where output rows are off the 16-byte grid); the
 // last epilogue is not hidden, and where K is split adding up costs 0.9 us + 0.4
-// us per split.  (1600 x 72 x 21952: 86 us in tiles of 64 rows, 43 in tiles of 256.)
+// us per split.  (An epilogue's fixed part measures 0.5 us; counted as that, the
+// model takes narrower tiles that are up to 18 % slower.  3200 x 72 x 21952: 73 us
+// in tiles of 64 rows, 52 in tiles of 256.)
 LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   LinearI8Plan c{};
   const int div = d.epilogue == RFX_EPI_GEGLU ? 2 : 1;  // weight rows per output column
