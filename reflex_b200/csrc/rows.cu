@@ -11,7 +11,7 @@
 // instructions in block_norm, half of them reductions, divisions and
 // addresses) and, for few rows, the latency of one row's chain of reductions.
 // Measured: int8 rows of 768 x 16384 bf16 10.3 us (3.7 TB/s); block_norm with
-// everything on, 3200 x 1024 bf16 to int8, 9.5 us (2.5 TB/s), 768 x 2048 fp32
+// everything on, 3200 x 1024 bf16 to int8, 9.2 us (2.6 TB/s), 768 x 2048 fp32
 // 7.5 us (3.3 TB/s), 50 x 1024 2.6 us.  Rows off the 16-byte grid take element
 // accesses: 3200 x 1025 24 us.
 #include "quant_i8.cuh"
@@ -392,12 +392,20 @@ __global__ void __launch_bounds__(TPR* rows_per_cta<TPR>(), TPR <= 128 ? 6 : NV 
   if (kAhead) load(0);
   f32x2 gain[4], a12[4], b2[4];  // of the current stream, when kept
   const float *gate = nullptr, *pa2 = nullptr, *pb2 = nullptr;
-  int held = -1;
-  for (int r = 0; r < n; ++r) {
+  // the stream of the row, and its rows left: one division per CTA
+  int b = first / p.S, left = p.S - (first - b * p.S);
+  bool fresh = true;
+  auto step = [&] {
+    if (--left == 0) {
+      left = p.S;
+      ++b;
+      fresh = true;
+    }
+  };
+  for (int r = 0; r < n; ++r, step()) {
     const int i = r & 1;
-    const int b = (first + r) / p.S;
-    if (b != held) {
-      held = b;
+    if (fresh) {
+      fresh = false;
       gate = p.gate ? p.gate + b * p.gate_stride : nullptr;
       pa2 = p.a2 ? p.a2 + b * p.ab_stride : nullptr;
       pb2 = p.b2 ? p.b2 + b * p.ab_stride : nullptr;
