@@ -617,7 +617,8 @@ __global__ void __launch_bounds__(kSideThreads, 3)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int N = p.n_tile, splits = p.splits, stages = p.stages;
   const int stage = (kTileM + N) * kStepK;
-  const int mine = (N / 4 + splits - 1) / splits;  // groups of 4 tokens per CTA, at most
+  const int shift = 31 - __clz(splits);            // splits is a power of 2
+  const int mine = (N / 4 + splits - 1) >> shift;  // groups of 4 tokens per CTA, at most
   const bool joined = kGeglu || splits > 1;
   // one CTA's own sums go where its ring was
   const int ring = splits == 1 && kGeglu ? max(stages * stage, N * kTileM * 4) : stages * stage;
@@ -628,7 +629,7 @@ __global__ void __launch_bounds__(kSideThreads, 3)
   uint64_t* acc_full = empty + stages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int rank = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int o0 = static_cast<int>(blockIdx.x) / splits * kRows;
+  const int o0 = (static_cast<int>(blockIdx.x) >> shift) * kRows;
   const int k0 = static_cast<int>(static_cast<long>(rank) * p.k_steps / splits);
   const int nk = static_cast<int>(static_cast<long>(rank + 1) * p.k_steps / splits) - k0;
   const uint32_t cols = N <= 32 ? 32 : N <= 64 ? 64 : 128;
@@ -728,11 +729,14 @@ __global__ void __launch_bounds__(kSideThreads, 3)
         tmem_wait_ld();
         if (o < p.F) {
           Tout* y = static_cast<Tout*>(p.y) + 16l * j * p.ldy + o;
+          float v[16];
 #pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            if (16 * j + q < p.T)
-              put1(y + q * p.ldy, activate<ACT>(fmaf(static_cast<float>(static_cast<int>(r[q])) * sx[16 * j + q], ws, bs)));
-          }
+          for (int q = 0; q < 16; ++q)
+            v[q] = activate<ACT>(fmaf(static_cast<float>(static_cast<int>(r[q])) * sx[16 * j + q], ws, bs));
+          // (the values first: behind its own branch each would wait for the one before it)
+#pragma unroll
+          for (int q = 0; q < 16; ++q, y += p.ldy)
+            if (16 * j + q < p.T) put1(y, v[q]);
         }
       }
     }
@@ -753,7 +757,7 @@ __global__ void __launch_bounds__(kSideThreads, 3)
           if (splits == 1) {
             reinterpret_cast<int4*>(red)[g * kTileM + rowt] = make_int4(v[0], v[1], v[2], v[3]);
           } else {
-            const int owner = g % splits, slot = (rank * mine + g / splits) * kTileM + rowt;
+            const int owner = g & (splits - 1), slot = (rank * mine + (g >> shift)) * kTileM + rowt;
             st_dsmem_i4(mapa_shared(smem_u32(red), static_cast<uint32_t>(owner)) + static_cast<uint32_t>(slot) * 16u, v);
           }
         }
@@ -765,30 +769,42 @@ __global__ void __launch_bounds__(kSideThreads, 3)
       __syncthreads();
     if (warp >= 2 && summed && o < p.F) {
       const int4* in = reinterpret_cast<const int4*>(red) + et % kRows;
-      for (int it = et / kRows; it < mine; it += 256 / kRows) {
-        const int t = (it * splits + rank) * 4;
-        if (t >= p.T) break;
-        int4 a = make_int4(0, 0, 0, 0), b = a;
-        for (int src = 0; src < splits; ++src) {
-          const int4 v = in[(src * mine + it) * kTileM];
-          a = make_int4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
-          if (kGeglu) {
-            const int4 u = in[(src * mine + it) * kTileM + kRows];
-            b = make_int4(b.x + u.x, b.y + u.y, b.z + u.z, b.w + u.w);
+      constexpr int kStep = 256 / kRows;  // groups that the warps take at a time
+      constexpr int kAhead = kGeglu ? 1 : 2;  // of them per thread, values first and then their stores
+      for (int it0 = et / kRows; it0 < mine && (it0 * splits + rank) * 4 < p.T; it0 += kAhead * kStep) {
+        float v[kAhead][4];
+#pragma unroll
+        for (int h = 0; h < kAhead; ++h) {
+          const int it = min(it0 + h * kStep, mine - 1), t = min((it * splits + rank) * 4, N - 4);
+          int4 a = make_int4(0, 0, 0, 0), b = a;
+          for (int src = 0; src < splits; ++src) {
+            const int4 x = in[(src * mine + it) * kTileM];
+            a = make_int4(a.x + x.x, a.y + x.y, a.z + x.z, a.w + x.w);
+            if (kGeglu) {
+              const int4 u = in[(src * mine + it) * kTileM + kRows];
+              b = make_int4(b.x + u.x, b.y + u.y, b.z + u.z, b.w + u.w);
+            }
+          }
+          const float4 s4 = *reinterpret_cast<const float4*>(sx + t);
+          const int av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+          const float sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            v[h][q] = fmaf(static_cast<float>(av[q]) * sv[q], ws, bs);
+            if (kGeglu)
+              v[h][q] = gelu_i8(v[h][q]) * fmaf(static_cast<float>(bv[q]) * sv[q], wu, bu);
+            else
+              v[h][q] = activate<ACT>(v[h][q]);
           }
         }
-        const int av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-        Tout* y = static_cast<Tout*>(p.y) + t * p.ldy + o;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (t + q < p.T) {
-            float v = fmaf(static_cast<float>(av[q]) * sx[t + q], ws, bs);
-            if (kGeglu)
-              v = gelu_i8(v) * fmaf(static_cast<float>(bv[q]) * sx[t + q], wu, bu);
-            else
-              v = activate<ACT>(v);
-            put1(y + q * p.ldy, v);
-          }
+        for (int h = 0; h < kAhead; ++h) {
+          const int it = it0 + h * kStep, t = (it * splits + rank) * 4;
+          const int live = it < mine ? p.T - t : 0;
+          Tout* y = static_cast<Tout*>(p.y) + t * p.ldy + o;
+#pragma unroll
+          for (int q = 0; q < 4; ++q, y += p.ldy)
+            if (q < live) put1(y, v[h][q]);
         }
       }
     }
