@@ -590,9 +590,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // Bound by what an SM takes in, 16 KB of weights and T x 128 bytes of tokens per
 // K step, about 75 GB/s of the former, and by 3 to 4 us around the product.
 // Measured (captured; in brackets as pair tiles): 50 x 1024 x 8192 GeGLU 6.5 us
-// (7.5), 50 x 4096 x 1024 5.7 (9.4), 16 x 1024 x 2560 3.5 (5.4), 50 x 2048 x
-// 32768 GeGLU 16.0, 4.2 TB/s of weights (19.7), 16 x 16384 x 2048 10.4 (16.3).
-constexpr int kSideTokens = 128;
+// (7.5), 50 x 4096 x 1024 5.5 (9.4), 16 x 1024 x 2560 3.4 (5.4), 50 x 2048 x
+// 32768 GeGLU 15.4, 4.4 TB/s of weights (19.7), 16 x 16384 x 2048 10.2 (16.3).
+constexpr int kSideTokens = 128;  // the registers of an SM allow three CTAs: 384 of its 512 TMEM columns
 constexpr int kSideThreads = 320;
 constexpr int kSideMaxSplits = 8;
 constexpr int kSideMaxStages = 16;
@@ -1031,11 +1031,11 @@ void plan_side(const rfx_linear_i8_desc& d, int nsm, int k_steps, LinearI8Plan* 
 // 8000 3.3 and 4.8, of 256 x 21953 5.8 and 3.8; 4 tokens of 1024 x 8000 4.7 and
 // 4.8, of 16384 x 2048 12.3 and 10.1.
 //
-// The weights lie on the M side up to 64 tokens and, but for K from 768 to 2048,
-// up to 128.  Measured there and as pair tiles: 50 tokens of 1024 x 8192 GeGLU
-// 6.5 and 7.5 us, of 4096 x 1024 5.7 and 9.4, of 2048 x 32768 GeGLU 16.0 and
-// 19.7, of 72 x 21953 7.7 and 19.9; 96 tokens of 1152 x 4304 8.0 and 7.3, 128 of
-// 1024 x 8192 GeGLU 8.8 and 7.8, of 4096 x 1024 6.9 and 9.5.
+// The weights lie on the M side up to 128 tokens.  Measured there and as pair
+// tiles: 50 tokens of 1024 x 8192 GeGLU 6.5 and 7.5 us, of 4096 x 1024 5.5 and 9.4,
+// of 2048 x 32768 GeGLU 15.4 and 19.7; 96 tokens of 1152 x 4304 GELU 6.0 and 6.9;
+// 128 of 800 x 20000 8.5 and 10.2, of 1024 x 2560 5.6 and 5.6, of 1024 x 8192 GeGLU
+// 7.7 and 7.5.
 //
 // Pair tiles: the width N and the split of K that finish soonest by this
 // model, whose figures are fitted to measured times of these projections at
@@ -1063,7 +1063,7 @@ LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
     return c;
   }
   const int k_steps = (d.K + kStepK - 1) / kStepK;
-  if (d.T <= 64 || (d.T <= kSideTokens && (d.K <= 768 || d.K >= 2048))) {
+  if (d.T <= kSideTokens) {
     plan_side(d, nsm, k_steps, &c);
     return c;
   }
