@@ -574,12 +574,13 @@ int rfx_block_norm(const rfx_block_norm_desc* desc, void* stream);
 /* Rotary positions on QKV rows x[b*S + s] = [num_q_heads q heads | num_kv_heads
  * k heads | num_kv_heads v heads (with v_out)], split into q, k and v, element
  * (b, h, s, d) at b * stride_b + h * stride_h + s * stride_s + d (head-major,
- * token-major, or over x itself).
+ * token-major, or over x itself; three strides of 0: packed, [B][heads][S][D]).
  * Pair i < rot_dim/2 of a q or k head is dims (i, i + rot_dim/2)
  * (RFX_ROPE_HALF) or (2i, 2i + 1) (RFX_ROPE_INTERLEAVED) and turns by
  * positions[b*S + s] * inv_freq[i] radians, times `magnitude`; dims past
  * rot_dim and v are copied.  An output lies over x exactly (each element at its
- * own input's address) or apart from it; else it is refused.  inv_freq is fp64 on the device (positions far
+ * own input's address) or apart from it, and none of its elements share an
+ * address; else it is refused.  inv_freq is fp64 on the device (positions far
  * beyond fp32's reach keep their angle), scaled by the caller for long
  * contexts.  head_dim <= 256, rot_dim even. */
 #define RFX_ROPE_HALF 0

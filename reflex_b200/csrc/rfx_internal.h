@@ -65,6 +65,17 @@ bool rows_shared(Rows a, Rows b);
 // Whether b is a, element for element: what an operator in place may be given.
 bool rows_same(const Rows& a, const Rows& b);
 
+// Places in memory: n[i] of them along each of three dimensions, step[i]
+// elements of `elem` bytes from one to the next, `width` elements at each.
+struct Places {
+  const void* p;
+  long elem, width;
+  long n[3], step[3];
+};
+// Whether two of the places share an element (exact, at any strides; true where
+// the strides are so tangled that a few thousand steps do not settle it).
+bool places_overlap(const Places& a);
+
 // Clusters of cluster_x CTAs of this kernel that can be resident at once (memoised; 0 when no device answers).
 int max_active_clusters(const void* func, int threads, int smem, int cluster_x);
 

@@ -307,7 +307,22 @@ static bool rope_place_ok(const rfx_rope_desc& d, const void* out, long heads, l
   return hi <= x || lo >= x + (static_cast<__int128>(T - 1) * d.ldx + heads * d.head_dim) * esz;
 }
 
-int validate_rope(const rfx_rope_desc& d) {
+// The descriptor with the strides of packed outputs written out.
+static rfx_rope_desc with_strides(rfx_rope_desc d) {
+  auto pack = [&](long H, long& sb, long& sh, long& ss) {
+    if (sb || sh || ss) return;
+    sb = H * d.S * d.head_dim;
+    sh = static_cast<long>(d.S) * d.head_dim;
+    ss = d.head_dim;
+  };
+  pack(d.num_q_heads, d.qs_b, d.qs_h, d.qs_s);
+  pack(d.num_kv_heads, d.ks_b, d.ks_h, d.ks_s);
+  pack(d.num_kv_heads, d.vs_b, d.vs_h, d.vs_s);
+  return d;
+}
+
+int validate_rope(const rfx_rope_desc& desc) {
+  const rfx_rope_desc d = with_strides(desc);
   if (d.B < 0 || d.S < 0 || static_cast<long>(d.B) * d.S > 0x7fffffffL - 1024)
     return set_error(RFX_E_INVAL, "rfx_rope: bad B/S (B=%d S=%d)", d.B, d.S);
   if (d.num_q_heads < 1 || d.num_kv_heads < 0 || d.num_q_heads > 1024 || d.num_kv_heads > 1024)
@@ -328,6 +343,15 @@ int validate_rope(const rfx_rope_desc& d) {
   if (!al(d.x, esz) || !al(d.q_out, esz) || !al(d.k_out, esz) || !al(d.v_out, esz) || !al(d.positions, 4) ||
       !al(d.inv_freq, 8))
     return set_error(RFX_E_INVAL, "rfx_rope: misaligned pointer");
+  const Places out[3] = {
+      {d.q_out, esz, d.head_dim, {d.B, d.num_q_heads, d.S}, {d.qs_b, d.qs_h, d.qs_s}},
+      {d.k_out, esz, d.head_dim, {d.B, d.num_kv_heads, d.S}, {d.ks_b, d.ks_h, d.ks_s}},
+      {d.v_out, esz, d.head_dim, {d.B, d.num_kv_heads, d.S}, {d.vs_b, d.vs_h, d.vs_s}},
+  };
+  for (const Places& o : out)
+    if (o.p && places_overlap(o))
+      return set_error(RFX_E_INVAL, "rfx_rope: heads or tokens of an output overlap (strides %ld, %ld, %ld)", o.step[0],
+                       o.step[1], o.step[2]);
   if (!rope_place_ok(d, d.q_out, heads, 0, d.num_q_heads, d.qs_b, d.qs_h, d.qs_s) ||
       !rope_place_ok(d, d.k_out, heads, d.num_q_heads, d.num_kv_heads, d.ks_b, d.ks_h, d.ks_s) ||
       !rope_place_ok(d, d.v_out, heads, d.num_q_heads + d.num_kv_heads, d.num_kv_heads, d.vs_b, d.vs_h, d.vs_s))
@@ -335,9 +359,10 @@ int validate_rope(const rfx_rope_desc& d) {
   return RFX_OK;
 }
 
-int launch_rope(const rfx_rope_desc& d, cudaStream_t stream, bool pdl) {
-  const int rc = validate_rope(d);
-  if (rc || d.B == 0 || d.S == 0) return rc;
+int launch_rope(const rfx_rope_desc& desc, cudaStream_t stream, bool pdl) {
+  const int rc = validate_rope(desc);
+  if (rc || desc.B == 0 || desc.S == 0) return rc;
+  const rfx_rope_desc d = with_strides(desc);
   RopeParams p{};
   p.T = d.B * d.S;
   p.S = d.S;

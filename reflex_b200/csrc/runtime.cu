@@ -3,6 +3,7 @@
 // word, and execution plans (ordered launch lists with CUDA-graph capture).
 #include "rfx_internal.h"
 
+#include <algorithm>
 #include <atomic>
 #include <cstdarg>
 #include <memory>
@@ -170,6 +171,75 @@ bool rows_shared(Rows a, Rows b) {
 
 bool rows_same(const Rows& a, const Rows& b) {
   return a.p == b.p && a.n == b.n && a.width == b.width && (a.pitch == b.pitch || a.n == 1);
+}
+
+// Two places i and j share an element where sum_k (j_k - i_k) step_k is within
+// a width of 0: one bounded equation in whole numbers.
+namespace {
+struct Term {
+  long step, lo, hi;  // step > 0; the difference of the indexes lies in lo..hi
+};
+long floor_div(long a, long b) { return a / b - (a % b != 0 && (a < 0)); }  // b > 0
+
+// Whether sum_k d_k step_k + r = off has a solution with d_k in lo..hi and r in
+// r_lo..r_hi, the terms in falling order of their steps: each index is within
+// what the later terms can make up, which are few candidates.
+bool solvable(const Term* t, int n, long off, long r_lo, long r_hi, int* budget) {
+  if (n == 0) return r_lo <= off && off <= r_hi;
+  long lo = r_lo, hi = r_hi;
+  for (int i = 1; i < n; ++i) {
+    lo += t[i].lo * t[i].step;
+    hi += t[i].hi * t[i].step;
+  }
+  const long first = std::max(t->lo, -floor_div(hi - off, t->step)), last = std::min(t->hi, floor_div(off - lo, t->step));
+  for (long d = first; d <= last; ++d) {
+    if (--*budget < 0) return true;
+    if (solvable(t + 1, n - 1, off - d * t->step, r_lo, r_hi, budget)) return true;
+  }
+  return false;
+}
+constexpr int kOverlapBudget = 4096;
+constexpr long kFarthest = 1l << 60;  // bytes: farther than any memory, and sums of a few stay within a long
+
+// The steps along which there is more than one place, in bytes, positive and
+// falling; false if they lead out of any memory.
+bool places_terms(const Places& a, Term (&t)[3], int* n) {
+  *n = 0;
+  __int128 reach = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (a.n[i] <= 1) continue;
+    const __int128 step = static_cast<__int128>(a.step[i]) * a.elem, size = step < 0 ? -step : step;
+    reach += size * (a.n[i] - 1);
+    if (reach > kFarthest) return false;
+    t[(*n)++] = Term{static_cast<long>(size), 0, a.n[i] - 1};
+  }
+  std::sort(t, t + *n, [](const Term& x, const Term& y) { return x.step > y.step; });
+  return true;
+}
+}  // namespace
+
+bool places_overlap(const Places& a) {
+  Term t[3];
+  int n;
+  if (!places_terms(a, t, &n)) return true;
+  const long width = a.width * a.elem;
+  // nested steps, each past all that the smaller ones reach: the usual layouts
+  long reach = width;
+  int i = n;
+  while (i > 0 && t[i - 1].step >= reach) {
+    --i;
+    reach += t[i].step * t[i].hi;
+  }
+  if (i == 0) return false;
+  if (t[n - 1].step == 0) return true;
+  // two places differ first in one index, and by symmetry it grows
+  int budget = kOverlapBudget;
+  for (i = 0; i < n; ++i) {
+    Term d[3];
+    for (int k = i; k < n; ++k) d[k - i] = Term{t[k].step, k == i ? 1 : -t[k].hi, t[k].hi};
+    if (solvable(d, n - i, 0, 1 - width, width - 1, &budget)) return true;
+  }
+  return false;
 }
 
 int max_active_clusters(const void* func, int threads, int smem, int cluster_x) {

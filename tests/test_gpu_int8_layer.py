@@ -774,3 +774,24 @@ def test_captured_direct_calls_follow_their_inputs():
         want = step()
         done()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_rope_packed_without_strides():
+    """A descriptor whose strides are all 0 writes packed [B][heads][S][D] outputs."""
+    r = gen(40)
+    x = r(2 * 5, 8 * 64).to(BF).cuda()
+    freq, _ = K.rope_frequencies(64)
+    pos = torch.arange(10, dtype=torch.int32, device="cuda")
+    q, k, v = (torch.empty(2, H, 5, 64, dtype=BF, device="cuda") for H in (4, 2, 2))
+    d = K.rope_desc(x=x, positions=pos, inv_freq=freq, q_out=q, k_out=k, v_out=v)
+    K.Plan.run_direct(d)
+    done()
+    want = [t.clone() for t in (q, k, v)]
+    for t in (q, k, v):
+        t.zero_()
+    for s in ("qs", "ks", "vs"):
+        for c in "bhs":
+            setattr(d, f"{s}_{c}", 0)
+    K.Plan.run_direct(d)
+    done()
+    assert all(torch.equal(a, b) for a, b in zip((q, k, v), want))

@@ -4,6 +4,7 @@ frequencies against their formulas."""
 import ctypes
 import math
 import os
+import random
 import subprocess
 
 import pytest
@@ -267,3 +268,82 @@ def test_rope_frequencies():
 def test_rope_frequencies_refusals(kw):
     with pytest.raises(ValueError):
         K.rope_frequencies(device="cpu", **kw)
+
+
+def plan_add(name, d):
+    """The plan add's return code and, where it refused, its message."""
+    lib = _lib.load()
+    plan = ctypes.c_void_p()
+    assert lib.rfx_plan_create(ctypes.byref(plan)) == _lib.RFX_OK
+    try:
+        rc = getattr(lib, "rfx_plan_add_" + name)(plan, ctypes.byref(d))
+        return rc, lib.rfx_last_error() if rc else b""
+    finally:
+        lib.rfx_plan_destroy(plan)
+
+
+def rope_at(**change):
+    """rope()'s tensors (x, positions, inv_freq, q, k, v at 1 to 6 A), every output packed head-major."""
+    d = rope()
+    for k, v in change.items():
+        setattr(d, k, v)
+    for n, h in (("q", d.num_q_heads), ("k", d.num_kv_heads), ("v", d.num_kv_heads)):
+        for s, packed in (("b", h * d.S * d.head_dim), ("h", d.S * d.head_dim), ("s", d.head_dim)):
+            if f"{n}s_{s}" not in change:
+                setattr(d, f"{n}s_{s}", packed)
+    d.ldx = max(d.ldx, (d.num_q_heads + 2 * d.num_kv_heads) * d.head_dim)
+    return d
+
+
+OWN_PLACES = [  # the strides of one rope output: whether its heads and tokens lie apart
+    ({}, True), (dict(B=3, num_kv_heads=2), True),
+    (dict(qs_h=64, qs_s=64), False),                      # head 1 of a token over head 0 of the next
+    (dict(qs_h=63), False), (dict(qs_s=63), False), (dict(B=2, qs_b=511), False), (dict(B=2, qs_b=448), False),
+    (dict(qs_h=64, qs_s=128), True), (dict(qs_h=64, qs_s=127), False),
+    (dict(qs_h=0), False), (dict(qs_s=0), False), (dict(qs_h=0, qs_s=0), False),
+    (dict(qs_h=192, qs_s=128), True),                     # 0, 128, 256, 384 and 192, 320, 448, 576: apart, nested in no order
+    (dict(qs_h=191, qs_s=128), False),
+    (dict(qs_h=-64, qs_s=128), True), (dict(qs_h=-256, qs_s=-64), True), (dict(qs_h=-64, qs_s=-64), False),
+    (dict(qs_b=1), True),                                 # one stream: its stride is not used
+    (dict(S=1, qs_s=0), True), (dict(ks_h=0), True), (dict(num_kv_heads=2, ks_h=0), False),
+    (dict(num_kv_heads=2, vs_h=64, vs_s=64), False), (dict(num_kv_heads=2, vs_h=64, vs_s=128), True),
+    (dict(B=2, qs_b=0, qs_h=0, qs_s=0), True),            # none given: packed, head-major
+    (dict(B=2, num_kv_heads=4, vs_b=0, vs_h=0, vs_s=0), True),
+]
+
+
+@pytest.mark.parametrize("change,fine", OWN_PLACES)
+def test_rope_outputs_lie_apart_from_themselves(change, fine):
+    """Two heads or tokens of an output at one place would be written by two
+    threads at once; three strides of 0 stand for a packed output."""
+    rc, why = plan_add("rope", rope_at(**change))
+    assert rc == (_lib.RFX_OK if fine else _lib.RFX_E_INVAL), why
+    assert fine or (b"rfx_rope" in why and b"overlap" in why)
+
+
+def places(d, n, heads):
+    """Every element's offset of output `n`, one per (stream, head, token, dim)."""
+    sb, sh, ss = (getattr(d, f"{n}s_{c}") for c in "bhs")
+    if not (sb or sh or ss):
+        sb, sh, ss = heads * d.S * d.head_dim, d.S * d.head_dim, d.head_dim
+    return [b * sb + h * sh + s * ss + e for b in range(d.B) for h in range(heads) for s in range(d.S)
+            for e in range(d.head_dim)]
+
+
+def test_rope_overlap_of_any_strides():
+    """Random strides, negative and tangled ones among them, against the
+    places written down one by one."""
+    rng = random.Random(1)
+    seen = [0, 0]
+    for _ in range(4000):
+        D = rng.choice([2, 4, 6])
+        top = rng.choice([8, 30, 100])
+        d = rope_at(B=rng.randint(1, 3), S=rng.randint(1, 4), num_q_heads=rng.randint(1, 4), num_kv_heads=0, head_dim=D,
+                    rot_dim=2, k_out=None, v_out=None, qs_b=rng.randint(-top, top), qs_h=rng.randint(-top, top),
+                    qs_s=rng.randint(-top, top))
+        at = places(d, "q", d.num_q_heads)
+        fine = len(set(at)) == len(at)
+        seen[fine] += 1
+        rc, why = plan_add("rope", d)
+        assert rc == (_lib.RFX_OK if fine else _lib.RFX_E_INVAL), (why, d.B, d.num_q_heads, d.S, D, d.qs_b, d.qs_h, d.qs_s)
+    assert min(seen) > 400, seen
