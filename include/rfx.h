@@ -579,8 +579,9 @@ int rfx_block_norm(const rfx_block_norm_desc* desc, void* stream);
  * (RFX_ROPE_HALF) or (2i, 2i + 1) (RFX_ROPE_INTERLEAVED) and turns by
  * positions[b*S + s] * inv_freq[i] radians, times `magnitude`; dims past
  * rot_dim and v are copied.  An output lies over x exactly (each element at its
- * own input's address) or apart from it, and none of its elements share an
- * address; else it is refused.  inv_freq is fp64 on the device (positions far
+ * own input's address) or apart from it, apart from positions, inv_freq and the
+ * other outputs, and none of its elements share an address; else it is refused.
+ * inv_freq is fp64 on the device (positions far
  * beyond fp32's reach keep their angle), scaled by the caller for long
  * contexts.  head_dim <= 256, rot_dim even. */
 #define RFX_ROPE_HALF 0

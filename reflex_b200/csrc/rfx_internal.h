@@ -72,9 +72,11 @@ struct Places {
   long elem, width;
   long n[3], step[3];
 };
-// Whether two of the places share an element (exact, at any strides; true where
-// the strides are so tangled that a few thousand steps do not settle it).
+// Whether two of the places share an element, or two sets of places do (false
+// with a null pointer).  Exact, at any strides; true where they are so tangled
+// that a few thousand steps do not settle it.
 bool places_overlap(const Places& a);
+bool places_shared(const Places& a, const Places& b);
 
 // Clusters of cluster_x CTAs of this kernel that can be resident at once (memoised; 0 when no device answers).
 int max_active_clusters(const void* func, int threads, int smem, int cluster_x);

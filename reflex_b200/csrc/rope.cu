@@ -290,21 +290,11 @@ const void* rope_ptr(bool half, bool vec) {
 
 }  // namespace
 
-// Whether an output whose first head is head `at` of x may be written: over x
-// element for element, or apart from it.
-static bool rope_place_ok(const rfx_rope_desc& d, const void* out, long heads, long at, int H, long sb, long sh, long ss) {
-  if (!out) return true;
-  const long esz = d.dtype == kDtypeBF16 ? 2 : 4;
-  const bool rows = (d.S == 1 || ss == d.ldx) && (d.B == 1 || sb == d.S * d.ldx);  // token rows at x's pitch
-  const uintptr_t x = reinterpret_cast<uintptr_t>(d.x), o = reinterpret_cast<uintptr_t>(out);
-  if (rows && (H == 1 || sh == d.head_dim) && o == x + at * d.head_dim * esz) return true;
-  const long T = static_cast<long>(d.B) * d.S;
-  const Rows in{d.x, T, d.ldx * esz, heads * d.head_dim * esz};
-  if (rows && sh >= 0) return !rows_shared(in, {out, T, d.ldx * esz, ((H - 1) * sh + d.head_dim) * esz});
-  __int128 lo = o, hi = o + static_cast<__int128>(d.head_dim) * esz;
-  const long n[3] = {d.B, H, d.S}, stride[3] = {sb, sh, ss};
-  for (int i = 0; i < 3; ++i) (stride[i] < 0 ? lo : hi) += static_cast<__int128>(n[i] - 1) * stride[i] * esz;
-  return hi <= x || lo >= x + (static_cast<__int128>(T - 1) * d.ldx + heads * d.head_dim) * esz;
+// Whether an output whose first head is head `at` of x lies over it element for element.
+static bool over_x(const rfx_rope_desc& d, const Places& out, long at) {
+  return (d.S == 1 || out.step[2] == d.ldx) && (d.B == 1 || out.step[0] == static_cast<__int128>(d.S) * d.ldx) &&
+         (out.n[1] == 1 || out.step[1] == d.head_dim) &&
+         reinterpret_cast<uintptr_t>(out.p) == reinterpret_cast<uintptr_t>(d.x) + at * d.head_dim * out.elem;
 }
 
 // The descriptor with the strides of packed outputs written out.
@@ -321,8 +311,7 @@ static rfx_rope_desc with_strides(rfx_rope_desc d) {
   return d;
 }
 
-int validate_rope(const rfx_rope_desc& desc) {
-  const rfx_rope_desc d = with_strides(desc);
+int validate_rope(const rfx_rope_desc& d) {
   if (d.B < 0 || d.S < 0 || static_cast<long>(d.B) * d.S > 0x7fffffffL - 1024)
     return set_error(RFX_E_INVAL, "rfx_rope: bad B/S (B=%d S=%d)", d.B, d.S);
   if (d.num_q_heads < 1 || d.num_kv_heads < 0 || d.num_q_heads > 1024 || d.num_kv_heads > 1024)
@@ -343,19 +332,31 @@ int validate_rope(const rfx_rope_desc& desc) {
   if (!al(d.x, esz) || !al(d.q_out, esz) || !al(d.k_out, esz) || !al(d.v_out, esz) || !al(d.positions, 4) ||
       !al(d.inv_freq, 8))
     return set_error(RFX_E_INVAL, "rfx_rope: misaligned pointer");
+  const rfx_rope_desc s = with_strides(d);
   const Places out[3] = {
-      {d.q_out, esz, d.head_dim, {d.B, d.num_q_heads, d.S}, {d.qs_b, d.qs_h, d.qs_s}},
-      {d.k_out, esz, d.head_dim, {d.B, d.num_kv_heads, d.S}, {d.ks_b, d.ks_h, d.ks_s}},
-      {d.v_out, esz, d.head_dim, {d.B, d.num_kv_heads, d.S}, {d.vs_b, d.vs_h, d.vs_s}},
+      {d.q_out, esz, d.head_dim, {d.B, d.num_q_heads, d.S}, {s.qs_b, s.qs_h, s.qs_s}},
+      {d.k_out, esz, d.head_dim, {d.B, d.num_kv_heads, d.S}, {s.ks_b, s.ks_h, s.ks_s}},
+      {d.v_out, esz, d.head_dim, {d.B, d.num_kv_heads, d.S}, {s.vs_b, s.vs_h, s.vs_s}},
   };
   for (const Places& o : out)
     if (o.p && places_overlap(o))
       return set_error(RFX_E_INVAL, "rfx_rope: heads or tokens of an output overlap (strides %ld, %ld, %ld)", o.step[0],
                        o.step[1], o.step[2]);
-  if (!rope_place_ok(d, d.q_out, heads, 0, d.num_q_heads, d.qs_b, d.qs_h, d.qs_s) ||
-      !rope_place_ok(d, d.k_out, heads, d.num_q_heads, d.num_kv_heads, d.ks_b, d.ks_h, d.ks_s) ||
-      !rope_place_ok(d, d.v_out, heads, d.num_q_heads + d.num_kv_heads, d.num_kv_heads, d.vs_b, d.vs_h, d.vs_s))
-    return set_error(RFX_E_INVAL, "rfx_rope: an output lies across x (over its own heads exactly, or apart from x)");
+  const long T = static_cast<long>(d.B) * d.S;
+  const Places x{d.x, esz, heads * d.head_dim, {T, 1, 1}, {d.ldx, 0, 0}};
+  const Places pos{d.positions, 4, T, {1, 1, 1}, {}}, freq{d.inv_freq, 8, d.rot_dim / 2, {1, 1, 1}, {}};
+  bool over[3];
+  for (int i = 0; i < 3; ++i) {
+    over[i] = over_x(d, out[i], i == 0 ? 0 : i == 1 ? d.num_q_heads : d.num_q_heads + d.num_kv_heads);
+    if (!over[i] && places_shared(out[i], x))
+      return set_error(RFX_E_INVAL, "rfx_rope: an output lies across x (over its own heads exactly, or apart from x)");
+    if (places_shared(out[i], pos) || places_shared(out[i], freq))
+      return set_error(RFX_E_INVAL, "rfx_rope: an output shares memory with positions or inv_freq");
+    // (what lies over x is apart from what does not, and from x's other heads)
+    for (int j = 0; j < i; ++j)
+      if (!over[i] && !over[j] && places_shared(out[i], out[j]))
+        return set_error(RFX_E_INVAL, "rfx_rope: two outputs share memory");
+  }
   return RFX_OK;
 }
 

@@ -173,8 +173,9 @@ bool rows_same(const Rows& a, const Rows& b) {
   return a.p == b.p && a.n == b.n && a.width == b.width && (a.pitch == b.pitch || a.n == 1);
 }
 
-// Two places i and j share an element where sum_k (j_k - i_k) step_k is within
-// a width of 0: one bounded equation in whole numbers.
+// Two places i and j share an element where their addresses are less than a
+// width apart: with addresses p + sum_k i_k step_k one bounded equation in whole
+// numbers.
 namespace {
 struct Term {
   long step, lo, hi;  // step > 0; the difference of the indexes lies in lo..hi
@@ -240,6 +241,37 @@ bool places_overlap(const Places& a) {
     if (solvable(d, n - i, 0, 1 - width, width - 1, &budget)) return true;
   }
   return false;
+}
+
+bool places_shared(const Places& a, const Places& b) {
+  if (!a.p || !b.p) return false;
+  Term ta[3], tb[3], t[6];
+  int na, nb, n = 0;
+  if (!places_terms(a, ta, &na) || !places_terms(b, tb, &nb)) return true;
+  // lowest address of either, and how far its places reach from there
+  auto lowest = [](const Places& x) {
+    __int128 at = static_cast<__int128>(reinterpret_cast<uintptr_t>(x.p));
+    for (int i = 0; i < 3; ++i)
+      if (x.n[i] > 1 && x.step[i] < 0) at += static_cast<__int128>(x.n[i] - 1) * x.step[i] * x.elem;
+    return at;
+  };
+  const long wa = a.width * a.elem, wb = b.width * b.elem;
+  long ra = wa, rb = wb;
+  for (int i = 0; i < na; ++i) ra += ta[i].hi * ta[i].step;
+  for (int i = 0; i < nb; ++i) rb += tb[i].hi * tb[i].step;
+  const __int128 off = lowest(b) - lowest(a);
+  if (off >= ra || -off >= rb) return false;
+  // off = sum i_k step_k - sum j_k step_k + r; equal steps are one term
+  for (int i = 0, j = 0; i < na || j < nb;) {
+    const long sa = i < na ? ta[i].step : -1, sb = j < nb ? tb[j].step : -1;
+    Term d{std::max(sa, sb), 0, 0};
+    if (d.step == 0) break;  // places on top of one another
+    for (; i < na && ta[i].step == d.step; ++i) d.hi += ta[i].hi;
+    for (; j < nb && tb[j].step == d.step; ++j) d.lo -= tb[j].hi;
+    t[n++] = d;
+  }
+  int budget = kOverlapBudget;
+  return solvable(t, n, static_cast<long>(off), 1 - wb, wa - 1, &budget);
 }
 
 int max_active_clusters(const void* func, int threads, int smem, int cluster_x) {

@@ -347,3 +347,83 @@ def test_rope_overlap_of_any_strides():
         rc, why = plan_add("rope", d)
         assert rc == (_lib.RFX_OK if fine else _lib.RFX_E_INVAL), (why, d.B, d.num_q_heads, d.S, D, d.qs_b, d.qs_h, d.qs_s)
     assert min(seen) > 400, seen
+
+
+# q 1024 bytes at 4 A, k and v 512 bytes at 5 A and 6 A, positions 16 bytes at 2 A, inv_freq 256 at 3 A
+STREAMS = dict(B=2, positions=2 * A, qs_b=1024, qs_h=64, qs_s=128)  # a workspace of 1024 elements per stream
+FAR = dict(B=64, S=6344, num_q_heads=8, num_kv_heads=4, x=1 << 40, q_out=2 << 40, k_out=3 << 40, v_out=(3 << 40) + 128)
+OTHER_PLACES = [  # rope outputs beside one another and beside the inputs
+    ({}, True),
+    (dict(k_out=4 * A), False), (dict(k_out=4 * A + 1022), False), (dict(k_out=4 * A + 1024), True),
+    (dict(k_out=4 * A - 510), False), (dict(k_out=4 * A - 512), True),
+    (dict(v_out=5 * A), False), (dict(v_out=5 * A + 510), False), (dict(v_out=5 * A + 512), True),
+    (dict(v_out=4 * A + 512), False),
+    (dict(k_out=5 * A, ks_s=128, v_out=5 * A + 128, vs_s=128), True),   # one cache, [S][k | v]
+    (dict(k_out=5 * A, ks_s=128, v_out=5 * A + 126, vs_s=128), False),
+    (dict(k_out=5 * A, ks_s=127, v_out=5 * A + 128, vs_s=127), False),
+    (dict(k_out=5 * A, ks_s=128, v_out=5 * A + 128, vs_s=192), False),  # the third token of each meets
+    (dict(num_kv_heads=2, ks_h=128, ks_s=256, v_out=5 * A + 128, vs_h=128, vs_s=256), True),  # [S][heads][k | v]
+    (dict(num_kv_heads=2, ks_h=128, ks_s=256, v_out=5 * A + 128, vs_h=64, vs_s=256), False),
+    (dict(STREAMS, k_out=4 * A + 1024, ks_b=1024, v_out=4 * A + 1536, vs_b=1024), True),
+    (dict(STREAMS, k_out=4 * A + 1024, ks_b=1024, v_out=4 * A + 1408, vs_b=1024), False),
+    (dict(STREAMS, k_out=4 * A + 896, ks_b=1024, v_out=4 * A + 1536, vs_b=1024), False),
+    (dict(STREAMS, k_out=4 * A + 1024, ks_b=512, v_out=6 * A, vs_b=256), False),  # stream 1's k over its q
+    (dict(k_out=5 * A + 384, ks_s=-64, v_out=5 * A + 512), True), (dict(k_out=5 * A + 384, ks_s=-64, v_out=5 * A), False),
+    (dict(q_out=2 * A), False), (dict(q_out=2 * A + 14), False), (dict(q_out=2 * A + 16), True),
+    (dict(q_out=2 * A - 1022), False), (dict(q_out=2 * A - 1024), True), (dict(v_out=2 * A), False),
+    (dict(k_out=3 * A), False), (dict(k_out=3 * A + 254), False), (dict(k_out=3 * A + 256), True),
+    (dict(v_out=3 * A + 2), False), (dict(rot_dim=32, v_out=3 * A + 128), True),
+    (dict(positions=4 * A + 128, qs_h=64, qs_s=256), False),            # positions in q's rows,
+    (dict(positions=4 * A + 256, qs_h=64, qs_s=256), True),             # or in the columns between them
+    (dict(q_out=4 * A, k_out=4 * A, v_out=4 * A, positions=4 * A, inv_freq=4 * A), False),
+    # caches of 64 streams, [stream][S][heads][k | v] and [stream][heads][S][k | v]
+    (dict(FAR, ks_b=6400 * 512, ks_h=128, ks_s=512, vs_b=6400 * 512, vs_h=128, vs_s=512), True),
+    (dict(FAR, ks_b=6400 * 512, ks_h=6400 * 128, ks_s=128, vs_b=6400 * 512, vs_h=6400 * 128, vs_s=128), True),
+    (dict(FAR, ks_b=6400 * 512, ks_h=6400 * 128, ks_s=128, vs_b=6400 * 512, vs_h=6400 * 128, vs_s=126), False),
+    (OVER_X, True), (dict(OVER_X, k_out=5 * A, ks_b=256, ks_s=64), True),
+    (dict(OVER_X, positions=A + 512), False), (dict(OVER_X, positions=A + 2048), True),
+    (dict(OVER_X, k_out=5 * A, ks_b=256, ks_s=64, v_out=5 * A, vs_b=256, vs_s=64), False),
+]
+
+
+@pytest.mark.parametrize("change,fine", OTHER_PLACES)
+def test_rope_outputs_lie_apart_from_the_rest(change, fine):
+    """CTAs read positions and inv_freq, and write q, k and v, in no order."""
+    rc, why = plan_add("rope", rope_at(**change))
+    assert rc == (_lib.RFX_OK if fine else _lib.RFX_E_INVAL), why
+    assert fine or (b"rfx_rope" in why and (b"share memory" in why or b"shares memory" in why or b"lies across" in why))
+
+
+def test_rope_sharing_of_any_strides():
+    """Random layouts of q, k and x in one small buffer, against the places
+    written down one by one."""
+    rng = random.Random(2)
+    seen = [0, 0]
+    for _ in range(6000):
+        D, S, B = rng.choice([2, 4]), rng.randint(1, 4), rng.randint(1, 2)
+        Hq, Hk = rng.randint(1, 2), rng.randint(1, 3)
+        T, width = B * S, (Hq + Hk) * D
+        ldx = width + rng.choice([0, 0, 2, 8, 13])
+        st = {}
+        for n in "qk":
+            st.update({f"{n}s_b": rng.choice([S * ldx, ldx * S + 5, 64, 31]), f"{n}s_h": rng.choice([D, S * D, -D, 9, 17]),
+                       f"{n}s_s": rng.choice([ldx, D, 2 * D, 33])})
+        at = lambda: A + 2 * rng.randint(-40, 160)  # noqa: E731
+        d = rope_at(B=B, S=S, num_q_heads=Hq, num_kv_heads=Hk, head_dim=D, rot_dim=2, v_out=None, **st)
+        d.ldx, d.x, d.q_out, d.k_out = ldx, A, rng.choice([A, at()]), rng.choice([A + 2 * Hq * D, at(), at()])
+        x = {t * ldx + e for t in range(T) for e in range(width)}
+        sets = []
+        fine = True
+        for n, h, own in (("q", Hq, 0), ("k", Hk, Hq * D)):
+            p = places(d, n, h)
+            off = (getattr(d, n + "_out") - A) // 2
+            p = [off + e for e in p]
+            over = p == [own + (b * S + s) * ldx + i * D + e for b in range(B) for i in range(h) for s in range(S)
+                         for e in range(D)]
+            fine &= len(set(p)) == len(p) and (over or not x & set(p))
+            sets.append(set(p))
+        fine &= not sets[0] & sets[1]
+        seen[fine] += 1
+        rc, why = plan_add("rope", d)
+        assert rc == (_lib.RFX_OK if fine else _lib.RFX_E_INVAL), (why, st, B, S, Hq, Hk, D, ldx, d.q_out - A, d.k_out - A)
+    assert min(seen) > 300, seen
