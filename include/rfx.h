@@ -544,7 +544,7 @@ int rfx_linear_i8(const rfx_linear_i8_desc* desc, void* stream);
  * with the scheme of rfx_quant_rows, to z_q / z_scale; with neither, only the
  * stream is updated; with y == NULL only the norm is computed (h' = h).
  * h_out may be h and z may be h or y (same stride); any other overlap of h, y
- * and the outputs is refused.  1 <= K <= 16384. */
+ * and the outputs, or of an output and a vector, is refused.  1 <= K <= 16384. */
 typedef struct rfx_block_norm_desc {
   int T, K, tokens_per_batch;
   int dtype;     /* of h, y, h_out and z: RFX_DTYPE_BF16 or RFX_DTYPE_F32 */

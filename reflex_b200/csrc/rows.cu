@@ -608,6 +608,24 @@ int validate_block_norm(const rfx_block_norm_desc& d) {
       (!rows_same(z, y) && rows_shared(z, y)) || rows_shared(z, ho) || rows_shared(q, h) || rows_shared(q, y) ||
       rows_shared(q, ho) || rows_shared(zs, h) || rows_shared(zs, y) || rows_shared(zs, ho) || rows_shared(zs, q))
     return set_error(RFX_E_INVAL, "rfx_block_norm: outputs overlap (in place only h_out or z over h, or z over y, at the same stride)");
+  const long B = (static_cast<long>(d.T) - 1) / d.tokens_per_batch + 1;
+  const Places vectors[5] = {
+      {d.post_w, 4, d.K, {1, 1, 1}, {}},
+      {d.gate, 4, d.K, {B, 1, 1}, {d.gate_stride, 0, 0}},
+      {d.norm_a1, 4, d.K, {1, 1, 1}, {}},
+      {d.norm_a2, 4, d.K, {B, 1, 1}, {d.norm_ab_stride, 0, 0}},
+      {d.norm_b2, 4, d.K, {B, 1, 1}, {d.norm_ab_stride, 0, 0}},
+  };
+  const Places outputs[4] = {
+      {d.h_out, esz, d.K, {d.T, 1, 1}, {d.ldho, 0, 0}},
+      {d.z, esz, d.K, {d.T, 1, 1}, {d.ldz, 0, 0}},
+      {d.z_q, 1, d.K, {d.T, 1, 1}, {d.ldzq, 0, 0}},
+      {d.z_scale, 4, d.T, {1, 1, 1}, {}},
+  };
+  for (const Places& o : outputs)
+    for (const Places& v : vectors)
+      if (places_shared(o, v))
+        return set_error(RFX_E_INVAL, "rfx_block_norm: an output shares memory with post_w, gate or a norm vector");
   if (!d.z && !d.z_q && (d.norm_a1 || d.norm_a2 || d.norm_b2))
     return set_error(RFX_E_INVAL, "rfx_block_norm: norm vectors without a norm output");
   if (!aligned(d.h, elem_size(d.dtype)) || !aligned(d.y, elem_size(d.dtype)) || !aligned(d.h_out, elem_size(d.dtype)) ||

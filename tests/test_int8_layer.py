@@ -427,3 +427,45 @@ def test_rope_sharing_of_any_strides():
         rc, why = plan_add("rope", d)
         assert rc == (_lib.RFX_OK if fine else _lib.RFX_E_INVAL), (why, st, B, S, Hq, Hk, D, ldx, d.q_out - A, d.k_out - A)
     assert min(seen) > 300, seen
+
+
+def norm_at(**change):
+    """norm() over two streams of two tokens, with all five vectors, gate and a2 / b2 at a batch stride of 64."""
+    d = norm()
+    d.tokens_per_batch = 2
+    d.post_w, d.gate, d.norm_a1, d.norm_a2, d.norm_b2 = (i * A for i in range(7, 12))
+    d.gate_stride = d.norm_ab_stride = 64
+    for k, v in change.items():
+        setattr(d, k, v)
+    return d
+
+
+TO_INT8 = dict(z=None, z_q=5 * A, z_scale=6 * A)
+VECTOR_PLACES = [  # block_norm's outputs (512 bytes each of h_out and z, 256 of z_q, 16 of z_scale) and its vectors
+    ({}, True), (TO_INT8, True),
+    (dict(post_w=3 * A), False), (dict(post_w=3 * A + 508), False), (dict(post_w=3 * A + 512), True),
+    (dict(post_w=3 * A - 252), False), (dict(post_w=3 * A - 256), True),
+    (dict(norm_a1=4 * A), False), (dict(norm_a1=3 * A), False), (dict(norm_a1=4 * A + 512), True),
+    (dict(gate=4 * A), False), (dict(gate=4 * A - 256), False), (dict(gate=4 * A - 512), True),  # its second stream's row
+    (dict(gate=4 * A - 256, gate_stride=0), True), (dict(gate=4 * A - 252, gate_stride=0), False),
+    (dict(gate=4 * A - 256, tokens_per_batch=4), True),                                          # one stream only
+    (dict(norm_a2=3 * A), False), (dict(norm_b2=3 * A), False), (dict(norm_a2=4 * A), False), (dict(norm_b2=4 * A), False),
+    (dict(norm_b2=4 * A - 1024, norm_ab_stride=256), False), (dict(norm_b2=4 * A - 1280, norm_ab_stride=256), True),
+    (dict(TO_INT8, norm_a1=5 * A), False), (dict(TO_INT8, gate=5 * A + 252), False), (dict(TO_INT8, gate=5 * A + 256), True),
+    (dict(TO_INT8, post_w=6 * A), False), (dict(TO_INT8, norm_b2=6 * A + 12), False), (dict(TO_INT8, norm_b2=6 * A + 16), True),
+    (dict(T=3, gate=4 * A - 256), False), (dict(T=2, gate=4 * A - 256), True),                   # the last stream cut short
+    # vectors in the columns between the outputs' rows
+    (dict(ldho=192, post_w=3 * A + 128), True), (dict(ldho=190, post_w=3 * A + 128), False),
+    (dict(ldho=192, gate=3 * A + 128, gate_stride=192), True), (dict(ldho=192, gate=3 * A + 128, gate_stride=96), True),
+    (dict(ldho=192, gate=3 * A + 128, gate_stride=64), False),
+    (dict(h_out=A, post_w=A), False), (dict(h_out=A, z=2 * A, norm_a1=2 * A), False),            # outputs in place
+    (dict(gate=7 * A), True), (dict(norm_a1=A), True), (dict(norm_b2=10 * A), True),             # inputs may share
+]
+
+
+@pytest.mark.parametrize("change,fine", VECTOR_PLACES)
+def test_block_norm_outputs_lie_apart_from_the_vectors(change, fine):
+    """Every CTA reads the vectors while others write their rows."""
+    rc, why = plan_add("block_norm", norm_at(**change))
+    assert rc == (_lib.RFX_OK if fine else _lib.RFX_E_INVAL), why
+    assert fine or (b"rfx_block_norm" in why and b"share" in why)
