@@ -356,6 +356,7 @@ def copy_rows(**kw) -> None:
 # each tensor as seldom as they can.
 _CODES = {torch.bfloat16: L.RFX_DTYPE_BF16, torch.float32: L.RFX_DTYPE_F32}
 _F32, _I8 = torch.float32, torch.int8
+_MOST = 0x7FFFFFFF  # what a descriptor's sizes hold; ctypes cuts off the rest
 _ENTRIES: dict = {}
 
 
@@ -388,6 +389,8 @@ def _matrix(name: str, t: torch.Tensor):
         T, K = t.shape
     except ValueError:
         raise ValueError(f"{name} must be a matrix, not {list(t.shape)}") from None
+    if T > _MOST or K > _MOST:
+        raise ValueError(f"{name}: at most 2^31 - 1 rows and columns, not {list(t.shape)}")
     return T, K
 
 
@@ -402,7 +405,7 @@ def _rows(name: str, t: torch.Tensor, T: int, K: int, align: int = 1) -> int:
         raise ValueError(f"{name} must be [{T}, {K}] with contiguous rows, not {list(t.shape)} (strides {t.stride()})")
     if T < 2:
         return -(-K // align) * align
-    if ld < K or T > 0x7FFFFFFF:
+    if ld < K or T > _MOST:
         raise ValueError(f"{name}: rows overlap (stride {ld}, length {K}), or more than 2^31 - 1 of them")
     return ld
 
@@ -531,7 +534,7 @@ def _block_norm(h, S, y, post_w, gate, residual_scale, h_out, norm_a1, norm_a2, 
         apart, s_at = apart or z_scale.get_device() != dev, _vector("z_scale", z_scale, T)
     if apart:
         raise _apart(h, y, post_w, gate, h_out, norm_a1, norm_a2, norm_b2, z, z_q, z_scale)
-    return L.BlockNormDesc(T, K, S if S <= 0x7FFFFFFF else 0x7FFFFFFF, _code("h", h), h.data_ptr(),
+    return L.BlockNormDesc(T, K, S if S <= _MOST else _MOST, _code("h", h), h.data_ptr(),
                            _rows("h", h, T, K), y_at, ldy, post_at, gate_at, gate_ld, residual_scale, ho_at, ldho,
                            a1_at, a2_at, b2_at, ab, eps, z_at, ldz, q_at, ldq, s_at), dev
 
@@ -631,7 +634,10 @@ def _rope(x, positions, inv_freq, q_out, k_out, v_out, pairs, magnitude):
             heads += Hkv
     elif v_out is not None:
         raise ValueError("v_out goes with k_out")
-    return L.RopeDesc(B, S, Hq, Hkv, D, 2 * inv_freq.shape[0], pairs, _code("x", x), x.data_ptr(),
+    rot = 2 * inv_freq.shape[0]
+    if max(B, Hq, S, D, Hkv, rot) > _MOST:
+        raise ValueError(f"sizes above 2^31 - 1: q_out {list(shape)}, {Hkv} KV heads, {rot} rotated dims")
+    return L.RopeDesc(B, S, Hq, Hkv, D, rot, pairs, _code("x", x), x.data_ptr(),
                       _rows("x", x, T, heads * D, 8), positions.data_ptr(), inv_freq.data_ptr(), magnitude,
                       *_heads("q_out", q_out, x, shape), *k, *v), dev
 

@@ -469,3 +469,50 @@ def test_block_norm_outputs_lie_apart_from_the_vectors(change, fine):
     rc, why = plan_add("block_norm", norm_at(**change))
     assert rc == (_lib.RFX_OK if fine else _lib.RFX_E_INVAL), why
     assert fine or (b"rfx_block_norm" in why and b"share" in why)
+
+
+HUGE = (1 << 32) + 16  # a 32-bit size would hold 16 of it
+
+
+@pytest.fixture
+def meta(monkeypatch):
+    """Makes the descriptor builders take meta tensors, which have sizes and no memory."""
+    monkeypatch.setattr(K, "_current", lambda dev: dev)
+    return lambda *shape, dt=torch.float32: torch.empty(*shape, dtype=dt, device="meta")
+
+
+@pytest.mark.parametrize("T,Kc", [(1, HUGE), (2, HUGE), (HUGE, 1), (1 << 31, 1), (1, 1 << 31)])
+def test_sizes_past_32_bits_are_refused(meta, T, Kc):
+    """Descriptors hold sizes in 32 bits: a larger one is refused, not cut."""
+    i8 = torch.int8
+    with pytest.raises(ValueError, match="2\\^31"):
+        K.quant_rows_desc(x=meta(T, Kc), q=meta(T, Kc, dt=i8), scale=meta(T))
+    with pytest.raises(ValueError, match="2\\^31"):
+        K.block_norm_desc(h=meta(T, Kc), S=1, z=meta(T, Kc))
+    with pytest.raises(ValueError, match="2\\^31"):
+        K.linear_i8_desc(w=meta(8, Kc, dt=i8), w_scale=meta(8), x=meta(T, Kc, dt=i8), x_scale=meta(T), y=meta(T, 8))
+    with pytest.raises(ValueError, match="2\\^31"):
+        K.linear_i8_desc(w=meta(T, Kc, dt=i8), w_scale=meta(T), x=meta(1, Kc, dt=i8), x_scale=meta(1), y=meta(1, T))
+
+
+@pytest.mark.parametrize("B,Hq,S,D,Hkv,pairs", [
+    (1, 1, 1, HUGE, 0, 8), (1, HUGE, 1, 16, 0, 8), (1, 1, HUGE, 16, 0, 8), (HUGE, 1, 1, 16, 0, 8), (1 << 16, 1, 1 << 16, 16, 0, 8),
+    (1, 1, 1, 16, HUGE, 8), (1, 1, 1, 16, 0, (1 << 31) + 8), (1, 1, 1, 16, 0, 1 << 30),
+])
+def test_rope_sizes_past_32_bits_are_refused(meta, B, Hq, S, D, Hkv, pairs):
+    kv = dict(k_out=meta(B, Hkv, S, D)) if Hkv else {}
+    with pytest.raises(ValueError, match="2\\^31"):
+        K.rope_desc(x=meta(B * S, (Hq + Hkv) * D), positions=meta(B * S, dt=torch.int32),
+                    inv_freq=meta(pairs, dt=torch.float64), q_out=meta(B, Hq, S, D), **kv)
+
+
+def test_largest_sizes_are_passed_on(meta):
+    """Sizes that fit reach the C entry's own limits unchanged."""
+    top = (1 << 31) - 1
+    d = K.quant_rows_desc(x=meta(1, top), q=meta(1, top, dt=torch.int8), scale=meta(1))
+    assert (d.T, d.K) == (1, top)
+    d = K.quant_rows_desc(x=meta(top, 1), q=meta(top, 1, dt=torch.int8), scale=meta(top))
+    assert (d.T, d.K) == (top, 1)
+    d = K.rope_desc(x=meta(top, 2), positions=meta(top, dt=torch.int32), inv_freq=meta(1, dt=torch.float64),
+                    q_out=meta(1, 1, top, 2))
+    assert (d.B, d.S, d.rot_dim) == (1, top, 2)
