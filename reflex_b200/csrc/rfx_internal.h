@@ -78,7 +78,7 @@ struct Places {
 bool places_overlap(const Places& a);
 bool places_shared(const Places& a, const Places& b);
 
-// Clusters of cluster_x CTAs of this kernel that can be resident at once (memoised; 0 when no device answers).
+// Clusters of cluster_x CTAs of this kernel that can be resident at once (memoised; 0 when the query fails).
 int max_active_clusters(const void* func, int threads, int smem, int cluster_x);
 
 // Raises the dynamic shared-memory limit of a kernel once per process.

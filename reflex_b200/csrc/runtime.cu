@@ -277,7 +277,7 @@ bool places_shared(const Places& a, const Places& b) {
 int max_active_clusters(const void* func, int threads, int smem, int cluster_x) {
   struct Entry {
     const void* func;
-    int smem, cluster, dev, n;
+    int threads, smem, cluster, dev, n;
   };
   static std::mutex mu;
   static Entry memo[256];  // a few kernels x cluster sizes x devices; the rest is asked again
@@ -289,9 +289,11 @@ int max_active_clusters(const void* func, int threads, int smem, int cluster_x) 
   }
   std::lock_guard<std::mutex> lk(mu);
   for (int i = 0; i < used; ++i)
-    if (memo[i].func == func && memo[i].smem == smem && memo[i].cluster == cluster_x && memo[i].dev == dev)
+    if (memo[i].func == func && memo[i].threads == threads && memo[i].smem == smem && memo[i].cluster == cluster_x &&
+        memo[i].dev == dev)
       return memo[i].n;
   int n = 0;
+  bool known = false;  // a query that failed is asked again
   if (ensure_smem_attr(func, smem) == RFX_OK) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(cluster_x));
@@ -304,10 +306,12 @@ int max_active_clusters(const void* func, int threads, int smem, int cluster_x) 
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess) n = 0;
+    known = cudaOccupancyMaxActiveClusters(&n, func, &cfg) == cudaSuccess;
+    if (!known) n = 0;
     cudaGetLastError();
   }
-  if (used < static_cast<int>(sizeof(memo) / sizeof(memo[0]))) memo[used++] = Entry{func, smem, cluster_x, dev, n};
+  if (known && used < static_cast<int>(sizeof(memo) / sizeof(memo[0])))
+    memo[used++] = Entry{func, threads, smem, cluster_x, dev, n};
   return n;
 }
 
