@@ -149,11 +149,12 @@ bool cluster_fits(const void* func, dim3 grid, int threads, int smem, int cluste
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   int n = 0;
-  const bool ok = cudaOccupancyMaxActiveClusters(&n, func, &cfg) == cudaSuccess && n > 0;
+  const bool known = cudaOccupancyMaxActiveClusters(&n, func, &cfg) == cudaSuccess;
   cudaGetLastError();
+  if (!known) return false;  // and asked again the next time
   std::lock_guard<std::mutex> lk(mu);
-  memo[key] = ok;
-  return ok;
+  memo[key] = n > 0;
+  return n > 0;
 }
 
 bool rows_shared(Rows a, Rows b) {

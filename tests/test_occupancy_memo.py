@@ -49,6 +49,17 @@ int main() {
   clusters(cudaSuccess, 5, 320, 1000, 4);                // known
   clusters(cudaSuccess, 0, 320, 3000, 4);                // none fits
   clusters(cudaSuccess, 5, 320, 3000, 4);                // known too
+  queries = 0;
+  auto fits = [&](cudaError_t s, int a, int cluster) {
+    status = s, answer = a;
+    const bool f = rfx::cluster_fits(fn, dim3(64), 192, 1000, cluster);
+    printf("fits %d %d\n", f ? 1 : 0, queries);
+  };
+  fits(cudaErrorMemoryAllocation, 9, 16);
+  fits(cudaSuccess, 9, 16);
+  fits(cudaSuccess, 0, 16);
+  fits(cudaSuccess, 0, 8);
+  fits(cudaSuccess, 9, 8);
 }
 """
 
@@ -71,3 +82,7 @@ def test_active_clusters_are_remembered_by_what_they_depend_on(said):
     """(answer, queries so far): a failed query answers 0 and is asked again;
     threads, shared memory, cluster size and device are told apart."""
     assert said("clusters") == [(0, 1), (37, 2), (37, 2), (12, 3), (11, 4), (7, 5), (30, 6), (37, 6), (0, 7), (0, 7)]
+
+
+def test_cluster_fits_is_remembered_once_it_is_known(said):
+    assert said("fits") == [(0, 1), (1, 2), (1, 2), (0, 3), (0, 3)]
