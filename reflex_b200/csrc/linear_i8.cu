@@ -37,7 +37,6 @@ struct I8Params {
   int n_tail;       // of the tiles from column cols_a on
   int cols_a, units;
   int stages;
-  int rows_a;       // token rows per copy: 128, or T rounded up to 8
   const int8_t* x;
   long ldx;
   const int8_t* w;
@@ -327,7 +326,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // both CTAs' copies count on the even CTA's barrier; a half without
       // tokens copies none (what its rows multiply is not stored)
       const bool has_x = t0 < p.T;
-      const int x_rows = p.rows_a * (has_x && t0 + kTileM < p.T ? 2 : 1);
+      const int x_rows = has_x && t0 + kTileM < p.T ? 2 * kTileM : kTileM;
       const uint32_t bytes = static_cast<uint32_t>(x_rows + tile.N) * kStepK;
       for (int i = 0; i < nk; ++i) {
         if (issued >= stages && !(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase ^ 1, p.status, kDevTimeoutStageEmpty))))
@@ -1018,7 +1017,6 @@ void plan_side(const rfx_linear_i8_desc& d, int nsm, int k_steps, LinearI8Plan* 
     }
   }
   c->nt = N;
-  c->rows_a = d.T;
   c->clusters = static_cast<int>(tiles);
 }
 
@@ -1037,9 +1035,9 @@ void plan_side(const rfx_linear_i8_desc& d, int nsm, int k_steps, LinearI8Plan* 
 // 128 of 800 x 20000 8.5 and 10.2, of 1024 x 2560 5.6 and 5.6, of 1024 x 8192 GeGLU
 // 7.7 and 7.5.
 //
-// Pair tiles: the width N and the split of K that finish soonest by this
-// model, whose figures are fitted to measured times of these projections at
-// 16 to 4096 tokens.  A K step takes 150 ns + 0.45 ns per weight row while the
+// Pair tiles, above 128 tokens: the width N and the split of K that finish
+// soonest by this model, whose figures are fitted to measured times of these
+// projections at 16 to 4096 tokens.  A K step takes 150 ns + 0.45 ns per weight row while the
 // copies into the SM bound it, 1.12 ns per weight row once the MMAs do, and
 // 1.17 times that over several rounds of tiles, each at least its epilogue's
 // 1.7 us + 10.5 ns per weight row (14.5 with GeGLU, 18.5 with an activation, 4
@@ -1130,7 +1128,6 @@ LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
     }
   }
   c.m_tiles = m;
-  c.rows_a = d.T < kTileM ? (d.T + 7) / 8 * 8 : kTileM;
   c.stages = std::min(kPairMaxStages, kPairRing / ((kTileM + c.nt / 2) * kStepK));
   return c;
 }
@@ -1177,7 +1174,7 @@ int build_linear_i8_maps(const rfx_linear_i8_desc& d, LinearI8Maps* maps) {
   maps->plan = plan_i8(d, nsm);
   const LinearI8Plan& c = maps->plan;
   if (c.form == kI8Few) return RFX_OK;
-  rc = make_tmap_2d(&maps->x, d.x, 1, d.K, d.T, d.ldx, kStepK, c.rows_a, true);
+  rc = make_tmap_2d(&maps->x, d.x, 1, d.K, d.T, d.ldx, kStepK, c.form == kI8Side ? d.T : kTileM, true);
   if (rc) return rc;
   if (c.form == kI8Side)
     return make_tmap_2d(&maps->w, d.w, 1, d.K, d.O, d.ldw, kStepK, d.epilogue == RFX_EPI_GEGLU ? kTileM / 2 : kTileM, true);
@@ -1216,7 +1213,6 @@ int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cuda
   p.cols_a = c.n_tiles;
   p.units = c.m_tiles * (c.n_tiles + c.n_tiles2);
   p.stages = c.stages;
-  p.rows_a = c.rows_a;
   p.x = static_cast<const int8_t*>(d.x);
   p.ldx = d.ldx;
   p.w = static_cast<const int8_t*>(d.w);

@@ -156,7 +156,7 @@ struct LinearI8Plan {
   int form;         // kI8Few: `clusters` CTAs, `splits` warps per pair of rows
   int nt, n_tiles;  // CTA pairs: weight rows per tile, tiles per token tile
   int nt2, n_tiles2;  // the narrower last tiles
-  int splits, stages, rows_a, m_tiles, clusters;
+  int splits, stages, m_tiles, clusters;
 };
 struct LinearI8Maps {
   CUtensorMap x, w, w2, y;
