@@ -795,3 +795,84 @@ def test_rope_packed_without_strides():
     K.Plan.run_direct(d)
     done()
     assert all(torch.equal(a, b) for a, b in zip((q, k, v), want))
+
+
+FAR = 1 << 31  # elements
+
+
+@pytest.fixture(scope="module")
+def far_buffer():
+    """4.3 GB whose rows can lie 2^31 elements of bf16 (2^32 of int8) apart."""
+    return torch.empty(FAR + (1 << 20), dtype=BF, device="cuda")
+
+
+@pytest.mark.parametrize("epi", [L.RFX_EPI_STORE, L.RFX_EPI_GEGLU])
+@pytest.mark.parametrize("T,off", [(129, 0), (129, 1), (129, 2), (129, 4), (300, 0), (300, 1)])
+def test_linear_i8_pair_tiles_past_32_bits(far_buffer, T, off, epi):
+    """Pair tiles (more than 128 tokens) into output rows whose offsets pass
+    2^31 elements: by the copy where rows lie on 16 bytes, in units of 2, 4 and
+    8 bytes where they do not."""
+    F, Kc = 96, 256
+    O = 2 * F if epi == L.RFX_EPI_GEGLU else F
+    ld = FAR // (T - 1) // 8 * 8 + 64 + off
+    q, x = ints(T, T, Kc)
+    w, wd = ints(T + 1, O, Kc)
+    sx, sw = torch.full((T,), 1e-2), torch.full((O,), 1e-2)
+    y = far_buffer.as_strided((T, F), (ld, 1))
+    y.fill_(7.0)
+    K.linear_i8(w=wd, w_scale=sw.cuda(), x=x, x_scale=sx.cuda(), y=y, epilogue=epi)
+    done()
+    want, tol = ref_linear(q, w, sx, sw, None, epi)
+    within(y, want, tol + 1.01 * HALF[BF] * np.abs(want))
+
+
+@pytest.mark.parametrize("T", [2, 50, 200])
+@pytest.mark.parametrize("which", ["x", "w"])
+def test_linear_i8_operands_past_32_bits(far_buffer, T, which):
+    """Token or weight rows whose offsets pass 2^32 bytes, in each of the three
+    forms: integer units, weights on the M side, pair tiles."""
+    O, Kc = 96, 272
+    q, x = ints(T, T, Kc)
+    w, wd = ints(T + 1, O, Kc)
+    n = T if which == "x" else O
+    ld = ((1 << 32) // (n - 1) // 16 + 4) * 16
+    far = far_buffer.view(torch.int8).as_strided((n, Kc), (ld, 1))
+    far.copy_(q if which == "x" else w)
+    sx, sw = torch.full((T,), 1e-2), torch.full((O,), 1e-2)
+    y = torch.empty(T, O, device="cuda")
+    K.linear_i8(w=far if which == "w" else wd, w_scale=sw.cuda(), x=far if which == "x" else x, x_scale=sx.cuda(), y=y)
+    done()
+    want, tol = ref_linear(q, w, sx, sw, None, L.RFX_EPI_STORE)
+    within(y, want, tol + 1.01 * U32 * np.abs(want))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("epi", [L.RFX_EPI_STORE, L.RFX_EPI_SILU, L.RFX_EPI_GELU, L.RFX_EPI_GEGLU])
+@pytest.mark.parametrize("T,Kc", [(4, 256), (50, 256), (50, 4096), (300, 256), (300, 16384)])
+def test_linear_i8_nonfinite_rows_and_channels_show(T, Kc, epi, dtype):
+    """In every form and with every activation a token, and an output channel,
+    whose scale is NaN or infinite with q 0 comes out as NaN; everything else
+    has the bits that it has without them."""
+    O = 128
+    F = O // 2 if epi == L.RFX_EPI_GEGLU else O
+    r = gen(T + Kc)
+    x, w = r(T, Kc).cuda(), (r(O, Kc) / math.sqrt(Kc)).cuda()
+    ys = []
+    for bad in (False, True):
+        xb, wb = x.clone(), w.clone()
+        if bad:
+            xb[1, 5], xb[T - 1, Kc - 1] = float("nan"), float("inf")
+            wb[3, 0], wb[F - 1, 7] = float("-inf"), float("nan")
+        q, s = torch.empty(T, Kc, dtype=torch.int8, device="cuda"), torch.empty(T, device="cuda")
+        wq, ws = torch.empty(O, Kc, dtype=torch.int8, device="cuda"), torch.empty(O, device="cuda")
+        K.quant_rows(x=xb, q=q, scale=s)
+        K.quant_rows(x=wb, q=wq, scale=ws)
+        y = torch.empty(T, F, dtype=dtype, device="cuda")
+        K.linear_i8(w=wq, w_scale=ws, x=q, x_scale=s, y=y, epilogue=epi)
+        ys.append(y)
+    done()
+    gone = torch.zeros(T, F, dtype=torch.bool, device="cuda")
+    gone[[1, T - 1]] = True
+    gone[:, [3, F - 1]] = True
+    assert torch.isfinite(ys[0]).all()
+    assert torch.isnan(ys[1][gone]).all() and torch.equal(ys[1][~gone], ys[0][~gone])
