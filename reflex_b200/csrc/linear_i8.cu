@@ -95,14 +95,14 @@ __device__ __forceinline__ void st_dsmem_i4(uint32_t addr, const int (&v)[4]) {
 // split owns into that CTA's (now idle) operand ring through DSMEM and adds
 // what it receives to its own.
 //
-// Measured: 4096 x 4096 x 4096 47 us, 2.9 POP/s (87 % of twice the measured
-// bf16 burst rate; 55 us, 89 % of twice the sustained one, in a loop under the
-// power cap); 768 x 32768 x 2048 GeGLU 40 us (2.6 POP/s); 768 x 2048 x 16384
-// 24 us (2.2 POP/s, two splits).  With the MMAs left out the first takes 34 us
-// and with the copies left out 39: both streams are near their limit, and they
-// share the SM's shared memory.  Calls of one tile per pair spend about 7 us
-// outside the product: set-up 1, the first copy 1.2 - 1.8, the last epilogue
-// 2 - 3 and the pair's exit 0.8.
+// Measured, T x O x K: 4096 x 4096 x 4096 48 us, 2.8 POP/s (85 % of twice the
+// measured bf16 burst rate; 55 us, 89 % of twice the sustained one, in a loop under
+// the power cap); 768 x 32768 x 2048 GeGLU 39 us (2.6 POP/s; this instance spills
+// 32 bytes at its 168 registers); 768 x 2048 x 16384 24 us (2.1 POP/s, two
+// splits).  With the MMAs left out the first takes 34 us and with the copies left
+// out 39: both streams are near their limit, and they share the SM's shared
+// memory.  Calls of one tile per pair spend about 7 us outside the product: set-up
+// 1, the first copy 1.2 - 1.8, the last epilogue 2 - 3 and the pair's exit 0.8.
 constexpr int kPairThreads = 320;
 constexpr int kPairMaxStages = 10;
 constexpr int kPairRing = 6 * 2 * kTileM * kStepK;     // operand ring: 6 stages of N = 256, more of a narrower N
@@ -588,9 +588,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 //
 // Bound by what an SM takes in, 16 KB of weights and T x 128 bytes of tokens per
 // K step, about 75 GB/s of the former, and by 3 to 4 us around the product.
-// Measured (captured; in brackets as pair tiles): 50 x 1024 x 8192 GeGLU 6.5 us
-// (7.5), 50 x 4096 x 1024 5.5 (9.4), 16 x 1024 x 2560 3.4 (5.4), 50 x 2048 x
-// 32768 GeGLU 15.4, 4.4 TB/s of weights (19.7), 16 x 16384 x 2048 10.2 (16.3).
+// Measured, T x O x K (captured; in brackets as pair tiles): 50 x 8192 x 1024 GeGLU
+// 6.6 us (7.5), 50 x 1024 x 4096 5.5 (9.4), 16 x 2560 x 1024 3.3 (5.4), 50 x 32768 x
+// 2048 GeGLU 14.8, 4.5 TB/s of weights (19.7), 16 x 2048 x 16384 10.0 (16.3).
 constexpr int kSideTokens = 128;  // the registers of an SM allow three CTAs: 384 of its 512 TMEM columns
 constexpr int kSideThreads = 320;
 constexpr int kSideMaxSplits = 8;
@@ -824,10 +824,9 @@ __global__ void __launch_bounds__(kSideThreads, 3)
 // Up to 4 tokens: the weights are read once, 16 bytes per lane and load, and
 // multiplied on the integer units (4 products per instruction): no tiles, no
 // shared-memory round trip, nothing to set up, so a single token's call costs
-// little more than the memory's latency (3.0 us for 2048 x 2560, 14.6 us or
-// 4.6 TB/s for the 67 MB of a 2048 x 32768 GeGLU).  A
-// warp takes two weight rows (GeGLU: a gate row and its up row) over a 1/kw
-// part of K; x comes through L1.
+// little more than the memory's latency (O x K: 3.0 us for 2560 x 2048, 12.1 us or
+// 5.5 TB/s for the 67 MB of a 32768 x 2048 GeGLU).  A warp takes two weight rows
+// (GeGLU: a gate row and its up row) over a 1/kw part of K; x comes through L1.
 constexpr int kFewTokens = 4;
 constexpr long kFewSmall = 16 << 20;  // bytes of weights for 3 and 4 tokens
 constexpr int kFewThreads = 256;
@@ -1025,14 +1024,14 @@ void plan_side(const rfx_linear_i8_desc& d, int nsm, int k_steps, LinearI8Plan* 
 // Up to 4 tokens go to the integer units, unless the layer is wide and short
 // (16 output rows and more per column of K: a warp's part is then too small) or,
 // with 3 or 4 tokens, large (the products bound them).  Measured there and with
-// the weights on the M side: 1 token of 1024 x 2560 2.8 and 3.1 us, of 1024 x
-// 8000 3.3 and 4.8, of 256 x 21953 5.8 and 3.8; 4 tokens of 1024 x 8000 4.7 and
-// 4.8, of 16384 x 2048 12.3 and 10.1.
+// the weights on the M side, O x K: 1 token of 2560 x 1024 2.8 and 3.1 us, of 8000 x
+// 1024 3.3 and 4.8, of 21953 x 256 5.8 and 3.8; 4 tokens of 8000 x 1024 4.7 and
+// 4.8, of 2048 x 16384 12.3 and 10.1.
 //
 // The weights lie on the M side up to 128 tokens.  Measured there and as pair
-// tiles: 50 tokens of 1024 x 8192 GeGLU 6.5 and 7.5 us, of 4096 x 1024 5.5 and 9.4,
-// of 2048 x 32768 GeGLU 15.4 and 19.7; 96 tokens of 1152 x 4304 GELU 6.0 and 6.9;
-// 128 of 800 x 20000 8.5 and 10.2, of 1024 x 2560 5.6 and 5.6, of 1024 x 8192 GeGLU
+// tiles, O x K: 50 tokens of 8192 x 1024 GeGLU 6.5 and 7.5 us, of 1024 x 4096 5.5 and
+// 9.4, of 32768 x 2048 GeGLU 15.4 and 19.7; 96 tokens of 4304 x 1152 GELU 6.0 and 6.9;
+// 128 of 20000 x 800 8.5 and 10.2, of 2560 x 1024 5.6 and 5.6, of 8192 x 1024 GeGLU
 // 7.7 and 7.5.
 //
 // Pair tiles, above 128 tokens: the width N and the split of K that finish
@@ -1044,7 +1043,7 @@ void plan_side(const rfx_linear_i8_desc& d, int nsm, int k_steps, LinearI8Plan* 
 // more for fp32 and 16 more where output rows are off the 16-byte grid); the
 // last epilogue is not hidden, and where K is split adding up costs 0.9 us + 0.4
 // us per split.  (An epilogue's fixed part measures 0.5 us; counted as that, the
-// model takes narrower tiles that are up to 18 % slower.  3200 x 72 x 21952: 73 us
+// model takes narrower tiles that are up to 18 % slower.  3200 x 21952 x 72: 73 us
 // in tiles of 64 rows, 52 in tiles of 256.)
 LinearI8Plan plan_i8(const rfx_linear_i8_desc& d, int nsm) {
   LinearI8Plan c{};

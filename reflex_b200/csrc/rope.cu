@@ -9,9 +9,11 @@
 // the angle is formed in fp64 turns, p * f_i / (2 pi), of which only the
 // fraction goes on to fp32 (a fp32 angle would be off by 0.03 rad at position
 // 10^6), once per token and pair; all heads of the token share it through
-// shared memory.  Bound by the rows' one read and one write: 6344 tokens of 10
-// heads x 256 (half of each interleaved) take 14.9 us, 4.3 TB/s, 66 % of the
-// measured copy rate; 3200 tokens (64 streams) 11.4 us; one stream's 50 2.2 us.
+// shared memory.  The floor is the rows' one read and one write: 6344 tokens of
+// 10 heads x 256 (half of each interleaved) take 15.1 us, 4.3 TB/s, 66 % of the
+// measured copy rate, the rest of the time waiting for loads (a thread requests
+// two tokens, turns and stores them, and then requests the next two); 3200 tokens
+// (64 streams) 11.5 us; one stream's 50 2.2 us.
 #include "rfx_internal.h"
 
 #include <algorithm>
@@ -161,8 +163,9 @@ __device__ __forceinline__ void token_angles(const RopeParams& p, int t0, int nt
   }
 }
 
-// Threads on an SM, and tokens whose loads a thread has in flight: a half-split
-// item is two loads, an interleaved one is one.
+// Resident threads on an SM, which limit a thread to 64 or 40 registers: a
+// half-split item is two loads, an interleaved one is one.  (The bf16 vector kernels
+// spill 12 and 16 bytes at these limits.)
 template <bool TWO_LOADS>
 constexpr int resident_threads() {
   return TWO_LOADS ? 1024 : 1536;

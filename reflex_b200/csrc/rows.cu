@@ -6,14 +6,18 @@
 // that read it, through every reduction, until its outputs are written: TPR
 // threads per row, NV vectors of 8 elements per thread.
 //
-// Both operators are bound by memory traffic in principle; what keeps them
-// from it is the instructions per element (a row of 1024 costs 360 warp
-// instructions in block_norm, half of them reductions, divisions and
-// addresses) and, for few rows, the latency of one row's chain of reductions.
-// Measured: int8 rows of 768 x 16384 bf16 10.3 us (3.7 TB/s); block_norm with
-// everything on, 3200 x 1024 bf16 to int8, 9.2 us (2.6 TB/s), 768 x 2048 fp32
-// 7.5 us (3.3 TB/s), 50 x 1024 2.6 us.  Rows off the 16-byte grid take element
-// accesses: 3200 x 1025 24 us.
+// Both operators would be bound by memory traffic; what keeps them from it is
+// latency.  With everything on, block_norm of 3200 x 1024 bf16 to int8 has 5
+// warps on a scheduler, which issues in 52 % of its active clocks: each warp
+// waits for its loads, then for dependent arithmetic (340 instructions in each of
+// a row's four warps) and for the shuffles and shared memory of up to three
+// reductions in a chain.  768 x 2048 fp32 issues in 29 %, mostly waiting for the
+// loads and the reductions of 5 or 6 rows per SM.  Quantizing 768 rows of 16384
+// issues in 56 %, and the rows are whole: 296 CTAs take 2 or 3 of them, 6 on the
+// busiest SM where 5.2 is the mean (888 rows, 6 on each, take 10.9 us).
+// Measured: int8 rows of 768 x 16384 bf16 10.4 us (3.6 TB/s); block_norm 3200 x
+// 1024 bf16 to int8 9.3 us (2.5 TB/s), 768 x 2048 fp32 7.8 us (3.2 TB/s), 50 x 1024
+// 2.6 us.  Rows off the 16-byte grid take element accesses: 3200 x 1025 25 us.
 #include "quant_i8.cuh"
 #include "rfx_internal.h"
 
@@ -365,7 +369,9 @@ __device__ __forceinline__ void column_shift(const float* b, int K, int tid, int
 //   h' = h + (u * rstd_u) * [residual_scale * gate * post_w],
 //   z  = (h' * rstd_h) * [a1 * a2] + b2,
 // which with one vector of 8 per thread stays in registers from row to row and
-// with longer rows is formed again from L1.
+// with longer rows is formed again from L1.  (The register limit of 768 resident
+// threads spills 8 to 20 bytes in four instances: fp32 rows of up to 256, and
+// without vector accesses bf16 rows of up to 256 and fp32 rows of 1025 to 2048.)
 template <typename T, int TPR, int NV, bool VEC>
 __global__ void __launch_bounds__(TPR* rows_per_cta<TPR>(), TPR <= 128 ? 6 : NV == 1 ? 768 / TPR : 1)
     block_norm_kernel(const BlockNormParams p) {
