@@ -606,6 +606,90 @@ typedef struct rfx_rope_desc {
 } rfx_rope_desc;
 int rfx_rope(const rfx_rope_desc* desc, void* stream);
 
+/* ------------------------------------------------ 4-bit layer operators ---- */
+/* Rows of 4-bit floating point numbers with a scale per block.  No counterpart
+ * in the reference, whose layers stay in bf16 (reflex/layers/linear.py:72-148).
+ *
+ * A row of K values is ceil(K / 2) bytes of e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * and their negatives), element k in byte k / 2, the even one in the low half;
+ * with an odd K the last high half is 0.  Rows begin on 16-byte boundaries.
+ *   RFX_FP4_MX: blocks of 32, scale 2^(byte - 127) (e8m0; 255 is NaN).
+ *   RFX_FP4_NV: blocks of 16, e4m3 scale, times row_scale[t] (fp32).
+ * The scale bytes lie in tiles of 128 rows x 4 blocks, 512 bytes each, in the
+ * order in which the tensor cores take them: row t's byte of block j is at
+ *   ((t / 128) * ceil(K / (4 * block)) + j / 4) * 512 + (t % 32) * 16 + (t % 128) / 32 * 4 + j % 4.
+ * A row's last group of 4 holds zeros past its last block; bytes of rows past
+ * the last one are never used.  With rows_per_part > 0 the tiles begin anew at
+ * every rows_per_part rows (RFX_EPI_GEGLU takes a weight [Wgate; Wup] of two
+ * parts), t above being the row in its part and the parts' tiles following
+ * one another. */
+#define RFX_FP4_MX 0
+#define RFX_FP4_NV 1
+
+/* Rows of bf16 or fp32 to 4 bits.  absmax is a block's (NV: and a row's)
+ * largest magnitude; every quotient is one correctly rounded fp32 division.
+ *   MX: e = max(floor(log2 absmax) - 2, -127); q = e2m1(x / 2^e).
+ *   NV: row_scale = 2^max(floor(log2 absmax_row) - 10, -100);
+ *       s = e4m3(absmax / 6 / row_scale); q = e2m1(x / (s * row_scale)), 0 where s is 0.
+ * e2m1 and e4m3 round to nearest even, e2m1 to at most 6.  A block (NV: a row)
+ * that holds a NaN or an infinity has q = 0 and scale NaN (NV: row_scale NaN,
+ * scale bytes 0): what is computed from it is NaN, never a plausible number.
+ * The outputs share no memory with x or one another.  K <= 65536. */
+typedef struct rfx_quant_fp4_desc {
+  int T, K;
+  int format;   /* RFX_FP4_* */
+  int in_dtype; /* RFX_DTYPE_BF16 or RFX_DTYPE_F32 */
+  int rows_per_part; /* 0: one part */
+  const void* x; /* [T][ldx] */
+  long ldx;
+  void* q;  /* [T][ldq] bytes, 16-byte aligned, ldq a multiple of 16 */
+  long ldq;
+  void* scale;      /* 16-byte aligned */
+  float* row_scale; /* [T], RFX_FP4_NV only */
+} rfx_quant_fp4_desc;
+int rfx_quant_fp4(const rfx_quant_fp4_desc* desc, void* stream);
+
+/* What 4-bit rows stand for, as bf16 or fp32 (one rounding). */
+typedef struct rfx_dequant_fp4_desc {
+  int T, K;
+  int format;
+  int out_dtype;
+  int rows_per_part;
+  const void* q; /* [T][ldq] bytes */
+  long ldq;
+  const void* scale;
+  const float* row_scale; /* RFX_FP4_NV only */
+  void* y; /* [T][ldy] */
+  long ldy;
+} rfx_dequant_fp4_desc;
+int rfx_dequant_fp4(const rfx_dequant_fp4_desc* desc, void* stream);
+
+/* y = act(x_row[t] * w_row[o] * (x . w^T) + bias[o]) of two matrices of 4-bit
+ * rows of one format (row scales 1 with MX), products and sums in fp32 on the
+ * tensor cores, one rounding to the output type.  Epilogues STORE, SILU, GELU
+ * and GEGLU (w = [Wgate; Wup], its scales in two parts of O / 2 rows; y has
+ * O / 2 columns).  The order of the sum depends on the shape alone.  A row or
+ * channel with a NaN scale gives NaN outputs, no others.
+ * y shares no memory with an input.  1 <= K <= 65536. */
+typedef struct rfx_linear_fp4_desc {
+  int T, O, K;
+  int format;    /* RFX_FP4_* of x and w */
+  int epilogue;  /* RFX_EPI_STORE, SILU, GELU or GEGLU */
+  int out_dtype; /* RFX_DTYPE_BF16 or RFX_DTYPE_F32 */
+  const void* x; /* [T][ldx] bytes */
+  long ldx;
+  const void* x_scale;
+  const float* x_row_scale; /* [T], RFX_FP4_NV only */
+  const void* w; /* [O][ldw] bytes */
+  long ldw;
+  const void* w_scale;
+  const float* w_row_scale; /* [O], RFX_FP4_NV only */
+  const float* bias;        /* [O] or NULL */
+  void* y;                  /* [T][ldy] */
+  long ldy;
+} rfx_linear_fp4_desc;
+int rfx_linear_fp4(const rfx_linear_fp4_desc* desc, void* stream);
+
 /* ------------------------------------------------ fused chunk executor ---- */
 /* The whole PI0.5 denoising loop of one chunk (all Euler steps x layers:
  * input norm, QKV+RoPE, partitioned attention over the context ring,
@@ -712,6 +796,9 @@ int rfx_plan_add_quant_rows(rfx_plan* plan, const rfx_quant_rows_desc* desc);
 int rfx_plan_add_linear_i8(rfx_plan* plan, const rfx_linear_i8_desc* desc);
 int rfx_plan_add_block_norm(rfx_plan* plan, const rfx_block_norm_desc* desc);
 int rfx_plan_add_rope(rfx_plan* plan, const rfx_rope_desc* desc);
+int rfx_plan_add_quant_fp4(rfx_plan* plan, const rfx_quant_fp4_desc* desc);
+int rfx_plan_add_dequant_fp4(rfx_plan* plan, const rfx_dequant_fp4_desc* desc);
+int rfx_plan_add_linear_fp4(rfx_plan* plan, const rfx_linear_fp4_desc* desc);
 /* The chunk (not owned by the plan) is run at this point: counter clear + one launch. */
 int rfx_plan_add_chunk(rfx_plan* plan, rfx_chunk* chunk);
 /* The next op added is launched without programmatic dependent launch: it

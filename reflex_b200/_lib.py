@@ -46,6 +46,9 @@ RFX_PACK_GATE_UP = 1
 RFX_ROPE_HALF = 0
 RFX_ROPE_INTERLEAVED = 1
 
+RFX_FP4_MX = 0
+RFX_FP4_NV = 1
+
 RFX_ADARMS_GATE = 0
 RFX_ADARMS_SSG = 1
 
@@ -246,6 +249,31 @@ class RopeDesc(Structure):
     ]
 
 
+class QuantFp4Desc(Structure):
+    _fields_ = [
+        ("T", c_int), ("K", c_int), ("format", c_int), ("in_dtype", c_int), ("rows_per_part", c_int),
+        ("x", c_void_p), ("ldx", c_long), ("q", c_void_p), ("ldq", c_long), ("scale", c_void_p),
+        ("row_scale", c_void_p),
+    ]
+
+
+class DequantFp4Desc(Structure):
+    _fields_ = [
+        ("T", c_int), ("K", c_int), ("format", c_int), ("out_dtype", c_int), ("rows_per_part", c_int),
+        ("q", c_void_p), ("ldq", c_long), ("scale", c_void_p), ("row_scale", c_void_p), ("y", c_void_p),
+        ("ldy", c_long),
+    ]
+
+
+class LinearFp4Desc(Structure):
+    _fields_ = [
+        ("T", c_int), ("O", c_int), ("K", c_int), ("format", c_int), ("epilogue", c_int), ("out_dtype", c_int),
+        ("x", c_void_p), ("ldx", c_long), ("x_scale", c_void_p), ("x_row_scale", c_void_p),
+        ("w", c_void_p), ("ldw", c_long), ("w_scale", c_void_p), ("w_row_scale", c_void_p),
+        ("bias", c_void_p), ("y", c_void_p), ("ldy", c_long),
+    ]
+
+
 # Every entry point declared in include/rfx.h: name -> (argtypes, restype).
 SIGNATURES = {
     "rfx_version": ([], c_int),
@@ -285,6 +313,12 @@ SIGNATURES = {
     "rfx_plan_add_linear_i8": ([c_void_p, POINTER(LinearI8Desc)], c_int),
     "rfx_plan_add_block_norm": ([c_void_p, POINTER(BlockNormDesc)], c_int),
     "rfx_plan_add_rope": ([c_void_p, POINTER(RopeDesc)], c_int),
+    "rfx_quant_fp4": ([POINTER(QuantFp4Desc), c_void_p], c_int),
+    "rfx_dequant_fp4": ([POINTER(DequantFp4Desc), c_void_p], c_int),
+    "rfx_linear_fp4": ([POINTER(LinearFp4Desc), c_void_p], c_int),
+    "rfx_plan_add_quant_fp4": ([c_void_p, POINTER(QuantFp4Desc)], c_int),
+    "rfx_plan_add_dequant_fp4": ([c_void_p, POINTER(DequantFp4Desc)], c_int),
+    "rfx_plan_add_linear_fp4": ([c_void_p, POINTER(LinearFp4Desc)], c_int),
     "rfx_plan_add_chunk": ([c_void_p, c_void_p], c_int),
     "rfx_chunk_workspace_size": ([POINTER(ChunkDesc), POINTER(c_size_t)], c_int),
     "rfx_chunk_create": ([POINTER(ChunkDesc), c_void_p, c_size_t, POINTER(c_void_p)], c_int),
@@ -346,5 +380,6 @@ def ptr(t) -> int | None:
 __all__ = [n for n in dir() if n.startswith(("RFX_", "Rfx"))] + [
     "KvQuantDesc", "LinearDesc", "AttnDesc", "TimeCondDesc", "ModulationDesc", "ActionIoDesc", "CopyRowsDesc",
     "NormDesc", "ChunkDesc", "QuantRowsDesc", "LinearI8Desc", "BlockNormDesc", "RopeDesc",
+    "QuantFp4Desc", "DequantFp4Desc", "LinearFp4Desc",
     "SIGNATURES", "load", "check", "call", "ptr", "LIB_PATH", "c_ubyte",
 ]

@@ -238,6 +238,37 @@ __device__ __forceinline__ void umma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uin
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// D (TMEM, fp32) (+)= (A * scale A) (B * scale B)^T over 64 values of e2m1, with
+// scales in TMEM: an e8m0 number per 32 of them (kind::mxf4) or an e4m3 one per 16
+// (kind::mxf4nvf4).
+template <bool MX, bool PAIR>
+__device__ __forceinline__ void umma_fp4_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t a_scale, uint32_t b_scale, uint32_t accumulate) {
+#define RFX_UMMA_FP4(GROUP, KIND, VEC)                                                                      \
+  asm volatile(                                                                                             \
+      "{\n\t.reg .pred p;\n\t"                                                                              \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                           \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" KIND ".block_scale.scale_vec::" VEC                         \
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),                                               \
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale), "r"(b_scale), "r"(accumulate)                     \
+      : "memory")
+  if (MX && PAIR) RFX_UMMA_FP4("2", "mxf4", "2X");
+  if (MX && !PAIR) RFX_UMMA_FP4("1", "mxf4", "2X");
+  if (!MX && PAIR) RFX_UMMA_FP4("2", "mxf4nvf4", "4X");
+  if (!MX && !PAIR) RFX_UMMA_FP4("1", "mxf4nvf4", "4X");
+#undef RFX_UMMA_FP4
+}
+// 512 bytes of shared memory (32 rows of 16) into lanes 0-31 of 4 TMEM columns,
+// and the same into the other three quarters of the lanes; with PAIR in both
+// CTAs of the pair, each from its own shared memory.  In order with the MMAs
+// that the same thread issues after it.
+template <bool PAIR>
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t s_desc) {
+  if (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+}
 // Arrives once on the mbarrier when all previously issued tcgen05.mma of this
 // thread have completed (their smem operands are free, TMEM results final).
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
@@ -258,6 +289,25 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool bf16, b
 __host__ __device__ constexpr uint32_t make_idesc_i8(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
          (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// Instruction descriptor for kind::mxf4 / mxf4nvf4, e2m1 operands, both K-major:
+// [4,6) / [29,31) which of the 4 scale bytes of a row B / A begin with (MX: 0 or
+// 2), [7,10) and [10,12) 1 = e2m1, [17,23) N>>3, [23] scales e8m0, [27,29) M>>7.
+__host__ __device__ constexpr uint32_t make_idesc_fp4(int M, int N, bool mx, int first_scale) {
+  return (static_cast<uint32_t>(first_scale) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
+         ((mx ? 1u : 0u) << 23) | (static_cast<uint32_t>(M >> 7) << 27) | (static_cast<uint32_t>(first_scale) << 29);
+}
+
+// Shared-memory matrix descriptor without swizzle of rows of 16 bytes that lie
+// one after another (8 rows, 128 bytes, per core matrix).
+__device__ __forceinline__ uint64_t make_sdesc_rows16(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(128 >> 4) << 16;
+  d |= static_cast<uint64_t>(128 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle.

@@ -137,6 +137,9 @@ int validate_quant_rows(const rfx_quant_rows_desc& d);
 int validate_block_norm(const rfx_block_norm_desc& d);
 int validate_rope(const rfx_rope_desc& d);
 int validate_linear_i8(const rfx_linear_i8_desc& d);
+int validate_quant_fp4(const rfx_quant_fp4_desc& d);
+int validate_dequant_fp4(const rfx_dequant_fp4_desc& d);
+int validate_linear_fp4(const rfx_linear_fp4_desc& d);
 
 int launch_time_cond(const rfx_time_cond_desc& d, cudaStream_t stream, bool pdl);
 int launch_modulation(const rfx_modulation_desc& d, cudaStream_t stream, bool pdl);
@@ -164,6 +167,25 @@ struct LinearI8Maps {
 };
 int build_linear_i8_maps(const rfx_linear_i8_desc& d, LinearI8Maps* maps);
 int launch_linear_i8(const rfx_linear_i8_desc& d, const LinearI8Maps& maps, cudaStream_t stream, bool pdl);
+
+int launch_quant_fp4(const rfx_quant_fp4_desc& d, cudaStream_t stream, bool pdl);
+int launch_dequant_fp4(const rfx_dequant_fp4_desc& d, cudaStream_t stream, bool pdl);
+// Bytes of the scale tiles of T 4-bit rows.
+long fp4_scale_bytes(int T, int K, int format, int rows_per_part);
+// How rfx_linear_fp4 cuts a call up; its tensor maps are made for it.
+enum { kFp4Pair, kFp4Side };
+struct LinearFp4Plan {
+  int form;
+  int nt, n_tiles;    // weight rows per tile (side: tokens), tiles per token tile
+  int nt2, n_tiles2;  // the narrower last tiles
+  int splits, stages, m_tiles, clusters;
+};
+struct LinearFp4Maps {
+  CUtensorMap x, w, w2, y, xs, ws;
+  LinearFp4Plan plan;
+};
+int build_linear_fp4_maps(const rfx_linear_fp4_desc& d, LinearFp4Maps* maps);
+int launch_linear_fp4(const rfx_linear_fp4_desc& d, const LinearFp4Maps& maps, cudaStream_t stream, bool pdl);
 int run_chunk_op(rfx_chunk* c, cudaStream_t s);
 
 }  // namespace rfx

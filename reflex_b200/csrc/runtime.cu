@@ -530,12 +530,23 @@ struct LinearI8Op {
   rfx_linear_i8_desc d;
   LinearI8Maps maps;
 };
+struct QuantFp4Op {
+  rfx_quant_fp4_desc d;
+};
+struct DequantFp4Op {
+  rfx_dequant_fp4_desc d;
+};
+struct LinearFp4Op {
+  rfx_linear_fp4_desc d;
+  LinearFp4Maps maps;
+};
 struct BarrierOp {};
 struct ChunkOp {
   rfx_chunk* c;
 };
 using Op = std::variant<LinearOp, AttnOp, QuantOp, TimeOp, ModOp, InOp, TailOp, CopyOp, NormOp, BarrierOp, ChunkOp,
-                        PatchOp, LayerNormOp, VitAttnOp, QuantRowsOp, BlockNormOp, RopeOp, LinearI8Op>;
+                        PatchOp, LayerNormOp, VitAttnOp, QuantRowsOp, BlockNormOp, RopeOp, LinearI8Op, QuantFp4Op,
+                        DequantFp4Op, LinearFp4Op>;
 }  // namespace
 
 struct rfx_plan {
@@ -565,6 +576,9 @@ int run_op(const Op& op, cudaStream_t s, bool pdl) {
   if (auto* o = std::get_if<BlockNormOp>(&op)) return launch_block_norm(o->d, s, pdl);
   if (auto* o = std::get_if<RopeOp>(&op)) return launch_rope(o->d, s, pdl);
   if (auto* o = std::get_if<LinearI8Op>(&op)) return launch_linear_i8(o->d, o->maps, s, pdl);
+  if (auto* o = std::get_if<QuantFp4Op>(&op)) return launch_quant_fp4(o->d, s, pdl);
+  if (auto* o = std::get_if<DequantFp4Op>(&op)) return launch_dequant_fp4(o->d, s, pdl);
+  if (auto* o = std::get_if<LinearFp4Op>(&op)) return launch_linear_fp4(o->d, o->maps, s, pdl);
   return set_error(RFX_E_STATE, "plan: unknown op");
 }
 // Launches every op in order; an op that follows a BarrierOp runs without PDL.
@@ -751,6 +765,26 @@ extern "C" int rfx_plan_add_linear_i8(rfx_plan* plan, const rfx_linear_i8_desc* 
   PLAN_GUARD(plan);
   LinearI8Op op{*desc, {}};
   const int rc = build_linear_i8_maps(op.d, &op.maps);
+  if (rc) return rc;
+  return plan_push(plan, op, desc->T > 0);
+}
+
+extern "C" int rfx_plan_add_quant_fp4(rfx_plan* plan, const rfx_quant_fp4_desc* desc) {
+  PLAN_GUARD(plan);
+  const int rc = validate_quant_fp4(*desc);
+  if (rc) return rc;
+  return plan_push(plan, QuantFp4Op{*desc}, desc->T > 0);
+}
+extern "C" int rfx_plan_add_dequant_fp4(rfx_plan* plan, const rfx_dequant_fp4_desc* desc) {
+  PLAN_GUARD(plan);
+  const int rc = validate_dequant_fp4(*desc);
+  if (rc) return rc;
+  return plan_push(plan, DequantFp4Op{*desc}, desc->T > 0);
+}
+extern "C" int rfx_plan_add_linear_fp4(rfx_plan* plan, const rfx_linear_fp4_desc* desc) {
+  PLAN_GUARD(plan);
+  LinearFp4Op op{*desc, {}};
+  const int rc = build_linear_fp4_maps(op.d, &op.maps);
   if (rc) return rc;
   return plan_push(plan, op, desc->T > 0);
 }

@@ -657,6 +657,133 @@ def rope(*, x, positions, inv_freq, q_out, k_out=None, v_out=None, pairs=L.RFX_R
     _launch("rfx_rope", *_rope(x, positions, inv_freq, q_out, k_out, v_out, pairs, magnitude))
 
 
+# ------------------------------------------------------- 4-bit layer path ---
+_U8 = torch.uint8
+
+
+@dataclass
+class Fp4Rows:
+    """Rows of 4-bit floating point numbers (e2m1) with a scale per block: q
+    uint8 [T, ceil(K / 2)], rows on 16-byte boundaries; scale uint8, the scale
+    bytes in tiles of 128 rows x 4 blocks (512 bytes each, in the order that
+    include/rfx.h gives); row_scale fp32 [T] with RFX_FP4_NV, else None.  With
+    `parts` > 1 each of that many equal parts of the rows has tiles of its own."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    row_scale: torch.Tensor | None
+    K: int
+    fmt: int
+    parts: int = 1
+
+    @staticmethod
+    def allocate(T: int, K: int, fmt: int, parts: int = 1, device="cuda") -> "Fp4Rows":
+        """Room for T rows of K values; a GeGLU weight [Wgate; Wup] has two parts."""
+        if T < 0 or K < 1 or parts < 1 or T % parts:
+            raise ValueError(f"need T >= 0 whole parts and K >= 1 (T={T} K={K} parts={parts})")
+        q = torch.zeros(T, -(-K // 32) * 16, dtype=_U8, device=device)[:, :(K + 1) // 2]
+        scale = torch.zeros(fp4_scale_bytes(T, K, fmt, parts), dtype=_U8, device=device)
+        row = torch.zeros(T, device=device) if fmt == L.RFX_FP4_NV else None
+        return Fp4Rows(q, scale, row, K, fmt, parts)
+
+
+def fp4_scale_bytes(T: int, K: int, fmt: int, parts: int = 1) -> int:
+    """Bytes of the scale tiles of T rows of K values."""
+    if fmt not in (L.RFX_FP4_MX, L.RFX_FP4_NV):
+        raise ValueError(f"unknown 4-bit format {fmt!r}")
+    k_tiles = -(-K // (128 if fmt == L.RFX_FP4_MX else 64))
+    return parts * -(-T // (parts * 128)) * k_tiles * 512
+
+
+def _fp4(name: str, r: Fp4Rows, dev: int) -> tuple:
+    """(T, address, row stride, scale address, row scale address) of 4-bit rows on device `dev`."""
+    q, scale, row, K, parts = r.q, r.scale, r.row_scale, r.K, r.parts
+    if q.dtype is not _U8 or scale.dtype is not _U8:
+        raise ValueError(f"{name}: values and scales must be uint8, not {q.dtype} and {scale.dtype}")
+    if q.get_device() != dev or scale.get_device() != dev or (row is not None and row.get_device() != dev):
+        raise _apart(q, scale, row)
+    if not 1 <= K <= _MOST:
+        raise ValueError(f"{name}: rows of {K} values")
+    T = _matrix(name, q)[0]
+    ld = _rows(name, q, T, (K + 1) // 2, 16)
+    if parts < 1 or T % parts:
+        raise ValueError(f"{name}: {T} rows are not {parts} equal parts")
+    if not scale.is_contiguous() or scale.numel() != fp4_scale_bytes(T, K, r.fmt, parts):
+        raise ValueError(f"{name}: scales must be {fp4_scale_bytes(T, K, r.fmt, parts)} contiguous bytes, not "
+                         f"{list(scale.shape)} (strides {scale.stride()})")
+    if (row is None) != (r.fmt == L.RFX_FP4_MX):
+        raise ValueError(f"{name}: row_scale goes with RFX_FP4_NV, and only with it")
+    return T, q.data_ptr(), ld, scale.data_ptr(), None if row is None else _vector(name + ".row_scale", row, T)
+
+
+def _quant_fp4(x, out):
+    dev = _current(x.get_device())
+    T, K = _matrix("x", x)
+    rows, q, ldq, scale, row = _fp4("out", out, dev)
+    if rows != T or out.K != K:
+        raise ValueError(f"out holds {rows} rows of {out.K}, x is {list(x.shape)}")
+    return L.QuantFp4Desc(T, K, out.fmt, _code("x", x), T // out.parts, x.data_ptr(), _rows("x", x, T, K), q, ldq,
+                          scale, row), dev
+
+
+def quant_fp4_desc(*, x: torch.Tensor, out: Fp4Rows) -> L.QuantFp4Desc:
+    """Rows x [T, K] (bf16 or fp32) to 4-bit rows `out`."""
+    return _quant_fp4(x, out)[0]
+
+
+def quant_fp4(*, x, out) -> None:
+    """Rows to 4-bit floating point with a scale per block: a power of two per 32
+    values (RFX_FP4_MX), or an e4m3 number per 16 under a power of two per row
+    (RFX_FP4_NV).  A block (NV: a row) with a NaN or an infinity becomes NaN."""
+    _launch("rfx_quant_fp4", *_quant_fp4(x, out))
+
+
+def _dequant_fp4(x, out):
+    dev = _current(out.get_device())
+    T, q, ldq, scale, row = _fp4("x", x, dev)
+    return L.DequantFp4Desc(T, x.K, x.fmt, _code("out", out), T // x.parts, q, ldq, scale, row, out.data_ptr(),
+                            _rows("out", out, T, x.K)), dev
+
+
+def dequant_fp4_desc(*, x: Fp4Rows, out: torch.Tensor) -> L.DequantFp4Desc:
+    """out [T, K] (bf16 or fp32): what the 4-bit rows x stand for."""
+    return _dequant_fp4(x, out)[0]
+
+
+def dequant_fp4(*, x, out) -> None:
+    """What 4-bit rows stand for, as bf16 or fp32."""
+    _launch("rfx_dequant_fp4", *_dequant_fp4(x, out))
+
+
+def _linear_fp4(w, x, y, epilogue, bias):
+    dev = _current(y.get_device())
+    T, xq, ldx, xs, xr = _fp4("x", x, dev)
+    O, wq, ldw, ws, wr = _fp4("w", w, dev)
+    geglu = epilogue == L.RFX_EPI_GEGLU
+    if x.K != w.K or x.fmt != w.fmt:
+        raise ValueError(f"x and w must be rows of one length and format, not {x.K}, {w.K} and {x.fmt}, {w.fmt}")
+    if x.parts != 1 or w.parts != (2 if geglu else 1):
+        raise ValueError(f"x has one part and w {'two' if geglu else 'one'}, not {x.parts} and {w.parts}")
+    if bias is not None and bias.get_device() != dev:
+        raise _apart(y, bias)
+    return L.LinearFp4Desc(T, O, x.K, x.fmt, epilogue, _code("y", y), xq, ldx, xs, xr, wq, ldw, ws, wr,
+                           None if bias is None else _vector("bias", bias, O), y.data_ptr(),
+                           _rows("y", y, T, O // 2 if geglu else O)), dev
+
+
+def linear_fp4_desc(*, w: Fp4Rows, x: Fp4Rows, y: torch.Tensor, epilogue: int = L.RFX_EPI_STORE,
+                    bias: torch.Tensor | None = None) -> L.LinearFp4Desc:
+    """y = act(x @ w^T + bias): 4-bit rows x of T tokens and w of O output
+    channels, y [T, O] bf16 or fp32 ([T, O/2] with RFX_EPI_GEGLU, w =
+    [Wgate; Wup] quantized in two parts)."""
+    return _linear_fp4(w, x, y, epilogue, bias)[0]
+
+
+def linear_fp4(*, w, x, y, epilogue=L.RFX_EPI_STORE, bias=None) -> None:
+    """Linear layer in 4-bit floating point with a scale per block of either operand."""
+    _launch("rfx_linear_fp4", *_linear_fp4(w, x, y, epilogue, bias))
+
+
 def device_status() -> int:
     v = ctypes.c_int(0)
     L.call("rfx_device_status", _stream(), ctypes.byref(v))
@@ -682,6 +809,9 @@ class Plan:
         L.LinearI8Desc: "rfx_plan_add_linear_i8",
         L.BlockNormDesc: "rfx_plan_add_block_norm",
         L.RopeDesc: "rfx_plan_add_rope",
+        L.QuantFp4Desc: "rfx_plan_add_quant_fp4",
+        L.DequantFp4Desc: "rfx_plan_add_dequant_fp4",
+        L.LinearFp4Desc: "rfx_plan_add_linear_fp4",
     }
     # direct (non-plan) entry point of each descriptor kind, for eager execution
     DIRECT = {
@@ -699,6 +829,9 @@ class Plan:
         L.LinearI8Desc: "rfx_linear_i8",
         L.BlockNormDesc: "rfx_block_norm",
         L.RopeDesc: "rfx_rope",
+        L.QuantFp4Desc: "rfx_quant_fp4",
+        L.DequantFp4Desc: "rfx_dequant_fp4",
+        L.LinearFp4Desc: "rfx_linear_fp4",
     }
 
     @classmethod
