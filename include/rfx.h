@@ -309,6 +309,63 @@ int rfx_attention_workspace_size(const rfx_attn_desc* desc, size_t* bytes);
  *     race on it and corrupt each other; order them. */
 int rfx_attention_noalloc(const rfx_attn_desc* desc, void* stream);
 
+/* --------------------------------------- attention over a shared context ---- */
+/* Attention of the S new tokens of B streams over (1) one quantized context that
+ * all streams share, (2) each stream's own quantized context of its own length,
+ * (3) the stream's new tokens: rows of all streams are multiplied with the
+ * shared keys together, which are read once for all of them.  For a batch of
+ * candidate chunks of one observation (the reference repeats the context per
+ * stream: reflex/policies/pi05/modeling_pi05.py:1403-1425 at batch B) and for
+ * streams that branch off a common prefix, down to one token each (S = 1).
+ *
+ * out[b*S + s][h*256 + d] = sum_j p_j v_j / sum_j p_j,
+ * p_j = exp(softmax_scale * q[b][h][s] . k_j - max), over the shared slots
+ * [0, n_shared) with shared_valid, the own slots [0, own_len[b]) and the new
+ * keys j with new_block[j] <= new_block[s]; q head h reads KV head h / (num_q_heads
+ * / num_kv_heads).  A row that sees no key is 0.  own_len values are clamped to
+ * 0..own_max.  A NaN or infinity that only some rows see reaches no others.
+ *
+ * Numerics as in rfx_attention: scores and sums in fp32, P (times the key's
+ * value scale) and V in f16 in P V, exact while a context token's value absmax
+ * stays below about 32,000; a new token with a value beyond f16 makes the rows
+ * that see it NaN.  Results do not depend on the order in which SMs finish. */
+typedef struct rfx_kv_view { /* a quantized ring: rows of 256 bytes at byte strides, scales at element strides */
+  const void* k;
+  const void* v;
+  const void* k_scale;
+  const void* v_scale;
+  const void* k_zp; /* RFX_QUANT_U8_REF */
+  const void* v_zp;
+  long qs_b, qs_h, qs_c;
+  long ss_b, ss_h, ss_c;
+} rfx_kv_view;
+typedef struct rfx_attn_shared_desc {
+  int B, S, num_q_heads, num_kv_heads, head_dim; /* head_dim 256 */
+  int quant_mode, scale_dtype; /* of both rings */
+  int n_shared;
+  int own_max; /* slots of a stream's own context at most; 0: none */
+  const void* q; /* bf16, element strides (rows of 256 on 16-byte boundaries) */
+  long qs_b, qs_h, qs_s;
+  rfx_kv_view shared; /* qs_b and ss_b are not used */
+  const unsigned char* shared_valid; /* [n_shared] 0/1 or NULL */
+  rfx_kv_view own;
+  const int* own_len; /* device [B], or NULL: own_max each */
+  const void* k_new;  /* bf16 [B][Hkv][S] x 256 at element strides, or NULL: no new keys */
+  long ks_b, ks_h, ks_s;
+  const void* v_new;
+  long vs_b, vs_h, vs_s;
+  const int* new_block; /* [S] or NULL */
+  float softmax_scale;
+  void* out; /* bf16 [B*S][ldo] */
+  long ldo;
+  void* workspace; /* 1024-byte aligned; nothing in it has to be zeroed */
+  size_t workspace_bytes;
+} rfx_attn_shared_desc;
+int rfx_attention_shared(const rfx_attn_shared_desc* desc, void* stream);
+/* Workspace needed for this descriptor's sizes.  Calls that may overlap have
+ * workspaces of their own. */
+int rfx_attention_shared_workspace_size(const rfx_attn_shared_desc* desc, size_t* bytes);
+
 /* ----------------------------------------- timestep conditioning + heads ---- */
 /* cond[i] = silu(W_out · silu(W_in · bf16(sinusoid(t[i])) + b_in) + b_out), bf16.
  * With w_in == NULL only the embedding is computed: cond[i] = bf16(sinusoid(t[i])).
@@ -799,6 +856,7 @@ int rfx_plan_add_rope(rfx_plan* plan, const rfx_rope_desc* desc);
 int rfx_plan_add_quant_fp4(rfx_plan* plan, const rfx_quant_fp4_desc* desc);
 int rfx_plan_add_dequant_fp4(rfx_plan* plan, const rfx_dequant_fp4_desc* desc);
 int rfx_plan_add_linear_fp4(rfx_plan* plan, const rfx_linear_fp4_desc* desc);
+int rfx_plan_add_attention_shared(rfx_plan* plan, const rfx_attn_shared_desc* desc);
 /* The chunk (not owned by the plan) is run at this point: counter clear + one launch. */
 int rfx_plan_add_chunk(rfx_plan* plan, rfx_chunk* chunk);
 /* The next op added is launched without programmatic dependent launch: it

@@ -274,6 +274,27 @@ class LinearFp4Desc(Structure):
     ]
 
 
+class KvView(Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("k_zp", c_void_p),
+        ("v_zp", c_void_p), ("qs_b", c_long), ("qs_h", c_long), ("qs_c", c_long), ("ss_b", c_long), ("ss_h", c_long),
+        ("ss_c", c_long),
+    ]
+
+
+class AttnSharedDesc(Structure):
+    _fields_ = [
+        ("B", c_int), ("S", c_int), ("num_q_heads", c_int), ("num_kv_heads", c_int), ("head_dim", c_int),
+        ("quant_mode", c_int), ("scale_dtype", c_int), ("n_shared", c_int), ("own_max", c_int),
+        ("q", c_void_p), ("qs_b", c_long), ("qs_h", c_long), ("qs_s", c_long),
+        ("shared", KvView), ("shared_valid", c_void_p), ("own", KvView), ("own_len", c_void_p),
+        ("k_new", c_void_p), ("ks_b", c_long), ("ks_h", c_long), ("ks_s", c_long),
+        ("v_new", c_void_p), ("vs_b", c_long), ("vs_h", c_long), ("vs_s", c_long),
+        ("new_block", c_void_p), ("softmax_scale", c_float), ("out", c_void_p), ("ldo", c_long),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 # Every entry point declared in include/rfx.h: name -> (argtypes, restype).
 SIGNATURES = {
     "rfx_version": ([], c_int),
@@ -319,6 +340,9 @@ SIGNATURES = {
     "rfx_plan_add_quant_fp4": ([c_void_p, POINTER(QuantFp4Desc)], c_int),
     "rfx_plan_add_dequant_fp4": ([c_void_p, POINTER(DequantFp4Desc)], c_int),
     "rfx_plan_add_linear_fp4": ([c_void_p, POINTER(LinearFp4Desc)], c_int),
+    "rfx_attention_shared": ([POINTER(AttnSharedDesc), c_void_p], c_int),
+    "rfx_attention_shared_workspace_size": ([POINTER(AttnSharedDesc), POINTER(c_size_t)], c_int),
+    "rfx_plan_add_attention_shared": ([c_void_p, POINTER(AttnSharedDesc)], c_int),
     "rfx_plan_add_chunk": ([c_void_p, c_void_p], c_int),
     "rfx_chunk_workspace_size": ([POINTER(ChunkDesc), POINTER(c_size_t)], c_int),
     "rfx_chunk_create": ([POINTER(ChunkDesc), c_void_p, c_size_t, POINTER(c_void_p)], c_int),
@@ -380,6 +404,7 @@ def ptr(t) -> int | None:
 __all__ = [n for n in dir() if n.startswith(("RFX_", "Rfx"))] + [
     "KvQuantDesc", "LinearDesc", "AttnDesc", "TimeCondDesc", "ModulationDesc", "ActionIoDesc", "CopyRowsDesc",
     "NormDesc", "ChunkDesc", "QuantRowsDesc", "LinearI8Desc", "BlockNormDesc", "RopeDesc",
-    "QuantFp4Desc", "DequantFp4Desc", "LinearFp4Desc",
+    "QuantFp4Desc", "DequantFp4Desc", "LinearFp4Desc", "KvView",
+    "AttnSharedDesc",
     "SIGNATURES", "load", "check", "call", "ptr", "LIB_PATH", "c_ubyte",
 ]

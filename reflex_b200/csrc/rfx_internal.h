@@ -140,6 +140,7 @@ int validate_linear_i8(const rfx_linear_i8_desc& d);
 int validate_quant_fp4(const rfx_quant_fp4_desc& d);
 int validate_dequant_fp4(const rfx_dequant_fp4_desc& d);
 int validate_linear_fp4(const rfx_linear_fp4_desc& d);
+int validate_attention_shared(const rfx_attn_shared_desc& d);
 
 int launch_time_cond(const rfx_time_cond_desc& d, cudaStream_t stream, bool pdl);
 int launch_modulation(const rfx_modulation_desc& d, cudaStream_t stream, bool pdl);
@@ -185,6 +186,9 @@ struct LinearFp4Maps {
   LinearFp4Plan plan;
 };
 int build_linear_fp4_maps(const rfx_linear_fp4_desc& d, LinearFp4Maps* maps);
+// Kernel launches of one rfx_attention_shared call.
+int attention_shared_launches(const rfx_attn_shared_desc& d);
+int launch_attention_shared(const rfx_attn_shared_desc& d, cudaStream_t stream, bool pdl);
 int launch_linear_fp4(const rfx_linear_fp4_desc& d, const LinearFp4Maps& maps, cudaStream_t stream, bool pdl);
 int run_chunk_op(rfx_chunk* c, cudaStream_t s);
 

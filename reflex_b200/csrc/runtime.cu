@@ -540,13 +540,16 @@ struct LinearFp4Op {
   rfx_linear_fp4_desc d;
   LinearFp4Maps maps;
 };
+struct AttnSharedOp {
+  rfx_attn_shared_desc d;
+};
 struct BarrierOp {};
 struct ChunkOp {
   rfx_chunk* c;
 };
 using Op = std::variant<LinearOp, AttnOp, QuantOp, TimeOp, ModOp, InOp, TailOp, CopyOp, NormOp, BarrierOp, ChunkOp,
                         PatchOp, LayerNormOp, VitAttnOp, QuantRowsOp, BlockNormOp, RopeOp, LinearI8Op, QuantFp4Op,
-                        DequantFp4Op, LinearFp4Op>;
+                        DequantFp4Op, LinearFp4Op, AttnSharedOp>;
 }  // namespace
 
 struct rfx_plan {
@@ -579,6 +582,7 @@ int run_op(const Op& op, cudaStream_t s, bool pdl) {
   if (auto* o = std::get_if<QuantFp4Op>(&op)) return launch_quant_fp4(o->d, s, pdl);
   if (auto* o = std::get_if<DequantFp4Op>(&op)) return launch_dequant_fp4(o->d, s, pdl);
   if (auto* o = std::get_if<LinearFp4Op>(&op)) return launch_linear_fp4(o->d, o->maps, s, pdl);
+  if (auto* o = std::get_if<AttnSharedOp>(&op)) return launch_attention_shared(o->d, s, pdl);
   return set_error(RFX_E_STATE, "plan: unknown op");
 }
 // Launches every op in order; an op that follows a BarrierOp runs without PDL.
@@ -730,15 +734,15 @@ extern "C" int rfx_plan_add_vit_attention(rfx_plan* plan, const rfx_vit_attn_des
 }
 
 namespace {
-// Appends an op of one launch (none if it has no rows); no exception leaves a C entry.
+// Appends an op of so many launches (none if it has no rows); no exception leaves a C entry.
 template <typename T>
-int plan_push(rfx_plan* plan, T&& op, bool launches) {
+int plan_push(rfx_plan* plan, T&& op, int launches) {
   try {
     plan->ops.emplace_back(std::forward<T>(op));
   } catch (...) {
     return set_error(RFX_E_INVAL, "plan: out of host memory");
   }
-  plan->launches += launches ? 1 : 0;
+  plan->launches += launches;
   return RFX_OK;
 }
 }  // namespace
@@ -787,6 +791,13 @@ extern "C" int rfx_plan_add_linear_fp4(rfx_plan* plan, const rfx_linear_fp4_desc
   const int rc = build_linear_fp4_maps(op.d, &op.maps);
   if (rc) return rc;
   return plan_push(plan, op, desc->T > 0);
+}
+
+extern "C" int rfx_plan_add_attention_shared(rfx_plan* plan, const rfx_attn_shared_desc* desc) {
+  PLAN_GUARD(plan);
+  const int rc = validate_attention_shared(*desc);
+  if (rc) return rc;
+  return plan_push(plan, AttnSharedOp{*desc}, attention_shared_launches(*desc));
 }
 
 extern "C" int rfx_plan_add_chunk(rfx_plan* plan, rfx_chunk* chunk) {

@@ -355,7 +355,7 @@ def copy_rows(**kw) -> None:
 # These wrappers run once per launch and a launch takes 2.5 us, so they look at
 # each tensor as seldom as they can.
 _CODES = {torch.bfloat16: L.RFX_DTYPE_BF16, torch.float32: L.RFX_DTYPE_F32}
-_F32, _I8 = torch.float32, torch.int8
+_F32, _I8, _BF16 = torch.float32, torch.int8, torch.bfloat16
 _MOST = 0x7FFFFFFF  # what a descriptor's sizes hold; ctypes cuts off the rest
 _ENTRIES: dict = {}
 
@@ -661,13 +661,24 @@ def rope(*, x, positions, inv_freq, q_out, k_out=None, v_out=None, pairs=L.RFX_R
 _U8 = torch.uint8
 
 
-@dataclass
+def fp4_scale_bytes(T: int, K: int, fmt: int, parts: int = 1) -> int:
+    """Bytes of the scale tiles of T rows of K values."""
+    if fmt not in (L.RFX_FP4_MX, L.RFX_FP4_NV):
+        raise ValueError(f"unknown 4-bit format {fmt!r}")
+    k_tiles = -(-K // (128 if fmt == L.RFX_FP4_MX else 64))
+    return parts * -(-T // (parts * 128)) * k_tiles * 512
+
+
+@dataclass(frozen=True)
 class Fp4Rows:
     """Rows of 4-bit floating point numbers (e2m1) with a scale per block: q
     uint8 [T, ceil(K / 2)], rows on 16-byte boundaries; scale uint8, the scale
     bytes in tiles of 128 rows x 4 blocks (512 bytes each, in the order that
     include/rfx.h gives); row_scale fp32 [T] with RFX_FP4_NV, else None.  With
-    `parts` > 1 each of that many equal parts of the rows has tiles of its own."""
+    `parts` > 1 each of that many equal parts of the rows has tiles of its own.
+
+    The tensors are looked at once, when the object is made: they keep their
+    shapes and memory for as long as it is used (their contents may change)."""
 
     q: torch.Tensor
     scale: torch.Tensor
@@ -675,6 +686,27 @@ class Fp4Rows:
     K: int
     fmt: int
     parts: int = 1
+
+    def __post_init__(self):
+        q, scale, row, K, fmt, parts = self.q, self.scale, self.row_scale, self.K, self.fmt, self.parts
+        if q.dtype is not _U8 or scale.dtype is not _U8:
+            raise ValueError(f"q and scale must be uint8, not {q.dtype} and {scale.dtype}")
+        if q.device != scale.device or (row is not None and row.device != q.device):
+            raise _apart(q, scale, row)
+        if not 1 <= K <= _MOST:
+            raise ValueError(f"rows of {K} values")
+        T = _matrix("q", q)[0]
+        ld = _rows("q", q, T, (K + 1) // 2, 16)
+        if parts < 1 or T % parts:
+            raise ValueError(f"{T} rows are not {parts} equal parts")
+        if not scale.is_contiguous() or scale.numel() != fp4_scale_bytes(T, K, fmt, parts):
+            raise ValueError(f"scale must be {fp4_scale_bytes(T, K, fmt, parts)} contiguous bytes, not "
+                             f"{list(scale.shape)} (strides {scale.stride()})")
+        if (row is None) != (fmt == L.RFX_FP4_MX):
+            raise ValueError("row_scale goes with RFX_FP4_NV, and only with it")
+        at = None if row is None else _vector("row_scale", row, T)
+        # device, rows and where they lie, for the descriptors
+        object.__setattr__(self, "_at", (q.get_device(), T, q.data_ptr(), ld, scale.data_ptr(), at))
 
     @staticmethod
     def allocate(T: int, K: int, fmt: int, parts: int = 1, device="cuda") -> "Fp4Rows":
@@ -687,39 +719,12 @@ class Fp4Rows:
         return Fp4Rows(q, scale, row, K, fmt, parts)
 
 
-def fp4_scale_bytes(T: int, K: int, fmt: int, parts: int = 1) -> int:
-    """Bytes of the scale tiles of T rows of K values."""
-    if fmt not in (L.RFX_FP4_MX, L.RFX_FP4_NV):
-        raise ValueError(f"unknown 4-bit format {fmt!r}")
-    k_tiles = -(-K // (128 if fmt == L.RFX_FP4_MX else 64))
-    return parts * -(-T // (parts * 128)) * k_tiles * 512
-
-
-def _fp4(name: str, r: Fp4Rows, dev: int) -> tuple:
-    """(T, address, row stride, scale address, row scale address) of 4-bit rows on device `dev`."""
-    q, scale, row, K, parts = r.q, r.scale, r.row_scale, r.K, r.parts
-    if q.dtype is not _U8 or scale.dtype is not _U8:
-        raise ValueError(f"{name}: values and scales must be uint8, not {q.dtype} and {scale.dtype}")
-    if q.get_device() != dev or scale.get_device() != dev or (row is not None and row.get_device() != dev):
-        raise _apart(q, scale, row)
-    if not 1 <= K <= _MOST:
-        raise ValueError(f"{name}: rows of {K} values")
-    T = _matrix(name, q)[0]
-    ld = _rows(name, q, T, (K + 1) // 2, 16)
-    if parts < 1 or T % parts:
-        raise ValueError(f"{name}: {T} rows are not {parts} equal parts")
-    if not scale.is_contiguous() or scale.numel() != fp4_scale_bytes(T, K, r.fmt, parts):
-        raise ValueError(f"{name}: scales must be {fp4_scale_bytes(T, K, r.fmt, parts)} contiguous bytes, not "
-                         f"{list(scale.shape)} (strides {scale.stride()})")
-    if (row is None) != (r.fmt == L.RFX_FP4_MX):
-        raise ValueError(f"{name}: row_scale goes with RFX_FP4_NV, and only with it")
-    return T, q.data_ptr(), ld, scale.data_ptr(), None if row is None else _vector(name + ".row_scale", row, T)
-
-
 def _quant_fp4(x, out):
     dev = _current(x.get_device())
     T, K = _matrix("x", x)
-    rows, q, ldq, scale, row = _fp4("out", out, dev)
+    where, rows, q, ldq, scale, row = out._at
+    if where != dev:
+        raise _apart(x, out.q)
     if rows != T or out.K != K:
         raise ValueError(f"out holds {rows} rows of {out.K}, x is {list(x.shape)}")
     return L.QuantFp4Desc(T, K, out.fmt, _code("x", x), T // out.parts, x.data_ptr(), _rows("x", x, T, K), q, ldq,
@@ -740,7 +745,9 @@ def quant_fp4(*, x, out) -> None:
 
 def _dequant_fp4(x, out):
     dev = _current(out.get_device())
-    T, q, ldq, scale, row = _fp4("x", x, dev)
+    where, T, q, ldq, scale, row = x._at
+    if where != dev:
+        raise _apart(x.q, out)
     return L.DequantFp4Desc(T, x.K, x.fmt, _code("out", out), T // x.parts, q, ldq, scale, row, out.data_ptr(),
                             _rows("out", out, T, x.K)), dev
 
@@ -757,15 +764,15 @@ def dequant_fp4(*, x, out) -> None:
 
 def _linear_fp4(w, x, y, epilogue, bias):
     dev = _current(y.get_device())
-    T, xq, ldx, xs, xr = _fp4("x", x, dev)
-    O, wq, ldw, ws, wr = _fp4("w", w, dev)
+    x_dev, T, xq, ldx, xs, xr = x._at
+    w_dev, O, wq, ldw, ws, wr = w._at
+    if x_dev != dev or w_dev != dev or (bias is not None and bias.get_device() != dev):
+        raise _apart(x.q, w.q, y, bias)
     geglu = epilogue == L.RFX_EPI_GEGLU
     if x.K != w.K or x.fmt != w.fmt:
         raise ValueError(f"x and w must be rows of one length and format, not {x.K}, {w.K} and {x.fmt}, {w.fmt}")
     if x.parts != 1 or w.parts != (2 if geglu else 1):
         raise ValueError(f"x has one part and w {'two' if geglu else 'one'}, not {x.parts} and {w.parts}")
-    if bias is not None and bias.get_device() != dev:
-        raise _apart(y, bias)
     return L.LinearFp4Desc(T, O, x.K, x.fmt, epilogue, _code("y", y), xq, ldx, xs, xr, wq, ldw, ws, wr,
                            None if bias is None else _vector("bias", bias, O), y.data_ptr(),
                            _rows("y", y, T, O // 2 if geglu else O)), dev
@@ -782,6 +789,149 @@ def linear_fp4_desc(*, w: Fp4Rows, x: Fp4Rows, y: torch.Tensor, epilogue: int = 
 def linear_fp4(*, w, x, y, epilogue=L.RFX_EPI_STORE, bias=None) -> None:
     """Linear layer in 4-bit floating point with a scale per block of either operand."""
     _launch("rfx_linear_fp4", *_linear_fp4(w, x, y, epilogue, bias))
+
+
+# ------------------------------------------ attention over a shared context ---
+def _kv_view(name: str, ring: KVRing, B: int, H: int, D: int, n: int, dev: int) -> L.KvView:
+    k, v, ks, vs, kz, vz = ring.k_q, ring.v_q, ring.k_scale, ring.v_scale, ring.k_zp, ring.v_zp
+    if k.get_device() != dev or v.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev or (
+            kz is not None and (kz.get_device() != dev or vz.get_device() != dev)):
+        raise _apart(k, v, ks, vs, kz, vz)
+    shape, want = k.shape, torch.int8 if ring.mode == L.RFX_QUANT_I8_SYM else _U8
+    if len(shape) != 4 or shape[0] < B or shape[1] != H or shape[2] < n or shape[3] != D or v.shape != shape:
+        raise ValueError(f"{name}: keys and values must be [{B}, {H}, {n} or more, {D}], not {list(shape)} and "
+                         f"{list(v.shape)}")
+    if k.dtype is not want or v.dtype is not want:
+        raise ValueError(f"{name}: keys and values must be {want}, not {k.dtype} and {v.dtype}")
+    qb, qh, qc, qd = k.stride()
+    if qd != 1 or v.stride() != k.stride():
+        raise ValueError(f"{name}: keys and values must have one layout with contiguous heads")
+    sb, sh, sc = ks.stride()
+    for s in (vs, kz, vz) if kz is not None else (vs,):
+        if s.shape != shape[:3] or s.stride() != (sb, sh, sc) or s.dtype is not ks.dtype:
+            raise ValueError(f"{name}: scales must be [B, H, slots] of one type and layout")
+    if ks.shape != shape[:3]:
+        raise ValueError(f"{name}: scales must be {list(shape[:3])}, not {list(ks.shape)}")
+    if ring.mode == L.RFX_QUANT_U8_REF and kz is None:
+        raise ValueError(f"{name}: the uint8 scheme needs zero points")
+    return L.KvView(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), None if kz is None else kz.data_ptr(),
+                    None if vz is None else vz.data_ptr(), qb, qh, qc, sb, sh, sc)
+
+
+def _attention_shared(q, shared, n_shared, out, softmax_scale, own, own_len, own_max, k_new, v_new, new_block,
+                      shared_valid):
+    dev = _current(q.get_device())
+    if out.get_device() != dev or (k_new is not None and k_new.get_device() != dev) or (
+            v_new is not None and v_new.get_device() != dev):
+        raise _apart(q, out, k_new, v_new)
+    try:
+        B, Hq, S, D = q.shape
+    except ValueError:
+        raise ValueError(f"q must be [B, Hq, S, D], not {list(q.shape)}") from None
+    if q.dtype is not _BF16 or out.dtype is not _BF16:
+        raise ValueError(f"q and out must be bf16, not {q.dtype} and {out.dtype}")
+    if q.stride(3) != 1 and D > 1:
+        raise ValueError("q must have contiguous heads")
+    ring = shared if shared is not None else own
+    if ring is not None:
+        Hkv = ring.k_q.shape[1] if ring.k_q.dim() == 4 else 0
+    else:
+        Hkv = k_new.shape[1] if k_new is not None and k_new.dim() == 4 else 1
+    if max(B, Hq, S, D, Hkv, n_shared) > _MOST:
+        raise ValueError(f"sizes above 2^31 - 1: q {list(q.shape)}, n_shared {n_shared}")
+    d = L.AttnSharedDesc()
+    d.B, d.S, d.num_q_heads, d.num_kv_heads, d.head_dim = B, S, Hq, Hkv, D
+    d.quant_mode = ring.mode if ring is not None else L.RFX_QUANT_I8_SYM
+    d.scale_dtype = _code("scales", ring.k_scale) if ring is not None else L.RFX_DTYPE_F32
+    d.n_shared = n_shared
+    d.q = q.data_ptr()
+    d.qs_b, d.qs_h, d.qs_s = q.stride()[:3]
+    if n_shared > 0:
+        if shared is None:
+            raise ValueError("n_shared slots of no ring")
+        d.shared = _kv_view("shared", shared, 1, Hkv, D, n_shared, dev)
+    if own is not None:
+        if own.mode != ring.mode or own.k_scale.dtype is not ring.k_scale.dtype:
+            raise ValueError("the shared and the own ring must be of one scheme")
+        if own_max is None:
+            own_max = own.capacity
+        d.own_max = own_max
+        if own_max > 0:
+            d.own = _kv_view("own", own, B, Hkv, D, own_max, dev)
+    elif own_max or own_len is not None:
+        raise ValueError("own_len and own_max go with a ring")
+    for name, t, dt, n in (("own_len", own_len, torch.int32, B), ("new_block", new_block, torch.int32, S),
+                           ("shared_valid", shared_valid, _U8, n_shared)):
+        if t is not None:
+            if t.get_device() != dev:
+                raise _apart(q, t)
+            if t.dtype is not dt and not (dt is _U8 and t.dtype is torch.bool):
+                raise ValueError(f"{name} must be {dt}, not {t.dtype}")
+            if t.dim() != 1 or t.shape[0] < n or t.stride(0) != 1:
+                raise ValueError(f"{name} must be a contiguous vector of at least {n}, not {list(t.shape)}")
+            setattr(d, name, t.data_ptr())
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new come together")
+    if k_new is not None:
+        for name, t in (("k_new", k_new), ("v_new", v_new)):
+            if t.dtype is not _BF16 or t.shape != (B, Hkv, S, D) or (t.stride(3) != 1 and D > 1):
+                raise ValueError(f"{name} must be bf16 {[B, Hkv, S, D]} with contiguous heads, not {t.dtype} {list(t.shape)}")
+        d.k_new, d.v_new = k_new.data_ptr(), v_new.data_ptr()
+        d.ks_b, d.ks_h, d.ks_s = k_new.stride()[:3]
+        d.vs_b, d.vs_h, d.vs_s = v_new.stride()[:3]
+    d.softmax_scale = softmax_scale
+    d.out, d.ldo = out.data_ptr(), _rows("out", out, B * S, Hq * D, 8)
+    return d, dev
+
+
+def attention_shared_desc(*, q: torch.Tensor, shared: KVRing | None, n_shared: int, out: torch.Tensor,
+                          softmax_scale: float, own: KVRing | None = None, own_len: torch.Tensor | None = None,
+                          own_max: int | None = None, k_new: torch.Tensor | None = None,
+                          v_new: torch.Tensor | None = None, new_block: torch.Tensor | None = None,
+                          shared_valid: torch.Tensor | None = None,
+                          workspace: torch.Tensor | None = None) -> L.AttnSharedDesc:
+    """q bf16 [B, Hq, S, 256] of any strides; shared: a ring of one stream, of
+    which every stream sees the slots [0, n_shared) (those with shared_valid);
+    own: a ring of B streams, stream b's slots [0, own_len[b]) (int32 on the
+    device; at most own_max, by default its capacity); k_new and v_new bf16 [B,
+    Hkv, S, 256] views, key j visible to token i iff new_block[j] <=
+    new_block[i]; out bf16 [B*S, Hq*256].  A plan's descriptor needs a workspace
+    whose 1024-byte aligned part holds attention_shared_workspace_bytes."""
+    d = _attention_shared(q, shared, n_shared, out, softmax_scale, own, own_len, own_max, k_new, v_new, new_block,
+                          shared_valid)[0]
+    if workspace is not None:
+        _give_workspace(d, workspace)
+    return d
+
+
+def _give_workspace(d: L.AttnSharedDesc, ws: torch.Tensor) -> None:
+    at = ws.data_ptr()
+    skip = -at % 1024
+    d.workspace, d.workspace_bytes = at + skip, max(ws.numel() * ws.element_size() - skip, 0)
+
+
+def attention_shared_workspace_bytes(d: L.AttnSharedDesc) -> int:
+    n = ctypes.c_size_t(0)
+    L.call("rfx_attention_shared_workspace_size", ctypes.byref(d), ctypes.byref(n))
+    return n.value
+
+
+def attention_shared(*, q, shared, n_shared, out, softmax_scale, own=None, own_len=None, own_max=None, k_new=None,
+                     v_new=None, new_block=None, shared_valid=None, workspace=None) -> None:
+    """Attention of B streams over one shared context, each stream's own and its
+    new tokens; allocates the workspace if the caller gives none large enough."""
+    d, dev = _attention_shared(q, shared, n_shared, out, softmax_scale, own, own_len, own_max, k_new, v_new,
+                               new_block, shared_valid)
+    need = attention_shared_workspace_bytes(d)
+    if need:
+        if workspace is not None:
+            if workspace.get_device() != dev or not workspace.is_contiguous():
+                raise ValueError("workspace must be contiguous, on the tensors' device")
+            _give_workspace(d, workspace)
+        if workspace is None or d.workspace_bytes < need:
+            workspace = torch.empty(need + 1024, dtype=_U8, device=q.device)
+            _give_workspace(d, workspace)
+    _launch("rfx_attention_shared", d, dev)
 
 
 def device_status() -> int:
@@ -812,6 +962,7 @@ class Plan:
         L.QuantFp4Desc: "rfx_plan_add_quant_fp4",
         L.DequantFp4Desc: "rfx_plan_add_dequant_fp4",
         L.LinearFp4Desc: "rfx_plan_add_linear_fp4",
+        L.AttnSharedDesc: "rfx_plan_add_attention_shared",
     }
     # direct (non-plan) entry point of each descriptor kind, for eager execution
     DIRECT = {
@@ -832,6 +983,7 @@ class Plan:
         L.QuantFp4Desc: "rfx_quant_fp4",
         L.DequantFp4Desc: "rfx_dequant_fp4",
         L.LinearFp4Desc: "rfx_linear_fp4",
+        L.AttnSharedDesc: "rfx_attention_shared",
     }
 
     @classmethod

@@ -103,9 +103,8 @@ def rows_for(T, Kc, fmt, parts=1, fill=0xA5):
     """Fp4Rows whose memory holds `fill` everywhere, and a check of what lies around the rows."""
     r = K.Fp4Rows.allocate(T, Kc, fmt, parts)
     view, clean = framed(T, (Kc + 1) // 2, torch.uint8, -(-Kc // 32) * 16 + 16, fill)
-    r.q = view
     r.scale.fill_(fill)
-    return r, clean
+    return K.Fp4Rows(view, r.scale, r.row_scale, Kc, fmt, parts), clean
 
 
 def quantized(x, fmt, parts=1):
