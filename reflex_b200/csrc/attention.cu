@@ -933,6 +933,10 @@ __global__ void __launch_bounds__(kDThreads, 1)
       if (lane == 0) mbar_arrive(&p_ready[jl & 1]);
     }
     // ---- epilogue (the layout of attention_kernel's) ----
+    // (P V of the block before the last one may be on its way too, where its values
+    // came late: a wait for the last one's parity alone would take the one two
+    // before it for done)
+    if (ok && nbl > 1) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (nbl - 2) & 1, p.status, kDevTimeoutMmaDone));
     if (ok && nbl > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (nbl - 1) & 1, p.status, kDevTimeoutMmaDone));
     tc_fence_after();
     // the row sum over both halves, in a fixed order (every pair takes this
