@@ -677,7 +677,8 @@ __global__ void __launch_bounds__(kDThreads, 1)
   uint64_t* sc_full = bars + 15;  // [3] per scale stage
   uint64_t* p_ready = bars + 18;  // [2] per S buffer: P_jl written (blocks jl, jl + 2, ... on one barrier)
   uint64_t* o_done = bars + 20;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  uint64_t* o_last = bars + 21;   // every P V is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
   if (threadIdx.x == 0) trace(p, kTrStart);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -693,6 +694,7 @@ __global__ void __launch_bounds__(kDThreads, 1)
     for (int i = 0; i < 3; ++i) mbar_init(&sc_full[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&p_ready[i], kDWorkers / 32);
     mbar_init(o_done, 1);
+    mbar_init(o_last, 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
@@ -802,6 +804,7 @@ __global__ void __launch_bounds__(kDThreads, 1)
         if (jl >= 1) pv(jl - 1);
       }
       if (ok) pv(nbl - 1);
+      if (ok) umma_commit(o_last);
     }
   } else {
     pdl_wait();
@@ -933,11 +936,8 @@ __global__ void __launch_bounds__(kDThreads, 1)
       if (lane == 0) mbar_arrive(&p_ready[jl & 1]);
     }
     // ---- epilogue (the layout of attention_kernel's) ----
-    // (P V of the block before the last one may be on its way too, where its values
-    // came late: a wait for the last one's parity alone would take the one two
-    // before it for done)
-    if (ok && nbl > 1) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (nbl - 2) & 1, p.status, kDevTimeoutMmaDone));
-    if (ok && nbl > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (nbl - 1) & 1, p.status, kDevTimeoutMmaDone));
+    // (o_done's parity cannot tell the last P V from the one two before it)
+    if (ok && nbl > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_last, 0, p.status, kDevTimeoutMmaDone));
     tc_fence_after();
     // the row sum over both halves, in a fixed order (every pair takes this
     // barrier once, whatever happened in the loop)
