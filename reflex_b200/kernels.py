@@ -792,96 +792,120 @@ def linear_fp4(*, w, x, y, epilogue=L.RFX_EPI_STORE, bias=None) -> None:
 
 
 # ------------------------------------------ attention over a shared context ---
+_NO_VIEW = L.KvView()
+
+
 def _kv_view(name: str, ring: KVRing, B: int, H: int, D: int, n: int, dev: int) -> L.KvView:
-    k, v, ks, vs, kz, vz = ring.k_q, ring.v_q, ring.k_scale, ring.v_scale, ring.k_zp, ring.v_zp
-    if k.get_device() != dev or v.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev or (
-            kz is not None and (kz.get_device() != dev or vz.get_device() != dev)):
-        raise _apart(k, v, ks, vs, kz, vz)
-    shape, want = k.shape, torch.int8 if ring.mode == L.RFX_QUANT_I8_SYM else _U8
+    k, v, ks, vs = ring.k_q, ring.v_q, ring.k_scale, ring.v_scale
+    kz = vz = None
+    shape, lay, scale_shape, scale_lay = k.shape, k.stride(), ks.shape, ks.stride()
     if len(shape) != 4 or shape[0] < B or shape[1] != H or shape[2] < n or shape[3] != D or v.shape != shape:
         raise ValueError(f"{name}: keys and values must be [{B}, {H}, {n} or more, {D}], not {list(shape)} and "
                          f"{list(v.shape)}")
+    if lay[3] != 1 or v.stride() != lay:
+        raise ValueError(f"{name}: keys and values must have one layout with contiguous heads")
+    want = _I8
+    if ring.mode == L.RFX_QUANT_U8_REF:
+        want, kz, vz = _U8, ring.k_zp, ring.v_zp
+        if kz is None or vz is None:
+            raise ValueError(f"{name}: the uint8 scheme needs zero points")
     if k.dtype is not want or v.dtype is not want:
         raise ValueError(f"{name}: keys and values must be {want}, not {k.dtype} and {v.dtype}")
-    qb, qh, qc, qd = k.stride()
-    if qd != 1 or v.stride() != k.stride():
-        raise ValueError(f"{name}: keys and values must have one layout with contiguous heads")
-    sb, sh, sc = ks.stride()
-    for s in (vs, kz, vz) if kz is not None else (vs,):
-        if s.shape != shape[:3] or s.stride() != (sb, sh, sc) or s.dtype is not ks.dtype:
+    if scale_shape != shape[:3]:
+        raise ValueError(f"{name}: scales must be {list(shape[:3])}, not {list(scale_shape)}")
+    for s in (vs,) if kz is None else (vs, kz, vz):
+        if s.shape != scale_shape or s.stride() != scale_lay or s.dtype is not ks.dtype:
             raise ValueError(f"{name}: scales must be [B, H, slots] of one type and layout")
-    if ks.shape != shape[:3]:
-        raise ValueError(f"{name}: scales must be {list(shape[:3])}, not {list(ks.shape)}")
-    if ring.mode == L.RFX_QUANT_U8_REF and kz is None:
-        raise ValueError(f"{name}: the uint8 scheme needs zero points")
+    if k.get_device() != dev or v.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev or (
+            kz is not None and (kz.get_device() != dev or vz.get_device() != dev)):
+        raise _apart(k, v, ks, vs, kz, vz)
     return L.KvView(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), None if kz is None else kz.data_ptr(),
-                    None if vz is None else vz.data_ptr(), qb, qh, qc, sb, sh, sc)
+                    None if vz is None else vz.data_ptr(), lay[0], lay[1], lay[2], *scale_lay)
+
+
+def _flags(name: str, t: torch.Tensor, dtype, n: int, dev: int) -> int:
+    """Address of a vector of at least n (bool stands for uint8)."""
+    if t.dtype is not dtype and not (dtype is _U8 and t.dtype is torch.bool):
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.dim() != 1 or t.shape[0] < n or t.stride(0) != 1:
+        raise ValueError(f"{name} must be a contiguous vector of at least {n}, not {list(t.shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the others on cuda:{dev}")
+    return t.data_ptr()
 
 
 def _attention_shared(q, shared, n_shared, out, softmax_scale, own, own_len, own_max, k_new, v_new, new_block,
-                      shared_valid):
+                      shared_valid, workspace=None):
     dev = _current(q.get_device())
-    if out.get_device() != dev or (k_new is not None and k_new.get_device() != dev) or (
-            v_new is not None and v_new.get_device() != dev):
-        raise _apart(q, out, k_new, v_new)
+    if out.get_device() != dev:
+        raise _apart(q, out)
     try:
-        B, Hq, S, D = q.shape
+        (B, Hq, S, D), (qb, qh, qs, qd) = q.shape, q.stride()
     except ValueError:
         raise ValueError(f"q must be [B, Hq, S, D], not {list(q.shape)}") from None
     if q.dtype is not _BF16 or out.dtype is not _BF16:
         raise ValueError(f"q and out must be bf16, not {q.dtype} and {out.dtype}")
-    if q.stride(3) != 1 and D > 1:
+    if qd != 1 and D > 1:
         raise ValueError("q must have contiguous heads")
     ring = shared if shared is not None else own
+    mode, scales = L.RFX_QUANT_I8_SYM, L.RFX_DTYPE_F32
     if ring is not None:
-        Hkv = ring.k_q.shape[1] if ring.k_q.dim() == 4 else 0
+        rows = ring.k_q.shape
+        Hkv, mode, scales = rows[1] if len(rows) == 4 else 0, ring.mode, _code("scales", ring.k_scale)
     else:
         Hkv = k_new.shape[1] if k_new is not None and k_new.dim() == 4 else 1
     if max(B, Hq, S, D, Hkv, n_shared) > _MOST:
         raise ValueError(f"sizes above 2^31 - 1: q {list(q.shape)}, n_shared {n_shared}")
-    d = L.AttnSharedDesc()
-    d.B, d.S, d.num_q_heads, d.num_kv_heads, d.head_dim = B, S, Hq, Hkv, D
-    d.quant_mode = ring.mode if ring is not None else L.RFX_QUANT_I8_SYM
-    d.scale_dtype = _code("scales", ring.k_scale) if ring is not None else L.RFX_DTYPE_F32
-    d.n_shared = n_shared
-    d.q = q.data_ptr()
-    d.qs_b, d.qs_h, d.qs_s = q.stride()[:3]
+    shared_view = own_view = _NO_VIEW
+    valid_at = len_at = block_at = k_at = v_at = None
     if n_shared > 0:
         if shared is None:
             raise ValueError("n_shared slots of no ring")
-        d.shared = _kv_view("shared", shared, 1, Hkv, D, n_shared, dev)
+        shared_view = _kv_view("shared", shared, 1, Hkv, D, n_shared, dev)
+        if shared_valid is not None:
+            valid_at = _flags("shared_valid", shared_valid, _U8, n_shared, dev)
     if own is not None:
-        if own.mode != ring.mode or own.k_scale.dtype is not ring.k_scale.dtype:
+        if own.mode != mode or own.k_scale.dtype is not ring.k_scale.dtype:
             raise ValueError("the shared and the own ring must be of one scheme")
         if own_max is None:
             own_max = own.capacity
-        d.own_max = own_max
         if own_max > 0:
-            d.own = _kv_view("own", own, B, Hkv, D, own_max, dev)
+            own_view = _kv_view("own", own, B, Hkv, D, own_max, dev)
+        if own_len is not None:
+            len_at = _flags("own_len", own_len, torch.int32, B, dev)
     elif own_max or own_len is not None:
         raise ValueError("own_len and own_max go with a ring")
-    for name, t, dt, n in (("own_len", own_len, torch.int32, B), ("new_block", new_block, torch.int32, S),
-                           ("shared_valid", shared_valid, _U8, n_shared)):
-        if t is not None:
-            if t.get_device() != dev:
-                raise _apart(q, t)
-            if t.dtype is not dt and not (dt is _U8 and t.dtype is torch.bool):
-                raise ValueError(f"{name} must be {dt}, not {t.dtype}")
-            if t.dim() != 1 or t.shape[0] < n or t.stride(0) != 1:
-                raise ValueError(f"{name} must be a contiguous vector of at least {n}, not {list(t.shape)}")
-            setattr(d, name, t.data_ptr())
-    if (k_new is None) != (v_new is None):
+    k_lay = v_lay = (0, 0, 0)
+    if k_new is not None and v_new is not None:
+        want = (B, Hkv, S, D)
+        k_lay, v_lay = k_new.stride(), v_new.stride()
+        if k_new.dtype is not _BF16 or v_new.dtype is not _BF16 or k_new.shape != want or v_new.shape != want or (
+                D > 1 and (k_lay[3] != 1 or v_lay[3] != 1)):
+            raise ValueError(f"k_new and v_new must be bf16 {list(want)} with contiguous heads, not {k_new.dtype} "
+                             f"{list(k_new.shape)} and {v_new.dtype} {list(v_new.shape)}")
+        if k_new.get_device() != dev or v_new.get_device() != dev:
+            raise _apart(q, k_new, v_new)
+        k_at, v_at = k_new.data_ptr(), v_new.data_ptr()
+        if new_block is not None:
+            block_at = _flags("new_block", new_block, torch.int32, S, dev)
+    elif k_new is not None or v_new is not None:
         raise ValueError("k_new and v_new come together")
-    if k_new is not None:
-        for name, t in (("k_new", k_new), ("v_new", v_new)):
-            if t.dtype is not _BF16 or t.shape != (B, Hkv, S, D) or (t.stride(3) != 1 and D > 1):
-                raise ValueError(f"{name} must be bf16 {[B, Hkv, S, D]} with contiguous heads, not {t.dtype} {list(t.shape)}")
-        d.k_new, d.v_new = k_new.data_ptr(), v_new.data_ptr()
-        d.ks_b, d.ks_h, d.ks_s = k_new.stride()[:3]
-        d.vs_b, d.vs_h, d.vs_s = v_new.stride()[:3]
-    d.softmax_scale = softmax_scale
-    d.out, d.ldo = out.data_ptr(), _rows("out", out, B * S, Hq * D, 8)
-    return d, dev
+    ws_at, ws_bytes = None, 0
+    if workspace is not None:
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous, on the tensors' device")
+        ws_at, ws_bytes = _workspace(workspace)
+    return L.AttnSharedDesc(B, S, Hq, Hkv, D, mode, scales, n_shared, own_max or 0, q.data_ptr(), qb, qh, qs, shared_view,
+                            valid_at, own_view, len_at, k_at, k_lay[0], k_lay[1], k_lay[2], v_at, v_lay[0], v_lay[1],
+                            v_lay[2], block_at, softmax_scale, out.data_ptr(), _rows("out", out, B * S, Hq * D, 8), ws_at,
+                            ws_bytes), dev
+
+
+def _workspace(ws: torch.Tensor) -> tuple:
+    """The 1024-byte aligned part of a buffer and its size."""
+    at = ws.data_ptr()
+    skip = -at % 1024
+    return at + skip, max(ws.numel() * ws.element_size() - skip, 0)
 
 
 def attention_shared_desc(*, q: torch.Tensor, shared: KVRing | None, n_shared: int, out: torch.Tensor,
@@ -897,17 +921,8 @@ def attention_shared_desc(*, q: torch.Tensor, shared: KVRing | None, n_shared: i
     Hkv, S, 256] views, key j visible to token i iff new_block[j] <=
     new_block[i]; out bf16 [B*S, Hq*256].  A plan's descriptor needs a workspace
     whose 1024-byte aligned part holds attention_shared_workspace_bytes."""
-    d = _attention_shared(q, shared, n_shared, out, softmax_scale, own, own_len, own_max, k_new, v_new, new_block,
-                          shared_valid)[0]
-    if workspace is not None:
-        _give_workspace(d, workspace)
-    return d
-
-
-def _give_workspace(d: L.AttnSharedDesc, ws: torch.Tensor) -> None:
-    at = ws.data_ptr()
-    skip = -at % 1024
-    d.workspace, d.workspace_bytes = at + skip, max(ws.numel() * ws.element_size() - skip, 0)
+    return _attention_shared(q, shared, n_shared, out, softmax_scale, own, own_len, own_max, k_new, v_new, new_block,
+                             shared_valid, workspace)[0]
 
 
 def attention_shared_workspace_bytes(d: L.AttnSharedDesc) -> int:
@@ -921,16 +936,17 @@ def attention_shared(*, q, shared, n_shared, out, softmax_scale, own=None, own_l
     """Attention of B streams over one shared context, each stream's own and its
     new tokens; allocates the workspace if the caller gives none large enough."""
     d, dev = _attention_shared(q, shared, n_shared, out, softmax_scale, own, own_len, own_max, k_new, v_new,
-                               new_block, shared_valid)
+                               new_block, shared_valid, workspace)
+    try:
+        if workspace is not None:  # (the call itself says if it is too small)
+            return _launch("rfx_attention_shared", d, dev)
+    except L.RfxError:
+        if attention_shared_workspace_bytes(d) <= d.workspace_bytes:
+            raise
     need = attention_shared_workspace_bytes(d)
     if need:
-        if workspace is not None:
-            if workspace.get_device() != dev or not workspace.is_contiguous():
-                raise ValueError("workspace must be contiguous, on the tensors' device")
-            _give_workspace(d, workspace)
-        if workspace is None or d.workspace_bytes < need:
-            workspace = torch.empty(need + 1024, dtype=_U8, device=q.device)
-            _give_workspace(d, workspace)
+        workspace = torch.empty(need + 1024, dtype=_U8, device=q.device)
+        d.workspace, d.workspace_bytes = _workspace(workspace)
     _launch("rfx_attention_shared", d, dev)
 
 

@@ -167,6 +167,9 @@ def want_of(c):
 
 
 SHAPES = [
+    (1, 1, 8, 1, 5000, 0, False),
+    (64, 50, 8, 1, 300, 0, True),
+    (30, 9, 8, 1, 3000, 100, True),
     # B, S, Hq, Hkv, n_shared, own, new
     (1, 1, 1, 1, 1, 0, False),
     (1, 1, 8, 1, 100, 0, True),
@@ -193,13 +196,13 @@ def test_matches_formula(shape):
     check(run(c), *want_of(c))
 
 
-@pytest.mark.parametrize("shape", [SHAPES[i] for i in (1, 4, 5, 10)], ids=str)
+@pytest.mark.parametrize("shape", [SHAPES[i] for i in (4, 7, 8, 13)], ids=str)
 def test_uint8_scheme(shape):
     c = case(*shape, mode=U8)
     check(run(c), *want_of(c))
 
 
-@pytest.mark.parametrize("shape", [SHAPES[i] for i in (3, 4, 7, 10, 13)], ids=str)
+@pytest.mark.parametrize("shape", [SHAPES[i] for i in (1, 2, 6, 7, 10, 13, 16)], ids=str)
 @pytest.mark.parametrize("holes", [False, True])
 def test_masks(shape, holes):
     """Block-causal new tokens (ids from -1 on), masked shared slots."""
