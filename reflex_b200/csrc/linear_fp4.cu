@@ -14,6 +14,7 @@
 // 128-byte swizzle; what lies past T, O or K is filled with zeros by the copy or
 // not copied, and not stored.  MMAs whose 64 values all lie past K are left out,
 // so no scale tile past a row's last one is used.
+#include "quant_i8.cuh"
 #include "rfx_internal.h"
 #include "tile_epilogue.cuh"
 
@@ -53,7 +54,7 @@ struct Fp4Params {
   int n_tail;       // of the tiles from column cols_a on
   int cols_a, units;
   int stages;
-  const float* x_row;  // NULL: 1
+  const float* x_row;  // NV
   const float* w_row;
   const float* bias;
   void* y;
@@ -66,54 +67,86 @@ struct Fp4Params {
 // CTA stages its 128 tokens and half of the weight rows per K step, its tokens'
 // scales and the scales of all N weight rows (an MMA reads those from either
 // CTA's own TMEM).  With GeGLU half of a tile's weight rows are gate rows and half
-// up rows, by MMAs of their own, and a thread of the epilogue finds both halves
-// of its outputs in its own TMEM lane.
+// up rows, and a thread of the epilogue finds both halves of its outputs in its own
+// TMEM lane.  256 weight rows are one MMA's N, the gate rows from the even CTA and the
+// up rows from the odd one, each a whole tile of scales; 128 are two MMAs, since their
+// scales lie in halves of two tiles.
 //
-// TMEM: two accumulators of up to 192 columns that alternate, so that a tile's
-// epilogue (8 warps) runs under the next tile's MMAs, and two sets of scales, one
-// per K step in turn.  A set is copied into once the MMAs of two steps before are
-// done.
+// TMEM: one accumulator of up to 256 columns, or two of up to 128 that alternate,
+// and as many sets of scales as the ring has stages: a stage that has been filled
+// again was free, and so is its set.  The 16 epilogue warps take all of their columns
+// into registers and free the accumulator at once, so that the epilogue runs under
+// the next tile's MMAs also where there is one accumulator.
 //
 // splits == 1: persistent, the pair walks the tiles.  splits > 1: a cluster of
 // `splits` pairs computes one tile, each pair a part of K; at the end each CTA
 // pushes the fp32 sums of the columns that another split owns into that CTA's
 // (now idle) operand ring through DSMEM, and the owner adds them in split order.
-constexpr int kPairThreads = 320;
-constexpr int kPairMaxStages = 10;
-constexpr int kPairMaxN = 192;
-constexpr int kAcc1 = 192;             // TMEM columns: the second accumulator,
-constexpr int kSets = 384;             // the two sets of scales,
+constexpr int kEpiWarps = 16;
+constexpr int kPairThreads = 64 + 32 * kEpiWarps;
+constexpr int kAcc1 = 128;             // TMEM columns: the second accumulator,
+constexpr int kSets = 256;             // the sets of scales,
 constexpr int kSetCols = 48;           // each tokens' (16) and weight rows' (32)
-constexpr int kPairRing = 6 * ((kTileM + kPairMaxN / 2) * kStepB + 3 * 4 * kScaleTile);
+constexpr int kPairMaxStages = (512 - kSets) / kSetCols;
+constexpr int kPairSmem = kSmemMax;
+constexpr int kPairRing = (kPairSmem - 1024 - 256 - kEpiWarps * 2048 - 2 * 2 * 256 * 4) & ~1023;
 constexpr int kPairOffVec = kPairRing;                      // [2][w_row | bias][256]
 constexpr int kPairOffOut = kPairOffVec + 2 * 2 * 256 * 4;  // output staging, 2 KB per epilogue warp
-constexpr int kPairOffBars = kPairOffOut + 8 * 32 * 64;
-constexpr int kPairSmem = kPairOffBars + 256 + 1024;
+constexpr int kPairOffBars = kPairOffOut + kEpiWarps * 32 * 64;
 constexpr int kMaxSplits = 4;                               // clusters of at most 8 CTAs
-static_assert(kPairSmem <= kSmemMax, "pair tiles fit in shared memory");
+static_assert(kPairOffBars + 256 + 1024 <= kPairSmem, "pair tiles fit in shared memory");
 static_assert((kPairMaxStages * 2 + 4) * 8 + 4 <= 256, "barriers fit");
-static_assert(kSets + 2 * kSetCols <= 512, "scales fit in TMEM");
 
-// 16 outputs of one token: row scales and bias from shared memory.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ bool epi_all(bool ok) {  // (also a barrier of the epilogue's warps)
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(ok ? 1u : 0u), "n"(32 * kEpiWarps)
+      : "memory");
+  return all != 0;
+}
+
+// GELU (as in gelu_ex2) and SiLU of two values.
 template <int ACT>
-__device__ __forceinline__ void finish16(const uint32_t (&acc)[16], const uint32_t (&up)[16], float sx,
-                                         const float* ws, const float* bs, int half, float (&v)[16]) {
+__device__ __forceinline__ f32x2 activate2(f32x2 v) {
+  if (ACT == kActNone) return v;
+  f32x2 e;
+  if (ACT == kActSilu) {
+    e = mul_f32x2(v, pack_f32x2(-1.4426950409f, -1.4426950409f));
+  } else {
+    constexpr float kA = -2.3022081986f, kB = kA * 0.044715f;  // -2 sqrt(2/pi) log2(e)
+    e = mul_f32x2(v, fma_f32x2(mul_f32x2(v, v), pack_f32x2(kB, kB), pack_f32x2(kA, kA)));
+  }
+  const f32x2 d = add_f32x2(pack_f32x2(ex2_approx(lo_f32(e)), ex2_approx(hi_f32(e))), pack_f32x2(1.f, 1.f));
+  return mul_f32x2(v, pack_f32x2(rcp_approx(lo_f32(d)), rcp_approx(hi_f32(d))));
+}
+
+// 16 outputs of one token: row scales (NV) and bias from shared memory, packed as
+// they are stored.  `up`: the up half with GeGLU.
+template <int ACT, bool MX, typename Tout>
+__device__ __forceinline__ void finish16(const uint32_t (&acc)[16], const uint32_t (&up)[16], float sx, const float* ws,
+                                         const float* bs, bool bias, int half, uint32_t* out) {
+  const f32x2 s2 = pack_f32x2(sx, sx);
+  auto scaled = [&](const uint32_t (&a)[16], int g, int at) {  // values g, g + 1 of 4 at a time
+    f32x2 v = pack_f32x2(__uint_as_float(a[g]), __uint_as_float(a[g + 1]));
+    if (!MX) v = mul_f32x2(v, mul_f32x2(s2, *reinterpret_cast<const f32x2*>(ws + at + g)));
+    if (bias) v = add_f32x2(v, *reinterpret_cast<const f32x2*>(bs + at + g));
+    return v;
+  };
 #pragma unroll
-  for (int g = 0; g < 16; g += 4) {
-    const float4 w = *reinterpret_cast<const float4*>(ws + g);
-    const float4 b = *reinterpret_cast<const float4*>(bs + g);
-    const float wv[4] = {w.x, w.y, w.z, w.w}, bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[g + j] = fmaf(__uint_as_float(acc[g + j]) * sx, wv[j], bv[j]);
-    if (ACT == kActGeglu) {
-      const float4 w2 = *reinterpret_cast<const float4*>(ws + half + g);
-      const float4 b2 = *reinterpret_cast<const float4*>(bs + half + g);
-      const float wu[4] = {w2.x, w2.y, w2.z, w2.w}, bu[4] = {b2.x, b2.y, b2.z, b2.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[g + j] = gelu_ex2(v[g + j]) * fmaf(__uint_as_float(up[g + j]) * sx, wu[j], bu[j]);
+  for (int g = 0; g < 16; g += 2) {
+    f32x2 v = scaled(acc, g, 0);
+    if (ACT == kActGeglu)
+      v = mul_f32x2(activate2<kActGelu>(v), scaled(up, g, half));
+    else
+      v = activate2<ACT>(v);
+    if (sizeof(Tout) == 2) {
+      out[g >> 1] = pack_bf16x2(lo_f32(v), hi_f32(v));
     } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[g + j] = activate<ACT>(v[g + j]);
+      out[g] = __float_as_uint(lo_f32(v));
+      out[g + 1] = __float_as_uint(hi_f32(v));
     }
   }
 }
@@ -187,7 +220,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_free[i], 16);  // both CTAs' epilogue warps, on the even CTA's barrier
+      mbar_init(&acc_free[i], 2 * kEpiWarps);  // both CTAs' epilogue warps, on the even CTA's barrier
     }
     fence_mbar_init();
     tma_prefetch_desc(&tmX);
@@ -207,8 +240,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   pdl_wait();
 
   const bool tma_y = (p.ldy * sizeof(Tout)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
-  constexpr int kGroup = 128 / static_cast<int>(sizeof(Tout));  // output columns of 128 bytes
-  constexpr int kHalf = kGroup / 2;                              // of which a warp finishes half
+  constexpr int kPiece = 64 / static_cast<int>(sizeof(Tout));  // output columns that a warp stores at a time
+  constexpr int kPieces = 4 * (kGeglu ? 32 : 64) / (4 * kPiece);  // of a warp, at most: every fourth
+  const bool one = p.n_tile > kAcc1;                             // one accumulator
   uint8_t* out_st = smem + kPairOffOut + (warp - 2) * 32 * 64;
   bool failed = false;
   int issued = 0;
@@ -223,7 +257,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int t0 = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM;
       const CUtensorMap* tw = tile.tail ? &tmW2 : &tmW;
       const int quarter = tile.N / 4;
-      const int wrow = tile.o0 + static_cast<int>(rank) * (kGeglu ? quarter : tile.N / 2);
+      const bool halves = kGeglu && tile.N < 256;
+      const int wrow = kGeglu && !halves ? tile.o0 + static_cast<int>(rank) * p.F
+                                         : tile.o0 + static_cast<int>(rank) * (kGeglu ? quarter : tile.N / 2);
       const int wst = w_scale_tiles(tile);
       // both CTAs' copies count on the even CTA's barrier; a half without
       // tokens copies none (what its rows multiply is not stored)
@@ -245,7 +281,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             tma_load_2d_pair(st, &tmX, bar, kb, t0);
             tma_load_2d_pair(st + off_xs, &tmXS, bar, 0, xs0 + kt);
           }
-          if (kGeglu) {
+          if (halves) {
             tma_load_2d_pair(st + kTileM * kStepB, tw, bar, kb, wrow);
             tma_load_2d_pair(st + (kTileM + quarter) * kStepB, tw, bar, kb, p.F + wrow);
           } else {
@@ -271,77 +307,96 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const uint64_t b0 = make_sdesc_sw128(smem_u32(smem + kTileM * kStepB), 16, 1024);
       const uint64_t s0 = make_sdesc_rows16(smem_u32(smem + off_xs));
       bool ok = true;
-      int s = 0, tl = 0, done = 0;      // done: K steps issued
-      int s2 = 0;                       // the stage of two steps before,
-      uint32_t phase = 0, phase2 = 0;   // and its parity
+      int s = 0, tl = 0;
+      uint32_t phase = 0;
+      const uint16_t both = static_cast<uint16_t>(3u << crank);
+      const bool lead = elect_one();
       for (Walk k = first; k.un < p.units && ok; next(k), ++tl) {
-        const int buf = tl & 1;
+        const int buf = one ? 0 : tl & 1, turn = one ? tl : tl >> 1;
         const Tile tile = tile_of(k);
         const int wst = w_scale_tiles(tile);
         const uint32_t shift = static_cast<uint32_t>(tile.o0 & 127) / 32;  // columns of the first row's scales
-        const int nb = kGeglu ? tile.N / 2 : tile.N;
-        if (tl >= 2 &&
-            !(ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[buf], ((tl >> 1) - 1) & 1, p.status, kDevTimeoutMmaDone))))
+        const bool halves = kGeglu && tile.N < 256;
+        const int nb = halves ? tile.N / 2 : tile.N;
+        const uint32_t n_field = static_cast<uint32_t>(nb >> 3) << 17;
+        if (turn > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[buf], (turn - 1) & 1, p.status, kDevTimeoutMmaDone))))
           break;
         tc_fence_after();
         const uint32_t acc = tmem + buf * kAcc1;
-        for (int i = 0; i < nk; ++i, ++done) {
-          // the MMAs of two steps before have read this set of scales
-          if (done >= 2) {
-            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s2], phase2, p.status, kDevTimeoutMmaDone)))) break;
-            if (++s2 == stages) {
-              s2 = 0;
-              phase2 ^= 1;
-            }
-          }
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase, p.status, kDevTimeoutTmaFull)))) break;
-          tc_fence_after();
-          const uint64_t off = static_cast<uint64_t>((s * stage) >> 4);
-          const uint32_t xs = tmem + kSets + (done & 1) * kSetCols, ws = xs + 16;
-          const int mmas = min(kStepK / kMmaK, p.k_mmas - (k0 + i) * (kStepK / kMmaK));
-          if (elect_one()) {
+        // two K steps at a time: what this warp spends around them (waits, votes, the
+        // loop) is otherwise longer than a step's MMAs
+        for (int i = 0; i < nk; i += 2) {
+          const bool two = i + 1 < nk;
+          const int s1 = s + 1 == stages ? 0 : s + 1;
+          const uint32_t phase1 = s1 ? phase : phase ^ 1;
+          bool fine = true;
+          if (lead) {
+            auto scales = [&](int st, int mmas) {
+              const uint32_t xs = tmem + kSets + st * kSetCols, ws = xs + 16;
+              const uint64_t sc0 = s0 + static_cast<uint64_t>((st * stage) >> 4);
 #pragma unroll
-            for (int c = 0; c < F::kTiles; ++c) {
-              if (c * F::kMmas < mmas) {
-                const uint64_t sc = s0 + off + c * (kScaleTile >> 4);
-                tmem_copy_scales<true>(xs + c * 4, sc);
-                tmem_copy_scales<true>(ws + c * 8, sc + (F::kBytes >> 4));
-                if (wst == 2) tmem_copy_scales<true>(ws + c * 8 + 4, sc + 2 * (F::kBytes >> 4));
+              for (int c = 0; c < F::kTiles; ++c) {
+                if (c * F::kMmas < mmas) {
+                  const uint64_t sc = sc0 + c * (kScaleTile >> 4);
+                  tmem_copy_scales<true>(xs + c * 4, sc);
+                  tmem_copy_scales<true>(ws + c * 8, sc + (F::kBytes >> 4));
+                  if (wst == 2) tmem_copy_scales<true>(ws + c * 8 + 4, sc + 2 * (F::kBytes >> 4));
+                }
+              }
+            };
+            auto multiply = [&](int st, int mmas, bool first_step, bool last_step) {
+              const uint32_t xs = tmem + kSets + st * kSetCols, ws = xs + 16 + shift;
+              const uint64_t off = static_cast<uint64_t>((st * stage) >> 4), ad = a0 + off, bd = b0 + off;
+#pragma unroll
+              for (int kk = 0; kk < kStepK / kMmaK; ++kk) {
+                if (kk < mmas) {
+                  const int c = kk / F::kMmas;
+                  const uint32_t idesc = make_idesc_fp4(2 * kTileM, 0, MX, 2 * (kk % F::kMmas)) | n_field;
+                  const uint32_t add = (!first_step || kk > 0) ? 1u : 0u;
+                  umma_fp4_ss<MX, true>(acc, ad + kk * 2, bd + kk * 2, idesc, xs + c * 4, ws + c * 8, add);
+                  if (halves)
+                    umma_fp4_ss<MX, true>(acc + nb, ad + kk * 2, bd + kk * 2 + ((nb / 2 * kStepB) >> 4), idesc, xs + c * 4,
+                                          ws + c * 8 + 4, add);
+                }
+              }
+              umma_commit_pair_mask(&empty[st], both);
+              if (last_step) umma_commit_pair_mask(&acc_full[buf], both);
+            };
+            const int left = p.k_mmas - (k0 + i) * (kStepK / kMmaK);
+            fine = mbar_wait(&full[s], phase, p.status, kDevTimeoutTmaFull);
+            if (fine) {
+              scales(s, left);
+              multiply(s, left, i == 0, i == nk - 1);
+              if (two) {
+                fine = mbar_wait(&full[s1], phase1, p.status, kDevTimeoutTmaFull);
+                if (fine) {
+                  scales(s1, left - kStepK / kMmaK);
+                  multiply(s1, left - kStepK / kMmaK, false, i + 1 == nk - 1);
+                }
               }
             }
-#pragma unroll
-            for (int kk = 0; kk < kStepK / kMmaK; ++kk) {
-              if (kk < mmas) {
-                const int c = kk / F::kMmas;
-                const uint32_t idesc = make_idesc_fp4(2 * kTileM, 0, MX, 2 * (kk % F::kMmas)) | (static_cast<uint32_t>(nb >> 3) << 17);
-                const uint32_t add = (i > 0 || kk > 0) ? 1u : 0u;
-                umma_fp4_ss<MX, true>(acc, a0 + off + kk * 2, b0 + off + kk * 2, idesc, xs + c * 4, ws + c * 8 + shift, add);
-                if (kGeglu)
-                  umma_fp4_ss<MX, true>(acc + nb, a0 + off + kk * 2, b0 + off + kk * 2 + ((nb / 2 * kStepB) >> 4), idesc,
-                                        xs + c * 4, ws + c * 8 + 4 + shift, add);
-              }
-            }
-            umma_commit_pair(smem_u32(&empty[s]));
-            umma_commit_pair(mapa_shared(smem_u32(&empty[s]), crank | 1u));
-            if (i == nk - 1) {
-              umma_commit_pair(smem_u32(&acc_full[buf]));
-              umma_commit_pair(mapa_shared(smem_u32(&acc_full[buf]), crank | 1u));
-            }
           }
-          __syncwarp();
-          if (++s == stages) {
+          if (!(ok = __all_sync(0xffffffffu, fine))) break;
+          if (two && s1 + 1 < stages) {
+            s = s1 + 1;
+            phase = phase1;
+          } else if (two) {
             s = 0;
-            phase ^= 1;
+            phase = phase1 ^ 1;
+          } else {
+            s = s1;
+            phase = phase1;
           }
         }
       }
     }
   } else {
-    const int et = threadIdx.x - 64;  // 0..255
+    const int et = threadIdx.x - 64;
     const int quad = warp & 3;
-    const int hw = (warp - 2) >> 2;  // which of the two warps of this TMEM quadrant
+    const int hw = (warp - 2) >> 2;  // which of the four warps of this TMEM quadrant
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t free_bar = mapa_shared(smem_u32(&acc_free[0]), crank & ~1u);
+    const bool bias = p.bias != nullptr;
     int tl = 0;
     // a tile's scales and bias come asynchronously while the tile before it is
     // finished (a short K's products are there at once: the loads would be
@@ -354,65 +409,72 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const bool in = tile.o0 + c < p.F;
         const int o = tile.o0 + c + (kGeglu && et >= nh ? p.F : 0);
         float* ws = vec + b * 512 + et;
-        if (in && p.w_row)
+        if (!MX && in)
           cp_async4(ws, p.w_row + o);
         else
           *ws = 1.f;
-        if (in && p.bias)
+        if (in && bias)
           cp_async4(ws + 256, p.bias + o);
         else
           ws[256] = 0.f;
       }
       cp_async_commit();
       const int t = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32 + lane;
-      sx_next = t < p.T && p.x_row ? p.x_row[t] : 1.f;
+      sx_next = !MX && t < p.T ? p.x_row[t] : 1.f;
     };
     if (first.un < p.units) request(tile_of(first), 0);
     for (Walk k = first; k.un < p.units; next(k), ++tl) {
-      const int buf = tl & 1;
+      const int buf = one ? 0 : tl & 1, vbuf = tl & 1;
       const Tile tile = tile_of(k);
       const int N = tile.N, nh = N / 2, oc = kGeglu ? nh : N;  // oc output columns
       const int tw = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32;  // the warp's first token
       const int o0 = tile.o0;
-      const float* ws = vec + buf * 512;
+      const float* ws = vec + vbuf * 512;
       const float* bs = ws + 256;
       const float sx = sx_next;
+      const bool full_ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (one ? tl : tl >> 1) & 1, p.status, kDevTimeoutMmaDone));
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * kAcc1 + lane_base;
+      // pieces hw, hw + 4, ... of the tile's columns, all of them at once: then the
+      // accumulator is free
+      uint32_t r[kPieces][kPiece / 16][16], u[kGeglu ? kPieces : 1][kPiece / 16][16];
+      if (full_ok && p.splits == 1) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int c = (hw + 4 * i) * kPiece;
+          if (c < oc) {
+#pragma unroll
+            for (int q = 0; q < kPiece / 16; ++q) {
+              tmem_ld16(acc + c + 16 * q, r[i][q]);
+              if (kGeglu) tmem_ld16(acc + nh + c + 16 * q, u[i][q]);
+            }
+          }
+        }
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(free_bar + 8u * buf);
+      }
       cp_async_wait_all();
-      // every epilogue warp agrees before anyone leaves the loop
-      if (!epi_agree(mbar_wait(&acc_full[buf], (tl >> 1) & 1, p.status, kDevTimeoutMmaDone))) {
+      // (the scales are there; every epilogue warp agrees before anyone leaves the loop)
+      if (!epi_all(full_ok)) {
         failed = true;
         break;
       }
-      tc_fence_after();
-      const uint32_t acc = tmem + buf * kAcc1 + lane_base;
       if (p.splits > 1) break;  // one tile per cluster: summed below
       Walk ahead = k;
       next(ahead);
-      if (ahead.un < p.units) request(tile_of(ahead), buf ^ 1);
-      // groups of 128 output bytes, of which each warp of the quadrant finishes
-      // and stores 64
-#pragma unroll 1
-      for (int g = hw * kHalf; g < oc; g += kGroup) {
-        uint32_t w[16];
-        uint32_t r[kHalf / 16][16], u[kHalf / 16][16];
+      if (ahead.un < p.units) request(tile_of(ahead), vbuf ^ 1);
 #pragma unroll
-        for (int q = 0; q < kHalf / 16; ++q) {
-          tmem_ld16(acc + g + 16 * q, r[q]);
-          if (kGeglu) tmem_ld16(acc + nh + g + 16 * q, u[q]);
-        }
-        tmem_wait_ld();
-        if (g + kGroup >= oc) {  // this warp's last read of the accumulator
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(free_bar + 8u * buf);
-        }
+      for (int i = 0; i < kPieces; ++i) {
+        const int c = (hw + 4 * i) * kPiece;
+        if (c < oc) {
+          uint32_t w[16];
 #pragma unroll
-        for (int q = 0; q < kHalf / 16; ++q) {
-          float v[16];
-          finish16<ACT>(r[q], u[q], sx, ws + g + 16 * q, bs + g + 16 * q, nh, v);
-          pack16(v, w + q * 8, static_cast<const Tout*>(nullptr));
+          for (int q = 0; q < kPiece / 16; ++q)
+            finish16<ACT, MX, Tout>(r[i][q], u[kGeglu ? i : 0][q], sx, ws + c + 16 * q, bs + c + 16 * q, bias, nh, w + q * 8);
+          store_part<Tout>(p, &tmY, out_st, w, tw, o0 + c, p.T - tw, min(kPiece, p.F - o0 - c), tma_y, lane);
         }
-        store_part<Tout>(p, &tmY, out_st, w, tw, o0 + g, p.T - tw, min(kHalf, p.F - o0 - g), tma_y, lane);
       }
     }
   }
@@ -424,6 +486,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     // own in split order.
     const Tile tile = tile_of(first);
     const int nh = tile.N / 2, oc = kGeglu ? nh : tile.N;
+    constexpr int kGroup = 2 * kPiece;
     const int quad = warp & 3, hw = (warp - 2) >> 2;
     const int rowt = quad * 32 + lane;
     const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16);
@@ -435,7 +498,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (warp >= 2 && !failed) {
       const uint32_t base = smem_u32(smem) + static_cast<uint32_t>(rowt) * 16u;
 #pragma unroll 1
-      for (int j = hw; j < groups * (kGroup / 16); j += 2) {  // 16-column chunks
+      for (int j = hw; j < groups * (kGroup / 16); j += 4) {  // 16-column chunks
         const int grp = j / (kGroup / 16), q = j % (kGroup / 16);
         const int owner = grp % p.splits;
         if (owner == split || j * 16 >= oc) continue;
@@ -459,14 +522,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (warp >= 2 && !failed) {
       const int tw = tile.m * 2 * kTileM + static_cast<int>(rank) * kTileM + quad * 32;
       const int o0 = tile.o0;
-      const float sx = tw + lane < p.T && p.x_row ? p.x_row[tw + lane] : 1.f;
+      const float sx = !MX && tw + lane < p.T ? p.x_row[tw + lane] : 1.f;
 #pragma unroll 1
-      for (int lg = 0; lg * p.splits + split < groups; ++lg) {
+      for (int lg = hw >> 1; lg * p.splits + split < groups; lg += 2) {
         const int g0 = (lg * p.splits + split) * kGroup;
         uint32_t w[16];
 #pragma unroll
-        for (int qq = 0; qq < kHalf / 16; ++qq) {
-          const int q = hw * (kHalf / 16) + qq;
+        for (int qq = 0; qq < kPiece / 16; ++qq) {
+          const int q = (hw & 1) * (kPiece / 16) + qq;
           const int c = g0 + 16 * q;
           if (c < oc) {
             uint32_t r[kParts][16], sum[kParts][16];
@@ -497,13 +560,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 }
               }
             }
-            float v[16];
-            finish16<ACT>(sum[0], sum[kParts - 1], sx, vec + c, vec + 256 + c, nh, v);
-            pack16(v, w + qq * 8, static_cast<const Tout*>(nullptr));
+            finish16<ACT, MX, Tout>(sum[0], sum[kParts - 1], sx, vec + c, vec + 256 + c, p.bias != nullptr, nh, w + qq * 8);
           }
         }
-        const int g = g0 + hw * kHalf;
-        store_part<Tout>(p, &tmY, out_st, w, tw, o0 + g, p.T - tw, min(min(kHalf, oc - g), p.F - o0 - g), tma_y, lane);
+        const int g = g0 + (hw & 1) * kPiece;
+        store_part<Tout>(p, &tmY, out_st, w, tw, o0 + g, p.T - tw, min(min(kPiece, oc - g), p.F - o0 - g), tma_y, lane);
       }
     }
     __syncwarp();
@@ -694,14 +755,14 @@ __global__ void __launch_bounds__(kSideThreads, 3)
       }
     }
   } else {
-    if (et < N) sx[et] = et < p.T && p.x_row ? p.x_row[et] : 1.f;
+    if (et < N) sx[et] = !MX && et < p.T ? p.x_row[et] : 1.f;
     o = o0 + rowt;
     if (splits > 1) o = o0 + et % kTileM;
     if (o < p.F) {
-      if (p.w_row) ws = p.w_row[o];
+      if (!MX) ws = p.w_row[o];
       if (p.bias) bs = p.bias[o];
       if (kGeglu) {
-        if (p.w_row) wu = p.w_row[p.F + o];
+        if (!MX) wu = p.w_row[p.F + o];
         if (p.bias) bu = p.bias[p.F + o];
       }
     }
@@ -851,7 +912,16 @@ void plan_side(const rfx_linear_fp4_desc& d, int nsm, int k_steps, LinearFp4Plan
   c->stages = stages;
 }
 
+// Pair tiles, above 128 tokens: the width and the split of K that finish soonest by
+// this model, in ns, fitted to measured times of 17 projections of 129 to 4096 tokens
+// at every width and split.  Launch, first copies and last epilogue take kBase +
+// kBaseRow per weight row; a K step what kStep says of its width, and kHalves more
+// where the gate and up rows are MMAs of their own; from one tile to the next kTurn,
+// more where one accumulator has to be emptied in between; adding up a split K kSplit
+// per split.
 LinearFp4Plan plan_fp4(const rfx_linear_fp4_desc& d, int nsm) {
+  constexpr double kBase = 4300, kBaseRow = 5.8, kStep[4] = {310, 320, 365, 385}, kHalves = 130;
+  constexpr double kTurn[2] = {600, 1600}, kSplit = 1200;
   LinearFp4Plan c{};
   const bool geglu = d.epilogue == RFX_EPI_GEGLU, mx = d.format == RFX_FP4_MX;
   const int div = geglu ? 2 : 1;  // weight rows per output column
@@ -862,16 +932,66 @@ LinearFp4Plan plan_fp4(const rfx_linear_fp4_desc& d, int nsm) {
     return c;
   }
   const int m = (d.T - 1) / (2 * kTileM) + 1;
+  const int width = 64 * div;  // scale tiles are taken from multiples of 64 rows on
+  const void* fn = fp4_kernel(d, kFp4Pair);
+  auto tiles_of = [&](int cols, int nt) { return static_cast<int>((static_cast<long>(cols) * div + nt - 1) / nt); };
+  auto sum_ns = [&](int nt, int s) {
+    return (k_steps + s - 1) / s * (kStep[nt / 64 - 1] + (geglu && nt < 256 ? kHalves : 0.0));
+  };
+  auto epi_ns = [&](int nt) { return kBase + kBaseRow * nt; };
+  auto tile_ns = [&](int nt) { return sum_ns(nt, 1) + kTurn[nt > kAcc1]; };
+  double best = 0;
+  for (int s = 1; s <= std::min(kMaxSplits, k_steps); ++s) {
+    // clusters of 2s CTAs that are resident at once (GPCs hold whole clusters)
+    int slots = max_active_clusters(fn, kPairThreads, kPairSmem, 2 * s);
+    if (slots <= 0) {
+      if (s > 1) break;
+      slots = std::max(1, nsm / 2);
+    }
+    for (int nt = width; nt <= 256; nt += width) {
+      const int n = tiles_of(F, nt);
+      const long tiles = static_cast<long>(m) * n;
+      const long rounds = (tiles + slots - 1) / slots;
+      if (s > 1 && rounds > 1) continue;
+      auto consider = [&](double cost, int n_a, int nt2, int n_b) {
+        if (c.nt != 0 && cost >= best) return;
+        best = cost;
+        c.nt = nt;
+        c.splits = s;
+        c.n_tiles = n_a;
+        c.nt2 = nt2;
+        c.n_tiles2 = n_b;
+        c.clusters = static_cast<int>(std::min<long>(static_cast<long>(m) * (n_a + n_b), slots));
+      };
+      if (s > 1) {
+        consider(sum_ns(nt, s) + epi_ns(nt) + kSplit * s, n, 0, 0);
+        continue;
+      }
+      consider((rounds - 1) * tile_ns(nt) + sum_ns(nt, 1) + epi_ns(nt), n, 0, 0);
+      if (rounds < 2) continue;
+      // the full rounds at this width, the rest in narrower tiles
+      const int n_a = static_cast<int>((rounds - 1) * slots / m);
+      if (n_a < 1 || n_a >= n) continue;
+      for (int nt2 = width; nt2 < nt; nt2 += width) {
+        const int n_b = tiles_of(F - n_a * (nt / div), nt2);
+        const long ua = static_cast<long>(n_a) * m, ub = static_cast<long>(n_b) * m;
+        // the tiles go round the slots: the busiest slot's time
+        const double ta = tile_ns(nt), tb = tile_ns(nt2), end = epi_ns(nt2) - kTurn[nt2 > kAcc1];
+        const long qa = ua / slots, ra = ua % slots, first = slots - ra;  // `first` slots have one wide tile less
+        double time;
+        if (ub <= first) {
+          time = std::max(qa * ta + tb, (qa + (ra ? 1 : 0)) * ta);
+        } else {
+          const long qb = (ub - first) / slots, rb = (ub - first) % slots;
+          time = std::max(ra ? (qa + 1) * ta + (qb + (rb ? 1 : 0)) * tb : 0.0, qa * ta + (1 + qb + (rb > ra ? 1 : 0)) * tb);
+        }
+        // (a gain of a hundredth by this model is none by the clock)
+        consider(1.01 * (time + end), n_a, nt2, n_b);
+      }
+    }
+  }
   c.form = kFp4Pair;
   c.m_tiles = m;
-  const int slots = std::max(1, max_active_clusters(fp4_kernel(d, kFp4Pair), kPairThreads, kPairSmem, 2));
-  c.nt = geglu ? 128 : kPairMaxN;
-  // narrower tiles while they are fewer than the pairs
-  auto tiles = [&](int nt) { return static_cast<long>(m) * ((static_cast<long>(F) * div + nt - 1) / nt); };
-  while (!geglu && c.nt > 64 && tiles(c.nt) < slots) c.nt -= 64;
-  c.n_tiles = static_cast<int>(tiles(c.nt) / m);
-  c.splits = 1;
-  c.clusters = static_cast<int>(std::min<long>(tiles(c.nt), slots));
   const int stage = (kTileM + c.nt / 2) * kStepB + 3 * (mx ? Fmt<true>::kBytes : Fmt<false>::kBytes);
   c.stages = std::min(kPairMaxStages, kPairRing / stage);
   return c;
@@ -940,12 +1060,12 @@ int build_linear_fp4_maps(const rfx_linear_fp4_desc& d, LinearFp4Maps* maps) {
   rc = make_tmap_2d(&maps->ws, d.w_scale, 4, kScaleTile / 4, ws / kScaleTile, kScaleTile, kScaleTile / 4, tiles, false);
   if (rc) return rc;
   if (c.form == kFp4Side) return make_tmap_2d(&maps->w, d.w, 1, kb, d.O, d.ldw, kStepB, kTileM, true);
-  const int div = geglu ? 4 : 2;
-  rc = make_tmap_2d(&maps->w, d.w, 1, kb, d.O, d.ldw, kStepB, c.nt / div, true);
+  auto box = [&](int nt) { return geglu && nt < 256 ? nt / 4 : nt / 2; };
+  rc = make_tmap_2d(&maps->w, d.w, 1, kb, d.O, d.ldw, kStepB, box(c.nt), true);
   if (rc) return rc;
   maps->w2 = maps->w;
   if (c.n_tiles2 > 0) {
-    rc = make_tmap_2d(&maps->w2, d.w, 1, kb, d.O, d.ldw, kStepB, c.nt2 / div, true);
+    rc = make_tmap_2d(&maps->w2, d.w, 1, kb, d.O, d.ldw, kStepB, box(c.nt2), true);
     if (rc) return rc;
   }
   const int esz = d.out_dtype == kDtypeBF16 ? 2 : 4;
