@@ -247,7 +247,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   bool failed = false;
   int issued = 0;
   if (warp == 0) {
-    // as in the MMA warp, the whole warp walks the steps and one lane issues
+    // as in the MMA warp, the whole warp walks the steps and one lane waits and issues
+    const bool lead = elect_one();
+    const int leader_lane = __ffs(__ballot_sync(0xffffffffu, lead)) - 1;
     bool ok = true;
     int s = 0;
     uint32_t phase = 0;
@@ -269,32 +271,47 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                                                    2 * wst * F::kBytes);
       const int xs0 = (t0 / kTileM) * p.k_tiles;
       const int ws0 = (tile.o0 / 128) * p.k_tiles, ws1 = ws0 + (kGeglu ? p.up_tiles : 1) * p.k_tiles;
-      for (int i = 0; i < nk; ++i) {
-        if (issued >= stages && !(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase ^ 1, p.status, kDevTimeoutStageEmpty))))
-          break;
-        if (elect_one()) {
-          uint8_t* st = smem + s * stage;
-          const uint32_t bar = full0 + 8u * s;
-          const int kb = (k0 + i) * kStepB, kt = (k0 + i) * F::kTiles;
-          if (leader) mbar_arrive_expect_tx(&full[s], bytes);
-          if (has_x) {
-            tma_load_2d_pair(st, &tmX, bar, kb, t0);
-            tma_load_2d_pair(st + off_xs, &tmXS, bar, 0, xs0 + kt);
-          }
-          if (halves) {
+      for (int i = 0; i < nk; i += 2) {
+        const bool two = i + 1 < nk;
+        const int s1 = s + 1 == stages ? 0 : s + 1;
+        const uint32_t phase1 = s1 ? phase : phase ^ 1;
+        int done = 0;
+        if (lead) {
+          auto copy = [&](int sg, int step) {
+            uint8_t* st = smem + sg * stage;
+            const uint32_t bar = full0 + 8u * sg;
+            const int kb = (k0 + step) * kStepB, kt = (k0 + step) * F::kTiles;
+            if (leader) mbar_arrive_expect_tx(&full[sg], bytes);
+            if (has_x) {
+              tma_load_2d_pair(st, &tmX, bar, kb, t0);
+              tma_load_2d_pair(st + off_xs, &tmXS, bar, 0, xs0 + kt);
+            }
             tma_load_2d_pair(st + kTileM * kStepB, tw, bar, kb, wrow);
-            tma_load_2d_pair(st + (kTileM + quarter) * kStepB, tw, bar, kb, p.F + wrow);
-          } else {
-            tma_load_2d_pair(st + kTileM * kStepB, tw, bar, kb, wrow);
+            if (halves) tma_load_2d_pair(st + (kTileM + quarter) * kStepB, tw, bar, kb, p.F + wrow);
+            tma_load_2d_pair(st + off_xs + F::kBytes, &tmWS, bar, 0, ws0 + kt);
+            if (wst == 2) tma_load_2d_pair(st + off_xs + 2 * F::kBytes, &tmWS, bar, 0, ws1 + kt);
+          };
+          if (issued < stages || mbar_wait(&empty[s], phase ^ 1, p.status, kDevTimeoutStageEmpty)) {
+            copy(s, i);
+            done = 1;
+            if (two && (issued + 1 < stages || mbar_wait(&empty[s1], phase1 ^ 1, p.status, kDevTimeoutStageEmpty))) {
+              copy(s1, i + 1);
+              done = 2;
+            }
           }
-          tma_load_2d_pair(st + off_xs + F::kBytes, &tmWS, bar, 0, ws0 + kt);
-          if (wst == 2) tma_load_2d_pair(st + off_xs + 2 * F::kBytes, &tmWS, bar, 0, ws1 + kt);
         }
-        __syncwarp();
-        ++issued;
-        if (++s == stages) {
+        done = __shfl_sync(0xffffffffu, done, leader_lane);
+        issued += done;
+        if (!(ok = done == (two ? 2 : 1))) break;
+        if (two && s1 + 1 < stages) {
+          s = s1 + 1;
+          phase = phase1;
+        } else if (two) {
           s = 0;
-          phase ^= 1;
+          phase = phase1 ^ 1;
+        } else {
+          s = s1;
+          phase = phase1;
         }
       }
     }
