@@ -77,6 +77,8 @@ struct SharedAttnParams {
   int cluster;      // CTAs per tile, or 0: runs of units over `ctas` CTAs,
   int ctas;
   int run, longer;  // `run` units each, the first `longer` CTAs one more
+  int join;         // of the CTAs of a tile the last to finish joins the parts
+  int early;        // q is there once this grid runs: the keys' copy went before
   // dense keys [block][64][256], shared blocks of each head first, then (stream,
   // head, own block); per block the words of its keys: [ks | vs | add | nb][64]
   __nv_bfloat16* kd;
@@ -85,6 +87,7 @@ struct SharedAttnParams {
   // parts of tiles, a slot per CTA of a cluster, or two per CTA
   float* part_o;    // [slot][256 / 4][tile_rows][4]
   float2* part_ml;  // [slot][tile_rows]: m (log2 units), l
+  int* arrived;     // [tile] CTAs whose part is there
   int* status;
 };
 
@@ -202,8 +205,12 @@ __device__ __forceinline__ float round_to(float x, bool bf16) { return bf16 ? bf
 // rows in the same tile multiply them by 0.
 __global__ void __launch_bounds__(256) shared_dense_kernel(const __grid_constant__ SharedAttnParams p) {
   constexpr int kPer = 16;
+  // (before the grid behind this one may begin: what went before is done, and that
+  // grid's early reads of q are safe)
   pdl_wait();
   pdl_launch_dependents();
+  if (p.join)
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < p.tiles; i += gridDim.x * 256) p.arrived[i] = 0;
   const int block = blockIdx.x / (kKeys / kPer), q0 = blockIdx.x % (kKeys / kPer) * kPer;
   const bool sbf16 = p.scale_bf16 != 0;
   const int n_sh = p.Hkv * p.shared_blocks;
@@ -351,6 +358,7 @@ constexpr int kTmS = 384;
 constexpr int kWorkers = 256;
 constexpr int kFirstWorker = 128;
 constexpr int kThreads = kFirstWorker + kWorkers;
+constexpr int kJoinMost = 4;  // parts of a tile that the last CTA joins, at most
 constexpr int kFewMost = 64;  // rows per KV head up to which the form for few is taken
 
 // Barrier over the two worker warps of a TMEM lane quadrant that also ANDs a
@@ -438,6 +446,24 @@ __device__ __forceinline__ float4* part_at(const SharedAttnParams& p, long slot,
   return reinterpret_cast<float4*>(p.part_o) + (slot * (kD / 4) + col4) * p.tile_rows + r;
 }
 
+// 32 columns of a row's O, or zeros where no block was seen.
+__device__ __forceinline__ void load_o(bool live, uint32_t at, uint32_t (&o)[2][16]) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    if (live) tmem_ld16(at + q * 16, o[q]);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (!live) o[q][e] = 0u;
+  }
+  if (live) tmem_wait_ld();
+}
+
+__device__ __forceinline__ int ld_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
 // Columns 8 g .. 8 g + 7 of a row, from parts that are added in order.
 struct Joined {
   float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -521,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* o_free = bars + 24;
   uint64_t* m_set = bars + 25;    // [4 quadrants][2 groups]: the running maxima after a block
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 33);
+  volatile int* last_x = reinterpret_cast<volatile int*>(bars + 34);
   if (threadIdx.x == 0) {
     mbar_init(q_ready, kWorkers / 32);
     for (int i = 0; i < kStages; ++i) {
@@ -555,14 +582,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmO = tmem, tmQ = tmem + kTmQ;
   auto tmS = [&](int j) { return tmem + kTmS + static_cast<uint32_t>(j & 1) * kKeys; };
   pdl_launch_dependents();
-  pdl_wait();
+  const bool worker = threadIdx.x >= kFirstWorker;
+  if (!worker || !p.early) pdl_wait();
   const Share share(p);
   int issued = 0;  // blocks whose K (warp 0) or V (warp 2) was requested
 
   if (warp == 0 || warp == 2) {
     // warp 0 copies K and the words, warp 2 V
+    const bool is_v = warp == 2;
+    if (is_v && share.tile1 > share.tile0) {
+      // the second tile's Q into L2: the CTAs get there at about the same time, and
+      // would wait for memory together
+      const int tile = share.tile0 + 1, h = tile / p.head_tiles;
+#pragma unroll 1
+      for (int r = lane; r < kRows; r += 32) {
+        const RowOf row(p, min((tile - h * p.head_tiles) * kRows + r, p.rows - 1));
+        const __nv_bfloat16* q = p.q + row.b * p.qs_b + (h * p.G + row.g) * p.qs_h + row.s * p.qs_s;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + 64 * i));
+      }
+    }
     if (lane == 0) {
-      const bool is_v = warp == 2;
       const int stages = is_v ? kStagesV : kStages;
       uint64_t* full = is_v ? v_full : k_full;
       uint64_t* empty = is_v ? v_empty : k_empty;
@@ -659,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) pv(j - 1, true);
       ++seg;
     }
-  } else if (threadIdx.x >= kFirstWorker) {
+  } else if (worker) {
     const int quad = warp & 3;
     const int ch = (threadIdx.x - kFirstWorker) >> 7;  // this warp's group: blocks in turn, half of the output columns
     const int r = quad * 32 + lane;                    // query row inside the tile == TMEM lane
@@ -718,6 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(q_ready);
       }
+      if (tile == share.tile0 && p.early) pdl_wait();
       for (; blk.unit >= 0 && ok; blocks.step(p, blk), ++j) {
         const int ws = wst;
         const uint32_t wp = wph;
@@ -860,26 +901,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       // (where scores were all NaN a maximum is -inf and its sum NaN)
       l_run = (m0 == m_run ? l_x[r] : l_x[r] * exp2f(m0 - m_run)) +
               (m1 == m_run ? l_x[kRows + r] : l_x[kRows + r] * exp2f(m1 - m_run));
-      if (ok) {
-        const bool parts = p.cluster > 1 || !s.whole;
-        const long slot = p.cluster > 1 ? blockIdx.x : 2 * blockIdx.x + (tile == share.tile0 ? 0 : 1);
-        const float inv_l = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f;
-        const long at = row_valid ? out_at(p, blocks.h, row) : -1;
-        if (parts && ch == 0) p.part_ml[slot * kRows + r] = make_float2(m_run, l_run);
+      const bool part = p.cluster > 1 || !s.whole;
+      const long slot = p.cluster > 1 ? blockIdx.x : 2 * blockIdx.x + (tile == share.tile0 ? 0 : 1);
+      // A tile of several CTAs without a cluster: the last of them to get here joins the
+      // parts, in their order whichever it is.  It is the last for sure where all others
+      // have arrived, and then leaves no part of its own.
+      const bool joins = part && p.join;
+      int c0 = 0, c1 = 0;
+      bool last = false;
+      if (joins) {
+        c0 = cta_of(p, tile * p.tile_units);
+        c1 = cta_of(p, (tile + 1) * p.tile_units - 1);
+        if (threadIdx.x == kFirstWorker) *last_x = ld_acquire(p.arrived + tile) == c1 - c0;
+        workers_all(true);
+        last = *last_x != 0;
+      }
+      const long at = row_valid ? out_at(p, blocks.h, row) : -1;
+      float inv_l = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f;
+      if (part && !last) {
+        if (ok) {
+          if (ch == 0) p.part_ml[slot * kRows + r] = make_float2(m_run, l_run);
 #pragma unroll 1
-        for (int c = 4 * ch; c < 4 * ch + 4; ++c) {  // 32 columns
-          uint32_t rr[2][16];
-          if (live) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) tmem_ld16(tmO + lane_base + c * 32 + q * 16, rr[q]);
-            tmem_wait_ld();
-          } else {
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) rr[q][e] = 0u;
-          }
-          if (parts) {
+          for (int c = 4 * ch; c < 4 * ch + 4; ++c) {  // 32 columns
+            uint32_t rr[2][16];
+            load_o(live, tmO + lane_base + c * 32, rr);
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -887,25 +932,86 @@ __global__ void __launch_bounds__(kThreads, 1)
                 *part_at(p, slot, c * 8 + q * 4 + e, r) =
                     make_float4(__uint_as_float(rr[q][4 * e]), __uint_as_float(rr[q][4 * e + 1]),
                                 __uint_as_float(rr[q][4 * e + 2]), __uint_as_float(rr[q][4 * e + 3]));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t* x = &rr[i >> 1][8 * (i & 1)];
-              *reinterpret_cast<uint4*>(own_chunk(st, lane, i)) =
-                  make_uint4(pack_bf16x2(__uint_as_float(x[0]) * inv_l, __uint_as_float(x[1]) * inv_l),
-                             pack_bf16x2(__uint_as_float(x[2]) * inv_l, __uint_as_float(x[3]) * inv_l),
-                             pack_bf16x2(__uint_as_float(x[4]) * inv_l, __uint_as_float(x[5]) * inv_l),
-                             pack_bf16x2(__uint_as_float(x[6]) * inv_l, __uint_as_float(x[7]) * inv_l));
-            }
-            __syncwarp();
-#pragma unroll
-            for (int it = 0; it < 4; ++it) {
-              const long to = __shfl_sync(0xffffffffu, at, it * 8 + (lane >> 2));
-              const uint4 x = *reinterpret_cast<const uint4*>(shared_chunk(st, lane, it));
-              if (to >= 0) *reinterpret_cast<uint4*>(p.out + to + c * 32 + (lane & 3) * 8) = x;
-            }
-            __syncwarp();
           }
+        }
+        if (joins) {
+          __threadfence();
+          workers_all(true);
+          if (threadIdx.x == kFirstWorker) *last_x = atomicAdd(p.arrived + tile, 1) == c1 - c0;
+          workers_all(true);
+          last = *last_x != 0;
+        }
+      }
+      if (ok && (!part || last)) {
+        // weights of the parts before and after this one, and of this one
+        const int mine = static_cast<int>(blockIdx.x) - c0;
+        const long first = 2l * c0 + (c0 != static_cast<int>(blockIdx.x) && cta_begin(p, c0) >= tile * p.tile_units ? 0 : 1);
+        auto slot_of = [&](int q) { return q == 0 ? first : 2l * (c0 + q); };
+        float M = m_run;
+        if (last) {
+          __threadfence();
+          for (int q = 0; q <= c1 - c0; ++q)
+            if (q != mine) M = fmaxf(M, __ldcg(&p.part_ml[slot_of(q) * kRows + r].x));
+          float L = 0.f;
+          for (int q = 0; q <= c1 - c0; ++q) {
+            const float2 ml = q == mine ? make_float2(m_run, l_run) : __ldcg(p.part_ml + slot_of(q) * kRows + r);
+            L = fmaf(ml.x == M ? 1.f : exp2f(ml.x - M), ml.y, L);
+          }
+          inv_l = L > 0.f || L != L ? 1.f / L : 0.f;
+        }
+#pragma unroll 1
+        for (int c = 4 * ch; c < 4 * ch + 4; ++c) {  // 32 columns
+          uint32_t rr[2][16];
+          load_o(live, tmO + lane_base + c * 32, rr);
+          if (last) {
+            float acc[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) acc[e] = 0.f;
+#pragma unroll 1
+            for (int q = 0; q <= c1 - c0; ++q) {
+              float4 x[8];
+              float m = m_run;
+              if (q == mine) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const uint32_t* o = &rr[e >> 2][4 * (e & 3)];
+                  x[e] = make_float4(__uint_as_float(o[0]), __uint_as_float(o[1]), __uint_as_float(o[2]), __uint_as_float(o[3]));
+                }
+              } else {
+                const long from = slot_of(q);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __ldcg(part_at(p, from, c * 8 + e, r));
+                m = __ldcg(&p.part_ml[from * kRows + r].x);
+              }
+              const float w = m == M ? 1.f : exp2f(m - M);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                acc[4 * e] = fmaf(w, x[e].x, acc[4 * e]);
+                acc[4 * e + 1] = fmaf(w, x[e].y, acc[4 * e + 1]);
+                acc[4 * e + 2] = fmaf(w, x[e].z, acc[4 * e + 2]);
+                acc[4 * e + 3] = fmaf(w, x[e].w, acc[4 * e + 3]);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) rr[e >> 4][e & 15] = __float_as_uint(acc[e]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t* x = &rr[i >> 1][8 * (i & 1)];
+            *reinterpret_cast<uint4*>(own_chunk(st, lane, i)) =
+                make_uint4(pack_bf16x2(__uint_as_float(x[0]) * inv_l, __uint_as_float(x[1]) * inv_l),
+                           pack_bf16x2(__uint_as_float(x[2]) * inv_l, __uint_as_float(x[3]) * inv_l),
+                           pack_bf16x2(__uint_as_float(x[4]) * inv_l, __uint_as_float(x[5]) * inv_l),
+                           pack_bf16x2(__uint_as_float(x[6]) * inv_l, __uint_as_float(x[7]) * inv_l));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            const long to = __shfl_sync(0xffffffffu, at, it * 8 + (lane >> 2));
+            const uint4 x = *reinterpret_cast<const uint4*>(shared_chunk(st, lane, it));
+            if (to >= 0) *reinterpret_cast<uint4*>(p.out + to + c * 32 + (lane & 3) * 8) = x;
+          }
+          __syncwarp();
         }
       }
       if (live) {
@@ -925,7 +1031,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // takes them faster than the SMs' network takes stores into one another); each
     // joins its share of the columns of all rows.
     cluster_sync();
-    const bool worker = threadIdx.x >= kFirstWorker;
     const int n = p.cluster, rank = static_cast<int>(cluster_ctarank());
     const int h = share.tile0 / p.head_tiles, r = (threadIdx.x - kFirstWorker) & (kRows - 1);
     const int R = (share.tile0 - h * p.head_tiles) * kRows + r;
@@ -1481,7 +1586,7 @@ struct Plan {
   bool few;     // the form for few rows
   long blocks;  // of the dense copy of the keys
   bool joined;  // some tile is several CTAs', without a cluster
-  size_t kd, vd, words, part_o, part_ml, total;
+  size_t kd, vd, words, part_o, part_ml, arrived, total;
 };
 
 // Clusters, or runs of units: what ends soonest by this model, in us.  A CTA's
@@ -1509,6 +1614,7 @@ void deal(Plan* out, int nsm) {
   p.ctas = p.cluster ? p.tiles * p.cluster : ctas;
   p.run = static_cast<int>(units / ctas);
   p.longer = static_cast<int>(units % ctas);
+  p.join = out->joined && p.tile_units <= (kJoinMost - 1) * p.run;
 }
 
 // The form for few rows: CTAs per tile (a cluster, or as many as there are SMs for,
@@ -1588,6 +1694,7 @@ int plan_shared(const rfx_attn_shared_desc& d, Plan* out) {
   const size_t slots = out->few ? p.ctas : out->joined ? 2 * static_cast<size_t>(p.ctas) : p.cluster > 1 ? p.ctas : 0;
   out->part_o = take(slots * tile_rows * kD * 4);
   out->part_ml = take(slots * tile_rows * 8);
+  out->arrived = take(p.join ? static_cast<size_t>(p.tiles) * 4 : 0);
   out->total = off;
   return RFX_OK;
 }
@@ -1699,7 +1806,7 @@ int validate(const rfx_attn_shared_desc& d, Plan* plan) {
 int attention_shared_launches(const rfx_attn_shared_desc& d) {
   Plan plan;
   if (d.B == 0 || d.S == 0 || plan_shared(d, &plan)) return 0;
-  return (plan.blocks > 0 ? 1 : 0) + 1 + (plan.joined ? 1 : 0);
+  return (plan.blocks > 0 ? 1 : 0) + 1 + (plan.joined && !plan.p.join ? 1 : 0);
 }
 
 int validate_attention_shared(const rfx_attn_shared_desc& d) {
@@ -1742,6 +1849,8 @@ int launch_attention_shared(const rfx_attn_shared_desc& d, cudaStream_t stream, 
   p.words = reinterpret_cast<float*>(ws + plan.words);
   p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
   p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
+  p.arrived = reinterpret_cast<int*>(ws + plan.arrived);
+  p.early = plan.blocks > 0;
   p.status = device_status_ptr();
   CUtensorMap k{}, v{};
   if (plan.blocks > 0) {
@@ -1765,7 +1874,7 @@ int launch_attention_shared(const rfx_attn_shared_desc& d, cudaStream_t stream, 
   }
   rc = launch_kernel(fn, dim3(p.ctas), dim3(kThreads), kSmemBytes, stream, pdl,
                      std::max(p.cluster, 1), k, v, p);
-  if (rc || !plan.joined) return rc;
+  if (rc || !plan.joined || p.join) return rc;
   // a few parts per tile are added one after another, many by eight threads
   if (p.ctas > 8 * p.tiles)
     return launch_kernel(reinterpret_cast<const void*>(shared_combine_kernel<kRows, 8>), dim3(p.tiles * (kD / 8)), dim3(8 * kRows), 0,
