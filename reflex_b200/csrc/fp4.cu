@@ -24,9 +24,9 @@ constexpr int kUnit = 16;
 // part ((j / 4) * 512 + j % 4).
 struct ScaleTiles {
   int per_part, tiles_per_part, k_tiles;  // rows and row tiles of a part, tiles along K
-  __device__ __forceinline__ long row(long t) const {
-    const long part = t / per_part, r = t - part * per_part;
-    return ((part * tiles_per_part + r / 128) * k_tiles) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
+  __device__ __forceinline__ long row(int t) const {
+    const int part = t / per_part, r = t - part * per_part;
+    return (static_cast<long>(part * tiles_per_part + r / 128) * k_tiles) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
   }
 };
 
@@ -41,6 +41,17 @@ struct QuantFp4Params {
   ScaleTiles tiles;
 };
 
+__device__ __forceinline__ void load_32(const void* from, uint4& a, uint4& b) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+               : "l"(from));
+}
+__device__ __forceinline__ void store_32(void* to, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+               "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
 // 16 values as they lie in memory.
 template <typename T>
 struct Unit {
@@ -48,9 +59,15 @@ struct Unit {
   static constexpr int kPer = 8 / static_cast<int>(sizeof(T)) * 2;  // values of a vector
   uint4 v[kVecs];
 
-  // Values k .. k+15 of a row, zeros past K.  VEC: the row lies on 16 bytes.
-  template <bool VEC>
+  // Values k .. k+15 of a row, zeros past K.  VEC: bytes that the row's start and
+  // stride are multiples of (32, 16, or 0 for the type's own).
+  template <int VEC>
   __device__ __forceinline__ void load(const T* row, int k, int K) {
+    if (VEC == 32 && k + kUnit <= K) {
+#pragma unroll
+      for (int i = 0; i < kVecs; i += 2) load_32(row + k + i * kPer, v[i], v[i + 1]);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const int at = k + i * kPer;
@@ -209,7 +226,7 @@ constexpr int rows_at_a_time(int tpr) { return tpr == 32 ? kWarpRows : 1; }
 
 // NU units per thread of a row's TPR threads; NU = 0: rows of any length, read
 // a second time where NV needs their maximum first.
-template <typename Tin, int FMT, int TPR, int NU, bool VEC>
+template <typename Tin, int FMT, int TPR, int NU, int VEC>
 __global__ void __launch_bounds__(TPR* rows_at_a_time(TPR)) quant_fp4_kernel(const QuantFp4Params p) {
   __shared__ uint32_t part[2][TPR / 32];
   pdl_wait();
@@ -300,55 +317,92 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t codes, float (&v)[8]) {
 
 __device__ __forceinline__ void put(float* y, float v) { *y = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* y, float v) { *y = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put8(float* y, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(y + 4) = make_float4(v[4], v[5], v[6], v[7]);
+template <int VEC>
+__device__ __forceinline__ void put16(float* y, const float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    const uint4 a = make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
+    const uint4 b = make_uint4(__float_as_uint(v[i + 4]), __float_as_uint(v[i + 5]), __float_as_uint(v[i + 6]), __float_as_uint(v[i + 7]));
+    if (VEC == 32) {
+      store_32(y + i, a, b);
+    } else {
+      *reinterpret_cast<uint4*>(y + i) = a;
+      *reinterpret_cast<uint4*>(y + i + 4) = b;
+    }
+  }
 }
-__device__ __forceinline__ void put8(__nv_bfloat16* y, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(y) =
-      make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+template <int VEC>
+__device__ __forceinline__ void put16(__nv_bfloat16* y, const float (&v)[16]) {
+  const uint4 a = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  const uint4 b = make_uint4(pack_bf16x2(v[8], v[9]), pack_bf16x2(v[10], v[11]), pack_bf16x2(v[12], v[13]), pack_bf16x2(v[14], v[15]));
+  if (VEC == 32) {
+    store_32(y, a, b);
+  } else {
+    *reinterpret_cast<uint4*>(y) = a;
+    *reinterpret_cast<uint4*>(y + 8) = b;
+  }
 }
 
-// A thread's unit: 16 values of one row under one scale byte.
-template <typename Tout, int FMT, bool VEC>
+// A CTA takes 256 / TPR rows and kTurn units per thread of them at a time: all codes and
+// scales are asked for before the first is used.
+template <typename Tout, int FMT, int TPR, int VEC>
 __global__ void __launch_bounds__(256) dequant_fp4_kernel(const DequantFp4Params p) {
+  constexpr int kRows = 256 / TPR, kTurn = TPR == 256 ? 2 : 1, kChunk = kTurn * TPR;
   pdl_wait();
   pdl_launch_dependents();
-  const long total = static_cast<long>(p.T) * p.units, step = static_cast<long>(gridDim.x) * 256;
-  for (long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
-    const long t = i / p.units;
-    const int u = static_cast<int>(i - t * p.units), k = u * kUnit;
-    const uint8_t* q = p.q + t * p.ldq + k / 2;
-    const int j = FMT == RFX_FP4_MX ? u >> 1 : u;
-    const uint32_t byte = p.scale[p.tiles.row(t) + (j >> 2) * 512l + (j & 3)];
-    uint2 codes = make_uint2(0u, 0u);
-    if (k + kUnit <= p.K) {
-      codes = *reinterpret_cast<const uint2*>(q);
-    } else {
-      const int n = (p.K - k + 1) / 2;
+  const int chunks = (p.units + kChunk - 1) / kChunk;
+  const long total = (static_cast<long>(p.T) + kRows - 1) / kRows * chunks;
+  for (long i = blockIdx.x; i < total; i += gridDim.x) {
+    const int rows = static_cast<int>(chunks == 1 ? i : i / chunks), t = rows * kRows + static_cast<int>(threadIdx.x) / TPR;
+    const int u0 = static_cast<int>(i - static_cast<long>(rows) * chunks) * kChunk + threadIdx.x % TPR;
+    if (t >= p.T) continue;
+    const uint8_t* q = p.q + t * p.ldq;
+    const uint8_t* scale = p.scale + p.tiles.row(t);
+    const float row_scale = FMT == RFX_FP4_NV ? p.row_scale[t] : 1.f;
+    Tout* y = static_cast<Tout*>(p.y) + t * p.ldy;
+    uint2 codes[kTurn];
+    uint32_t byte[kTurn];
 #pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        const uint32_t c = b < n ? static_cast<uint32_t>(q[b]) << (8 * (b & 3)) : 0u;
-        (b < 4 ? codes.x : codes.y) |= c;
+    for (int c = 0; c < kTurn; ++c) {
+      const int u = u0 + c * TPR, k = u * kUnit, j = FMT == RFX_FP4_MX ? u >> 1 : u;
+      codes[c] = make_uint2(0u, 0u);
+      byte[c] = 0;
+      if (u >= p.units) continue;
+      byte[c] = scale[(j >> 2) * 512l + (j & 3)];
+      if (k + kUnit <= p.K) {
+        codes[c] = *reinterpret_cast<const uint2*>(q + k / 2);
+      } else {
+        const int n = (p.K - k + 1) / 2;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          const uint32_t w = b < n ? static_cast<uint32_t>(q[k / 2 + b]) << (8 * (b & 3)) : 0u;
+          (b < 4 ? codes[c].x : codes[c].y) |= w;
+        }
       }
     }
-    // 2^(byte - 127) as two factors: byte 0 is below the smallest normal number
-    const float s0 = FMT == RFX_FP4_MX ? (byte == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(max(byte, 1u) << 23))
-                                       : from_e4m3(byte);
-    const float s1 = FMT == RFX_FP4_MX ? (byte == 0 ? 0.5f : 1.f) : p.row_scale[t];
-    Tout* y = static_cast<Tout*>(p.y) + t * p.ldy + k;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v[8];
-      unpack_e2m1(h ? codes.y : codes.x, v);
+    for (int c = 0; c < kTurn; ++c) {
+      const int u = u0 + c * TPR, k = u * kUnit;
+      if (u >= p.units) continue;
+      // 2^(byte - 127) as two factors: byte 0 is below the smallest normal number
+      const float s0 = FMT == RFX_FP4_MX
+                           ? (byte[c] == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(max(byte[c], 1u) << 23))
+                           : from_e4m3(byte[c]);
+      const float s1 = FMT == RFX_FP4_MX ? (byte[c] == 0 ? 0.5f : 1.f) : row_scale;
+      float v[16];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = v[e] * s0 * s1;
-      if (VEC && k + 8 * h + 8 <= p.K) {
-        put8(y + 8 * h, v);
+      for (int h = 0; h < 2; ++h) {
+        float x[8];
+        unpack_e2m1(h ? codes[c].y : codes[c].x, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * h + e] = x[e] * s0 * s1;
+      }
+      if (VEC && k + kUnit <= p.K) {
+        put16<VEC>(y + k, v);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k + 8 * h + e < p.K) put(y + 8 * h + e, v[e]);
+        for (int e = 0; e < 16; ++e)
+          if (k + e < p.K) put(y + k + e, v[e]);
       }
     }
   }
@@ -378,7 +432,7 @@ FpShape fp4_shape(int T, int K) {
   return {256, units <= 256 ? 1 : units <= 512 ? 2 : 4};
 }
 
-template <typename Tin, int FMT, bool VEC>
+template <typename Tin, int FMT, int VEC>
 const void* quant_ptr(FpShape s) {
 #define RFX_FP4_SHAPE(TPR, NU) \
   if (s.tpr == TPR && s.nu == NU) return reinterpret_cast<const void*>(quant_fp4_kernel<Tin, FMT, TPR, NU, VEC>)
@@ -394,18 +448,33 @@ const void* quant_ptr(FpShape s) {
 #undef RFX_FP4_SHAPE
   return reinterpret_cast<const void*>(quant_fp4_kernel<Tin, FMT, 256, 0, VEC>);
 }
+template <typename Tin, int FMT>
+const void* quant_vec(int vec, FpShape s) {
+  return vec == 32 ? quant_ptr<Tin, FMT, 32>(s) : vec == 16 ? quant_ptr<Tin, FMT, 16>(s) : quant_ptr<Tin, FMT, 0>(s);
+}
 template <typename Tin>
-const void* quant_kernel(int format, bool vec, FpShape s) {
-  if (format == RFX_FP4_MX) return vec ? quant_ptr<Tin, RFX_FP4_MX, true>(s) : quant_ptr<Tin, RFX_FP4_MX, false>(s);
-  return vec ? quant_ptr<Tin, RFX_FP4_NV, true>(s) : quant_ptr<Tin, RFX_FP4_NV, false>(s);
+const void* quant_kernel(int format, int vec, FpShape s) {
+  return format == RFX_FP4_MX ? quant_vec<Tin, RFX_FP4_MX>(vec, s) : quant_vec<Tin, RFX_FP4_NV>(vec, s);
+}
+template <typename Tout, int FMT, int TPR>
+const void* dequant_vec(int vec) {
+  return vec == 32   ? reinterpret_cast<const void*>(dequant_fp4_kernel<Tout, FMT, TPR, 32>)
+         : vec == 16 ? reinterpret_cast<const void*>(dequant_fp4_kernel<Tout, FMT, TPR, 16>)
+                     : reinterpret_cast<const void*>(dequant_fp4_kernel<Tout, FMT, TPR, 0>);
+}
+template <typename Tout, int FMT>
+const void* dequant_rows(int tpr, int vec) {
+  return tpr == 32 ? dequant_vec<Tout, FMT, 32>(vec) : tpr == 64 ? dequant_vec<Tout, FMT, 64>(vec) : dequant_vec<Tout, FMT, 256>(vec);
 }
 template <typename Tout>
-const void* dequant_kernel(int format, bool vec) {
-  if (format == RFX_FP4_MX)
-    return vec ? reinterpret_cast<const void*>(dequant_fp4_kernel<Tout, RFX_FP4_MX, true>)
-               : reinterpret_cast<const void*>(dequant_fp4_kernel<Tout, RFX_FP4_MX, false>);
-  return vec ? reinterpret_cast<const void*>(dequant_fp4_kernel<Tout, RFX_FP4_NV, true>)
-             : reinterpret_cast<const void*>(dequant_fp4_kernel<Tout, RFX_FP4_NV, false>);
+const void* dequant_kernel(int format, int tpr, int vec) {
+  return format == RFX_FP4_MX ? dequant_rows<Tout, RFX_FP4_MX>(tpr, vec) : dequant_rows<Tout, RFX_FP4_NV>(tpr, vec);
+}
+// Bytes at a time: what the rows' start and stride allow.
+int vec_of(const void* p, long stride, int rows) {
+  for (int bytes = 32; bytes >= 16; bytes /= 2)
+    if (aligned(p, bytes) && (rows == 1 || stride % bytes == 0)) return bytes;
+  return 0;
 }
 
 // What quantizing and its inverse have in common; `wide` is the bf16 / fp32 side.
@@ -457,7 +526,7 @@ int launch_quant_fp4(const rfx_quant_fp4_desc& d, cudaStream_t stream, bool pdl)
   QuantFp4Params p{d.T, d.K, d.x, d.ldx, static_cast<uint8_t*>(d.q), d.ldq, static_cast<uint8_t*>(d.scale), d.row_scale,
                    tiles_of(d.T, d.K, d.format, d.rows_per_part)};
   const long esz = d.in_dtype == kDtypeBF16 ? 2 : 4;
-  const bool vec = aligned(d.x, 16) && (d.T == 1 || d.ldx * esz % 16 == 0);
+  const int vec = vec_of(d.x, d.ldx * esz, d.T);
   const FpShape s = fp4_shape(d.T, d.K);
   const void* fn = d.in_dtype == kDtypeBF16 ? quant_kernel<__nv_bfloat16>(d.format, vec, s) : quant_kernel<float>(d.format, vec, s);
   int nsm = 148;
@@ -488,11 +557,13 @@ int launch_dequant_fp4(const rfx_dequant_fp4_desc& d, cudaStream_t stream, bool 
                      static_cast<const uint8_t*>(d.scale), d.row_scale, d.y, d.ldy,
                      tiles_of(d.T, d.K, d.format, d.rows_per_part)};
   const long esz = d.out_dtype == kDtypeBF16 ? 2 : 4;
-  const bool vec = aligned(d.y, 16) && (d.T == 1 || d.ldy * esz % 16 == 0);
-  const void* fn = d.out_dtype == kDtypeBF16 ? dequant_kernel<__nv_bfloat16>(d.format, vec) : dequant_kernel<float>(d.format, vec);
+  const int vec = vec_of(d.y, d.ldy * esz, d.T);
+  const int tpr = p.units <= 32 ? 32 : p.units <= 64 ? 64 : 256;
+  const void* fn = d.out_dtype == kDtypeBF16 ? dequant_kernel<__nv_bfloat16>(d.format, tpr, vec) : dequant_kernel<float>(d.format, tpr, vec);
   int nsm = 148;
   rfx_num_sms(&nsm);
-  const long ctas = (static_cast<long>(d.T) * p.units + 255) / 256;
+  const long rows = 256 / tpr, chunk = tpr == 256 ? 512 : tpr;
+  const long ctas = (d.T + rows - 1) / rows * ((p.units + chunk - 1) / chunk);
   return launch_kernel(fn, dim3(static_cast<unsigned>(std::min(ctas, 8l * nsm))), dim3(256), 0, stream, pdl, 1, p);
 }
 
