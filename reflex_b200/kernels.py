@@ -697,6 +697,8 @@ class Fp4Rows:
             raise ValueError(f"rows of {K} values")
         T = _matrix("q", q)[0]
         ld = _rows("q", q, T, (K + 1) // 2, 16)
+        if ld % 16 or q.data_ptr() % 16 or scale.data_ptr() % 16:
+            raise ValueError(f"rows of q and the scales must begin on 16-byte boundaries (row stride {ld})")
         if parts < 1 or T % parts:
             raise ValueError(f"{T} rows are not {parts} equal parts")
         if not scale.is_contiguous() or scale.numel() != fp4_scale_bytes(T, K, fmt, parts):

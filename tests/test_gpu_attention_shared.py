@@ -46,7 +46,7 @@ def make_ring(r, B, Hkv, n, mode=I8, capacity=None):
 
 
 def ring_values(ring):
-    """(k, v, v's quantized magnitudes) in 64 bits, [B, H, cap, D]."""
+    """(k, v) in 64 bits, [B, H, cap, D]."""
     kq, vq = ring.k_q.double().cpu(), ring.v_q.double().cpu()
     if ring.mode == I8:
         return (kq * ring.k_scale.double().cpu()[..., None]).numpy(), (vq * ring.v_scale.double().cpu()[..., None]).numpy()
@@ -62,9 +62,11 @@ def reference(q, shared, n_shared, scale, own=None, own_len=None, k_new=None, v_
     tol: scores are sums of 256 products in fp32, off by at most (256 / 16 + 2) 2u
     of the sum of magnitudes and u each for the two factors after it, which
     moves a weight by that (times the score scale) and by 2^-22 for its
-    exponential; a weight (times its value scale) is rounded to f16, 2^-11 of it or
-    2^-25 of the largest weight; sums over n keys in fp32 add (n / 16 + 4) 2u; the
-    output is rounded to bf16."""
+    exponential; a weight times its value scale is rounded to f16, by 2^-11 of it or,
+    among the subnormal numbers (steps of 2^-24), by 2^-25, and multiplies an integer
+    of at most 127 (a ring's int8 value, which its scale does not shrink there) or the
+    value itself (scale 1): (2^-25 / l) sum of those, with the largest weight 1; sums
+    over n keys in fp32 add (n / 16 + 4) 2u; the output is rounded to bf16."""
     q = q.double().cpu().numpy()
     B, Hq, S, _ = q.shape
     ring = shared if shared is not None else own
@@ -109,8 +111,11 @@ def reference(q, shared, n_shared, scale, own=None, own_len=None, k_new=None, v_
             u = 2.0 ** -24
             ds = (18 * 2 * u + 2 * u) * mag + 4 * u * np.abs(np.where(see, z, 0)) + 2.0 ** -21
             av = np.abs(v)
+            operand = av.copy()  # what the rounded weights multiply
+            if ring is not None and ring.mode == I8:
+                operand[:ctx] = 127.0
             d = (p * ds) @ av + (p * ds).sum(axis=1, keepdims=True) * (p @ av)
-            d += 2.0 ** -11 * (p @ av) + (2.0 ** -25 / np.maximum(l, 1e-300)) * (np.minimum(1, see) @ np.minimum(av, 127.0)) * ok_row
+            d += 2.0 ** -11 * (p @ av) + (2.0 ** -25 / np.maximum(l, 1e-300)) * (np.minimum(1, see) @ operand) * ok_row
             d += (len(k) / 16 + 4) * 2 * u * (p @ av)
             d += 2.0 ** -8 * (np.abs(o) + d) + 1e-38
             out[b, :, h * G:(h + 1) * G] = o.reshape(G, S, D).transpose(1, 0, 2)
@@ -208,3 +213,258 @@ def test_masks(shape, holes):
     """Block-causal new tokens (ids from -1 on), masked shared slots."""
     c = case(*shape, blocks=True, holes=holes, token_major=False, seed=3)
     check(run(c), *want_of(c))
+
+
+def test_rows_without_keys_are_zero():
+    """No keys at all, none valid, rings of length 0: rows of zeros; a stream
+    with keys beside one without."""
+    c = case(2, 3, 8, 1, 0, 0, False)
+    c["own"], c["own_max"] = make_ring(gen(1), 2, 1, 4), 0
+    assert (run(c) == 0).all()
+    for S in (1, 50):
+        c = case(3, S, 8, 1, 200, 0, False, holes=True)
+        c["shared_valid"].zero_()
+        assert (run(c) == 0).all()
+        c = case(5, S, 8, 1, 0, 70, False, lens=[0, 70, 0, 3, -5])
+        out = run(c)
+        check(out, *want_of(c))
+        assert (out.view(5, S, -1)[[0, 2, 4]] == 0).all()
+
+
+@pytest.mark.parametrize("S", [1, 40])
+def test_lengths_beyond_the_ring_are_clamped(S):
+    c = case(4, S, 8, 1, 100, 60, True, lens=[60, 60, 0, 10])
+    want = run(c).clone()
+    c["own_len"].copy_(torch.tensor([1000, 0x7fffffff, -0x80000000, 10], dtype=torch.int32))
+    assert torch.equal(run(c), want)
+
+
+@pytest.mark.parametrize("S", [1, 30])
+def test_nan_of_one_stream_stays_there(S):
+    """A NaN or an infinity in one stream's own ring or new keys (also values beyond
+    f16) makes that stream's rows NaN that see it, and changes no other stream's bits."""
+    c = case(6, S, 8, 1, 300, 90, True, lens=[90, 50, 90, 10, 0, 64], blocks=S > 1)
+    want = run(c).view(6, S, 8, D).clone()
+    c["own"].v_scale[1, :, 49] = float("nan")
+    c["v_new"][3, 0, 0, 5] = float("inf")
+    c["v_new"][4, 0, S - 1, 7] = 1e6
+    c["k_new"][5, 0, S - 1, 9] = float("nan")
+    got = run(c).view(6, S, 8, D)
+    assert torch.equal(got[[0, 2]], want[[0, 2]])
+    assert got[1].isnan().all() and got[3].isnan().all()
+    assert got[4, S - 1].isnan().all() and got[5, S - 1].isnan().all()
+    if S > 1:  # tokens of earlier blocks do not see the last block's
+        assert torch.equal(got[4:, 0], want[4:, 0])
+
+
+def test_masked_slots_may_hold_anything():
+    for S in (1, 50):
+        c = case(8, S, 8, 1, 500, 0, True, holes=True, seed=5)
+        want = run(c).clone()
+        off = c["shared_valid"] == 0
+        c["shared"].k_scale[0, 0, :500][off] = float("nan")
+        c["shared"].v_scale[0, 0, :500][off] = float("inf")
+        assert torch.equal(run(c), want)
+
+
+@pytest.mark.parametrize("shape", [(64, 50, 8, 1, 300, 0, True), (30, 9, 8, 1, 3000, 100, True), (16, 51, 8, 1, 2000, 48, True),
+                                   (3, 1, 8, 1, 9000, 20, True), (64, 1, 8, 1, 6000, 70, False)], ids=str)
+def test_same_bits_every_time(shape):
+    """Whichever CTA of a tile ends last, its parts are added in one order."""
+    c = case(*shape)
+    want = run(c).clone()
+    for _ in range(30):
+        assert torch.equal(run(c), want)
+
+
+@pytest.mark.parametrize("S", [1, 20])
+def test_layouts(S):
+    """Strided q, keys, rings and out (rings of a larger one's slots and layers): the same bits
+    as dense ones, and nothing beside out's rows is written."""
+    B, Hq = 5, 8
+    c = case(B, S, Hq, 1, 260, 40, True)
+    want = run(c).clone()
+
+    def spread(t, *dims):  # the same values, `dims` other strides
+        big = torch.full([2 * n if i in dims else n for i, n in enumerate(t.shape)], 99, dtype=t.dtype, device="cuda")
+        view = big[tuple(slice(0, 2 * n, 2) if i in dims else slice(None) for i, n in enumerate(t.shape))]
+        view.copy_(t)
+        return view
+    c["q"] = c["q"].transpose(1, 2).contiguous().transpose(1, 2)
+    c["k_new"], c["v_new"] = spread(c["k_new"], 0, 1), spread(c["v_new"], 2)
+    for name in ("shared", "own"):
+        ring = c[name]
+        c[name] = K.KVRing(spread(ring.k_q, 0, 2), spread(ring.v_q, 0, 2), spread(ring.k_scale, 1, 2), spread(ring.v_scale, 1, 2),
+                           None, None, ring.mode)
+    buf = torch.full((B * S + 2, Hq * D + 24), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = buf[1:-1, 8:8 + Hq * D]
+    assert torch.equal(run(c, out), want)
+    assert (buf[0] == 7).all() and (buf[-1] == 7).all() and (buf[:, :8] == 7).all() and (buf[:, 8 + Hq * D:] == 7).all()
+
+
+@pytest.mark.parametrize("S", [1, 40])
+def test_slots_past_32_bits(S):
+    """Slots so far apart that a byte's offset passes 2^32."""
+    c = case(2, S, 8, 1, 3, 2, False, lens=[2, 1])
+    want = run(c).clone()
+    big = torch.empty((1 << 32) + (1 << 22), dtype=torch.int8, device="cuda")
+
+    def far(t, n, at, step):
+        view = big[at:].as_strided((t.shape[0], 1, n, D), (1 << 16, D, step, 1))
+        view.copy_(t[:, :, :n])
+        return view
+    sh, own = c["shared"], c["own"]
+    c["shared"] = K.KVRing(far(sh.k_q, 3, 0, 1 << 31), far(sh.v_q, 3, 4096, 1 << 31), sh.k_scale[:, :, :3], sh.v_scale[:, :, :3], None, None, I8)
+    c["own"] = K.KVRing(far(own.k_q, 2, 8192, 1 << 32), far(own.v_q, 2, 12288, 1 << 32), own.k_scale[:, :, :2], own.v_scale[:, :, :2], None, None, I8)
+    assert torch.equal(run(c), want)
+
+
+@pytest.mark.parametrize("shape", [(3, 1, 8, 1, 700, 30, True), (64, 50, 8, 1, 300, 0, True), (64, 1, 8, 1, 6000, 70, True)], ids=str)
+def test_captured_calls_follow_their_inputs(shape):
+    """Two graphs captured over one workspace and a plan, replayed over changed inputs
+    and lengths on another stream: what the eager calls give, bit for bit."""
+    full = [shape[5]] * shape[0]  # (what lies past a length is NaN)
+    c, other = case(*shape, seed=1, lens=full), case(*shape, seed=2, lens=full)
+    out, out2 = torch.empty_like(run(c)), torch.empty_like(run(c))
+    need = K.attention_shared_workspace_bytes(K.attention_shared_desc(out=out, **c))
+    ws = torch.full((need + 1024,), 0xFF, dtype=torch.uint8, device="cuda")
+    K.attention_shared(out=out, workspace=ws, **c)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    with torch.cuda.graph(graphs[0]):
+        K.attention_shared(out=out, workspace=ws, **c)
+    with torch.cuda.graph(graphs[1]):
+        K.attention_shared(out=out2, workspace=ws, **other)
+    plan, out3 = K.Plan(), torch.empty_like(out)
+    plan.add(K.attention_shared_desc(out=out3, workspace=ws, **c))
+    st, r = torch.cuda.Stream(), gen(9)
+    for i in range(3):
+        c["q"].copy_(r(*c["q"].shape))
+        if "k_new" in c:
+            c["k_new"].copy_(r(*c["k_new"].shape))
+        if "own_len" in c:
+            c["own_len"].copy_(torch.randint(0, c["own_max"] + 1, c["own_len"].shape, generator=torch.Generator().manual_seed(i)))
+        want, want2 = run(c).clone(), run(other).clone()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            for g in graphs * 3:
+                g.replay()
+        st.synchronize()
+        plan.run()
+        done()
+        assert torch.equal(out2, want2) and torch.equal(out3, want) and torch.equal(out, want)
+
+
+def test_too_small_a_workspace_is_replaced():
+    c = case(64, 50, 8, 1, 300, 0, True)
+    want = run(c).clone()
+    assert torch.equal(run(dict(c, workspace=torch.empty(4096, dtype=torch.uint8, device="cuda"))), want)
+
+
+def test_two_streams_at_once():
+    cs = [case(64, 50, 8, 1, 300, 0, True), case(3, 1, 8, 1, 700, 30, True), case(64, 1, 8, 1, 6000, 70, True)]
+    outs = [run(c) for c in cs]
+    want = [o.clone() for o in outs]
+    sts = [torch.cuda.Stream() for _ in cs]
+    need = [K.attention_shared_workspace_bytes(K.attention_shared_desc(out=o, **c)) for c, o in zip(cs, outs)]
+    wss = [torch.empty(n + 1024, dtype=torch.uint8, device="cuda") for n in need]
+    for o, st in zip(outs, sts):
+        o.zero_()
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for c, o, ws, st in zip(cs, outs, wss, sts):
+            with torch.cuda.stream(st):
+                K.attention_shared(out=o, workspace=ws, **c)
+    done()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_wrong_sizes_are_refused():
+    c = case(2, 3, 8, 1, 64, 16, True)
+    out = run(c)
+    bad = [dict(q=c["q"].float()), dict(q=c["q"][0]), dict(q=c["q"].transpose(2, 3)), dict(n_shared=70), dict(shared=None),
+           dict(own_max=20), dict(own_len=c["own_len"].long()), dict(own_len=c["own_len"][:1]), dict(own=None),
+           dict(k_new=None), dict(v_new=c["v_new"][:, :, :2]), dict(k_new=c["k_new"].float()),
+           dict(new_block=torch.zeros(2, dtype=torch.int32, device="cuda")), dict(new_block=torch.zeros(3, device="cuda")),
+           dict(shared_valid=torch.ones(63, dtype=torch.uint8, device="cuda")), dict(shared_valid=torch.ones(64, device="cuda")),
+           dict(out=out[:5]), dict(out=out.float()), dict(out=out.cpu()), dict(workspace=torch.empty(4096, dtype=torch.uint8)),
+           dict(own=make_ring(gen(1), 2, 1, 16, U8)), dict(shared=make_ring(gen(1), 1, 2, 64))]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            K.attention_shared(**{**c, "out": out, **kw})
+    for kw in (dict(q=c["q"][..., :128]), dict(out=c["q"].view(-1)[:6 * 2048].view(6, 2048))):
+        with pytest.raises((ValueError, L.RfxError)):
+            K.attention_shared(**{**c, "out": out, **kw})
+    done()
+
+
+@pytest.mark.parametrize("fmt", [L.RFX_FP4_MX, L.RFX_FP4_NV])
+@pytest.mark.parametrize("B,S,W,H,F", [(1, 1, 512, 2, 1024), (4, 1, 1024, 8, 2048), (6, 50, 1024, 8, 2048)])
+def test_layer_run_together(fmt, B, S, W, H, F):
+    """A layer of candidate streams over one prompt on the 4-bit operators and the
+    attention, beside the norms and rotary positions that the library has: every stage
+    against the formula of what the stage before really left, and a captured plan's
+    replays on another stream bit-identical to the eager run."""
+    import math
+    import test_gpu_fp4 as P
+    r, T, ctx = gen(B + S), B * S, 300
+    e = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    w = {k: P.quantized(r(o, i) / math.sqrt(i), fmt, parts) for k, o, i, parts in
+         (("qkv", (H + 2) * D, W, 1), ("o", W, H * D, 1), ("gu", 2 * F, W, 2), ("down", W, F, 1))}
+    n = [(1 + 0.1 * r(W)).cuda() for _ in range(5)]
+    h0 = r(T, W).bfloat16().cuda()
+    h, z, qkv, att, y, act, last = h0.clone(), e(T, W), e(T, (H + 2) * D), e(T, H * D), e(T, W), e(T, F), e(T, W)
+    q, kn, vn = e(B, H, S, D), e(B, 1, S, D), e(B, 1, S, D)
+    zq, aq, fq = (K.Fp4Rows.allocate(T, k, fmt) for k in (W, H * D, F))
+    mq = K.Fp4Rows.allocate(T, W, fmt)
+    z2 = e(T, W)
+    shared = make_ring(r, 1, 1, ctx)
+    pos = (ctx + torch.arange(S, dtype=torch.int32)).repeat(B).cuda()
+    freq, _ = K.rope_frequencies(D)
+    ad = dict(q=q, shared=shared, n_shared=ctx, k_new=kn, v_new=vn, out=att, softmax_scale=D ** -0.5)
+    need = K.attention_shared_workspace_bytes(K.attention_shared_desc(**ad))
+    ws = torch.empty(need + 1024, dtype=torch.uint8, device="cuda")
+    descs = [
+        K.block_norm_desc(h=h, S=S, norm_a1=n[0], z=z),
+        K.quant_fp4_desc(x=z, out=zq),
+        K.linear_fp4_desc(w=w["qkv"], x=zq, y=qkv),
+        K.rope_desc(x=qkv, positions=pos, inv_freq=freq, q_out=q, k_out=kn, v_out=vn),
+        K.attention_shared_desc(workspace=ws, **ad),
+        K.quant_fp4_desc(x=att, out=aq),
+        K.linear_fp4_desc(w=w["o"], x=aq, y=y),
+        K.block_norm_desc(h=h, y=y, S=S, post_w=n[1], h_out=h, norm_a1=n[2], z=z2),
+        K.quant_fp4_desc(x=z2, out=mq),
+        K.linear_fp4_desc(w=w["gu"], x=mq, y=act, epilogue=L.RFX_EPI_GEGLU),
+        K.quant_fp4_desc(x=act, out=fq),
+        K.linear_fp4_desc(w=w["down"], x=fq, y=last),
+    ]
+    for d in descs:
+        K.Plan.run_direct(d)
+    done()
+
+    def stage(rows, weight, got, epi=L.RFX_EPI_STORE):
+        want, tol = P.ref_linear(P.values(rows), P.values(weight), None, epi)
+        check(got, want, tol + 2.0 ** -8 * (np.abs(want) + tol) + 1e-38)
+    for x, rows in ((z, zq), (att, aq), (z2, mq), (act, fq)):
+        again = P.quantized(x.cpu(), fmt)
+        assert torch.equal(again.q, rows.q) and torch.equal(again.scale, rows.scale)
+    stage(zq, w["qkv"], qkv)
+    check(att, *reference(q, shared, ctx, D ** -0.5, None, None, kn, vn))
+    stage(aq, w["o"], y)
+    stage(mq, w["gu"], act, L.RFX_EPI_GEGLU)
+    stage(fq, w["down"], last)
+    want = [t.clone() for t in (h, att, act, last)]
+    plan = K.Plan()
+    for d in descs:
+        plan.add(d)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        h.copy_(h0)
+        plan.capture(st)
+        for _ in range(3):
+            h.copy_(h0)
+            last.zero_()
+            plan.replay()
+    st.synchronize()
+    assert K.device_status() == 0
+    assert all(torch.equal(a, b) for a, b in zip((h, att, act, last), want))

@@ -307,3 +307,172 @@ def test_linear_any_length(fmt, T, Kc):
 def test_linear_any_output(fmt, T, O, pad, off, dtype):
     """Output rows of any length, stride and alignment; nothing beside them is written."""
     check_linear(T, O, 160, fmt, STORE, dtype, True, pad, off)
+
+
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("T,O,Kc,epi", [(129, 300, 9000, GELU), (200, 128, 16384, STORE), (700, 130, 5000, GEGLU),  # K in parts
+                                        (300, 2048, 4096, SILU), (2048, 2600, 512, STORE), (4000, 1100, 300, GELU),
+                                        (1300, 7000, 256, GEGLU), (600, 9000, 128, STORE)])                       # tiles of two widths
+def test_linear_as_it_is_cut_up(fmt, T, O, Kc, epi):
+    check_linear(T, O, Kc, fmt, epi, F32, epi != GEGLU)
+
+
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("T,O,Kc,epi", [(1, 300, 4096, STORE), (50, 512, 2048, GEGLU), (129, 300, 9000, GELU), (700, 2600, 512, STORE)])
+def test_same_bits_every_time(fmt, T, O, Kc, epi):
+    r = gen(3)
+    x, w = quantized(r(T, Kc), fmt), quantized(r(O, Kc) * Kc ** -0.5, fmt, 2 if epi == GEGLU else 1)
+    y = [torch.empty(T, O // 2 if epi == GEGLU else O, device="cuda") for _ in range(8)]
+    for t in y:
+        K.linear_fp4(w=w, x=x, y=t, epilogue=epi)
+    done()
+    assert all(torch.equal(t, y[0]) for t in y[1:])
+
+
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_nan_stays_in_its_row_and_column(fmt, T):
+    """A row of x or w that holds an infinity is NaN from quantizing on, and
+    reaches no other row's or column's products (in MX: its block)."""
+    r = gen(4)
+    x, w = r(T, 500), r(200, 500)
+    clean = torch.empty(T, 200, device="cuda")
+    K.linear_fp4(w=quantized(w, fmt), x=quantized(x, fmt), y=clean)
+    w[77, 499] = float("inf")
+    x[T - 1, 3] = float("nan")
+    y = torch.empty(T, 200, device="cuda")
+    xq, wq = quantized(x, fmt), quantized(w, fmt)
+    K.linear_fp4(w=wq, x=xq, y=y)
+    back = torch.empty(T, 500, device="cuda")
+    K.dequant_fp4(x=xq, out=back)
+    done()
+    assert y[T - 1].isnan().all() and y[:, 77].isnan().all()
+    keep = [c for c in range(200) if c != 77]
+    assert torch.equal(y[:T - 1][:, keep], clean[:T - 1][:, keep])
+    assert back[T - 1, :32].isnan().all() and not back[:T - 1].isnan().any()
+
+
+def test_no_rows():
+    for fmt in (MX, NV):
+        none, w = K.Fp4Rows.allocate(0, 64, fmt), quantized(gen(1)(8, 64), fmt)
+        e = torch.empty(0, 64, device="cuda")
+        K.quant_fp4(x=e, out=none)
+        K.dequant_fp4(x=none, out=e)
+        K.linear_fp4(w=w, x=none, y=torch.empty(0, 8, device="cuda"))
+    done()
+
+
+def test_wrong_sizes_are_refused():
+    r = gen(2)
+    x, w = quantized(r(4, 64), MX), quantized(r(8, 64), MX)
+    y = torch.empty(4, 8, device="cuda")
+    for kw in (dict(x=quantized(r(4, 96), MX)), dict(x=quantized(r(4, 64), NV)), dict(w=quantized(r(8, 64), MX, 2)),
+               dict(epilogue=GEGLU), dict(y=y[:3]), dict(y=y[:, :7]), dict(y=y.half()), dict(y=y.t().contiguous().t()),
+               dict(bias=torch.zeros(7, device="cuda")), dict(bias=torch.zeros(8, device="cuda").double()), dict(bias=torch.zeros(8)),
+               dict(y=y.cpu())):
+        with pytest.raises(ValueError):
+            K.linear_fp4(**{**dict(w=w, x=x, y=y), **kw})
+    for kw in (dict(x=r(5, 64).cuda()), dict(x=r(4, 63).cuda()), dict(x=r(4, 64).cuda().half()), dict(x=r(256).cuda())):
+        with pytest.raises(ValueError):
+            K.quant_fp4(**{**dict(x=r(4, 64).cuda(), out=x), **kw})
+    with pytest.raises(ValueError):
+        K.dequant_fp4(x=x, out=torch.empty(4, 65, device="cuda"))
+    with pytest.raises(L.RfxError):
+        K.linear_fp4(w=w, x=x, y=y, epilogue=L.RFX_EPI_RESIDUAL)
+    done()
+
+
+def test_rows_past_32_bits():
+    """Rows so far apart that an element's offset passes 2^31, one operand at a time
+    (rows of different pitches that interleave are refused)."""
+    r = gen(8)
+    big = torch.empty((1 << 32) + (1 << 20), dtype=torch.uint8, device="cuda")
+    x = r(2, 64).to(BF).cuda()
+    want = quantized(x, NV)
+    near = K.Fp4Rows.allocate(2, 64, NV)
+    far = K.Fp4Rows(big.as_strided((2, 32), ((1 << 32) + 64, 1)), near.scale, near.row_scale, 64, NV)
+    w = quantized(r(96, 64), NV)
+    y, back = torch.empty(2, 96, device="cuda"), torch.empty(2, 64, device="cuda")
+    K.quant_fp4(x=x, out=far)
+    K.linear_fp4(w=w, x=far, y=y)
+    K.dequant_fp4(x=far, out=back)
+    done()
+    assert torch.equal(far.q, want.q) and torch.equal(far.scale, want.scale)
+    v, tol = ref_linear(values(want), values(w), None, STORE)
+    assert (np.abs(y.double().cpu().numpy() - v) <= tol + HALF[F32] * np.abs(v)).all()
+    assert np.array_equal(back.double().cpu().numpy(), values(want))
+    wide = big.view(BF).as_strided((2, 64), ((1 << 31) + 64, 1))
+    wide.copy_(x)
+    K.quant_fp4(x=wide, out=near)
+    done()
+    assert torch.equal(near.q, want.q) and torch.equal(near.row_scale, want.row_scale)
+    K.dequant_fp4(x=near, out=wide.zero_())
+    done()
+    assert torch.equal(wide.double(), back.to(BF).double())
+    for T in (2, 5, 200):
+        xs = quantized(r(T, 64), NV)
+        ys = big.view(F32).as_strided((T, 96), ((1 << 30) // (T - 1) + 64, 1))
+        flat = torch.empty(T, 96, device="cuda")
+        K.linear_fp4(w=w, x=xs, y=ys)
+        K.linear_fp4(w=w, x=xs, y=flat)
+        done()
+        assert torch.equal(ys, flat)
+
+
+@pytest.mark.parametrize("T", [1, 50, 300])
+def test_captured_calls_follow_their_inputs(T):
+    """Captured into a graph and replayed on another stream over changed
+    inputs: what the eager calls give, bit for bit; so does a plan."""
+    r = gen(12)
+    Kc, O = 1000, 700
+    x, b = r(T, Kc).to(BF).cuda(), r(O).cuda()
+    w = quantized(r(O, Kc) * Kc ** -0.5, NV)
+    xq, y, back = K.Fp4Rows.allocate(T, Kc, NV), torch.empty(T, O, dtype=BF, device="cuda"), torch.empty(T, Kc, device="cuda")
+
+    def step():
+        K.quant_fp4(x=x, out=xq)
+        K.linear_fp4(w=w, x=xq, y=y, epilogue=SILU, bias=b)
+        K.dequant_fp4(x=xq, out=back)
+        return [t.clone() for t in (xq.q, xq.scale, xq.row_scale, y, back)]
+    step()
+    g, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g):
+        captured = step()
+    plan = K.Plan()
+    for d in (K.quant_fp4_desc(x=x, out=xq), K.linear_fp4_desc(w=w, x=xq, y=y, epilogue=SILU, bias=b), K.dequant_fp4_desc(x=xq, out=back)):
+        plan.add(d)
+    assert plan.num_launches == 3
+    for _ in range(3):
+        x.copy_(r(T, Kc))
+        want = step()
+        done()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            g.replay()
+        done()
+        assert all(torch.equal(a, c) for a, c in zip(captured, want))
+        y.zero_()
+        back.zero_()
+        plan.run()
+        done()
+        assert torch.equal(y, want[3]) and torch.equal(back, want[4])
+
+
+def test_two_streams_at_once():
+    cases = []
+    for i, (T, O, Kc) in enumerate([(50, 1024, 4096), (300, 300, 9000)]):
+        r = gen(20 + i)
+        x, w, y = quantized(r(T, Kc), NV), quantized(r(O, Kc), NV), torch.empty(T, O, device="cuda")
+        K.linear_fp4(w=w, x=x, y=y)
+        cases.append((w, x, y.clone(), y, torch.cuda.Stream()))
+    done()
+    for *_, y, st in cases:
+        y.zero_()
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for w, x, want, y, st in cases:
+            with torch.cuda.stream(st):
+                K.linear_fp4(w=w, x=x, y=y)
+    done()
+    for *_, want, y, st in cases:
+        assert torch.equal(want, y)
