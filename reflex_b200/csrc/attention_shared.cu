@@ -230,104 +230,84 @@ __global__ void __launch_bounds__(256) shared_dense_kernel(const __grid_constant
   const int held = is_shared ? p.n_shared : own_length(p, b);
   const int total = is_shared ? held : held + p.n_new;
   if (j * kKeys >= total) return;  // no unit visits it
-  __shared__ float dq[4][kPer];    // k scale, v scale, k zp, v zp of ring keys
-  __shared__ int seen[kPer];       // 0: no key, 1: of the ring, 2: new
-  __shared__ int bad[kPer];
-  float* words = p.words + static_cast<long>(block) * 4 * kKeys;
-  if (threadIdx.x < kPer) {
-    const int t = q0 + threadIdx.x, key = j * kKeys + t;
-    int kind = key < held ? 1 : key < total ? 2 : 0;
-    if (is_shared && kind == 1 && p.shared_valid && p.shared_valid[key] == 0) kind = 0;
-    float ks = 0.f, vs = 0.f;
-    int nb = kRingKey;
-    if (kind == 1) {
-      const long si = b * ring.ss_b + h * ring.ss_h + key * ring.ss_c;
-      const bool f32 = p.mode == kQuantI8Sym || !sbf16;
-      const float k = load_scalar(ring.k_scale, si, !f32), v = load_scalar(ring.v_scale, si, !f32);
-      if (p.mode == kQuantI8Sym) {
-        ks = k * p.scale_log2;
-        vs = v;
-      } else {
-        ks = p.scale_log2;
-        vs = 1.f;
-        dq[0][threadIdx.x] = k;
-        dq[1][threadIdx.x] = v;
-        dq[2][threadIdx.x] = load_scalar(ring.k_zp, si, sbf16);
-        dq[3][threadIdx.x] = load_scalar(ring.v_zp, si, sbf16);
-      }
-    } else if (kind == 2) {
-      ks = p.scale_log2;
-      vs = 1.f;
-      nb = block_id(p, key - held);
+  // 16 threads per key, 16 dims each.  A key's kind: 0 none, 1 of the ring, 2 new.
+  const int key = q0 + (threadIdx.x >> 4), g = threadIdx.x & 15, slot = j * kKeys + key;
+  int kind = slot < held ? 1 : slot < total ? 2 : 0;
+  uint4 raw[2][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) raw[i >> 1][i & 1] = make_uint4(0u, 0u, 0u, 0u);
+  float scale[2] = {0.f, 0.f}, zp[2] = {0.f, 0.f};
+  if (kind == 1) {
+    const long at = b * ring.qs_b + h * ring.qs_h + slot * ring.qs_c + g * 16;
+    raw[0][0] = *reinterpret_cast<const uint4*>(ring.k + at);
+    raw[1][0] = *reinterpret_cast<const uint4*>(ring.v + at);
+    const long si = b * ring.ss_b + h * ring.ss_h + slot * ring.ss_c;
+    const bool f32 = p.mode == kQuantI8Sym || !sbf16;
+    scale[0] = load_scalar(ring.k_scale, si, !f32);
+    scale[1] = load_scalar(ring.v_scale, si, !f32);
+    if (p.mode != kQuantI8Sym) {
+      zp[0] = load_scalar(ring.k_zp, si, sbf16);
+      zp[1] = load_scalar(ring.v_zp, si, sbf16);
     }
-    words[t] = ks;
-    words[kKeys + t] = vs;
-    words[2 * kKeys + t] = kind ? 0.f : -INFINITY;
-    reinterpret_cast<int*>(words)[3 * kKeys + t] = nb;
-    seen[threadIdx.x] = kind;
-    bad[threadIdx.x] = 0;
+    if (is_shared && p.shared_valid && p.shared_valid[slot] == 0) kind = 0;
+  } else if (kind == 2) {
+    const long n = slot - held;
+#pragma unroll
+    for (int isv = 0; isv < 2; ++isv) {
+      const __nv_bfloat16* src = isv ? p.v_new + b * p.vs_b + h * p.vs_h + n * p.vs_s : p.k_new + b * p.ks_b + h * p.ks_h + n * p.ks_s;
+      raw[isv][0] = *reinterpret_cast<const uint4*>(src + g * 16);
+      raw[isv][1] = *reinterpret_cast<const uint4*>(src + g * 16 + 8);
+    }
   }
-  __syncthreads();
-  // 16 keys x 16 chunks of 16 dims, K by the first half of the loop and V by the
-  // second; a new key's bad values are known only once all of it is looked at
-  const int key = q0 + (threadIdx.x >> 4), g = threadIdx.x & 15;
-  const int kind = seen[threadIdx.x >> 4];
+  float* words = p.words + static_cast<long>(block) * 4 * kKeys;
+  bool bad = false;
   const long row = (static_cast<long>(block) * kKeys + key) * kD + g * 16;
-  uint32_t wv[8];
 #pragma unroll
   for (int isv = 0; isv < 2; ++isv) {
     uint32_t w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = 0u;
     if (kind == 1) {
-      const uint4 raw = *reinterpret_cast<const uint4*>((isv ? ring.v : ring.k) + b * ring.qs_b + h * ring.qs_h +
-                                                        static_cast<long>(j * kKeys + key) * ring.qs_c + g * 16);
-      const uint8_t* b8 = reinterpret_cast<const uint8_t*>(&raw);
+      const uint8_t* b8 = reinterpret_cast<const uint8_t*>(&raw[isv][0]);
       float f[16];
       if (p.mode == kQuantI8Sym) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) f[e] = static_cast<float>(static_cast<int8_t>(b8[e]));
       } else {
-        const float sc = dq[isv ? 1 : 0][threadIdx.x >> 4], zp = dq[isv ? 3 : 2][threadIdx.x >> 4];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float t = round_to(__fsub_rn(static_cast<float>(b8[e]), zp), sbf16);
-          f[e] = round_to(__fmul_rn(t, sc), sbf16);
+          const float x = round_to(__fsub_rn(static_cast<float>(b8[e]), zp[isv]), sbf16);
+          f[e] = round_to(__fmul_rn(x, scale[isv]), sbf16);
         }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = isv ? pack_f16x2(f[2 * e], f[2 * e + 1]) : pack_bf16x2(f[2 * e], f[2 * e + 1]);
     } else if (kind == 2) {
-      const long n = j * kKeys + key - held;
-      const __nv_bfloat16* src = isv ? p.v_new + b * p.vs_b + h * p.vs_h + n * p.vs_s : p.k_new + b * p.ks_b + h * p.ks_h + n * p.ks_s;
-      const uint4 lo = *reinterpret_cast<const uint4*>(src + g * 16), hi = *reinterpret_cast<const uint4*>(src + g * 16 + 8);
+      const uint4 lo = raw[isv][0], hi = raw[isv][1];
       const uint32_t in[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = isv ? pack_f16x2(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u)) : in[e];
     }
     if (isv) {
-      bool out_of_range = false;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        out_of_range |= (w[e] & 0x7c00u) == 0x7c00u || (w[e] & 0x7c000000u) == 0x7c000000u;
-      if (out_of_range) bad[threadIdx.x >> 4] = 1;
+      for (int e = 0; e < 8; ++e) bad |= (w[e] & 0x7c00u) == 0x7c00u || (w[e] & 0x7c000000u) == 0x7c000000u;
+      // (a key's 16 threads are half of a warp)
+      const uint32_t all = __ballot_sync(0xffffffffu, bad);
+      bad = (all >> (threadIdx.x & 16) & 0xffffu) != 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) wv[e] = w[e];
-    } else {
-      uint4* dst = reinterpret_cast<uint4*>(p.kd + row);
-      dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      for (int e = 0; e < 8; ++e) w[e] = bad ? 0u : w[e];
     }
+    uint4* dst = reinterpret_cast<uint4*>(isv ? reinterpret_cast<uint16_t*>(p.vd) + row : reinterpret_cast<uint16_t*>(p.kd) + row);
+    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
-  __syncthreads();
-  if (bad[threadIdx.x >> 4]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) wv[e] = 0u;
-    if (g == 0) words[kKeys + key] = __uint_as_float(0x7fffffffu);
+  if (g == 0) {
+    const bool i8 = p.mode == kQuantI8Sym;
+    words[key] = kind == 0 ? 0.f : kind == 1 && i8 ? scale[0] * p.scale_log2 : p.scale_log2;
+    words[kKeys + key] = kind == 0 ? 0.f : bad ? __uint_as_float(0x7fffffffu) : kind == 1 && i8 ? scale[1] : 1.f;
+    words[2 * kKeys + key] = kind ? 0.f : -INFINITY;
+    reinterpret_cast<int*>(words)[3 * kKeys + key] = kind == 2 ? block_id(p, slot - held) : kRingKey;
   }
-  uint4* dst = reinterpret_cast<uint4*>(p.vd + row);
-  dst[0] = make_uint4(wv[0], wv[1], wv[2], wv[3]);
-  dst[1] = make_uint4(wv[4], wv[5], wv[6], wv[7]);
 }
 
 // ------------------------------------------------------------- attention ---
@@ -465,11 +445,12 @@ __device__ __forceinline__ int ld_acquire(const int* p) {
 }
 
 // Columns 8 g .. 8 g + 7 of a row, from parts that are added in order.
+template <int BATCH = 8>
 struct Joined {
   float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   template <typename Slot>
   __device__ __forceinline__ void add(const SharedAttnParams& p, int n, int r, int g, Slot slot) {
-    constexpr int kBatch = 8;
+    constexpr int kBatch = BATCH;
     for (int i0 = 0; i0 < n; i0 += kBatch) {
       float4 a[kBatch], b[kBatch];
       float2 ml[kBatch];
@@ -1039,7 +1020,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int slot0 = blockIdx.x - rank, groups = kD / 8 / n;
 #pragma unroll 1
       for (int g = rank * groups + ((threadIdx.x - kFirstWorker) >> 7); g < (rank + 1) * groups; g += 2) {
-        Joined j;
+        Joined<> j;
         j.add(p, n, r, g, [&](int i) { return static_cast<long>(slot0 + i); });
         *reinterpret_cast<uint4*>(p.out + at + g * 8) = j.result();
       }
@@ -1543,7 +1524,7 @@ __global__ void __launch_bounds__(ROWS * SLICES < 256 ? 256 : ROWS * SLICES) sha
   }
   const int h = tile / p.head_tiles, R = (tile - h * p.head_tiles) * ROWS + r;
   pdl_wait();
-  Joined j;
+  Joined<kThreads == 1024 ? 4 : 8> j;  // (64 registers a thread)
   if (R < p.rows) {
     const int mine = (n - slice + kSlices - 1) / kSlices;
     j.add(p, mine, r, g, [&](int i) {
