@@ -338,8 +338,9 @@ constexpr int kTmS = 384;
 constexpr int kWorkers = 256;
 constexpr int kFirstWorker = 128;
 constexpr int kThreads = kFirstWorker + kWorkers;
-constexpr int kJoinMost = 4;  // parts of a tile that the last CTA joins, at most
-constexpr int kFewMost = 64;  // rows per KV head up to which the form for few is taken
+constexpr int kJoinMost = 3;  // parts of a tile that the last CTA joins, at most
+constexpr int kFewMost = 2048;  // rows per KV head up to which the form for few may be taken (its time is above the
+                               // other's from about 1000 on, whatever the keys)
 
 // Barrier over the two worker warps of a TMEM lane quadrant that also ANDs a
 // flag over them.
@@ -1570,12 +1571,16 @@ struct Plan {
   size_t kd, vd, words, part_o, part_ml, arrived, total;
 };
 
-// Clusters, or runs of units: what ends soonest by this model, in us.  A CTA's
-// start and end cost kFix, a unit kUnit, a cluster's exchange kExchange, partial
-// results and the kernel that joins them kJoin and kPart per SM's worth of them.
-void deal(Plan* out, int nsm) {
+// Whole tiles, clusters, or runs of units: what ends soonest by this model, in us, fitted
+// to 13 batches at every way.  The keys' copy and the launches cost kCopy and kCopyBlock
+// per block of keys, a CTA's start and end on a tile kFix, a unit kUnit.  A cluster's
+// exchange is shorter the more CTAs share it.  Where a tile has at most kJoinMost parts the
+// last CTA joins them (kJoin), else a kernel of its own (kCombine and kCombineRow per row):
+// measured 62 and 70 us for 64 streams of 50 tokens over 818 slots (3 parts), 77 and 73 for
+// 16 of 51 over 6344 (4 parts).  Returns the time.
+double deal(Plan* out, int nsm) {
   SharedAttnParams& p = out->p;
-  constexpr double kFix = 3.0, kUnit = 0.75, kExchange = 1.5, kJoin = 4.0, kPart = 2.0;
+  constexpr double kCopy = 4.9, kCopyBlock = 0.0138, kFix = 5.5, kUnit = 1.22, kJoin = 13.0, kCombine = 6.0, kCombineRow = 0.0007;
   const long units = static_cast<long>(p.tiles) * p.tile_units;
   double best = 0;
   for (int c = 1; c <= kMaxCluster; c *= 2) {
@@ -1583,47 +1588,60 @@ void deal(Plan* out, int nsm) {
     const long slots = c == 1 ? nsm : static_cast<long>(max_active_clusters(reinterpret_cast<const void*>(attention_shared_kernel), kThreads, kSmemBytes, c)) * c;
     if (slots <= 0) continue;
     const long waves = (static_cast<long>(p.tiles) * c + slots - 1) / slots;
-    const double cost = waves * (kFix + (p.tile_units + c - 1) / c * kUnit + (c > 1 ? kExchange : 0.0));
+    const double cost = waves * (kFix + (p.tile_units + c - 1) / c * kUnit + (c > 1 ? 1.5 + 11.0 / c : 0.0));
     if (p.cluster && cost >= best) continue;
     best = cost;
     p.cluster = c;
   }
   const int ctas = static_cast<int>(std::min<long>(units, nsm));
-  const double cost = kFix + static_cast<double>((units + ctas - 1) / ctas) * kUnit + kJoin + kPart;
-  out->joined = cost < best;
-  if (out->joined) p.cluster = 0;
-  p.ctas = p.cluster ? p.tiles * p.cluster : ctas;
   p.run = static_cast<int>(units / ctas);
   p.longer = static_cast<int>(units % ctas);
-  p.join = out->joined && p.tile_units <= (kJoinMost - 1) * p.run;
+  const bool join = p.tile_units <= (kJoinMost - 1) * p.run;
+  const double ends = 1.0 + static_cast<double>(p.tiles) / ctas;  // of tiles, per CTA
+  const double cost = static_cast<double>((units + ctas - 1) / ctas) * kUnit + ends * kFix +
+                      (join ? kJoin : kCombine + kCombineRow * p.tiles * kRows);
+  out->joined = cost < best;
+  if (out->joined) p.cluster = 0;
+  p.join = out->joined && join;
+  p.ctas = p.cluster ? p.tiles * p.cluster : ctas;
+  return std::min(cost, best) + kCopy + kCopyBlock * out->blocks;
 }
 
-// The form for few rows: CTAs per tile (a cluster, or as many as there are SMs for,
-// whose parts a second kernel joins).  A warp's 16 keys cost kStep us, joining 3.
-void deal_few(Plan* out, int nsm) {
+// The form for few rows: CTAs per tile (a cluster, or as many as there are SMs for, whose
+// parts a second kernel joins).  16 keys of a warp cost kStep us, a CTA's start and end
+// kFix.  Returns the time, fitted like the other form's to 8 to 1024 rows of 64 to 16000
+// keys.
+double deal_few(Plan* out, int nsm) {
   SharedAttnParams& p = out->p;
-  constexpr double kStep = 0.55, kJoin = 3.0;
-  auto steps = [&](int ctas) { return (p.tile_units + ctas * kFewWarps - 1) / (ctas * kFewWarps); };
-  auto waves = [&](int ctas) { return (static_cast<long>(p.tiles) * ctas + nsm - 1) / nsm; };
+  constexpr double kFix = 4.0, kStep = 3.27, kJoin = 2.2, kJoinRow = 0.013;
+  auto time = [&](int ctas, long slots) {  // per tile, of all tiles at once
+    const long waves = (static_cast<long>(p.tiles) * ctas + slots - 1) / slots;
+    return waves * (kFix + (p.tile_units + ctas * kFewWarps - 1) / (ctas * kFewWarps) * kStep);
+  };
   p.cluster = 1;
-  double best = waves(1) * (2.0 + steps(1) * kStep);
-  for (int c = 2; c <= kFewMaxCluster; c *= 2) {
-    if (max_active_clusters(reinterpret_cast<const void*>(shared_few_kernel), 32 * kFewWarps, kFewSmem, c) <= 0) break;
-    const double cost = waves(c) * (2.0 + steps(c) * kStep + 0.8);
-    if (cost < best - 0.1) {
+  double best = time(1, nsm);
+  for (int c = 2; c <= kFewMaxCluster && c <= p.tile_units; c *= 2) {
+    const long slots = static_cast<long>(max_active_clusters(reinterpret_cast<const void*>(shared_few_kernel), 32 * kFewWarps, kFewSmem, c)) * c;
+    if (slots <= 0) break;
+    const double cost = time(c, slots) + 1.8 + 0.1 * c;
+    if (cost < best) {
       best = cost;
       p.cluster = c;
     }
   }
-  const int most = std::max(1, nsm / p.tiles);
-  if (most > p.cluster && 2.0 + steps(most) * kStep + kJoin < best) {
+  const int most = std::min(std::max(1, nsm / p.tiles), (p.tile_units + kFewWarps - 1) / kFewWarps);
+  const double cost = time(most, nsm) + kJoin + kJoinRow * p.tiles * kFewRows;
+  if (most > 1 && cost < best) {
+    best = cost;
     out->joined = true;
-    p.cluster = std::min<long>(most, (p.tile_units + kFewWarps - 1) / kFewWarps);
+    p.cluster = most;
   }
   p.ctas = out->joined ? p.tiles * p.cluster : 0;
+  return best;
 }
 
-int plan_shared(const rfx_attn_shared_desc& d, Plan* out) {
+// One form's plan and its time (few: tiles of 16 rows on the warps' matrix instructions).
+int plan_form(const rfx_attn_shared_desc& d, bool few, int nsm, Plan* out, double* time) {
   SharedAttnParams& p = out->p;
   *out = Plan{};
   p.B = d.B;
@@ -1636,8 +1654,8 @@ int plan_shared(const rfx_attn_shared_desc& d, Plan* out) {
   p.n_new = d.k_new ? d.S : 0;
   const long rows = static_cast<long>(d.B) * p.G * d.S;
   const long per = static_cast<long>(p.G) * d.S;
-  out->few = d.quant_mode == RFX_QUANT_I8_SYM && rows <= kFewMost;
-  const int tile_rows = out->few ? kFewRows : kRows, keys = out->few ? kFewKeys : kKeys;
+  out->few = few;
+  const int tile_rows = few ? kFewRows : kRows, keys = few ? kFewKeys : kKeys;
   // streams that a tile of rows can touch
   const long touch = per >= tile_rows ? (per % tile_rows ? 2 : 1) : tile_rows % per ? tile_rows / per + 2 : tile_rows / per;
   const long shared_blocks = (static_cast<long>(d.n_shared) + keys - 1) / keys;
@@ -1655,14 +1673,27 @@ int plan_shared(const rfx_attn_shared_desc& d, Plan* out) {
   p.own_blocks = static_cast<int>(own_blocks);
   p.streams = static_cast<int>(std::min<long>(touch, d.B));
   p.tile_units = static_cast<int>(units);
-  out->blocks = out->few ? 0 : p.Hkv * (shared_blocks + d.B * own_blocks);
+  out->blocks = few ? 0 : p.Hkv * (shared_blocks + d.B * own_blocks);
   if (out->blocks > 0x7fffffffl / kKeys) return set_error(RFX_E_INVAL, "rfx_attention_shared: too many keys");
+  *time = few ? deal_few(out, nsm) : deal(out, nsm);
+  return RFX_OK;
+}
+
+int plan_shared(const rfx_attn_shared_desc& d, Plan* out) {
+  SharedAttnParams& p = out->p;
   int nsm = 148;
   rfx_num_sms(&nsm);
-  if (out->few)
-    deal_few(out, nsm);
-  else
-    deal(out, nsm);
+  double time = 0;
+  int rc = plan_form(d, false, nsm, out, &time);
+  if (rc) return rc;
+  if (d.quant_mode == RFX_QUANT_I8_SYM && p.rows <= kFewMost) {
+    Plan few;
+    double few_time = 0;
+    rc = plan_form(d, true, nsm, &few, &few_time);
+    if (rc) return rc;
+    if (few_time < time) *out = few;
+  }
+  const int tile_rows = p.tile_rows;
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t o = off;

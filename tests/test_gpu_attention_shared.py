@@ -192,6 +192,10 @@ SHAPES = [
     (2, 16, 8, 1, 500, 128, True),
     (64, 2, 8, 4, 40, 8, True),
     (20, 50, 8, 1, 250, 0, True),
+    (64, 40, 8, 1, 1500, 0, True),   # tiles in parts that the last CTA joins
+    (70, 37, 8, 1, 1200, 30, True),
+    (64, 1, 8, 1, 1000, 70, True),
+    (130, 1, 4, 1, 5000, 20, True),
 ]
 
 
@@ -268,7 +272,7 @@ def test_masked_slots_may_hold_anything():
 
 
 @pytest.mark.parametrize("shape", [(64, 50, 8, 1, 300, 0, True), (30, 9, 8, 1, 3000, 100, True), (16, 51, 8, 1, 2000, 48, True),
-                                   (3, 1, 8, 1, 9000, 20, True), (64, 1, 8, 1, 6000, 70, False)], ids=str)
+                                   (3, 1, 8, 1, 9000, 20, True), (64, 1, 8, 1, 6000, 70, False), (64, 40, 8, 1, 1500, 0, True)], ids=str)
 def test_same_bits_every_time(shape):
     """Whichever CTA of a tile ends last, its parts are added in one order."""
     c = case(*shape)
@@ -319,7 +323,7 @@ def test_slots_past_32_bits(S):
     assert torch.equal(run(c), want)
 
 
-@pytest.mark.parametrize("shape", [(3, 1, 8, 1, 700, 30, True), (64, 50, 8, 1, 300, 0, True), (64, 1, 8, 1, 6000, 70, True)], ids=str)
+@pytest.mark.parametrize("shape", [(3, 1, 8, 1, 700, 30, True), (64, 50, 8, 1, 300, 0, True), (64, 1, 8, 1, 6000, 70, True), (64, 40, 8, 1, 1500, 0, True)], ids=str)
 def test_captured_calls_follow_their_inputs(shape):
     """Two graphs captured over one workspace and a plan, replayed over changed inputs
     and lengths on another stream: what the eager calls give, bit for bit."""
