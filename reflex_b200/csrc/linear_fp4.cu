@@ -676,6 +676,10 @@ __global__ void __launch_bounds__(kSideThreads, 3)
     tma_prefetch_desc(&tmXS);
     tma_prefetch_desc(&tmWS);
   }
+  // Waited for before the first store into a peer.  Before TMEM is asked for, and TMEM is
+  // given back before the peers' sums are waited for: CTAs that wait for TMEM which
+  // others on their SM hold would otherwise wait in a circle.
+  if (splits > 1) cluster_arrive_release();
   if (warp == 1) {
     tmem_alloc(tmem_slot, cols);
     tmem_relinquish();
@@ -684,7 +688,6 @@ __global__ void __launch_bounds__(kSideThreads, 3)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (splits > 1) cluster_arrive_release();  // waited for before the first store into a peer
   pdl_launch_dependents();
   pdl_wait();
 
@@ -728,7 +731,10 @@ __global__ void __launch_bounds__(kSideThreads, 3)
     int s = 0, s2 = 0;  // s2: the stage of two steps before
     uint32_t phase = 0, phase2 = 0;
     for (int i = 0; i < nk; ++i) {
-      if (i >= 2) {  // the MMAs of two steps before have read this set of scales
+      // The MMAs of two steps before have read this set of scales.  (A ring of one or two
+      // stages has been filled again, so they have; waiting for their phase there could
+      // miss it, since the next one of that parity may be over.)
+      if (i >= 2 && stages > 2) {
         if (!__all_sync(0xffffffffu, mbar_wait(&empty[s2], phase2, p.status, kDevTimeoutMmaDone))) break;
         if (++s2 == stages) {
           s2 = 0;
@@ -833,6 +839,13 @@ __global__ void __launch_bounds__(kSideThreads, 3)
         }
       }
     }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem, cols);
+    }
+    __syncwarp();
     cluster_sync();
     if (warp >= 2 && summed && o < p.F) {
       const float4* in = reinterpret_cast<const float4*>(red) + et % kTileM;
@@ -877,7 +890,7 @@ __global__ void __launch_bounds__(kSideThreads, 3)
     for (int i = (issued > stages ? issued - stages : 0); i < issued; ++i)
       mbar_wait(&full[i % stages], (i / stages) & 1, p.status, kDevTimeoutTmaFull);
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 1 && splits == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, cols);
   }
@@ -910,9 +923,14 @@ const void* fp4_kernel(const rfx_linear_fp4_desc& d, int form) {
   return nullptr;
 }
 
-// Tiles with the weights on the M side: the split of K that gives every SM work
-// with few K steps each; a ring as deep as a CTA's part of K, as far as it fits.
+// Tiles with the weights on the M side: the split of K that ends soonest by this model, in
+// us, fitted to 10 projections of 1, 16, 50 and 128 tokens at every split.  A K step takes
+// kStep (kStepGeglu with two weight rows per output; more where the ring has a stage or
+// two), launch and epilogue kFix and kFixToken per token, the exchange kSplit, kSplitStep
+// and kSplitToken.
 void plan_side(const rfx_linear_fp4_desc& d, int nsm, int k_steps, LinearFp4Plan* c) {
+  constexpr double kFix = 1.75, kFixToken = 0.0095, kStep = 0.365, kStepGeglu = 0.55;
+  constexpr double kSplit = 0.6, kSplitStep = 0.12, kSplitToken = 0.012;
   const bool geglu = d.epilogue == RFX_EPI_GEGLU, mx = d.format == RFX_FP4_MX;
   const void* fn = fp4_kernel(d, kFp4Side);
   const int N = (d.T + 15) / 16 * 16;
@@ -920,13 +938,27 @@ void plan_side(const rfx_linear_fp4_desc& d, int nsm, int k_steps, LinearFp4Plan
   c->form = kFp4Side;
   c->nt = N;
   c->clusters = static_cast<int>(tiles);
-  c->splits = 1;
-  while (c->splits < kSideMaxSplits && tiles * c->splits * 2 <= nsm && c->splits * 2 <= k_steps &&
-         max_active_clusters(fn, kSideThreads, kSmemMax, c->splits * 2) > 0)
-    c->splits *= 2;
-  int stages = std::min(kSideMaxStages, (k_steps + c->splits - 1) / c->splits);
-  while (stages > 1 && side_smem(N, c->splits, geglu, mx, stages) > kSmemMax) --stages;
-  c->stages = stages;
+  double best = 0;
+  for (int s = 1; s <= kSideMaxSplits && s <= k_steps; s *= 2) {
+    const int n = (k_steps + s - 1) / s;
+    int stages = std::min(kSideMaxStages, n);
+    while (stages > 1 && side_smem(N, s, geglu, mx, stages) > kSmemMax) --stages;
+    const int smem = side_smem(N, s, geglu, mx, stages);
+    if (smem > kSmemMax) break;
+    double waves = std::max(1.0, static_cast<double>(tiles) / nsm);
+    if (s > 1) {
+      const long slots = std::min<long>(max_active_clusters(fn, kSideThreads, smem, s), nsm * (512l / side_cols(N, geglu, mx)) / s);
+      if (slots <= 0) break;
+      waves = std::max<double>((tiles + slots - 1) / slots, static_cast<double>(tiles) * s / nsm);
+    }
+    const double step = (geglu ? kStepGeglu : kStep) + (n > stages ? (stages == 1 ? 0.8 : stages == 2 ? 0.35 : 0.0) : 0.0);
+    const double cost = kFix + kFixToken * d.T + waves * n * step + (waves > 1 ? (waves - 1) * kFixToken * d.T : 0.0) +
+                        (s > 1 ? kSplit + kSplitStep * n + kSplitToken * d.T : 0.0);
+    if (s > 1 && cost >= best) continue;
+    best = cost;
+    c->splits = s;
+    c->stages = stages;
+  }
 }
 
 // Pair tiles, above 128 tokens: the width and the split of K that finish soonest by
@@ -1124,11 +1156,7 @@ int launch_linear_fp4(const rfx_linear_fp4_desc& d, const LinearFp4Maps& maps, c
   p.status = device_status_ptr();
   CUtensorMap x = maps.x, w = maps.w, w2 = maps.w2, xs = maps.xs, ws = maps.ws, y = maps.y;
   if (c.form == kFp4Side) {
-    // Above 128 TMEM columns a CTA takes all of an SM's shared memory, so that no
-    // other CTA with TMEM of its own is beside it: two clusters that each wait for
-    // TMEM that the other holds would wait for good.  (Three CTAs' registers fill
-    // an SM, which is 384 columns.)
-    const int smem = side_cols(c.nt, geglu, mx) > 128 ? kSmemMax : side_smem(c.nt, c.splits, geglu, mx, c.stages);
+    const int smem = side_smem(c.nt, c.splits, geglu, mx, c.stages);
     return launch_kernel(fn, dim3(c.clusters * c.splits), dim3(kSideThreads), static_cast<size_t>(smem), stream, pdl,
                          c.splits, x, w, xs, ws, p);
   }

@@ -476,3 +476,11 @@ def test_two_streams_at_once():
     done()
     for *_, want, y, st in cases:
         assert torch.equal(want, y)
+
+
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("T,O,Kc", [(128, 8192, 4096), (120, 8192, 9000), (128, 2048, 16384), (97, 600, 8192)])
+def test_rings_of_one_stage(fmt, T, O, Kc):
+    """Many tokens and K steps beside the sums of a split K in shared memory: rings of a
+    stage or two, filled again many times."""
+    check_linear(T, O, Kc, fmt, GEGLU, F32, False)
