@@ -927,10 +927,10 @@ const void* fp4_kernel(const rfx_linear_fp4_desc& d, int form) {
 // us, fitted to 10 projections of 1, 16, 50 and 128 tokens at every split.  A K step takes
 // kStep (kStepGeglu with two weight rows per output; more where the ring has a stage or
 // two), launch and epilogue kFix and kFixToken per token, the exchange kSplit, kSplitStep
-// and kSplitToken.
+// and kSplitToken (twice the sums with two rows per output).
 void plan_side(const rfx_linear_fp4_desc& d, int nsm, int k_steps, LinearFp4Plan* c) {
   constexpr double kFix = 1.75, kFixToken = 0.0095, kStep = 0.365, kStepGeglu = 0.55;
-  constexpr double kSplit = 0.6, kSplitStep = 0.12, kSplitToken = 0.012;
+  const double kSplit = d.epilogue == RFX_EPI_GEGLU ? 1.6 : 0.6, kSplitStep = 0.12, kSplitToken = d.epilogue == RFX_EPI_GEGLU ? 0.025 : 0.012;
   const bool geglu = d.epilogue == RFX_EPI_GEGLU, mx = d.format == RFX_FP4_MX;
   const void* fn = fp4_kernel(d, kFp4Side);
   const int N = (d.T + 15) / 16 * 16;
@@ -952,8 +952,9 @@ void plan_side(const rfx_linear_fp4_desc& d, int nsm, int k_steps, LinearFp4Plan
       waves = std::max<double>((tiles + slots - 1) / slots, static_cast<double>(tiles) * s / nsm);
     }
     const double step = (geglu ? kStepGeglu : kStep) + (n > stages ? (stages == 1 ? 0.8 : stages == 2 ? 0.35 : 0.0) : 0.0);
-    const double cost = kFix + kFixToken * d.T + waves * n * step + (waves > 1 ? (waves - 1) * kFixToken * d.T : 0.0) +
-                        (s > 1 ? kSplit + kSplitStep * n + kSplitToken * d.T : 0.0);
+    // (without clusters CTAs follow one another on an SM, or share it)
+    const double cost = s == 1 ? kFix + waves * (kFixToken * d.T + n * step)
+                               : waves * (kFix + kFixToken * d.T + n * step + kSplit + kSplitStep * n + kSplitToken * d.T);
     if (s > 1 && cost >= best) continue;
     best = cost;
     c->splits = s;
