@@ -223,11 +223,16 @@ __device__ __forceinline__ void store_unit(const QuantFp4Params& p, uint8_t* q, 
 
 constexpr int kWarpRows = 4;  // rows of a CTA at a time where a warp has one
 constexpr int rows_at_a_time(int tpr) { return tpr == 32 ? kWarpRows : 1; }
+// The longest rows that are held: 64 registers a thread, so that 768 of 16384 values are
+// under way at once (left to itself the compiler takes 116, and 10.8 us instead of 9.3);
+// shorter ones lose more by it than they gain (4304 values: 5.7 us instead of 4.9).
+constexpr int ctas_per_sm(int tpr, int nu, int bytes) { return tpr == 256 && nu == 4 && bytes == 2 ? 4 : 0; }
 
 // NU units per thread of a row's TPR threads; NU = 0: rows of any length, read
 // a second time where NV needs their maximum first.
 template <typename Tin, int FMT, int TPR, int NU, int VEC>
-__global__ void __launch_bounds__(TPR* rows_at_a_time(TPR)) quant_fp4_kernel(const QuantFp4Params p) {
+__global__ void __launch_bounds__(TPR* rows_at_a_time(TPR), ctas_per_sm(TPR, NU, sizeof(Tin)))
+    quant_fp4_kernel(const QuantFp4Params p) {
   __shared__ uint32_t part[2][TPR / 32];
   pdl_wait();
   pdl_launch_dependents();
@@ -384,18 +389,23 @@ __global__ void __launch_bounds__(256) dequant_fp4_kernel(const DequantFp4Params
     for (int c = 0; c < kTurn; ++c) {
       const int u = u0 + c * TPR, k = u * kUnit;
       if (u >= p.units) continue;
-      // 2^(byte - 127) as two factors: byte 0 is below the smallest normal number
-      const float s0 = FMT == RFX_FP4_MX
-                           ? (byte[c] == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(max(byte[c], 1u) << 23))
-                           : from_e4m3(byte[c]);
-      const float s1 = FMT == RFX_FP4_MX ? (byte[c] == 0 ? 0.5f : 1.f) : row_scale;
+      // 2^(byte - 127), of byte 0 a subnormal number; an NV scale's 4 bits times the row's
+      // power of two, and a code's 3 bits times that, are exact
+      const float s = FMT == RFX_FP4_MX ? (byte[c] == 255 ? __uint_as_float(0x7fffffffu)
+                                           : byte[c] == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte[c] << 23))
+                                        : from_e4m3(byte[c]) * row_scale;
+      const unsigned long long s2 = pack_f32x2(s, s);
       float v[16];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float x[8];
         unpack_e2m1(h ? codes[c].y : codes[c].x, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[8 * h + e] = x[e] * s0 * s1;
+        for (int e = 0; e < 8; e += 2) {
+          const unsigned long long y = mul_f32x2(pack_f32x2(x[e], x[e + 1]), s2);
+          v[8 * h + e] = lo_f32(y);
+          v[8 * h + e + 1] = hi_f32(y);
+        }
       }
       if (VEC && k + kUnit <= p.K) {
         put16<VEC>(y + k, v);
