@@ -7,7 +7,9 @@
 // The 4 scale bytes of neighbouring blocks lie together in the tiles that the
 // tensor cores take, and are gathered by shuffles into one 4-byte store.
 //
-// Bound by memory traffic: 2 bytes per value in (bf16), 9/16 out.
+// Bound by memory traffic: 2 bytes per value in (bf16), 9/16 out.  768 x 16384 (NV): 9.3 us,
+// 3.5 TB/s, whole rows of 5 or 6 per SM; MX 7.5 us; 4096 x 4096 9.6 us, 4.5 TB/s.  Back:
+// 7.1 us, 4.5 TB/s.  Single rows take 1.3 us, a launch.
 #include "quant_i8.cuh"
 #include "rfx_internal.h"
 
