@@ -484,3 +484,27 @@ def test_rings_of_one_stage(fmt, T, O, Kc):
     """Many tokens and K steps beside the sums of a split K in shared memory: rings of a
     stage or two, filled again many times."""
     check_linear(T, O, Kc, fmt, GEGLU, F32, False)
+
+
+@pytest.mark.parametrize("epi", [GELU, SILU])
+@pytest.mark.parametrize("T", [2, 200])
+def test_activations_of_any_size(epi, T):
+    """Outputs from -1e30 to 1e30 side by side, infinities and NaN among them."""
+    big = torch.tensor([0.0, -1e-3, -0.5, -3.0, -9.0, -15.0, -40.0, -1e4, -1e30, 1e30, 1e4, 40.0, 9.0, 3.0, 0.5, 1e-3])
+    O = 16 * 12
+    b = big.repeat(12)
+    b[5 * 16 + 3], b[7 * 16 + 4], b[9 * 16 + 8] = float("nan"), float("inf"), float("-inf")
+    x, w = quantized(torch.zeros(T, 64), MX), quantized(torch.zeros(O, 64), MX)
+    y = torch.empty(T, O, device="cuda")
+    K.linear_fp4(w=w, x=x, y=y, epilogue=epi, bias=b.cuda())
+    done()
+    got, v = y.double().cpu().numpy(), b.double().numpy()
+    with np.errstate(over="ignore", invalid="ignore"):
+        e = v if epi == SILU else 1.5957691216057308 * (v + 0.044715 * v ** 3)
+        want = v / (1 + np.exp(-e))  # (-inf: NaN, as the formula's 0 times infinity)
+        want[v == -np.inf] = np.nan
+        tol = np.abs(want) * (3 * U32 * np.abs(e) * 1.5 + 2.0 ** -20) + 2.0 ** -58 * np.minimum(np.abs(v), 64)
+    assert np.array_equal(np.isnan(got), np.broadcast_to(np.isnan(want), got.shape))
+    ok = np.isfinite(want)
+    assert (np.abs(got[:, ok] - want[ok]) <= tol[ok]).all(), np.abs(got[:, ok] - want[ok]).max()
+    assert (got[:, v == np.inf] == np.inf).all()
