@@ -1012,6 +1012,10 @@ LinearFp4Plan plan_fp4(const rfx_linear_fp4_desc& d, int nsm) {
       const long tiles = static_cast<long>(m) * n;
       const long rounds = (tiles + slots - 1) / slots;
       if (s > 1 && rounds > 1) continue;
+      // what a CTA is sent has to fit into its ring: groups of 128 output bytes, of which
+      // it finishes one in `s`, from each of the other splits
+      const int group = 128 / (d.out_dtype == kDtypeBF16 ? 2 : 4), groups = (nt / div + group - 1) / group;
+      if (s > 1 && (groups + s - 1) / s * (s - 1) * div * (group / 4 * kTileM * 16) > kPairRing) continue;
       auto consider = [&](double cost, int n_a, int nt2, int n_b) {
         if (c.nt != 0 && cost >= best) return;
         best = cost;

@@ -508,3 +508,11 @@ def test_activations_of_any_size(epi, T):
     ok = np.isfinite(want)
     assert (np.abs(got[:, ok] - want[ok]) <= tol[ok]).all(), np.abs(got[:, ok] - want[ok]).max()
     assert (got[:, v == np.inf] == np.inf).all()
+
+
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("T,O,Kc", [(594, 40, 9598), (300, 200, 16384), (200, 256, 12000), (1024, 20, 8000)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_geglu_in_many_parts(fmt, T, O, Kc, dtype):
+    """Few outputs of a long K: what the parts of K send one another fits beside the scales."""
+    check_linear(T, O, Kc, fmt, GEGLU, dtype, True)
