@@ -328,7 +328,8 @@ int rfx_attention_noalloc(const rfx_attn_desc* desc, void* stream);
  * Numerics as in rfx_attention: scores and sums in fp32, P (times the key's
  * value scale) and V in f16 in P V, exact while a context token's value absmax
  * stays below about 32,000 (and fine down to about 0.01: a weight times its value
- * scale, absmax / 127, is rounded to steps of 2^-24 below 2^-14); a new token with
+ * scale, absmax / 127, is rounded to steps of 2^-24 below 2^-14, and so is a new
+ * token's value); a new token with
  * a value beyond f16 makes the rows that see it NaN.  Results do not depend on the
  * order in which SMs finish. */
 typedef struct rfx_kv_view { /* a quantized ring: rows of 256 bytes at byte strides, scales at element strides */

@@ -65,7 +65,9 @@ def reference(q, shared, n_shared, scale, own=None, own_len=None, k_new=None, v_
     exponential; a weight times its value scale is rounded to f16, by 2^-11 of it or,
     among the subnormal numbers (steps of 2^-24), by 2^-25, and multiplies an integer
     of at most 127 (a ring's int8 value, which its scale does not shrink there) or the
-    value itself (scale 1): (2^-25 / l) sum of those, with the largest weight 1; sums
+    value itself (scale 1): (2^-25 / l) sum of those, with the largest weight 1; a bf16
+    value is exact in f16 (8 of 11 bits) from 2^-14 on and off by 2^-25 below, which the
+    weights' mean keeps: 2^-25; sums
     over n keys in fp32 add (n / 16 + 4) 2u; the output is rounded to bf16."""
     q = q.double().cpu().numpy()
     B, Hq, S, _ = q.shape
@@ -116,7 +118,7 @@ def reference(q, shared, n_shared, scale, own=None, own_len=None, k_new=None, v_
                 operand[:ctx] = 127.0
             d = (p * ds) @ av + (p * ds).sum(axis=1, keepdims=True) * (p @ av)
             d += 2.0 ** -11 * (p @ av) + (2.0 ** -25 / np.maximum(l, 1e-300)) * (np.minimum(1, see) @ operand) * ok_row
-            d += (len(k) / 16 + 4) * 2 * u * (p @ av)
+            d += (len(k) / 16 + 4) * 2 * u * (p @ av) + 2.0 ** -25 * ok_row
             d += 2.0 ** -8 * (np.abs(o) + d) + 1e-38
             out[b, :, h * G:(h + 1) * G] = o.reshape(G, S, D).transpose(1, 0, 2)
             tol[b, :, h * G:(h + 1) * G] = d.reshape(G, S, D).transpose(1, 0, 2)
