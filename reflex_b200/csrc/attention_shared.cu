@@ -17,8 +17,8 @@
 // What bounds it: a block's MMAs take 1024 clocks, and a block comes every 2300.  That is
 // the chain of one softmax warp, whose two groups take the blocks in turn: 900
 // instructions of 64 keys at 2 warps per scheduler, which issues in 27 % of its clocks.
-// A third group found no registers (128 a thread; what the compiler then keeps in memory
-// made it a fifth slower).  64 streams of 50 tokens x 8 heads over 818 shared slots: 58 us,
+// A third group (152 registers a thread, a tile's end in smaller steps) gained 3 % on
+// the first batch below and lost 6 and 9 % on the last and on small ones.  64 streams of 50 tokens x 8 heads over 818 shared slots: 58 us,
 // 390 TFLOP/s; 16 of 51 over 6344: 72 us, 600 TFLOP/s; 64 single tokens over 32768: 51 us.
 //
 // K (bf16) and V (f16) of a block come by TMA from a dense copy of all keys that a
