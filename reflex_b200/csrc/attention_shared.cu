@@ -835,6 +835,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_st16(tmO + lane_base + (c0 + q) * 16, oo[q]);
               }
             }
+            // (the stores are asynchronous: they are done before P is announced, which
+            // lets the issuing warp add to O)
+            tmem_wait_st();
           }
           // P (times the value scales), where P of this group's block before was, once
           // its P V is done
@@ -865,6 +868,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<uint4*>(pt + sw128_offset(r, c)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
           }
           fence_proxy_async_smem();
+          tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_ready[ch]);
           const unsigned long long both = add_f32x2(sum[0], sum[1]);

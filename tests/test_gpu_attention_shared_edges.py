@@ -1,0 +1,66 @@
+"""Attention over a shared context on the GPU where a row's softmax is hard: maxima that
+rise from block to block.  Against the formula in 64 bits, with the tolerance that is
+derived beside it.
+"""
+import pytest
+import torch
+
+import test_gpu_attention_shared as A
+from reflex_b200 import kernels as K
+
+pytestmark = pytest.mark.gpu
+D, I8, U8 = A.D, A.I8, A.U8
+
+
+def ring_of(k, v, capacity=None, mode=I8, scale_dtype=None):
+    """A ring [B, H, n, D] of these keys and values; slots past them hold what no row may use."""
+    B, H, n, _ = k.shape
+    ring = K.KVRing.allocate(B, H, capacity or n, D, mode, **({} if scale_dtype is None else dict(scale_dtype=scale_dtype)))
+    ring.k_q.fill_(125)
+    ring.v_q.fill_(125)
+    for t in (ring.k_scale, ring.v_scale, ring.k_zp, ring.v_zp):
+        if t is not None:
+            t.fill_(float("nan"))
+    K.kv_quant_append(k.bfloat16().cuda(), v.bfloat16().cuda(), ring, 0, 0, ring.capacity)
+    return ring
+
+
+# B, S, Hq, n_shared, own: clusters, whole tiles, tiles that the last CTA joins, tiles that
+# a kernel joins, few rows
+RISING = [(4, 50, 8, 818, 0), (64, 50, 8, 818, 0), (64, 40, 8, 1500, 70), (16, 51, 8, 3000, 130), (64, 1, 8, 6000, 200),
+          (3, 5, 8, 700, 90), (1, 1, 8, 5000, 0)]
+
+
+def rising(B, S, Hq, n_shared, own, holes):
+    """Keys along 16 directions whose scores rise by 17 log2 units per 64 keys up to a block
+    that is another one for each, and rows of which two in three look along one of them."""
+    c = A.case(B, S, Hq, 1, n_shared, own, True, seed=11, holes=holes)
+    r = A.gen(B + S + n_shared)
+    blocks = (n_shared + own) // 64 + 1
+
+    def keys(B, n, first):
+        k = 0.3 * r(B, 1, n, D)
+        at = (first + torch.arange(n)) // 64
+        for d in range(16):
+            k[..., d] += 12.0 * torch.clamp(at, max=1 + (d + 1) * blocks // 16).float()
+        return k
+    c["shared"] = ring_of(keys(1, n_shared, 0), r(1, 1, n_shared, D), n_shared + 5)
+    if own:
+        c["own"] = ring_of(keys(B, own, n_shared), r(B, 1, own, D))
+    q = 0.3 * r(B, Hq, S, D)
+    row = torch.arange(B * Hq * S).view(B, Hq, S)
+    look = torch.nn.functional.one_hot(row * 7 % 16, D).float() * 16.0
+    c["q"] = torch.where((row % 3 != 0)[..., None], q + look, q).bfloat16().cuda()
+    return c
+
+
+@pytest.mark.parametrize("shape", RISING, ids=str)
+@pytest.mark.parametrize("holes", [False, True])
+def test_maxima_that_rise_in_every_block(shape, holes):
+    """O is rescaled in nearly every block, for some rows of a warp and not for others: the
+    formula's values, and the same bits each time."""
+    c = rising(*shape, holes)
+    want = A.run(c).clone()
+    A.check(want, *A.want_of(c))
+    for _ in range(20):
+        assert torch.equal(A.run(c), want)
