@@ -99,12 +99,10 @@ struct SharedAttnParams {
 };
 
 // Block ids: a key is visible to the rows of its stream whose id is not below its
-// own.  Ring keys come below every new key's id, other streams' rows below them.
-constexpr int kForeignRow = -0x7fffffff - 1;
-constexpr int kRingKey = kForeignRow + 1;
-__device__ __forceinline__ int block_id(const SharedAttnParams& p, int s) {
-  return p.new_block ? max(p.new_block[s], kRingKey) : 0;
-}
+// own.  They may be any numbers, and ring keys have the lowest; that a row is another
+// stream's, or that a key's place is empty, is told apart from them.
+constexpr int kRingKey = -0x7fffffff - 1;
+__device__ __forceinline__ int block_id(const SharedAttnParams& p, int s) { return p.new_block ? p.new_block[s] : 0; }
 
 __device__ __forceinline__ int own_length(const SharedAttnParams& p, int b) {
   if (p.own_max == 0) return 0;
@@ -789,13 +787,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                                      pack_f32x2(ka.z, ka.w));
           }
           if (kOwn) {
-            const int upto = blk.stream == b_row ? my_block : kForeignRow;
   #pragma unroll
             for (int c = 0; c < kKeys / 4; ++c) {
               const int4 nb = nb_s[c];
-              z[2 * c] = pack_f32x2(nb.x > upto ? -INFINITY : lo_f32(z[2 * c]), nb.y > upto ? -INFINITY : hi_f32(z[2 * c]));
-              z[2 * c + 1] = pack_f32x2(nb.z > upto ? -INFINITY : lo_f32(z[2 * c + 1]),
-                                        nb.w > upto ? -INFINITY : hi_f32(z[2 * c + 1]));
+              z[2 * c] = pack_f32x2(nb.x > my_block ? -INFINITY : lo_f32(z[2 * c]),
+                                    nb.y > my_block ? -INFINITY : hi_f32(z[2 * c]));
+              z[2 * c + 1] = pack_f32x2(nb.z > my_block ? -INFINITY : lo_f32(z[2 * c + 1]),
+                                        nb.w > my_block ? -INFINITY : hi_f32(z[2 * c + 1]));
+            }
+            // (on its own: as a second condition above it takes more registers)
+            if (blk.stream != b_row) {
+  #pragma unroll
+              for (int c = 0; c < kKeys / 2; ++c) z[c] = pack_f32x2(-INFINITY, -INFINITY);
             }
           }
   #pragma unroll
@@ -1281,17 +1284,19 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) shared_few_kernel(const __g
     blocks.step(p, ahead);
     const int key0 = b.j * kFewKeys;
     const bool has_new = b.total > b.held && key0 + kFewKeys > b.held;
-    // score and value scales of the thread's four keys, and the block ids from which on
-    // they are seen
+    // score and value scales of the thread's four keys, whether there is such a key, and
+    // the block id from which on it is seen
     float ks[4], vs[4];
     int nb[4];
+    bool there[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const int key = key0 + 2 * t + (n & 1) + 8 * (n >> 1);
       const bool seen = key < b.held && (raw.valid >> n & 1);
       ks[n] = seen ? raw.ks[n] * p.scale_log2 : 0.f;
       vs[n] = seen ? raw.vs[n] : 0.f;
-      nb[n] = seen ? kRingKey : 0x7fffffff;  // (no row's)
+      nb[n] = kRingKey;
+      there[n] = seen;
     }
     // a step with new tokens goes through the warp's (still unused) part of shared
     // memory, bf16 K and f16 V
@@ -1304,6 +1309,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) shared_few_kernel(const __g
           ks[n] = p.scale_log2;
           vs[n] = (bad >> i & 1) ? __uint_as_float(0x7fffffffu) : 1.f;
           nb[n] = block_id(p, key - b.held);
+          there[n] = true;
         }
       }
     }
@@ -1344,10 +1350,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) shared_few_kernel(const __g
     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int most = b.stream < 0 ? 0x7ffffffe : b.stream == stream[k] ? upto[k] : kForeignRow;
+      const bool ours = b.stream < 0 || b.stream == stream[k];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        z[k][n] = nb[n] <= most ? c[n >> 1][2 * k + (n & 1)] * ks[n] : -INFINITY;
+        z[k][n] = ours && there[n] && nb[n] <= upto[k] ? c[n >> 1][2 * k + (n & 1)] * ks[n] : -INFINITY;
         mx[k] = fmaxf(mx[k], z[k][n]);
       }
       mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 1));

@@ -64,3 +64,20 @@ def test_maxima_that_rise_in_every_block(shape, holes):
     A.check(want, *A.want_of(c))
     for _ in range(20):
         assert torch.equal(A.run(c), want)
+
+
+LOW, TOP = -0x80000000, 0x7fffffff
+IDS = [[TOP], [LOW], [LOW, LOW + 1], [LOW + 1, LOW, LOW], [TOP - 1, TOP, TOP - 1], [LOW, LOW + 1, -1, 0, TOP - 1, TOP],
+       [TOP] * 17, [LOW] * 9 + [TOP] * 11]
+
+
+@pytest.mark.parametrize("ids", IDS, ids=lambda v: "-".join(map(str, v[:6])))
+@pytest.mark.parametrize("B,n_shared,own", [(1, 0, 0), (3, 100, 20), (5, 0, 70), (70, 150, 9)])
+def test_block_ids_are_any_numbers(ids, B, n_shared, own):
+    """Ids from the lowest to the highest int32, in both forms: key j is seen by token i iff
+    id j <= id i, ring slots by all tokens of their stream, and places without a key by none."""
+    S = len(ids)
+    for Hq in (1, 8):
+        c = A.case(B, S, Hq, 1, n_shared, own, True, seed=S)
+        c["new_block"] = torch.tensor(ids, dtype=torch.int32).cuda()
+        A.check(A.run(c), *A.want_of(c))
