@@ -109,6 +109,14 @@ __device__ __forceinline__ int own_length(const SharedAttnParams& p, int b) {
   return p.own_len ? min(max(p.own_len[b], 0), p.own_max) : p.own_max;
 }
 
+// Whether a stream's rows see any key (each sees its own new one).
+__device__ __noinline__ bool sees_key(const SharedAttnParams& p, int b) {
+  if (p.n_new > 0 || own_length(p, b) > 0 || (p.n_shared > 0 && !p.shared_valid)) return true;
+  for (int i = 0; i < p.n_shared; ++i)
+    if (p.shared_valid[i]) return true;
+  return false;
+}
+
 // Runs of units.
 __device__ __forceinline__ int cta_begin(const SharedAttnParams& p, int cta) { return cta * p.run + min(cta, p.longer); }
 // The CTA that has unit u.
@@ -737,6 +745,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             w[4 * i + 2] = x.z;
             w[4 * i + 3] = x.w;
           }
+          // (a value that is not finite times a masked key's zeros would be NaN: where the
+          // row sees no key it counts as 0)
+          uint32_t most = 0u;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+          if (max(most & 0xffffu, most >> 16) >= 0x7f80u && !sees_key(p, row.b)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = 0u;
+          }
+          __syncwarp();
           tmem_st16(tmQ + lane_base + ch * 64 + c * 16, w);
           __syncwarp();
         }

@@ -81,3 +81,26 @@ def test_block_ids_are_any_numbers(ids, B, n_shared, own):
         c = A.case(B, S, Hq, 1, n_shared, own, True, seed=S)
         c["new_block"] = torch.tensor(ids, dtype=torch.int32).cuda()
         A.check(A.run(c), *A.want_of(c))
+
+
+@pytest.mark.parametrize("S", [1, 50])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_rows_without_keys_are_zero_whatever_their_query_holds(S, bad):
+    """A query that is not finite makes its row NaN where the row sees a key, and leaves it 0 where
+    it sees none; no other row's bits change."""
+    B = 6
+    c = A.case(B, S, 8, 1, 200, 70, False, lens=[0, 70, 0, 3, 70, 0], seed=2)
+    c["shared_valid"] = torch.zeros(200, dtype=torch.uint8).cuda()
+    want = A.run(c).view(B, S, 8, D).clone()
+    assert (want[[0, 2, 5]] == 0).all()
+    c["q"][0] = bad
+    c["q"][2, 3, S - 1, 200] = -bad
+    c["q"][4, 1, 0, 7] = bad
+    got = A.run(c).view(B, S, 8, D)
+    assert (got[[0, 2, 5]] == 0).all()
+    assert got[4, 0, 1].isnan().all()
+    got[4, 0, 1] = want[4, 0, 1]
+    assert torch.equal(got, want)
+    c["shared_valid"][199] = 1
+    got = A.run(c).view(B, S, 8, D)
+    assert got[0].isnan().all() and got[2, S - 1, 3].isnan().all() and not got[5].isnan().any()
