@@ -324,6 +324,14 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t codes, float (&v)[8]) {
 
 __device__ __forceinline__ void put(float* y, float v) { *y = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* y, float v) { *y = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put8(float* y, const float (&v)[8]) {
+  reinterpret_cast<float4*>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void put8(__nv_bfloat16* y, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(y) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                                            pack_bf16x2(v[6], v[7]));
+}
 template <int VEC>
 __device__ __forceinline__ void put16(float* y, const float (&v)[16]) {
 #pragma unroll
@@ -350,11 +358,44 @@ __device__ __forceinline__ void put16(__nv_bfloat16* y, const float (&v)[16]) {
   }
 }
 
+// a * b of a few bits by a float, rounded once to the output type: for bf16 to fp32 so
+// that the last bit is odd where bits are lost (of the two neighbours one is), which keeps
+// the second rounding from seeing a tie that is none.
+template <typename Tout>
+__device__ __forceinline__ float product(float a, float b) {
+  if (sizeof(Tout) == 4) return __fmul_rn(a, b);
+  const float lo = __fmul_rd(a, b), hi = __fmul_ru(a, b);
+  return (__float_as_uint(lo) & 1u) ? lo : hi;
+}
+// 16 values of a row whose scale is no power of two (`left`: those before the row's end),
+// 8 at a time, so that the rows that the quantizer makes lose no registers to it.
+template <typename Tout, int VEC>
+__device__ __forceinline__ void dequant_any_scale(Tout* y, int left, uint2 codes, float block_scale, float row_scale) {
+#pragma unroll 1
+  for (int h = 0; h < 16; h += 8) {
+    float v[8];
+    unpack_e2m1(h ? codes.y : codes.x, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = product<Tout>(v[e] * block_scale, row_scale);
+    if (VEC && left >= kUnit) {
+      put8(y + h, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (h + e < left) put(y + h + e, v[e]);
+    }
+  }
+}
+
 // A CTA takes 256 / TPR rows and kTurn units per thread of them at a time: all codes and
 // scales are asked for before the first is used.
 template <typename Tout, int FMT, int TPR, int VEC>
 __global__ void __launch_bounds__(256) dequant_fp4_kernel(const DequantFp4Params p) {
   constexpr int kRows = 256 / TPR, kTurn = TPR == 256 ? 2 : 1, kChunk = kTurn * TPR;
+  // bf16 rows whose scale is no power of two are written a second time, over the first: with
+  // the products that they need in one place with the others, 768 x 16384 of the quantizer's
+  // rows take 7.0 to 8.1 us instead of 6.7 (fp32 10.8 instead of 10.5: in one place).
+  constexpr bool kAgain = FMT == RFX_FP4_NV && sizeof(Tout) == 2;
   pdl_wait();
   pdl_launch_dependents();
   const int chunks = (p.units + kChunk - 1) / kChunk;
@@ -366,6 +407,10 @@ __global__ void __launch_bounds__(256) dequant_fp4_kernel(const DequantFp4Params
     const uint8_t* q = p.q + t * p.ldq;
     const uint8_t* scale = p.scale + p.tiles.row(t);
     const float row_scale = FMT == RFX_FP4_NV ? p.row_scale[t] : 1.f;
+    // a power of two (the quantizer makes no others) that times any block's scale neither
+    // overflows nor loses bits: one product per value
+    const uint32_t row_bits = __float_as_uint(row_scale);
+    const bool power = (row_bits & 0x007fffffu) == 0u && row_bits >= 1u << 23 && row_bits <= (119u + 127u) << 23;
     Tout* y = static_cast<Tout*>(p.y) + t * p.ldy;
     uint2 codes[kTurn];
     uint32_t byte[kTurn];
@@ -391,11 +436,11 @@ __global__ void __launch_bounds__(256) dequant_fp4_kernel(const DequantFp4Params
     for (int c = 0; c < kTurn; ++c) {
       const int u = u0 + c * TPR, k = u * kUnit;
       if (u >= p.units) continue;
-      // 2^(byte - 127), of byte 0 a subnormal number; an NV scale's 4 bits times the row's
-      // power of two, and a code's 3 bits times that, are exact
+      // 2^(byte - 127), of byte 0 a subnormal number; an NV scale's 4 bits times a power of
+      // two, and a code's 3 bits times either, are exact
       const float s = FMT == RFX_FP4_MX ? (byte[c] == 255 ? __uint_as_float(0x7fffffffu)
                                            : byte[c] == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte[c] << 23))
-                                        : from_e4m3(byte[c]) * row_scale;
+                                        : from_e4m3(byte[c]) * (kAgain || power ? row_scale : 1.f);
       const unsigned long long s2 = pack_f32x2(s, s);
       float v[16];
 #pragma unroll
@@ -409,12 +454,23 @@ __global__ void __launch_bounds__(256) dequant_fp4_kernel(const DequantFp4Params
           v[8 * h + e + 1] = hi_f32(y);
         }
       }
+      if (FMT == RFX_FP4_NV && !kAgain && !power) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = product<Tout>(v[e], row_scale);
+      }
       if (VEC && k + kUnit <= p.K) {
         put16<VEC>(y + k, v);
       } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (k + e < p.K) put(y + k + e, v[e]);
+      }
+    }
+    if (kAgain && !power) {
+#pragma unroll
+      for (int c = 0; c < kTurn; ++c) {
+        const int u = u0 + c * TPR, k = u * kUnit;
+        if (u < p.units) dequant_any_scale<Tout, VEC>(y + k, p.K - k, codes[c], from_e4m3(byte[c]), row_scale);
       }
     }
   }
