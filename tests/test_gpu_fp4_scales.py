@@ -67,3 +67,43 @@ def test_every_product_near_a_tie_is_rounded_once(dtype):
     K.dequant_fp4(x=out, out=y)
     P.done()
     assert torch.equal(y.cpu(), rounded(P.values(out), dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T", [1, 50, 128, 129, 300])
+@pytest.mark.parametrize("epi", [P.STORE, P.GEGLU])
+@pytest.mark.parametrize("ex,ew", [(74, 74), (-65, -65), (120, -90), (-90, 120), (110, -126), (-75, -60), (60, 60), (-126, 125)])
+def test_row_scales_whose_product_leaves_fp32(ex, ew, T, epi, dtype):
+    """x and w of such sizes (2^ex, 2^ew) that the product of two row scales, or of one and the
+    sum, is beyond fp32 or below it: the outputs are the formula's all the same, sums of 0 (rows
+    that share no places) are 0, and what is too large is infinite; in few tokens and in many."""
+    Kc, O = 192, 96
+    r = P.gen(T + ex)
+    x, w = r(T, Kc), r(O, Kc)
+    x[::2, 96:] = 0
+    w[::3, :96] = 0
+    xq = P.quantized(x.mul(2.0 ** ex) if ex > -120 else x, NV)
+    wq = P.quantized(w.mul(2.0 ** ew) if ew > -120 else w, NV, 2 if epi == P.GEGLU else 1)
+    for q, e in ((xq, ex), (wq, ew)):  # (smaller than the quantizer makes them)
+        if e <= -120:
+            q.row_scale.fill_(2.0 ** e)
+    y = torch.empty(T, O // 2 if epi == P.GEGLU else O, dtype=dtype, device="cuda")
+    K.linear_fp4(w=wq, x=xq, y=y, epilogue=epi)
+    P.done()
+    got = y.double().cpu().numpy()
+    with np.errstate(over="ignore", invalid="ignore"):
+        want, tol = P.ref_linear(P.values(xq), P.values(wq), None, P.STORE)
+        sure = np.ones(want.shape, bool)
+        if epi == P.GEGLU:  # (of gates and ups that are fp32 numbers: what infinities give is another test's)
+            sure = (np.abs(want) < 1e37)[:, :O // 2] & (np.abs(want) < 1e37)[:, O // 2:]
+            least = 2.0 ** -148 * (np.abs(want[:, :O // 2]) + np.abs(want[:, O // 2:]) + 1)
+            want, tol = P.ref_linear(P.values(xq), P.values(wq), None, P.GEGLU)
+            tol = tol + least
+        top = float(torch.finfo(dtype).max)
+        tol = tol + P.HALF[dtype] * (np.abs(want) + tol) + (2.0 ** -133 if dtype == BF else 2.0 ** -148)
+        close = np.abs(got - want) <= tol
+        over = (np.abs(want) >= top * (1 - 2.0 ** -7)) & (got == np.copysign(np.inf, want))
+    bad = ~(close | over) & sure
+    assert not bad.any(), (int(bad.sum()), bad.size, got[bad][:4], want[bad][:4], np.argwhere(bad)[:4].tolist())
+    nothing = (P.values(xq) @ P.values(wq).T == 0) & sure if epi == P.STORE else np.zeros_like(sure)
+    assert (got[nothing] == 0).all() and (epi == P.GEGLU or nothing.sum() >= (T + 1) // 2 * (O // 3))
