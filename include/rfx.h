@@ -325,13 +325,16 @@ int rfx_attention_noalloc(const rfx_attn_desc* desc, void* stream);
  * / num_kv_heads).  A row that sees no key is 0.  own_len values are clamped to
  * 0..own_max.  A NaN or infinity that only some rows see reaches no others.
  *
- * Numerics as in rfx_attention: scores and sums in fp32, P (times the key's
- * value scale) and V in f16 in P V, exact while a context token's value absmax
- * stays below about 32,000 (and fine down to about 0.01: a weight times its value
- * scale, absmax / 127, is rounded to steps of 2^-24 below 2^-14, and so is a new
- * token's value); a new token with
- * a value beyond f16 makes the rows that see it NaN.  Results do not depend on the
- * order in which SMs finish. */
+ * Numerics: scores and sums in fp32; P (times the key's value scale) and V in f16 in
+ * P V.  A weight times its value scale has 11 significant bits down to 2^-21 of the
+ * row's largest (score times the largest value scale of its 64 keys) and is rounded to
+ * steps of 2^-31 of that below, whatever the values' size (for value scales from 2^-64
+ * to 2^64).  The rings' int8 values are exact.  New tokens' values, and in
+ * RFX_QUANT_U8_REF the dequantized ones, are themselves f16: from 2^-14 on bf16
+ * numbers are exact and fp32 ones (fp32 scales) rounded to 11 bits, below they are
+ * rounded to steps of 2^-24, and one beyond 65504 makes the rows that see it NaN.  Keys
+ * are bf16, so that with fp32 scales in RFX_QUANT_U8_REF they are rounded to it.  Results do
+ * not depend on the order in which SMs finish. */
 typedef struct rfx_kv_view { /* a quantized ring: rows of 256 bytes at byte strides, scales at element strides */
   const void* k;
   const void* v;

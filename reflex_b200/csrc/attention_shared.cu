@@ -44,6 +44,7 @@ namespace {
 constexpr int kD = 256;
 constexpr int kRows = 128;  // query rows per tile
 constexpr int kKeys = 64;   // keys per block
+constexpr int kWords = 4 * kKeys + 4;  // of one block (the last 3 fill up 16 bytes)
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Quantized {  // a ring: quantized rows (bytes), scales and zero points (elements)
@@ -87,7 +88,8 @@ struct SharedAttnParams {
   int join;         // of the CTAs of a tile the last to finish joins the parts
   int early;        // q is there once this grid runs: the keys' copy went before
   // dense keys [block][64][256], shared blocks of each head first, then (stream,
-  // head, own block); per block the words of its keys: [ks | vs | add | nb][64]
+  // head, own block); per block the words of its keys: [ks | vs | add | nb][64], and the
+  // lift of all of them
   __nv_bfloat16* kd;
   __half* vd;
   float* words;
@@ -210,6 +212,21 @@ __device__ __forceinline__ float load_scalar(const void* p, long i, bool bf16) {
 }
 __device__ __forceinline__ float round_to(float x, bool bf16) { return bf16 ? bf16_round(x) : x; }
 
+// P times the value scales is f16, whose numbers are fine from 2^-14 to 2^16 only.  So a
+// row's weights are not taken relative to its largest score, but to the largest sum of
+// a block's largest score and its lift: the exponent of its largest value scale (all
+// are below 2^that) less 7.  Then the largest products are between 2^7 and 2^15 whatever
+// the values' size is, those down to 2^-21 of them have f16's 11 bits, and smaller ones
+// steps of 2^-31 of them.  (Scales of 0, NaN and infinity have no say; beyond 2^-64 and
+// 2^64 the lift stays what it is there, so that the sums of weights stay in range.)
+__device__ __forceinline__ uint32_t lift_bits(float value_scale) {
+  const uint32_t b = __float_as_uint(value_scale) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+__device__ __forceinline__ float lift_of(uint32_t bits) {
+  return static_cast<float>(min(max(static_cast<int>((bits + 0x7fffffu) >> 23) - 127, -64), 64) - 7);
+}
+
 // ------------------------------------------------------------ dense keys ---
 // One CTA per 16 keys of a block (768 blocks, 17 MB in and 50 out, 15 us from cold memory).  A key that no row may see has scores of -inf
 // and zero rows, so that what its memory holds (a NaN in a scale, say) reaches no
@@ -272,7 +289,7 @@ __global__ void __launch_bounds__(256) shared_dense_kernel(const __grid_constant
       raw[isv][1] = *reinterpret_cast<const uint4*>(src + g * 16 + 8);
     }
   }
-  float* words = p.words + static_cast<long>(block) * 4 * kKeys;
+  float* words = p.words + static_cast<long>(block) * kWords;
   bool bad = false;
   const long row = (static_cast<long>(block) * kKeys + key) * kD + g * 16;
 #pragma unroll
@@ -314,12 +331,27 @@ __global__ void __launch_bounds__(256) shared_dense_kernel(const __grid_constant
     dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
     dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
+  const bool i8 = p.mode == kQuantI8Sym;
+  const float vs = kind == 0 ? 0.f : bad ? __uint_as_float(0x7fffffffu) : kind == 1 && i8 ? scale[1] : 1.f;
   if (g == 0) {
-    const bool i8 = p.mode == kQuantI8Sym;
     words[key] = kind == 0 ? 0.f : kind == 1 && i8 ? scale[0] * p.scale_log2 : p.scale_log2;
-    words[kKeys + key] = kind == 0 ? 0.f : bad ? __uint_as_float(0x7fffffffu) : kind == 1 && i8 ? scale[1] : 1.f;
+    words[kKeys + key] = vs;
     words[2 * kKeys + key] = kind ? 0.f : -INFINITY;
     reinterpret_cast<int*>(words)[3 * kKeys + key] = kind == 2 ? block_id(p, slot - held) : kRingKey;
+  }
+  // the block's lift: one warp looks at all of its value scales
+  if (q0 == 0 && threadIdx.x < 32) {
+    uint32_t most = 0u;
+#pragma unroll
+    for (int i = 0; i < kKeys; i += 32) {
+      const int at = j * kKeys + i + threadIdx.x;
+      if (at < held && i8 && !(is_shared && p.shared_valid && p.shared_valid[at] == 0))
+        most = max(most, lift_bits(static_cast<const float*>(ring.v_scale)[b * ring.ss_b + h * ring.ss_h + at * ring.ss_c]));
+      else if (at < total && !(at < held && i8))
+        most = max(most, lift_bits(1.f));
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (threadIdx.x == 0) words[4 * kKeys] = lift_of(most);
   }
 }
 
@@ -331,7 +363,6 @@ constexpr int kTileP = kRows * kKeys * 2;
 constexpr int kOffK = 0;                     // [3] x 4 x [64 keys x 64 dims] bf16, K-major
 constexpr int kOffV = kOffK + kStages * kTile;   // [2] x 4 x [64 keys x 64 dims] f16, MN-major
 constexpr int kOffP = kOffV + kStagesV * kTile;  // [2] x [128 rows x 64 keys] f16, K-major
-constexpr int kWords = 4 * kKeys;            // of one block
 constexpr int kWordStages = 6;
 constexpr int kOffWords = kOffP + 2 * kTileP;
 constexpr int kOffXchg = kOffWords + kWordStages * kWords * 4;  // running maxima [2][128], the groups' sums and maxima [4][128]
@@ -821,6 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
   #pragma unroll
           for (int c = 0; c < kKeys / 2; ++c) mx[c & 3] = fmaxf(fmaxf(mx[c & 3], lo_f32(z[c])), hi_f32(z[c]));
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) + sc[4 * kKeys];
           // the row's running maximum, from the other group's block before
           float m_prev = -INFINITY;
           if (j > j0) {
@@ -828,8 +860,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) return;
             m_prev = m_x[(ch ^ 1) * kRows + r];
           }
-          const float m_new = fmaxf(m_prev, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-          // (moved by more than 2^8 only: P stays below 2^8, and O is seldom rescaled)
+          const float m_new = fmaxf(m_prev, top);
+          // (moved by more than 2^8 only: P stays below 2^15, and O is seldom rescaled)
           const bool need = m_prev != -INFINITY && m_new > m_prev + 8.f;
           const float m_use = need || m_prev == -INFINITY ? m_new : m_prev;
           m_x[ch * kRows + r] = m_use;
@@ -1363,6 +1395,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) shared_few_kernel(const __g
       }
     }
     if (ahead.unit >= 0) load_k(ahead);
+    uint32_t top = max(max(lift_bits(vs[0]), lift_bits(vs[1])), max(lift_bits(vs[2]), lift_bits(vs[3])));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float lift = lift_of(top);
     // c[n]: row g keys 8 n + 2t, + 1, row g + 8 the same
     float z[2][4];  // [row][key]
     float mx[2] = {-INFINITY, -INFINITY};
@@ -1382,7 +1418,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) shared_few_kernel(const __g
     bool need = false;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const float m_new = fmaxf(m_run[k], mx[k]);
+      const float m_new = fmaxf(m_run[k], mx[k] + lift);
       const bool up = m_run[k] != -INFINITY && m_new > m_run[k] + 8.f;
       const float m_use = up || m_run[k] == -INFINITY ? m_new : m_run[k];
       alpha[k] = up ? ex2_approx(m_run[k] - m_use) : 1.f;

@@ -1,7 +1,8 @@
 """Attention over a shared context on the GPU where a row's softmax is hard: maxima that
-rise from block to block.  Against the formula in 64 bits, with the tolerance that is
+rise from block to block, block ids at the ends of int32, values far from 1.  Against the formula in 64 bits, with the tolerance that is
 derived beside it.
 """
+import numpy as np
 import pytest
 import torch
 
@@ -104,3 +105,65 @@ def test_rows_without_keys_are_zero_whatever_their_query_holds(S, bad):
     c["shared_valid"][199] = 1
     got = A.run(c).view(B, S, 8, D)
     assert got[0].isnan().all() and got[2, S - 1, 3].isnan().all() and not got[5].isnan().any()
+
+
+def exact(c):
+    """(out, tol) of a call without new keys, in 64 bits, for values of any size.
+
+    As in the formula's other test, but what a weight times its value scale loses among the
+    small numbers of f16: weights are relative to the row's largest (score x block's largest value
+    scale, rounded up to a power of two), which is 2^15 to 2^7 there, so half a step of 2^-24 is
+    at most 2^-25 * 2^-7 * 2 * (the largest value scale) of the largest weight, times an integer of
+    at most 127 (times the value itself in the uint8 scheme, where the scale is 1)."""
+    q = c["q"].double().cpu().numpy()
+    B, Hq, S, _ = q.shape
+    i8 = c["shared"].mode == I8
+    n, own = c["n_shared"], c.get("own")
+    sk, sv = A.ring_values(c["shared"])
+    scale = c["shared"].v_scale.double().cpu().numpy()
+    ok, ov = A.ring_values(own) if own is not None else (None, None)
+    os_ = None if own is None else own.v_scale.double().cpu().numpy()
+    keep = np.ones(n, bool) if "shared_valid" not in c else c["shared_valid"].cpu().numpy() != 0
+    # (the shared part of all streams is one array: copies of it would be most of the time)
+    first = (sk[0, 0, :n][keep], sv[0, 0, :n][keep], scale[0, 0, :n][keep])
+    first_abs = np.abs(first[0]), np.abs(first[1])
+    out, tol = np.zeros((B, S, Hq, D)), np.zeros((B, S, Hq, D))
+    for b in range(B):
+        parts = [(*first, *first_abs)]
+        if own is not None:
+            m = int(c["own_len"][b])
+            parts.append((ok[b, 0, :m], ov[b, 0, :m], os_[b, 0, :m], np.abs(ok[b, 0, :m]), np.abs(ov[b, 0, :m])))
+        qq = q[b].reshape(Hq * S, D)
+        z = np.concatenate([qq @ k.T for k, *_ in parts], axis=1) * c["softmax_scale"]
+        mag = np.concatenate([np.abs(qq) @ ak.T for *_, ak, _ in parts], axis=1) * c["softmax_scale"]
+        w = np.exp(z - z.max(axis=1, keepdims=True))
+        l = w.sum(axis=1, keepdims=True)
+        p, u, keys = w / l, 2.0 ** -24, z.shape[1]
+        ds = p * (38 * u * mag + 4 * u * np.abs(z) + 2.0 ** -21)
+
+        def times(a, which):  # a [rows, keys] by the parts' values
+            at = np.cumsum([0] + [len(x[0]) for x in parts])
+            return sum(a[:, s:e] @ x[which] for s, e, x in zip(at, at[1:], parts))
+        o, pa = times(p, 1), times(p, 4)
+        d = times(ds, 4) + ds.sum(axis=1, keepdims=True) * pa + 2.0 ** -11 * pa
+        top = max(x[2].max(initial=0) for x in parts)
+        d += 2.0 ** -31 / l * (127.0 * keys * top if i8 else sum(x[4].sum(axis=0) for x in parts)) + (keys / 16 + 4) * 2 * u * pa
+        d += 0.0 if i8 else 2.0 ** -11 * pa + 2.0 ** -25  # (V itself in f16)
+        d += 2.0 ** -8 * (np.abs(o) + d)
+        out[b], tol[b] = (x.reshape(Hq, S, D).transpose(1, 0, 2) for x in (o, d))
+    return out.reshape(B * S, Hq * D), tol.reshape(B * S, Hq * D)
+
+
+@pytest.mark.parametrize("size", [1e-7, 1e-4, 0.01, 0.03, 1.0, 1e3, 1e6, 1e15])
+@pytest.mark.parametrize("shape", [(1, 1, 8, 5000, 0), (3, 5, 8, 700, 90), (64, 50, 8, 300, 40), (64, 1, 8, 32768, 70), (16, 51, 8, 3000, 0)],
+                         ids=str)
+def test_values_of_any_size(shape, size):
+    """Values far from 1, some keys' 1000 times as large as others': as exact as values near 1."""
+    B, S, Hq, n, own = shape
+    c = A.case(B, S, Hq, 1, n, own, False, seed=5)
+    r = A.gen(n + own)
+    spread = lambda *s: size * torch.exp(1.2 * r(*s, 1)) * r(*s, D)  # noqa: E731
+    c["shared"] = ring_of(r(1, 1, n, D), spread(1, 1, n), n + 5)
+    if own:
+        c["own"] = ring_of(r(B, 1, own, D), spread(B, 1, own))
+    A.check(A.run(c), *exact(c))
