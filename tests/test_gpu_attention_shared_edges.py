@@ -22,7 +22,8 @@ def ring_of(k, v, capacity=None, mode=I8, scale_dtype=None):
     for t in (ring.k_scale, ring.v_scale, ring.k_zp, ring.v_zp):
         if t is not None:
             t.fill_(float("nan"))
-    K.kv_quant_append(k.bfloat16().cuda(), v.bfloat16().cuda(), ring, 0, 0, ring.capacity)
+    t = scale_dtype or torch.bfloat16
+    K.kv_quant_append(k.to(t).cuda(), v.to(t).cuda(), ring, 0, 0, ring.capacity)
     return ring
 
 
@@ -107,6 +108,16 @@ def test_rows_without_keys_are_zero_whatever_their_query_holds(S, bad):
     assert got[0].isnan().all() and got[2, S - 1, 3].isnan().all() and not got[5].isnan().any()
 
 
+def values_of(ring):
+    """(k, v) in 64 bits, as the kernels multiply them: with fp32 scales in the uint8 scheme keys
+    are rounded to bf16 and values to f16."""
+    if ring.mode == I8 or ring.k_scale.dtype == torch.bfloat16:
+        return A.ring_values(ring)
+    dq = lambda q, s, z: (q.cpu().float() - z.cpu()[..., None]) * s.cpu()[..., None]  # noqa: E731
+    return (dq(ring.k_q, ring.k_scale, ring.k_zp).bfloat16().double().numpy(),
+            dq(ring.v_q, ring.v_scale, ring.v_zp).half().double().numpy())
+
+
 def exact(c):
     """(out, tol) of a call without new keys, in 64 bits, for values of any size.
 
@@ -119,9 +130,9 @@ def exact(c):
     B, Hq, S, _ = q.shape
     i8 = c["shared"].mode == I8
     n, own = c["n_shared"], c.get("own")
-    sk, sv = A.ring_values(c["shared"])
+    sk, sv = values_of(c["shared"])
     scale = c["shared"].v_scale.double().cpu().numpy()
-    ok, ov = A.ring_values(own) if own is not None else (None, None)
+    ok, ov = values_of(own) if own is not None else (None, None)
     os_ = None if own is None else own.v_scale.double().cpu().numpy()
     keep = np.ones(n, bool) if "shared_valid" not in c else c["shared_valid"].cpu().numpy() != 0
     # (the shared part of all streams is one array: copies of it would be most of the time)
@@ -166,4 +177,17 @@ def test_values_of_any_size(shape, size):
     c["shared"] = ring_of(r(1, 1, n, D), spread(1, 1, n), n + 5)
     if own:
         c["own"] = ring_of(r(B, 1, own, D), spread(B, 1, own))
+    A.check(A.run(c), *exact(c))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [0.01, 1.0, 300.0])
+@pytest.mark.parametrize("shape", [(1, 1, 8, 500, 0), (3, 5, 8, 257, 64), (64, 50, 8, 300, 40), (64, 1, 8, 6000, 70)], ids=str)
+def test_uint8_scheme_with_scales_of_either_type(shape, size, dtype):
+    B, S, Hq, n, own = shape
+    c = A.case(B, S, Hq, 1, n, own, False, seed=6, mode=U8, holes=True)
+    r = A.gen(n + own)
+    c["shared"] = ring_of(r(1, 1, n, D), size * r(1, 1, n, D), n + 5, U8, dtype)
+    if own:
+        c["own"] = ring_of(r(B, 1, own, D), size * r(B, 1, own, D), own, U8, dtype)
     A.check(A.run(c), *exact(c))
