@@ -275,24 +275,37 @@ bool places_shared(const Places& a, const Places& b) {
   return solvable(t, n, static_cast<long>(off), 1 - wb, wa - 1, &budget);
 }
 
+namespace {
+struct ClusterQuery {
+  const void* func;
+  int threads, smem, cluster, dev;
+  bool operator==(const ClusterQuery& o) const {
+    return func == o.func && threads == o.threads && smem == o.smem && cluster == o.cluster && dev == o.dev;
+  }
+};
+struct ClusterQueryHash {
+  size_t operator()(const ClusterQuery& q) const {
+    uint64_t h = reinterpret_cast<uintptr_t>(q.func);
+    for (const int v : {q.threads, q.smem, q.cluster, q.dev}) h = (h ^ static_cast<uint32_t>(v)) * 0x9e3779b97f4a7c15ull;
+    return static_cast<size_t>(h ^ (h >> 32));
+  }
+};
+}  // namespace
+
 int max_active_clusters(const void* func, int threads, int smem, int cluster_x) {
-  struct Entry {
-    const void* func;
-    int threads, smem, cluster, dev, n;
-  };
+  // The kernels whose shared memory follows the tokens and the length of K ask with sizes of
+  // their own (a few per layer shape and 16 tokens), so the table grows with them.
   static std::mutex mu;
-  static Entry memo[256];  // a few kernels x cluster sizes x devices; the rest is asked again
-  static int used = 0;
+  static std::unordered_map<ClusterQuery, int, ClusterQueryHash> memo;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
+  const ClusterQuery key{func, threads, smem, cluster_x, dev};
   std::lock_guard<std::mutex> lk(mu);
-  for (int i = 0; i < used; ++i)
-    if (memo[i].func == func && memo[i].threads == threads && memo[i].smem == smem && memo[i].cluster == cluster_x &&
-        memo[i].dev == dev)
-      return memo[i].n;
+  const auto it = memo.find(key);
+  if (it != memo.end()) return it->second;
   int n = 0;
   bool known = false;  // a query that failed is asked again
   if (ensure_smem_attr(func, smem) == RFX_OK) {
@@ -311,8 +324,12 @@ int max_active_clusters(const void* func, int threads, int smem, int cluster_x) 
     if (!known) n = 0;
     cudaGetLastError();
   }
-  if (known && used < static_cast<int>(sizeof(memo) / sizeof(memo[0])))
-    memo[used++] = Entry{func, threads, smem, cluster_x, dev, n};
+  if (known) {
+    try {
+      memo.emplace(key, n);
+    } catch (...) {  // out of host memory: asked again
+    }
+  }
   return n;
 }
 
