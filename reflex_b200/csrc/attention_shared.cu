@@ -80,8 +80,7 @@ struct SharedAttnParams {
   int tiles;        // Hkv * head_tiles
   int head_tiles;   // ceil(rows / tile_rows)
   int shared_blocks, own_blocks;  // of a head / of a stream and head
-  int streams;      // that a tile has rows of, at most
-  int tile_units;   // shared_blocks + streams * own_blocks
+  int tile_units;   // shared_blocks + own_blocks of each stream that a tile can have rows of
   int cluster;      // CTAs per tile, or 0: runs of units over `ctas` CTAs,
   int ctas;
   int run, longer;  // `run` units each, the first `longer` CTAs one more
@@ -1744,7 +1743,6 @@ int plan_form(const rfx_attn_shared_desc& d, bool few, int nsm, Plan* out, doubl
   p.tiles = p.Hkv * p.head_tiles;
   p.shared_blocks = static_cast<int>(shared_blocks);
   p.own_blocks = static_cast<int>(own_blocks);
-  p.streams = static_cast<int>(std::min<long>(touch, d.B));
   p.tile_units = static_cast<int>(units);
   out->blocks = few ? 0 : p.Hkv * (shared_blocks + d.B * own_blocks);
   if (out->blocks > 0x7fffffffl / kKeys) return set_error(RFX_E_INVAL, "rfx_attention_shared: too many keys");

@@ -42,7 +42,7 @@ struct Fmt {
 };
 
 struct Fp4Params {
-  int T, O, K;
+  int T;
   int F;            // output columns: O, or O / 2 with GeGLU
   int k_steps;      // of 256 values
   int k_mmas;       // of 64 values
@@ -1174,8 +1174,6 @@ int launch_linear_fp4(const rfx_linear_fp4_desc& d, const LinearFp4Maps& maps, c
   const int per_step = mx ? Fmt<true>::kTiles : Fmt<false>::kTiles;
   Fp4Params p{};
   p.T = d.T;
-  p.O = d.O;
-  p.K = d.K;
   p.F = out_cols(d);
   p.k_steps = (d.K + kStepK - 1) / kStepK;
   p.k_mmas = (d.K + kMmaK - 1) / kMmaK;
