@@ -323,12 +323,14 @@ int rfx_attention_noalloc(const rfx_attn_desc* desc, void* stream);
  * [0, n_shared) with shared_valid, the own slots [0, own_len[b]) and the new
  * keys j with new_block[j] <= new_block[s]; q head h reads KV head h / (num_q_heads
  * / num_kv_heads).  A row that sees no key is 0.  own_len values are clamped to
- * 0..own_max.  A NaN or infinity that only some rows see reaches no others.
+ * 0..own_max.  Block ids may be any numbers.  A NaN or infinity that only some rows see
+ * reaches no others.  The workspace and the way a call is cut up count own_max slots of
+ * every stream: an own_max far above the lengths in use costs memory and time.
  *
  * Numerics: scores and sums in fp32; P (times the key's value scale) and V in f16 in
  * P V.  A weight times its value scale has 11 significant bits down to 2^-21 of the
- * row's largest (score times the largest value scale of its 64 keys) and is rounded to
- * steps of 2^-31 of that below, whatever the values' size (for value scales from 2^-64
+ * row's largest (a block of keys' largest weight times its largest value scale) and is
+ * rounded to steps of 2^-31 of that below, whatever the values' size (for value scales from 2^-64
  * to 2^64).  The rings' int8 values are exact.  New tokens' values, and in
  * RFX_QUANT_U8_REF the dequantized ones, are themselves f16: from 2^-14 on bf16
  * numbers are exact and fp32 ones (fp32 scales) rounded to 11 bits, below they are
@@ -712,7 +714,7 @@ typedef struct rfx_quant_fp4_desc {
 } rfx_quant_fp4_desc;
 int rfx_quant_fp4(const rfx_quant_fp4_desc* desc, void* stream);
 
-/* What 4-bit rows stand for, as bf16 or fp32 (one rounding). */
+/* What 4-bit rows stand for, as bf16 or fp32: one rounding, whatever the row scale. */
 typedef struct rfx_dequant_fp4_desc {
   int T, K;
   int format;
@@ -731,7 +733,10 @@ int rfx_dequant_fp4(const rfx_dequant_fp4_desc* desc, void* stream);
  * rows of one format (row scales 1 with MX), products and sums in fp32 on the
  * tensor cores, one rounding to the output type.  Epilogues STORE, SILU, GELU
  * and GEGLU (w = [Wgate; Wup], its scales in two parts of O / 2 rows; y has
- * O / 2 columns).  The order of the sum depends on the shape alone.  A row or
+ * O / 2 columns).  Row scales may be any numbers, and their product may leave fp32
+ * where the output does not.  The order of the sum depends on the shape, the format, the
+ * types, and on what the device holds at once (its SMs and the clusters that it reports
+ * to have room for), not on when a call runs.  A row or
  * channel with a NaN scale gives NaN outputs, no others.
  * y shares no memory with an input.  1 <= K <= 65536. */
 typedef struct rfx_linear_fp4_desc {

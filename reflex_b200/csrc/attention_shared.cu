@@ -14,12 +14,13 @@
 // buffer is free as soon as its softmax has read it, so S runs two blocks ahead of P
 // V.  (Q in shared memory would make S wait for operands: 192 bytes a clock.)
 //
-// What bounds it: a block's MMAs take 1024 clocks, and a block comes every 2300.  That is
-// the chain of one softmax warp, whose two groups take the blocks in turn: 900
+// What bounds it: a block's MMAs take 1024 clocks, and a block comes about every 2400.  That
+// is the chain of one softmax warp, whose two groups take the blocks in turn: 940
 // instructions of 64 keys at 2 warps per scheduler, which issues in 27 % of its clocks.
-// A third group (152 registers a thread, a tile's end in smaller steps) gained 3 % on
-// the first batch below and lost 6 and 9 % on the last and on small ones.  64 streams of 50 tokens x 8 heads over 818 shared slots: 58 us,
-// 390 TFLOP/s; 16 of 51 over 6344: 72 us, 600 TFLOP/s; 64 single tokens over 32768: 51 us.
+// A third group (152 registers a thread, a tile's end in smaller steps) gained 3 % on the
+// first batch below and lost 6 and 9 % on the last and on small ones.  64 streams of 50
+// tokens x 8 heads over 818 shared slots: 61 us, 374 TFLOP/s; 16 of 51 over 6344: 75 us,
+// 575 TFLOP/s; 64 single tokens over 32768: 51 us.
 //
 // K (bf16) and V (f16) of a block come by TMA from a dense copy of all keys that a
 // first kernel makes (exact casts of int8, whose scales go to the scores and to P; the
@@ -211,7 +212,9 @@ __device__ __forceinline__ float load_scalar(const void* p, long i, bool bf16) {
 }
 __device__ __forceinline__ float round_to(float x, bool bf16) { return bf16 ? bf16_round(x) : x; }
 
-// P times the value scales is f16, whose numbers are fine from 2^-14 to 2^16 only.  So a
+// P times the value scales is f16, a product of the tensor cores' 16-bit kind (with the
+// int8 values exact, outputs are 2e-4 from the formula, 2-norm, before their rounding to
+// bf16, which is 1.7e-3).  f16's numbers are fine from 2^-14 to 2^16 only.  So a
 // row's weights are not taken relative to its largest score, but to the largest sum of
 // a block's largest score and its lift: the exponent of its largest value scale (all
 // are below 2^that) less 7.  Then the largest products are between 2^7 and 2^15 whatever

@@ -82,7 +82,7 @@ struct Fp4Params {
 // narrower ones every 600, which is what the issuing and the copying thread spend on a
 // step; between tiles of one accumulator 1600 ns pass, and 4.5 to 6 us of a call are
 // outside its products (set-up, first copies, last epilogue).  768 x 32768 x 2048 GeGLU 33 us,
-// 3.1 PFLOP/s; 3200 x 1024 x 4096 12 us, 2.2 PFLOP/s; 4096 x 4096 x 4096 35 us, 3.9 PFLOP/s (MX 31, 4.4).
+// 3.1 PFLOP/s; 3200 x 1024 x 4096 12.3 us, 2.2 PFLOP/s; 4096 x 4096 x 4096 35 us, 3.9 PFLOP/s (MX 31, 4.4).
 //
 // splits == 1: persistent, the pair walks the tiles.  splits > 1: a cluster of
 // `splits` pairs computes one tile, each pair a part of K; at the end each CTA

@@ -919,7 +919,8 @@ def attention_shared_desc(*, q: torch.Tensor, shared: KVRing | None, n_shared: i
     """q bf16 [B, Hq, S, 256] of any strides; shared: a ring of one stream, of
     which every stream sees the slots [0, n_shared) (those with shared_valid);
     own: a ring of B streams, stream b's slots [0, own_len[b]) (int32 on the
-    device; at most own_max, by default its capacity); k_new and v_new bf16 [B,
+    device; at most own_max, by default its capacity, of which the workspace and
+    the cut of the work count every slot); k_new and v_new bf16 [B,
     Hkv, S, 256] views, key j visible to token i iff new_block[j] <=
     new_block[i]; out bf16 [B*S, Hq*256].  A plan's descriptor needs a workspace
     whose 1024-byte aligned part holds attention_shared_workspace_bytes."""

@@ -70,18 +70,19 @@ def test_every_product_near_a_tie_is_rounded_once(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("T", [1, 50, 128, 129, 300])
+@pytest.mark.parametrize("T,Kc", [(1, 192), (50, 192), (128, 192), (129, 192), (300, 192), (60, 9000), (129, 9000)])
 @pytest.mark.parametrize("epi", [P.STORE, P.GEGLU])
 @pytest.mark.parametrize("ex,ew", [(74, 74), (-65, -65), (120, -90), (-90, 120), (110, -126), (-75, -60), (60, 60), (-126, 125)])
-def test_row_scales_whose_product_leaves_fp32(ex, ew, T, epi, dtype):
+def test_row_scales_whose_product_leaves_fp32(ex, ew, T, Kc, epi, dtype):
     """x and w of such sizes (2^ex, 2^ew) that the product of two row scales, or of one and the
     sum, is beyond fp32 or below it: the outputs are the formula's all the same, sums of 0 (rows
-    that share no places) are 0, and what is too large is infinite; in few tokens and in many."""
-    Kc, O = 192, 96
+    that share no places) are 0, and what is too large is infinite; in few tokens and in many, and
+    where K is in parts."""
+    O = 96
     r = P.gen(T + ex)
     x, w = r(T, Kc), r(O, Kc)
-    x[::2, 96:] = 0
-    w[::3, :96] = 0
+    x[::2, Kc // 2:] = 0
+    w[::3, :Kc // 2] = 0
     xq = P.quantized(x.mul(2.0 ** ex) if ex > -120 else x, NV)
     wq = P.quantized(w.mul(2.0 ** ew) if ew > -120 else w, NV, 2 if epi == P.GEGLU else 1)
     for q, e in ((xq, ex), (wq, ew)):  # (smaller than the quantizer makes them)
